@@ -42,6 +42,31 @@ class SeqCmd(C.Structure):
                 ("cbData", C.c_ubyte * 64), ("cbSize", C.c_uint), ("pad", C.c_uint * 1)]
 
 
+class Rotary(C.Structure):
+    """DctRotary: the shape, strides (batch, position, head) and frequencies of a dct_rotary call."""
+    _fields_ = [("batch", U32), ("length", U32), ("heads", U32), ("head_dim", U32),
+                ("x_stride", C.c_int64 * 3), ("y_stride", C.c_int64 * 3), ("rotated", U32),
+                ("interleaved", C.c_int), ("inverse", C.c_int), ("start", C.c_int), ("base", C.c_double),
+                ("factor", C.c_double), ("low", C.c_double), ("high", C.c_double), ("original", C.c_double),
+                ("magnitude", C.c_double)]
+
+
+class Attention(C.Structure):
+    """DctAttention: the shape, mask and strides (batch, position, head) of the attention calls."""
+    _fields_ = [("batch", U32), ("q_heads", U32), ("kv_heads", U32), ("q_len", U32), ("kv_len", U32),
+                ("head_dim", U32), ("causal", C.c_int), ("window", U32),
+                ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+                ("o_stride", C.c_int64 * 3), ("dq_stride", C.c_int64 * 3), ("dk_stride", C.c_int64 * 3),
+                ("dv_stride", C.c_int64 * 3), ("scale", F32), ("reserved", U32)]
+
+
+class Muon(C.Structure):
+    """DctMuon: the shape, polynomial and step of dct_orthogonalize and dct_muon."""
+    _fields_ = [("batch", U32), ("rows", U32), ("cols", U32), ("steps", U32), ("a", C.c_double), ("b", C.c_double),
+                ("c", C.c_double), ("eps", F32), ("lr", F32), ("momentum", F32), ("weight_decay", F32),
+                ("scale", F32), ("nesterov", C.c_int)]
+
+
 #: every exported symbol: name -> (argtypes, restype); None = leave ctypes' default
 SIGNATURES = {
     # -- reference entry points (nn_engine.py:43-119, :133-134) --
@@ -113,6 +138,12 @@ SIGNATURES = {
     "dct_sum_to_shape": ([VP, C.POINTER(C.c_int64), C.c_int, C.POINTER(C.c_int64), C.c_int, VP], C.c_int),
     "dct_broadcast_to": ([VP, C.POINTER(C.c_int64), C.c_int, C.POINTER(C.c_int64), C.c_int, VP], C.c_int),
     "dct_bias_relu_backward": ([VP, VP, VP, VP, U32, U32], C.c_int),
+    # transformer operators
+    "dct_rotary": ([C.POINTER(Rotary), VP, VP, VP], C.c_int),
+    "dct_attention_forward": ([C.POINTER(Attention)] + [VP] * 7, C.c_int),
+    "dct_attention_backward": ([C.POINTER(Attention)] + [VP] * 11, C.c_int),
+    "dct_orthogonalize": ([C.POINTER(Muon), VP, VP], C.c_int),
+    "dct_muon": ([C.POINTER(Muon), VP, VP, VP], C.c_int),
     # sharding over NCCL
     "dct_dist_available": ([], C.c_int),
     "dct_dist_nccl_version": ([], C.c_int),

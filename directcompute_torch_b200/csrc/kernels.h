@@ -243,4 +243,52 @@ cudaError_t launch_fill_random(float* y, uint64_t n, uint64_t seed, uint64_t off
 cudaError_t launch_scatter_values(float* x, const int64_t* idx, const float* vals, uint64_t k,
                                   cudaStream_t st);
 
+// ---- rotary positions (k_rotary.cu) -----------------------------------------
+struct RotaryTurns {
+  double turns[128];         // of pair j per position: frequency / 2 pi
+};
+struct RotaryArgs {
+  const float* x;
+  const int32_t* positions;  // [batch, length], or null: start + t
+  float* y;
+  uint32_t batch, length, heads, head_dim, rotated;   // batch * length < 2^31, heads * head_dim < 2^31
+  int64_t xs[3], ys[3];      // element strides of batch, position, head
+  int32_t start;
+  float magnitude;
+  bool interleaved, inverse, in_place;
+};
+cudaError_t launch_rotary(const RotaryArgs& a, const RotaryTurns& f, cudaStream_t st);
+
+// ---- attention (k_attention.cu) ------------------------------------------------
+// Rows of one key head: r = i * group + g, query position i of the group's query head g.
+struct AttnArgs {
+  const float *q, *k, *v;
+  const int32_t *q_lens, *kv_lens;       // [batch] or null
+  float *out, *lse;                      // lse [batch, q_heads, q_len] (may be null in the forward pass)
+  const float* dout;
+  float *dq, *dk, *dv;
+  int64_t qs[3], ks[3], vs[3], os[3], dqs[3], dks[3], dvs[3];   // element strides of batch, position, head
+  int batch, q_heads, kv_heads, group, q_len, kv_len, dim;
+  int causal, window;                    // window 0: none
+  float scale;
+  float* delta;                          // scratch [batch, q_heads, q_len]: sum_d dout out
+};
+// Float32 arithmetic on the CUDA cores, any finite or non-finite input.
+size_t attn_rows_ws_bytes(const AttnArgs& a);
+cudaError_t launch_attn_rows_forward(const AttnArgs& a, void* ws, cudaStream_t st);
+cudaError_t launch_attn_delta(const AttnArgs& a, cudaStream_t st);
+cudaError_t launch_attn_rows_backward(const AttnArgs& a, cudaStream_t st);
+
+// ---- orthogonalised update (k_muon.cu) -----------------------------------------
+struct MuonArgs {
+  const float* g;            // matrices [batch, rows, cols]
+  float *w, *m, *y;          // update: w and m in place; orthogonalize: y
+  uint32_t batch, rows, cols, steps;
+  double a, b, c, eps;
+  float momentum, keep, rate;   // w = keep w - rate orthogonalized
+  bool nesterov, update;
+};
+size_t muon_ws_bytes(const MuonArgs& a);
+cudaError_t launch_muon(const MuonArgs& a, void* ws, cudaStream_t st);
+
 }  // namespace dct

@@ -20,7 +20,10 @@ define these ops.  They run on the library's dct_* entry points:
   forward pass also writes dlogits, so the backward is one scaled copy;
 * `bias_relu` (the reference's bias_relu shader, nn_bias_relu.hlsl:8-12) whose
   backward is one fused pass (dct_bias_relu_backward), and `batch_norm2d`
-  (training statistics, running-stat update, fused backward).
+  (training statistics, running-stat update, fused backward);
+* the operators of a transformer: `rotary` positions and `attention` (grouped heads,
+  causal and windowed masks, ragged lengths), both differentiable, and the
+  `orthogonalize`d update with its optimizer step `muon_step`.
 
 The graph is built on a tensor type with the reference Tensor's protocol
 (`gpu_buf`, `shape`, `requires_grad`, `grad`, `_ctx`, `_accumulate_grad`,
@@ -40,12 +43,13 @@ import struct
 import numpy as np
 
 from . import load_library
-from ._abi import BINARY, REDUCE, UNARY, check
+from ._abi import BINARY, REDUCE, UNARY, Attention, Muon, Rotary, check
 from .tensor import DeviceTensor, Node
 
 __all__ = ["add", "sub", "mul", "div", "maximum", "minimum", "exp", "log_abs1p", "tanh", "sigmoid", "neg",
            "abs", "sum", "mean", "max", "min", "argmax", "argmin", "sum_to_shape", "broadcast_to",
-           "softmax_cross_entropy", "bias_relu", "batch_norm2d", "tensor", "to_numpy", "bind"]
+           "softmax_cross_entropy", "bias_relu", "batch_norm2d", "rotary", "attention", "orthogonalize", "muon_step",
+           "tensor", "to_numpy", "bind"]
 
 lib = load_library()
 Tensor = DeviceTensor
@@ -532,3 +536,172 @@ def batch_norm2d(x, gamma, beta, running_mean, running_var, training=True, momen
     _run_shader("batchnorm_forward", [x.gpu_buf, running_mean.gpu_buf, running_var.gpu_buf, gamma.gpu_buf,
                                       beta.gpu_buf], [h], ((x.size + 255) // 256, 1, 1), [N, C, H * W, _f2u(eps)])
     return _wrap(h, x.shape)
+
+
+# ---------------------------------------------------------------------------
+# rotary positions, attention
+# ---------------------------------------------------------------------------
+def _words(a, shape, what):
+    """A buffer of int32 words from array-like `a` (None stays None)."""
+    if a is None:
+        return None
+    a = np.asarray(a)
+    if not np.issubdtype(a.dtype, np.integer):
+        raise ValueError(f"{what}: integers expected, got {a.dtype}")
+    a = np.ascontiguousarray(np.broadcast_to(a, shape), dtype=np.int32)
+    if not a.size:
+        return _buf(1)
+    h = lib.CreateBuffer(a.ctypes.data_as(ctypes.POINTER(ctypes.c_float)), a.size)
+    if not h:
+        raise MemoryError("libdct_cuda: " + (lib.dct_last_error() or b"").decode())
+    return h
+
+
+def _strides(shape):
+    """Element strides of batch, position and head of an adjacent [batch, position, head, feature]."""
+    _, t, h, d = shape
+    return (t * h * d, h * d, d)
+
+
+class RotaryFunc(Node):
+    """Pairs of features turned by their position's angle; the backward turns the gradient back."""
+
+    def forward(self, x, positions, **kw):
+        if len(x.shape) != 4:
+            raise ValueError("rotary: x must be [batch, position, head, feature]")
+        self.inputs = (x,)
+        b, t, h, d = x.shape
+        self.positions = _words(positions, (b, t), "rotary positions")
+        self.p = Rotary(batch=b, length=t, heads=h, head_dim=d, x_stride=_strides(x.shape),
+                        y_stride=_strides(x.shape), **kw)
+        return _wrap(self._turn(x), x.shape, self, x.requires_grad)
+
+    def _turn(self, x):
+        y = _buf(x.size)
+        rc = lib.dct_rotary(ctypes.byref(self.p), x.gpu_buf, self.positions, y)
+        if rc:
+            _release(y)
+        check(lib, rc, "dct_rotary")
+        return y
+
+    def backward(self, g):
+        x = self.inputs[0]
+        if x.requires_grad:
+            self.p.inverse = 1
+            x._accumulate_grad(_wrap(self._turn(g), x.shape))
+
+    def __del__(self):
+        if getattr(self, "positions", None):
+            try:
+                lib.ReleaseBuffer(self.positions)
+            except Exception:
+                pass
+            self.positions = None
+
+
+def rotary(x, positions=None, start=0, rotated=None, interleaved=False, base=10000.0, factor=1.0, original=0.0,
+           low=1.0, high=32.0, magnitude=1.0):
+    """Rotary positions of x [batch, position, head, feature] (differentiable in x).
+
+    positions: integers [batch, position] (or broadcastable), else start + t.  rotated: the
+    first so many features turn (default all).  interleaved: pairs (2j, 2j+1) instead of
+    (j, j + rotated/2).  factor, original, low, high, magnitude: scaling for contexts longer
+    than `original` (see DctRotary in include/dct_cuda.h)."""
+    return RotaryFunc().forward(x, positions, start=start, rotated=x.shape[-1] if rotated is None else rotated,
+                                interleaved=bool(interleaved), base=base, factor=factor, original=original, low=low,
+                                high=high, magnitude=magnitude)
+
+
+class AttentionFunc(Node):
+    """softmax(scale q k^T + mask) v; the backward recomputes the probabilities from the
+    saved log-sums."""
+
+    def forward(self, q, k, v, causal, window, scale, q_lens, kv_lens):
+        if len(q.shape) != 4 or len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or \
+                q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+            raise ValueError(f"attention: q {q.shape}, k {k.shape} and v {v.shape} do not match")
+        self.inputs = (q, k, v)
+        b, t, h, d = q.shape
+        self.words = [_words(q_lens, (b,), "attention q_lens"), _words(kv_lens, (b,), "attention kv_lens")]
+        qs, ks = _strides(q.shape), _strides(k.shape)
+        self.p = Attention(batch=b, q_heads=h, kv_heads=k.shape[2], q_len=t, kv_len=k.shape[1], head_dim=d,
+                           causal=bool(causal), window=window, q_stride=qs, k_stride=ks, v_stride=ks, o_stride=qs,
+                           dq_stride=qs, dk_stride=ks, dv_stride=ks, scale=scale or 0.0)
+        oh, lh = _buf(q.size), _buf(b * t * h)
+        rc = lib.dct_attention_forward(ctypes.byref(self.p), q.gpu_buf, k.gpu_buf, v.gpu_buf, *self.words, oh, lh)
+        if rc:
+            _release(oh, lh)
+        check(lib, rc, "dct_attention_forward")
+        self.lse = _wrap(lh, (b, h, t))
+        lib.AddRefBuffer(oh)                  # the buffer, not the tensor: that would be a cycle
+        self.out = oh
+        return _wrap(oh, q.shape, self, q.requires_grad or k.requires_grad or v.requires_grad)
+
+    def backward(self, g):
+        q, k, v = self.inputs
+        grads = [_buf(t.size) for t in (q, k, v)]
+        rc = lib.dct_attention_backward(ctypes.byref(self.p), q.gpu_buf, k.gpu_buf, v.gpu_buf, *self.words,
+                                        self.out, self.lse.gpu_buf, g.gpu_buf, *grads)
+        if rc:
+            _release(*grads)
+        check(lib, rc, "dct_attention_backward")
+        for t, h in zip((q, k, v), grads):
+            if t.requires_grad:
+                t._accumulate_grad(_wrap(h, t.shape))
+            else:
+                _release(h)
+
+    def __del__(self):
+        for h in (*getattr(self, "words", ()), getattr(self, "out", None)):
+            if h:
+                try:
+                    lib.ReleaseBuffer(h)
+                except Exception:
+                    pass
+        self.words, self.out = (), None
+
+
+def attention(q, k, v, causal=False, window=0, scale=None, q_lens=None, kv_lens=None, return_lse=False):
+    """Attention of q [batch, position, head, feature] over k and v (as many heads, or a
+    divisor of them), differentiable in all three.
+
+    causal: a query sees the keys up to its own position, the last query standing at the
+    last key.  window > 0: only the nearest `window` positions.  scale: default
+    1/sqrt(features).  q_lens, kv_lens: valid positions of each batch entry.  A query that
+    sees nothing gets 0 (and log-sum -inf)."""
+    f = AttentionFunc()
+    out = f.forward(q, k, v, causal, window, scale, q_lens, kv_lens)
+    return (out, f.lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------
+# the orthogonalised update
+# ---------------------------------------------------------------------------
+def _muon(x, steps, coefficients, eps, **kw):
+    if len(x.shape) < 2:
+        raise ValueError("orthogonalize: matrices [..., rows, cols] expected")
+    a, b, c = coefficients
+    return Muon(batch=_size(x.shape[:-2]), rows=x.shape[-2], cols=x.shape[-1], steps=steps, a=a, b=b, c=c, eps=eps,
+                **kw)
+
+
+def orthogonalize(x, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """Matrices x [..., rows, cols] with their singular values moved toward 1 by
+    Newton-Schulz steps (no gradient)."""
+    h = _buf(x.size)
+    rc = lib.dct_orthogonalize(ctypes.byref(_muon(x, steps, coefficients, eps)), x.gpu_buf, h)
+    if rc:
+        _release(h)
+    check(lib, rc, "dct_orthogonalize")
+    return _wrap(h, x.shape)
+
+
+def muon_step(w, m, g, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, scale=0.0, steps=5,
+              coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """One optimizer step in place: m = momentum m + g; w = w (1 - lr weight_decay) - lr scale
+    orthogonalize(g + momentum m, or m without nesterov).  scale 0: sqrt(max(1, rows/cols))."""
+    if not (tuple(w.shape) == tuple(m.shape) == tuple(g.shape)):
+        raise ValueError(f"muon_step: w {w.shape}, m {m.shape} and g {g.shape} differ")
+    p = _muon(w, steps, coefficients, eps, lr=lr, momentum=momentum, nesterov=bool(nesterov),
+              weight_decay=weight_decay, scale=scale)
+    check(lib, lib.dct_muon(ctypes.byref(p), w.gpu_buf, m.gpu_buf, g.gpu_buf), "dct_muon")

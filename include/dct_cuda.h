@@ -291,6 +291,88 @@ DCT_API int dct_batchnorm_forward_train_noalloc(const float* x, const float* gam
                                                 float* batch_var, float* y, uint32_t N, uint32_t C, uint32_t S,
                                                 float eps, float momentum, void* stream);
 
+/* ======================= transformer operators =================================
+ * No kernels in the reference: its attention wrappers (nn_engine.py:1571-1792) name
+ * shaders that its snapshot does not hold, and its Muon (nn_engine.py:2244-2319)
+ * leaves the matrix products to a matmul outside this library.
+ *
+ * Tensors are float32 [batch, position, head, feature] with a head's features
+ * adjacent; the three other strides are given in elements, so a head of a packed
+ * projection or of a cache with spare room needs no copy (for a tensor that starts
+ * inside a buffer, wrap its first element).  Strides are not negative, the elements of
+ * an output are distinct, and no output shares its address range with an input, except
+ * where a call says that it works in place (DCT_ERR_ARG otherwise).  Index tensors are
+ * int32 words.  A size of 0 is allowed for batch and lengths.  The calls use the
+ * library's stream and scratch workspace; a stream that is being captured into a
+ * graph is refused (DCT_ERR_UNSUPPORTED), since a later call may move the workspace.
+ * Results are the same, bit for bit, from run to run. */
+
+/* Rotary positions: pair j of the first `rotated` features (even; the features behind
+ * them are copied) turns by the angle position * f[j] and is scaled by `magnitude`:
+ *   y1 = magnitude * (x1 cos - x2 sin),  y2 = magnitude * (x2 cos + x1 sin)
+ * Pairs are features (j, j + rotated/2), or (2j, 2j+1) when `interleaved`.  `inverse`
+ * turns the other way: with it the call is the gradient (the transpose) of the one
+ * without.  Positions: positions[b * length + t], or start + t when null.
+ * f[j] = base^(-2j/rotated).  With factor != 1 and original = 0 every f[j] is divided by
+ * factor.  With original > 0 (the context length that the frequencies were made for) a
+ * pair that turns r = original * f[j] / (2 pi) times in it keeps g = clamp((r - low) /
+ * (high - low), 0, 1) of its frequency: f[j] * (g + (1 - g) / factor).  Angles are formed
+ * and reduced in float64.  y may be x (same strides). */
+typedef struct DctRotary {
+  uint32_t batch, length, heads, head_dim;
+  int64_t x_stride[3], y_stride[3];        /* batch, position, head */
+  uint32_t rotated;
+  int32_t interleaved, inverse, start;
+  double base, factor, low, high, original, magnitude;
+} DctRotary;
+DCT_API int dct_rotary(const DctRotary* p, void* x, void* positions, void* y);
+
+/* Attention of q_heads query heads over kv_heads key/value heads (query head h reads
+ * key head h / (q_heads / kv_heads)); head_dim 1..128, scale 0 means 1/sqrt(head_dim).
+ * With m = q_lens[b] (null: q_len) and n = kv_lens[b] (null: kv_len) valid positions,
+ * clamped to [0, q_len] and [0, kv_len], query i < m stands at position p = i + n - m and
+ * sees the keys j < n with
+ *   causal: j <= p        window > 0: j > p - window, and j < p + window
+ *   out = sum_j softmax_j(scale q.k_j) v_j      lse[b, h, i] = log sum_j exp(scale q.k_j)
+ * A query that sees no key, and every query i >= m, gets out = 0 and lse = -inf, and its
+ * gradients are 0; keys and values at j >= n are not used and their gradients are 0.
+ * What a masked place holds, NaN and infinity too, does not reach a result.  lse is
+ * [batch, q_heads, q_len], adjacent; it may be null in the forward call.  The backward
+ * call takes the forward call's out and lse and recomputes the probabilities; dout has
+ * o_stride. */
+typedef struct DctAttention {
+  uint32_t batch, q_heads, kv_heads, q_len, kv_len, head_dim;
+  int32_t causal;
+  uint32_t window;
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];      /* batch, position, head */
+  int64_t dq_stride[3], dk_stride[3], dv_stride[3];                /* backward only */
+  float scale;
+  uint32_t reserved;
+} DctAttention;
+DCT_API int dct_attention_forward(const DctAttention* p, void* q, void* k, void* v, void* q_lens, void* kv_lens,
+                                  void* out, void* lse);
+DCT_API int dct_attention_backward(const DctAttention* p, void* q, void* k, void* v, void* q_lens, void* kv_lens,
+                                   void* out, void* lse, void* dout, void* dq, void* dk, void* dv);
+
+/* Orthogonalisation of `batch` matrices [rows, cols] (adjacent) by Newton-Schulz steps:
+ *   X = x / (|x|_F + eps);  `steps` times:  A = X X^T,  X = a X + (b A + c A A) X
+ * (on the shorter side; X^T X for tall matrices), which moves the singular values
+ * toward 1.  a = b = c = 0 means 3.4445, -4.7750, 2.0315; steps 0..16; the polynomial
+ * a s + b s^3 + c s^5 must keep [0, 1] below 64 over the steps (DCT_ERR_ARG).  y may be x. */
+typedef struct DctMuon {
+  uint32_t batch, rows, cols, steps;
+  double a, b, c;
+  float eps;
+  /* dct_muon only */
+  float lr, momentum, weight_decay, scale;   /* scale 0 means sqrt(max(1, rows / cols)) */
+  int32_t nesterov;
+} DctMuon;
+DCT_API int dct_orthogonalize(const DctMuon* p, void* x, void* y);
+/* One optimizer step in place on w and m:
+ *   m = momentum m + g;  u = nesterov ? g + momentum m : m;
+ *   w = w (1 - lr weight_decay) - lr scale orthogonalize(u) */
+DCT_API int dct_muon(const DctMuon* p, void* w, void* m, void* g);
+
 /* ======================= sharding over NCCL (one process per GPU) ==============
  * No counterpart in the reference, which drives one D3D11 device
  * (engine.cpp:61-129).  Each rank holds one contiguous shard of the sharded
