@@ -1,117 +1,611 @@
 // Orthogonalisation by Newton-Schulz steps, and the optimizer update around it.
+//
+// X = u / (|u| + eps), then `steps` times A = X X^T, P = c A A + b A, X = P X + a X (for tall
+// matrices A = X^T X, and P on the right).  The terms b A and a X are added in float32 after
+// the products: inside them, as multiples of the identity, they would be rounded with every
+// matrix instruction (see k_product), which measured 5 times the error.
+//
+// It is bound by the tensor cores: X, A and P live as split float16 chunks (dct_umma.cuh)
+// from the first kernel to the last, and one persistent kernel forms each product at float32
+// accuracy.  Of the symmetric A and P only the tiles up to the diagonal are formed and
+// stored; a chunk above it is read as the transpose of its mirror image, which the matrix
+// instructions do at no cost.  The powers of two are constants: no entry is larger than the
+// matrix's norm, which the polynomial bounds from the start.
+#include <algorithm>
+
 #include "dct_common.cuh"
+#include "dct_umma.cuh"
 #include "kernels.h"
 
 namespace dct {
 namespace {
 
-constexpr int kTile = 64, kDepth = 16;
-
-// C = alpha op(A) op(B) + beta D over a batch of matrices; element (i, k) of A lies at
-// i * ai + k * ak, likewise B (k, j).  64 x 64 tiles, 4 x 4 outputs a thread.
-struct Gemm {
-  const float *A, *B, *D;
-  float* C;
-  int64_t ai, ak, bk, bj, cs;       // C and D row stride
-  int64_t az, bz, cz;               // between matrices
-  int M, N, K;
-  float alpha, beta;
+// ---------------------------------------------------------------------------
+// C = sa A B + sd D over a batch, as chunks or as the final float32 result
+// ---------------------------------------------------------------------------
+struct Operand {
+  const uint8_t* p;
+  uint32_t cb;               // chunks per row of chunks
+  uint64_t z;                // bytes between matrices
+  bool mn;                   // its rows are the contraction
+  bool half;                 // symmetric, the tiles above the diagonal are not stored
 };
-__global__ void __launch_bounds__(256) k_gemm(const __grid_constant__ Gemm g) {
-  __shared__ float as[kDepth][kTile + 1], bs[kDepth][kTile + 1];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int i0 = blockIdx.y * kTile, j0 = blockIdx.x * kTile;
-  const float* A = g.A + blockIdx.z * g.az;
-  const float* B = g.B + blockIdx.z * g.bz;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < g.K; k0 += kDepth) {
-    for (int t = threadIdx.x; t < kTile * kDepth; t += 256) {
-      const int i = t / kDepth, k = t % kDepth;
-      as[k][i] = i0 + i < g.M && k0 + k < g.K ? A[(i0 + i) * g.ai + (k0 + k) * g.ak] : 0.f;
-      bs[k][i] = j0 + i < g.N && k0 + k < g.K ? B[(k0 + k) * g.bk + (j0 + i) * g.bj] : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kDepth; ++k)
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(as[k][ty + 16 * u], bs[k][tx + 16 * v], acc[u][v]);
-    __syncthreads();
+DCT_DEV const uint8_t* chunk_of(const Operand& o, uint32_t z, uint32_t rb, uint32_t cb) {
+  return o.p + z * o.z + ((uint64_t)rb * o.cb + cb) * kPairBytes;
+}
+struct Product {
+  Operand A, B, D;           // D.p null: no D; else stored where C is
+  uint8_t* C;                // chunks, or null: final
+  uint32_t c_cb;
+  uint64_t c_z;
+  float sa, sd;
+  uint32_t M, N, kb;         // rows, columns, contraction in chunks of 64
+  uint32_t mt, nt, tiles;    // rows and columns of tiles, tiles of a matrix
+  bool half;                 // C is symmetric: only the tiles up to the diagonal
+  // final result
+  float* out;                // y, or w
+  float keep, rate;
+  bool update;               // out = keep out - rate C, else out = C
+  float* parts;              // sums of cut tiles, two slots a worker and block
+  uint32_t* arrived;         // segments of a worker's cut tile that are summed (zero between launches)
+};
+
+constexpr int kRows = 128, kEpi = 8;            // tile rows of a block, epilogue warps
+constexpr int kThreads = 32 * (kEpi + 2);
+
+constexpr uint32_t kStaging = 4096;              // of an epilogue warp: its 32 rows of a chunk
+
+template <bool PAIR, int BN>
+struct Shape {
+  static constexpr uint32_t kTileRows = PAIR ? 2 * kRows : kRows;
+  static constexpr uint32_t kBChunks = (PAIR ? BN / 2 : BN) / 64;    // chunks of B's columns in this block
+  static constexpr uint32_t kA = 2 * kPairBytes, kB = kBChunks * kPairBytes, kStage = kA + kB;
+  static constexpr int kStages = 196608 / kStage > 4 ? 4 : 196608 / kStage;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kEpi * kStaging;
+};
+
+// tile number -> batch entry, row and column of tiles
+DCT_DEV void tile_at(const Product& g, uint32_t t, uint32_t& z, uint32_t& i, uint32_t& j) {
+  z = t / g.tiles;
+  uint32_t r = t - z * g.tiles;
+  if (!g.half) {
+    i = r % g.mt;            // neighbours share the B tile
+    j = r / g.mt;
+    return;
   }
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int i = i0 + ty + 16 * u, j = j0 + tx + 16 * v;
-      if (i < g.M && j < g.N) {
-        const int64_t at = blockIdx.z * g.cz + i * g.cs + j;
-        g.C[at] = g.D ? fmaf(g.alpha, acc[u][v], g.beta * g.D[at]) : g.alpha * acc[u][v];
-      }
-    }
+  for (i = 0; r > i; ++i) r -= i + 1;      // row i holds the tiles 0 .. i
+  j = r;
 }
 
-constexpr int kChunks = 64;         // partial sums of squares per matrix
+// The chunks of all tiles in a row are dealt to the workers (blocks, or pairs of blocks) in
+// equal runs of whole units: one chunk, so that every worker is busy to the end whatever the
+// number of tiles, or a whole tile.  A worker's share of one tile is a segment.
+struct Segment {
+  uint32_t tile, k0, k1;     // chunks [k0, k1) of the tile
+  uint32_t first, count;     // the worker with the tile's first segment, the tile's segments
+};
+struct Run {
+  uint64_t at, end, units;
+  uint32_t kb, unit, workers;
+  DCT_DEV Run(uint32_t tiles, uint32_t kb_, uint32_t unit_, uint32_t worker, uint32_t workers_)
+      : units((uint64_t)tiles * (kb_ / unit_)), kb(kb_), unit(unit_), workers(workers_) {
+    at = worker * units / workers * unit;
+    end = (worker + 1) * units / workers * unit;
+  }
+  DCT_DEV uint32_t worker_of(uint64_t chunk) const {
+    return (uint32_t)(((chunk / unit + 1) * workers - 1) / units);
+  }
+  DCT_DEV bool next(Segment& s) {
+    if (at >= end) return false;
+    s.tile = (uint32_t)(at / kb);
+    const uint64_t base = (uint64_t)s.tile * kb;
+    s.k0 = (uint32_t)(at - base);
+    s.k1 = (uint32_t)min((uint64_t)kb, end - base);
+    s.first = worker_of(base);
+    s.count = worker_of(base + kb - 1) - s.first + 1;
+    at = base + s.k1;
+    return true;
+  }
+};
 
-// u = the matrix to orthogonalise (with the momentum update), and its sums of squares
-__global__ void __launch_bounds__(256) k_muon_momentum(const __grid_constant__ MuonArgs a, float* u, double* part) {
+// acc[at .. at + 7] += f * the float16 numbers of v
+template <int N>
+DCT_DEV void add8(float (&acc)[N], int at, float f, uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+    acc[at + 2 * e] = fmaf(f, x.x, acc[at + 2 * e]);
+    acc[at + 2 * e + 1] = fmaf(f, x.y, acc[at + 2 * e + 1]);
+  }
+}
+
+DCT_DEV void epilogue_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// Warps 0..7 drain and store, warp 8 loads, warp 9 issues the matrix instructions.
+//
+// The tensor cores round every sum toward zero: a chain of n matrix instructions is off by
+// about n/2 * 2^-24 of a sum that grows steadily (5e-5 after 8192 columns, measured), so the
+// accumulator is drained to registers every kDrain chunks and added there with rounding to
+// nearest, and within a chunk the small cross products come first.
+//
+// Tiles that several blocks share meet in memory: every block leaves its sum, and the last
+// to arrive adds them in the order of the contraction, so the result does not depend on who
+// that was.
+constexpr uint32_t kDrain = 2;
+//
+// PAIR: two blocks on one tile of twice the rows.  A chunk of the contraction then costs a
+// block 64 KB of loads instead of 96 KB (tile 256 columns wide), and the loads are what
+// bounds the large products: 6.4 TB/s out of L2 at 2048 x 8192 without pairs.
+template <bool PAIR, int BN>
+__global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__ Product g, uint32_t total,
+                                                         uint32_t unit, uint32_t* err) {
+  using S = Shape<PAIR, BN>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+  __shared__ uint64_t full[4], empty[4], there[4], done[2], freed[2];   // there: the other block's chunk is in
+  __shared__ uint32_t tmem_base, order;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0, worker = PAIR ? blockIdx.x / 2 : blockIdx.x;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&there[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&done[s], 1);
+      mbar_init(&freed[s], PAIR ? 2 * kEpi : kEpi);
+    }
+    mbar_fence_init();
+  }
+  if (warp == kEpi + 1) {
+    if constexpr (PAIR) tmem_alloc_pair(&tmem_base, 2 * BN);
+    else tmem_alloc(&tmem_base, 2 * BN);
+  }
+  tc_fence_before();
+  if constexpr (PAIR) cluster_sync();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  pdl_entry();
+  const uint32_t mchunks = (g.M + 63) / 64, nchunks = (g.N + 63) / 64;
+  Run run(total, g.kb, unit, worker, PAIR ? gridDim.x / 2 : gridDim.x);
+  Segment sg;
+  // whether chunk k of an operand's tile is read with its rows as the contraction: its own
+  // layout, or the mirror image of a chunk above the diagonal
+  auto transposed = [](const Operand& o, uint32_t tile, uint32_t k) {
+    return o.half ? tile < k / (S::kTileRows / 64) : o.mn;
+  };
+
+  if (warp == kEpi) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      while (ok && run.next(sg)) {
+        uint32_t z, ti, tj;
+        tile_at(g, sg.tile, z, ti, tj);
+        const uint32_t m0 = ti * (S::kTileRows / 64) + rank * 2, n0 = tj * (BN / 64) + rank * S::kBChunks;
+        const uint32_t mc = m0 < mchunks ? min(2u, mchunks - m0) : 0;
+        const uint32_t nc = n0 < nchunks ? min(S::kBChunks, nchunks - n0) : 0;
+        for (uint32_t k = sg.k0; k < sg.k1; ++k, ++it) {
+          const uint32_t s = it % S::kStages;
+          ok = mbar_wait(&empty[s], ((it / S::kStages) & 1) ^ 1, err);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full[s], (mc + nc) * kPairBytes);
+          const bool a_mn = transposed(g.A, ti, k), b_mn = transposed(g.B, tj, k);
+          uint8_t* a = sm + s * S::kStage;
+          for (uint32_t p = 0; p < mc; ++p) {
+            const uint8_t* c = a_mn ? chunk_of(g.A, z, k, m0 + p) : chunk_of(g.A, z, m0 + p, k);
+            bulk_load(a + p * kChunkBytes, c, kChunkBytes, &full[s]);
+            bulk_load(a + (2 + p) * kChunkBytes, c + kChunkBytes, kChunkBytes, &full[s]);
+          }
+          uint8_t* b = a + S::kA;
+          for (uint32_t p = 0; p < nc; ++p) {
+            const uint8_t* c = b_mn ? chunk_of(g.B, z, k, n0 + p) : chunk_of(g.B, z, n0 + p, k);
+            bulk_load(b + p * kChunkBytes, c, kChunkBytes, &full[s]);
+            bulk_load(b + (S::kBChunks + p) * kChunkBytes, c + kChunkBytes, kChunkBytes, &full[s]);
+          }
+        }
+      }
+      // every copy has landed before the block may end
+      for (uint32_t u = it > (uint32_t)S::kStages ? it - S::kStages : 0; u < it; ++u)
+        mbar_wait(&full[u % S::kStages], (u / S::kStages) & 1, err);
+    }
+  } else if (warp == kEpi + 1 && rank != 0) {
+    if (lane == 0) {                              // tells the even block of each chunk that has come in
+      uint32_t it = 0;
+      bool ok = true;
+      while (ok && run.next(sg))
+        for (uint32_t k = sg.k0; k < sg.k1 && ok; ++k, ++it) {
+          const uint32_t s = it % S::kStages;
+          ok = mbar_wait(&full[s], (it / S::kStages) & 1, err);
+          if (ok) mbar_arrive_at(&there[s], 0);
+        }
+    }
+  } else if (warp == kEpi + 1) {
+    if (lane == 0) {
+      auto mma = [](uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+        if constexpr (PAIR) umma_pair(d, a, b, idesc, add);
+        else umma(d, a, b, idesc, add);
+      };
+      auto commit = [](uint64_t* bar) {
+        if constexpr (PAIR) umma_commit_pair(bar);
+        else umma_commit(bar);
+      };
+      uint32_t it = 0, part = 0;
+      bool ok = true;
+      while (ok && run.next(sg)) {
+        uint32_t z, ti, tj;
+        tile_at(g, sg.tile, z, ti, tj);
+        for (uint32_t k0 = sg.k0; k0 < sg.k1 && ok; k0 += kDrain, ++part) {
+          const uint32_t buf = part & 1, d = tmem + buf * BN, k1 = min(sg.k1, k0 + kDrain);
+          ok = mbar_wait_cluster(&freed[buf], ((part >> 1) & 1) ^ 1, err);
+          tc_fence_after();
+          for (uint32_t k = k0; k < k1 && ok; ++k, ++it) {
+            const uint32_t s = it % S::kStages;
+            ok = mbar_wait(&full[s], (it / S::kStages) & 1, err);
+            if (PAIR && ok) ok = mbar_wait_cluster(&there[s], (it / S::kStages) & 1, err);
+            if (!ok) break;
+            tc_fence_after();
+            const bool a_mn = transposed(g.A, ti, k), b_mn = transposed(g.B, tj, k);
+            const uint32_t idesc = umma_idesc(S::kTileRows, BN, a_mn, b_mn);
+            const uint32_t step_a = (a_mn ? 2048 : 32) / 16, step_b = (b_mn ? 2048 : 32) / 16;   // 16 rows, or 16 columns
+            const uint32_t a = smem_addr(sm + s * S::kStage), b = a + S::kA;
+            const uint64_t ah = umma_desc(a, kChunkBytes, 1024), bh = umma_desc(b, kChunkBytes, 1024);
+            const uint64_t al = ah + 2 * kChunkBytes / 16, bl = bh + S::kBChunks * kChunkBytes / 16;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              mma(d, al + q * step_a, bh + q * step_b, idesc, k != k0 || q != 0);
+              mma(d, ah + q * step_a, bl + q * step_b, idesc, true);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mma(d, ah + q * step_a, bh + q * step_b, idesc, true);
+            commit(&empty[s]);
+          }
+          commit(&done[buf]);
+        }
+      }
+    }
+  } else {
+    constexpr int W = BN / 2;                     // columns of a thread's row
+    const uint32_t side = warp >> 2;
+    uint8_t* stage = sm + S::kStages * S::kStage + warp * kStaging;
+    uint32_t part = 0;
+    bool ok = true;
+    while (ok && run.next(sg)) {
+      float acc[W];
+#pragma unroll
+      for (int c = 0; c < W; ++c) acc[c] = 0.f;
+      for (uint32_t k0 = sg.k0; k0 < sg.k1 && ok; k0 += kDrain, ++part) {
+        const uint32_t buf = part & 1;
+        ok = mbar_wait(&done[buf], (part >> 1) & 1, err);
+        tc_fence_after();
+        if (ok) {
+#pragma unroll
+          for (int c = 0; c < W; c += 32) {
+            uint32_t v[32];
+            tmem_load32(tmem + ((warp & 3) * 32u << 16) + buf * BN + side * W + c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) acc[c + e] += __uint_as_float(v[e]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (rank == 0) mbar_arrive(&freed[buf]);
+          else mbar_arrive_at(&freed[buf], 0);
+        }
+      }
+      if (!ok) break;
+      if (sg.count > 1) {                         // the tile is cut
+        auto slot = [&](uint32_t w) {
+          return g.parts + (size_t)(2 * (PAIR ? 2 * w + rank : w) + (w == sg.first)) * (kRows * BN) + threadIdx.x;
+        };
+        uint32_t* arrived = g.arrived + (PAIR ? 2 * sg.first + rank : sg.first);
+        float* mine = slot(worker);
+#pragma unroll
+        for (int c = 0; c < W; ++c) __stcg(mine + c * 256, acc[c]);
+        __threadfence();
+        epilogue_sync();
+        if (threadIdx.x == 0) order = atomicAdd(arrived, 1u);
+        epilogue_sync();
+        const bool last = order == sg.count - 1;
+        if (!last) continue;
+        __threadfence();
+        if (threadIdx.x == 0) *arrived = 0;
+#pragma unroll
+        for (int c = 0; c < W; ++c) acc[c] = 0.f;
+        for (uint32_t b = sg.first; b < sg.first + sg.count; ++b) {
+          const float* p = slot(b);
+#pragma unroll
+          for (int c = 0; c < W; ++c) acc[c] += __ldcg(p + c * 256);
+        }
+      }
+      uint32_t z, ti, tj;
+      tile_at(g, sg.tile, z, ti, tj);
+      // the warp's 32 rows from i0, the thread's row i, its columns from j0
+      const uint32_t i0 = ti * S::kTileRows + rank * kRows + (warp & 3) * 32, i = i0 + lane, j0 = tj * BN + side * W;
+#pragma unroll
+      for (int c = 0; c < W; ++c) acc[c] *= g.sa;
+      if (g.D.p && i0 < mchunks * 64) {
+        if constexpr (W < 64) {
+          const uint8_t* d = chunk_of(g.D, z, i >> 6, j0 >> 6);
+#pragma unroll
+          for (int e = 0; e < W; e += 8) {
+            const uint8_t* p = d + chunk_at(i & 63, ((j0 & 63) + e) >> 3);
+            add8(acc, e, g.sd, *reinterpret_cast<const uint4*>(p));
+            add8(acc, e, g.sd, *reinterpret_cast<const uint4*>(p + kChunkBytes));
+          }
+        } else
+#pragma unroll
+        for (int c = 0; c < W; c += 64) {         // whole rows into the staging, then each thread its row
+          if (j0 + c >= nchunks * 64) break;
+          const uint8_t* d = chunk_of(g.D, z, i0 >> 6, (j0 + c) >> 6) + (i0 & 32) * 128;
+#pragma unroll
+          for (int low = 0; low < 2; ++low) {
+            uint4 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              v[e] = *reinterpret_cast<const uint4*>(d + low * kChunkBytes + (e * 32 + lane) * 16);
+            if (lane == 0) bulk_store_read();     // an earlier tile's stores have left the staging
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(stage + (e * 32 + lane) * 16) = v[e];
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 64; e += 8)
+              add8(acc, c + e, g.sd, *reinterpret_cast<const uint4*>(stage + chunk_at(lane, e >> 3)));
+          }
+        }
+      }
+      if (g.C) {
+        // rows and columns behind M and N inside a chunk come out zero, as their operands are
+        if (i0 >= mchunks * 64) continue;
+        if constexpr (W < 64) {                   // half rows of a chunk do not lie together: no bulk copy
+          uint8_t* o = g.C + z * g.c_z + ((uint64_t)(i0 >> 6) * g.c_cb + (j0 >> 6)) * kPairBytes;
+#pragma unroll
+          for (int e = 0; e < W; e += 8) {
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) split2(acc[e + 2 * q], acc[e + 2 * q + 1], h[q], l[q]);
+            uint8_t* p = o + chunk_at(i & 63, ((j0 & 63) + e) >> 3);
+            *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(p + kChunkBytes) = make_uint4(l[0], l[1], l[2], l[3]);
+          }
+        } else
+#pragma unroll
+        for (int c = 0; c < W; c += 64) {
+          const uint32_t j = j0 + c;
+          if (j >= nchunks * 64) break;
+          uint8_t* o = g.C + z * g.c_z + ((uint64_t)(i0 >> 6) * g.c_cb + (j >> 6)) * kPairBytes + (i0 & 32) * 128;
+#pragma unroll
+          for (int low = 0; low < 2; ++low) {
+            if (lane == 0) bulk_store_read();     // the staging is free again
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 64; e += 8) {
+              uint32_t h[4], l[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) split2(acc[c + e + 2 * q], acc[c + e + 2 * q + 1], h[q], l[q]);
+              *reinterpret_cast<uint4*>(stage + chunk_at(lane, e >> 3)) =
+                  low ? make_uint4(l[0], l[1], l[2], l[3]) : make_uint4(h[0], h[1], h[2], h[3]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) bulk_store(o + low * kChunkBytes, stage, kStaging);
+          }
+        }
+      } else {
+        // through the staging, so that a warp reads and writes whole rows of 32 floats
+#pragma unroll
+        for (int c = 0; c < W; c += 32) {
+          float* t = reinterpret_cast<float*>(stage);
+          __syncwarp();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) t[lane * 32 + ((e + lane) & 31)] = acc[c + e];
+          __syncwarp();
+          const uint32_t j = j0 + c + lane;
+          if (j < g.N) {
+            float* o = g.out + ((uint64_t)z * g.M + i0) * g.N + j;
+            const uint32_t rows = i0 < g.M ? min(32u, g.M - i0) : 0;
+#pragma unroll 8
+            for (uint32_t r = 0; r < rows; ++r) {
+              const float v = t[r * 32 + ((lane + r) & 31)];
+              o[(uint64_t)r * g.N] = g.update ? fmaf(-g.rate, v, g.keep * o[(uint64_t)r * g.N]) : v;
+            }
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_store_done();
+  }
+  tc_fence_before();
+  if constexpr (PAIR) cluster_sync();             // no arrival may reach a block that has ended
+  else __syncthreads();
+  tc_fence_after();
+  if (warp == kEpi + 1) {
+    if constexpr (PAIR) tmem_free_pair(tmem, 2 * BN);
+    else tmem_free(tmem, 2 * BN);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// momentum, norm, first split
+// ---------------------------------------------------------------------------
+constexpr int kParts = 64;          // partial sums of squares per matrix
+
+DCT_DEV float direction(const MuonArgs& a, uint64_t i) {     // after the momentum update
+  if (!a.update) return a.g[i];
+  return a.nesterov ? fmaf(a.momentum, a.m[i], a.g[i]) : a.m[i];
+}
+
+// m = momentum m + g, and the sums of squares of the direction
+__global__ void __launch_bounds__(256) k_muon_momentum(const __grid_constant__ MuonArgs a, double* part,
+                                                       uint32_t* arrived, uint32_t blocks) {
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (uint32_t i = threadIdx.x; i < blocks; i += 256) arrived[i] = 0;
   __shared__ double sh[32];
-  const uint64_t n = (uint64_t)a.rows * a.cols, per = (n + kChunks - 1) / kChunks;
+  const uint64_t n = (uint64_t)a.rows * a.cols, per = (n + kParts - 1) / kParts;
   const uint64_t base = blockIdx.y * n, end = min(n, (blockIdx.x + 1) * per);
   double s = 0.0;
   for (uint64_t i = blockIdx.x * per + threadIdx.x; i < end; i += 256) {
-    float x = a.g[base + i];
-    if (a.update) {
-      const float m = fmaf(a.momentum, a.m[base + i], x);
-      a.m[base + i] = m;
-      x = a.nesterov ? fmaf(a.momentum, m, x) : m;
-    }
-    u[base + i] = x;
+    if (a.update) a.m[base + i] = fmaf(a.momentum, a.m[base + i], a.g[base + i]);
+    const float x = direction(a, base + i);
     s += (double)x * x;
   }
   s = block_sum(s, sh);
-  if (threadIdx.x == 0) part[blockIdx.y * kChunks + blockIdx.x] = s;
+  if (threadIdx.x == 0) part[blockIdx.y * kParts + blockIdx.x] = s;
 }
 
-__global__ void __launch_bounds__(256) k_muon_scale(const __grid_constant__ MuonArgs a, float* x, const double* part) {
+// the chunks of X = direction / (norm + eps): a warp per 8 rows x 64 columns... one thread
+// per 8 columns of a row
+__global__ void __launch_bounds__(256) k_muon_split(const __grid_constant__ MuonArgs a, const double* part, uint8_t* x,
+                                                    uint32_t rb, uint32_t cb, float scale) {
+  __shared__ double inv;
+  const uint32_t z = blockIdx.y;
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int i = 0; i < kParts; ++i) s += part[z * kParts + i];
+    inv = 1.0 / (sqrt(s) + a.eps);
+  }
+  __syncthreads();
+  const double f = inv * scale;
+  const uint64_t n = (uint64_t)a.rows * a.cols, groups = (uint64_t)rb * 64 * cb * 8;
+  for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < groups; t += 256ull * gridDim.x) {
+    const uint32_t i = (uint32_t)(t / (cb * 8)), c = (uint32_t)(t % (cb * 8));
+    uint32_t h[4] = {}, l[4] = {};
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t j = c * 8 + e;
+      v[e] = i < a.rows && j < a.cols ? (float)(direction(a, z * n + (uint64_t)i * a.cols + j) * f) : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split2(v[2 * e], v[2 * e + 1], h[e], l[e]);
+    uint8_t* o = x + (((uint64_t)z * rb + (i >> 6)) * cb + (c >> 3)) * kPairBytes + chunk_at(i & 63, c & 7);
+    *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(o + kChunkBytes) = make_uint4(l[0], l[1], l[2], l[3]);
+  }
+}
+
+// no steps: the result is X itself
+__global__ void __launch_bounds__(256) k_muon_apply(const __grid_constant__ MuonArgs a, const double* part) {
   const uint64_t n = (uint64_t)a.rows * a.cols;
   double s = 0.0;
-  for (int i = 0; i < kChunks; ++i) s += part[blockIdx.y * kChunks + i];
+  for (int i = 0; i < kParts; ++i) s += part[blockIdx.y * kParts + i];
   const double inv = 1.0 / (sqrt(s) + a.eps);
-  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += 256ull * gridDim.x)
-    x[blockIdx.y * n + i] = (float)(x[blockIdx.y * n + i] * inv);
-}
-
-__global__ void __launch_bounds__(256) k_muon_apply(const __grid_constant__ MuonArgs a, const float* x) {
-  const uint64_t n = (uint64_t)a.batch * a.rows * a.cols;
-  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += 256ull * gridDim.x) {
-    if (a.update) a.w[i] = fmaf(-a.rate, x[i], a.keep * a.w[i]);
-    else a.y[i] = x[i];
+  for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < n; t += 256ull * gridDim.x) {
+    const uint64_t i = blockIdx.y * n + t;
+    const float x = (float)(direction(a, i) * inv);
+    if (a.update) a.w[i] = fmaf(-a.rate, x, a.keep * a.w[i]);
+    else a.y[i] = x;
   }
 }
 
 struct Layout {
-  uint64_t n, r;                    // elements of a matrix, and of its Gram matrix
-  size_t x0, x1, gram, poly, part, total;
+  uint32_t rb, cb, sb;              // chunks of rows, columns, the shorter side
+  uint64_t x, s;                    // bytes of X's and of a Gram matrix's chunks
+  size_t x0, x1, gram, poly, part, cut, arrived, total;
   explicit Layout(const MuonArgs& a) {
-    n = (uint64_t)a.rows * a.cols;
-    const uint64_t s = a.rows < a.cols ? a.rows : a.cols;
-    r = s * s;
+    rb = (a.rows + 63) / 64;
+    cb = (a.cols + 63) / 64;
+    sb = rb < cb ? rb : cb;
+    x = (uint64_t)rb * cb * kPairBytes;
+    s = (uint64_t)sb * sb * kPairBytes;
     size_t at = 0;
-    auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) & ~size_t(255); return o; };
-    x0 = take(4 * n * a.batch);
-    x1 = take(4 * n * a.batch);
-    gram = take(4 * r * a.batch);
-    poly = take(4 * r * a.batch);
-    part = take(8 * kChunks * (size_t)a.batch);
+    auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 1023) & ~size_t(1023); return o; };
+    x0 = take(x * a.batch);
+    x1 = take(x * a.batch);
+    gram = take(s * a.batch);
+    poly = take(s * a.batch);
+    part = take(8 * kParts * (size_t)a.batch);
+    cut = take(2ull * dev_info().sm_count * kRows * 256 * sizeof(float));
+    arrived = take(sizeof(uint32_t) * dev_info().sm_count);
     total = at;
   }
 };
 
-cudaError_t gemm(const Gemm& g, uint32_t batch, cudaStream_t st) {
-  k_gemm<<<dim3((g.N + kTile - 1) / kTile, (g.M + kTile - 1) / kTile, batch), 256, 0, st>>>(g);
-  return cudaGetLastError();
+// Workers that run at once: every SM, or the pairs that the device can place.
+template <typename K>
+cudaError_t workers_of(K kernel, bool pair, size_t smem, int* workers) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  *workers = dev_info().sm_count;
+  if (e != cudaSuccess || !pair) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(2 * (dev_info().sm_count / 2));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaOccupancyMaxActiveClusters(workers, kernel, &cfg);
 }
+
+template <bool PAIR, int BN>
+cudaError_t product_as(Product g, uint32_t batch, cudaStream_t st) {
+  using S = Shape<PAIR, BN>;
+  const auto kernel = k_product<PAIR, BN>;
+  static int most = 0;
+  static const cudaError_t set = workers_of(kernel, PAIR, S::kSmem, &most);
+  if (set != cudaSuccess) return set;
+  if (most < 1 || (PAIR ? 2 : 1) * most > dev_info().sm_count) return cudaErrorInvalidConfiguration;
+  g.mt = (g.M + S::kTileRows - 1) / S::kTileRows;
+  g.nt = (g.N + BN - 1) / BN;
+  g.tiles = g.mt * g.nt;
+  if (g.half) g.tiles = g.mt * (g.mt + 1) / 2;
+  const uint64_t total = (uint64_t)g.tiles * batch, work = total * g.kb;
+  if (total >= (1ull << 31)) return cudaErrorInvalidConfiguration;
+  // Whole tiles, or cut ones: whichever has the shorter longest run.  A cut tile's meeting in
+  // memory costs about as much as 6 chunks (one matrix of 1024 x 8192: 700 us cut, 1079 us
+  // whole; twelve of 768 x 768: 552 and 550 us), and runs below 4 chunks gain nothing.
+  constexpr uint64_t kShortest = 4, kMeeting = 6;
+  const uint64_t whole = (total + most - 1) / most * g.kb;
+  const uint64_t cut = std::max<uint64_t>(kShortest, (work + most - 1) / most) + kMeeting;
+  const uint32_t unit = whole <= cut ? g.kb : 1;
+  const uint64_t runs = std::min<uint64_t>(unit == 1 ? (work + kShortest - 1) / kShortest : total, most);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)runs * (PAIR ? 2 : 1));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, g, (uint32_t)total, unit, device_error_word());
+}
+
+// The tile of a call's products: its rows and columns, of which symmetric results store
+// the lower half (64: one tile of a result no larger than that).
+cudaError_t product(int tile, const Product& g, uint32_t batch, cudaStream_t st) {
+  if (tile == 64) return product_as<false, 64>(g, batch, st);
+  if (tile == 128) return product_as<false, 128>(g, batch, st);
+  return product_as<true, 256>(g, batch, st);
+}
+
+// Pairs with tiles of 256 for large matrices, where the loads bound (4096 x 4096: 3.91 ms,
+// 4.94 with 128); below, smaller tiles divide better (1024 x 8192: 700 us, 962 with 256).
+int tile_of(const MuonArgs& a) {
+  const uint32_t s = std::min(a.rows, a.cols);
+  return s <= 64 ? 64 : s < 2048 ? 128 : 256;
+}
+
+// the power of two that brings `most` to at most 2^15
+int room(double most) {
+  int e;
+  frexp(most, &e);           // most <= 2^e
+  return 15 - e;
+}
+float pow2(int e) { return (float)ldexp(1.0, e); }
 
 }  // namespace
 
@@ -119,31 +613,68 @@ size_t muon_ws_bytes(const MuonArgs& a) { return Layout(a).total; }
 
 cudaError_t launch_muon(const MuonArgs& a, void* ws, cudaStream_t st) {
   const Layout L(a);
-  if (!L.n || !a.batch) return cudaSuccess;
-  char* w = static_cast<char*>(ws);
-  float *x = reinterpret_cast<float*>(w + L.x0), *y = reinterpret_cast<float*>(w + L.x1);
-  float *gram = reinterpret_cast<float*>(w + L.gram), *poly = reinterpret_cast<float*>(w + L.poly);
+  if (!a.rows || !a.cols || !a.batch) return cudaSuccess;
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  uint8_t *x = w + L.x0, *y = w + L.x1;
   double* part = reinterpret_cast<double*>(w + L.part);
-  k_muon_momentum<<<dim3(kChunks, a.batch), 256, 0, st>>>(a, x, part);
-  k_muon_scale<<<dim3(kChunks, a.batch), 256, 0, st>>>(a, x, part);
-  cudaError_t e = cudaGetLastError();
-  const int R = a.rows, C = a.cols;
-  const bool wide = R <= C;
-  const int S = wide ? R : C, T = wide ? C : R;
-  for (uint32_t i = 0; i < a.steps && e == cudaSuccess; ++i) {
-    const int64_t n = L.n, r = L.r;
-    e = gemm(wide ? Gemm{x, x, nullptr, gram, C, 1, 1, C, S, n, n, r, S, S, T, 1.f, 0.f}
-                  : Gemm{x, x, nullptr, gram, 1, C, C, 1, S, n, n, r, S, S, T, 1.f, 0.f}, a.batch, st);
-    if (e == cudaSuccess)
-      e = gemm(Gemm{gram, gram, gram, poly, S, 1, S, 1, S, r, r, r, S, S, S, (float)a.c, (float)a.b}, a.batch, st);
-    if (e == cudaSuccess)
-      e = gemm(wide ? Gemm{poly, x, x, y, S, 1, C, 1, C, r, n, n, R, C, S, 1.f, (float)a.a}
-                    : Gemm{x, poly, x, y, C, 1, S, 1, C, n, r, n, R, C, S, 1.f, (float)a.a}, a.batch, st);
-    float* t = x; x = y; y = t;
+  uint32_t* arrived = reinterpret_cast<uint32_t*>(w + L.arrived);
+  k_muon_momentum<<<dim3(kParts, a.batch), 256, 0, st>>>(a, part, arrived, dev_info().sm_count);
+  const uint64_t n = (uint64_t)a.rows * a.cols;
+  const unsigned across = std::max(1u, grid_for(n, 256 * 8, 4) / std::max(1u, a.batch / 8));
+  if (!a.steps) {
+    k_muon_apply<<<dim3(across, a.batch), 256, 0, st>>>(a, part);
+    return cudaGetLastError();
   }
-  if (e != cudaSuccess) return e;
-  k_muon_apply<<<grid_for((uint64_t)a.batch * L.n, 256), 256, 0, st>>>(a, x);
-  return cudaGetLastError();
+  // no entry of X exceeds its largest singular value, none of A that squared, none of P
+  // b t + c t^2 on those
+  const double top = a.bound * a.bound, most = std::max(1e-30, fabs(a.b) * top + fabs(a.c) * top * top);
+  const int ex = room(a.bound), eg = room(top), ep = room(most);
+  k_muon_split<<<dim3(across, a.batch), 256, 0, st>>>(a, part, x, L.rb, L.cb, pow2(ex));
+  cudaError_t e = cudaGetLastError();
+  const bool wide = a.rows <= a.cols;
+  const uint32_t S = wide ? a.rows : a.cols;
+  const int tile = tile_of(a);
+  Product base{};
+  base.parts = reinterpret_cast<float*>(w + L.cut);
+  base.arrived = arrived;
+  for (uint32_t i = 0; i < a.steps && e == cudaSuccess; ++i) {
+    const Operand X{x, L.cb, L.x, false, false}, XT{x, L.cb, L.x, true, false};
+    const Operand A{w + L.gram, L.sb, L.s, false, tile > 64}, P{w + L.poly, L.sb, L.s, false, tile > 64};
+    Product g = base;
+    g.A = g.B = wide ? X : XT;
+    g.C = w + L.gram; g.c_cb = L.sb; g.c_z = L.s;
+    g.sa = pow2(eg - 2 * ex);
+    g.M = g.N = S; g.kb = wide ? L.cb : L.rb;
+    g.half = tile > 64;
+    e = product(tile, g, a.batch, st);
+    if (e != cudaSuccess) break;
+    Product p = base;
+    p.A = p.B = p.D = A;
+    p.C = w + L.poly; p.c_cb = L.sb; p.c_z = L.s;
+    p.sa = (float)(a.c * pow2(ep - 2 * eg));
+    p.sd = (float)(a.b * pow2(ep - eg));
+    p.M = p.N = S; p.kb = L.sb;
+    p.half = tile > 64;
+    e = product(tile, p, a.batch, st);
+    if (e != cudaSuccess) break;
+    const bool last = i + 1 == a.steps;
+    Product q = base;
+    q.D = X;
+    q.A = wide ? P : X;
+    q.B = wide ? XT : P;
+    q.M = a.rows; q.N = a.cols; q.kb = L.sb;
+    q.sa = pow2((last ? 0 : ex) - ex - ep);
+    q.sd = (float)(a.a * pow2((last ? 0 : ex) - ex));
+    if (last) {
+      q.out = a.update ? a.w : a.y;
+      q.update = a.update; q.keep = a.keep; q.rate = a.rate;
+    } else {
+      q.C = y; q.c_cb = L.cb; q.c_z = L.x;
+    }
+    e = product(tile, q, a.batch, st);
+    std::swap(x, y);
+  }
+  return e;
 }
 
 }  // namespace dct

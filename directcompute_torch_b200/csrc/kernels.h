@@ -285,6 +285,7 @@ struct MuonArgs {
   float *w, *m, *y;          // update: w and m in place; orthogonalize: y
   uint32_t batch, rows, cols, steps;
   double a, b, c, eps;
+  double bound;              // of the singular values over the steps
   float momentum, keep, rate;   // w = keep w - rate orthogonalized
   bool nesterov, update;
 };

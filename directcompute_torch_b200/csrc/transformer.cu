@@ -187,8 +187,8 @@ int attention(const char* what, const DctAttention* p, void* q, void* k, void* v
 // ---------------------------------------------------------------------------
 // orthogonalisation
 // ---------------------------------------------------------------------------
-// Fills the shape and polynomial; `bound` gets the largest |singular value| over the steps.
-int muon_args(const char* what, const DctMuon* p, MuonArgs& a, double* bound) {
+// Fills the shape, the polynomial and the largest singular value that its steps can give.
+int muon_args(const char* what, const DctMuon* p, MuonArgs& a) {
   if (!p) return refuse(DCT_ERR_ARG, "%s: no parameters", what);
   if (p->batch > 65535 || (uint64_t)p->rows * p->cols >= kMost || p->rows >= (1u << 24) || p->cols >= (1u << 24))
     return refuse(DCT_ERR_ARG, "%s: %u matrices of %u x %u are too many or too large", what, p->batch, p->rows,
@@ -202,7 +202,7 @@ int muon_args(const char* what, const DctMuon* p, MuonArgs& a, double* bound) {
   // singular values start in [0, 1]; follow the largest that a step can give, on a grid
   // (and the slack that the grid's spacing and the arithmetic leave)
   double top = 1.0;
-  *bound = 1.0;
+  a.bound = 1.0;
   for (uint32_t i = 0; i < p->steps; ++i) {
     double next = 0.0;
     for (int j = 0; j <= 256; ++j) {
@@ -210,8 +210,8 @@ int muon_args(const char* what, const DctMuon* p, MuonArgs& a, double* bound) {
       next = std::max(next, fabs(s * (a.a + t * (a.b + t * a.c))));
     }
     top = 1.01 * next;
-    *bound = std::max(*bound, top);
-    if (!(*bound < 64.0))
+    a.bound = std::max(a.bound, top);
+    if (!(a.bound < 64.0))
       return refuse(DCT_ERR_ARG, "%s: the steps' polynomial grows past 64", what);
   }
   a.batch = p->batch; a.rows = p->rows; a.cols = p->cols; a.steps = p->steps;
@@ -299,8 +299,7 @@ DCT_API int dct_orthogonalize(const DctMuon* p, void* x, void* y) {
   const char* what = "dct_orthogonalize";
   if (const int rc = ready(what)) return rc;
   MuonArgs a{};
-  double bound;
-  if (const int rc = muon_args(what, p, a, &bound)) return rc;
+  if (const int rc = muon_args(what, p, a)) return rc;
   const int64_t none[3] = {(int64_t)p->rows * p->cols, (int64_t)p->cols, (int64_t)p->cols};
   Arg ax{"x", x, {p->batch, p->rows, 1}, p->cols, none, false};
   Arg ay{"y", y, {p->batch, p->rows, 1}, p->cols, none, true};
@@ -318,8 +317,7 @@ DCT_API int dct_muon(const DctMuon* p, void* w, void* m, void* g) {
   const char* what = "dct_muon";
   if (const int rc = ready(what)) return rc;
   MuonArgs a{};
-  double bound;
-  if (const int rc = muon_args(what, p, a, &bound)) return rc;
+  if (const int rc = muon_args(what, p, a)) return rc;
   const int64_t none[3] = {(int64_t)p->rows * p->cols, (int64_t)p->cols, (int64_t)p->cols};
   Arg aw{"w", w, {p->batch, p->rows, 1}, p->cols, none, true};
   Arg am{"m", m, {p->batch, p->rows, 1}, p->cols, none, true};

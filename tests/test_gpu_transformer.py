@@ -420,6 +420,20 @@ def test_orthogonalize_any_magnitude(dev, size):
         dev.free(hx)
 
 
+@pytest.mark.parametrize("coefficients", [(1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (1.875, -1.25, 0.375)], ids=str)
+def test_orthogonalize_other_polynomials(dev, coefficients):
+    """Polynomials that take singular values to 1 itself."""
+    x = np.random.default_rng(15).normal(size=(1, 140, 90)).astype(np.float32)
+    hx = dev.buf(x)
+    a, b, c = coefficients
+    try:
+        _abi.check(dev.lib, dev.lib.dct_orthogonalize(ctypes.byref(_muon(x.shape, a=a, b=b, c=c, steps=12)), hx, hx))
+        want, tol = T.orthogonalize(x[0], 12, coefficients)
+        assert np.linalg.norm(dev.read(hx).reshape(140, 90) - want) <= tol
+    finally:
+        dev.free(hx)
+
+
 def test_orthogonalize_zero_and_nan(dev):
     """A zero matrix stays zero; a NaN stays in its matrix of the batch."""
     x = np.random.default_rng(14).normal(size=(3, 66, 40)).astype(np.float32)
