@@ -61,6 +61,7 @@ struct Shape {
   static constexpr uint32_t kBChunks = (PAIR ? BN / 2 : BN) / 64;    // chunks of B's columns in this block
   static constexpr uint32_t kA = 2 * kPairBytes, kB = kBChunks * kPairBytes, kStage = kA + kB;
   static constexpr int kStages = 196608 / kStage > 4 ? 4 : 196608 / kStage;
+  static constexpr int kBufs = BN == 256 ? 2 : 4;                    // accumulators in tensor memory
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kEpi * kStaging;
 };
 
@@ -132,7 +133,8 @@ DCT_DEV void epilogue_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 // Tiles that several blocks share meet in memory: every block leaves its sum, and the last
 // to arrive adds them in the order of the contraction, so the result does not depend on who
 // that was.
-constexpr uint32_t kDrain = 2;
+// Draining costs about 230 cycles of the tensor cores: 5% of a large product every second
+// chunk, 9% every chunk; the smaller tiles do it every chunk.
 //
 // PAIR: two blocks on one tile of twice the rows.  A chunk of the contraction then costs a
 // block 64 KB of loads instead of 96 KB (tile 256 columns wide), and the loads are what
@@ -141,9 +143,10 @@ template <bool PAIR, int BN>
 __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__ Product g, uint32_t total,
                                                          uint32_t unit, uint32_t* err) {
   using S = Shape<PAIR, BN>;
+  constexpr uint32_t kDrain = PAIR ? 2 : 1;
   extern __shared__ uint8_t raw[];
   uint8_t* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-  __shared__ uint64_t full[4], empty[4], there[4], done[2], freed[2];   // there: the other block's chunk is in
+  __shared__ uint64_t full[4], empty[4], there[4], done[4], freed[4];   // there: the other block's chunk is in
   __shared__ uint32_t tmem_base, order;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_rank() : 0, worker = PAIR ? blockIdx.x / 2 : blockIdx.x;
@@ -153,15 +156,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
       mbar_init(&empty[s], 1);
       mbar_init(&there[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < S::kBufs; ++s) {
       mbar_init(&done[s], 1);
       mbar_init(&freed[s], PAIR ? 2 * kEpi : kEpi);
     }
     mbar_fence_init();
   }
   if (warp == kEpi + 1) {
-    if constexpr (PAIR) tmem_alloc_pair(&tmem_base, 2 * BN);
-    else tmem_alloc(&tmem_base, 2 * BN);
+    if constexpr (PAIR) tmem_alloc_pair(&tmem_base, S::kBufs * BN);
+    else tmem_alloc(&tmem_base, S::kBufs * BN);
   }
   tc_fence_before();
   if constexpr (PAIR) cluster_sync();
@@ -239,8 +242,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
         uint32_t z, ti, tj;
         tile_at(g, sg.tile, z, ti, tj);
         for (uint32_t k0 = sg.k0; k0 < sg.k1 && ok; k0 += kDrain, ++part) {
-          const uint32_t buf = part & 1, d = tmem + buf * BN, k1 = min(sg.k1, k0 + kDrain);
-          ok = mbar_wait_cluster(&freed[buf], ((part >> 1) & 1) ^ 1, err);
+          const uint32_t buf = part % S::kBufs, d = tmem + buf * BN, k1 = min(sg.k1, k0 + kDrain);
+          ok = mbar_wait_cluster(&freed[buf], ((part / S::kBufs) & 1) ^ 1, err);
           tc_fence_after();
           for (uint32_t k = k0; k < k1 && ok; ++k, ++it) {
             const uint32_t s = it % S::kStages;
@@ -278,8 +281,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
 #pragma unroll
       for (int c = 0; c < W; ++c) acc[c] = 0.f;
       for (uint32_t k0 = sg.k0; k0 < sg.k1 && ok; k0 += kDrain, ++part) {
-        const uint32_t buf = part & 1;
-        ok = mbar_wait(&done[buf], (part >> 1) & 1, err);
+        const uint32_t buf = part % S::kBufs;
+        ok = mbar_wait(&done[buf], (part / S::kBufs) & 1, err);
         tc_fence_after();
         if (ok) {
 #pragma unroll
@@ -426,64 +429,91 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
   else __syncthreads();
   tc_fence_after();
   if (warp == kEpi + 1) {
-    if constexpr (PAIR) tmem_free_pair(tmem, 2 * BN);
-    else tmem_free(tmem, 2 * BN);
+    if constexpr (PAIR) tmem_free_pair(tmem, S::kBufs * BN);
+    else tmem_free(tmem, S::kBufs * BN);
   }
 }
 
 // ---------------------------------------------------------------------------
 // momentum, norm, first split
 // ---------------------------------------------------------------------------
-constexpr int kParts = 64;          // partial sums of squares per matrix
+constexpr int kMostParts = 1024;    // partial sums of squares per matrix
 
-DCT_DEV float direction(const MuonArgs& a, uint64_t i) {     // after the momentum update
-  if (!a.update) return a.g[i];
-  return a.nesterov ? fmaf(a.momentum, a.m[i], a.g[i]) : a.m[i];
+DCT_DEV float updated(const MuonArgs& a, float m, float g) { return fmaf(a.momentum, m, g); }
+DCT_DEV float direction(const MuonArgs& a, float m, float g) {     // m after its update
+  return !a.update ? g : a.nesterov ? fmaf(a.momentum, m, g) : m;
 }
 
-// m = momentum m + g, and the sums of squares of the direction
+// m = momentum m + g, and the sums of squares of the direction, a part per block; 12 bytes
+// an element (4 without the update), bound by memory
+template <int V>
 __global__ void __launch_bounds__(256) k_muon_momentum(const __grid_constant__ MuonArgs a, double* part,
                                                        uint32_t* arrived, uint32_t blocks) {
+  __shared__ double sh[32];
   if (blockIdx.x == 0 && blockIdx.y == 0)
     for (uint32_t i = threadIdx.x; i < blocks; i += 256) arrived[i] = 0;
-  __shared__ double sh[32];
-  const uint64_t n = (uint64_t)a.rows * a.cols, per = (n + kParts - 1) / kParts;
-  const uint64_t base = blockIdx.y * n, end = min(n, (blockIdx.x + 1) * per);
+  const uint64_t n = (uint64_t)a.rows * a.cols / V, base = blockIdx.y * n;
   double s = 0.0;
-  for (uint64_t i = blockIdx.x * per + threadIdx.x; i < end; i += 256) {
-    if (a.update) a.m[base + i] = fmaf(a.momentum, a.m[base + i], a.g[base + i]);
-    const float x = direction(a, base + i);
-    s += (double)x * x;
-  }
-  s = block_sum(s, sh);
-  if (threadIdx.x == 0) part[blockIdx.y * kParts + blockIdx.x] = s;
-}
-
-// the chunks of X = direction / (norm + eps): a warp per 8 rows x 64 columns... one thread
-// per 8 columns of a row
-__global__ void __launch_bounds__(256) k_muon_split(const __grid_constant__ MuonArgs a, const double* part, uint8_t* x,
-                                                    uint32_t rb, uint32_t cb, float scale) {
-  __shared__ double inv;
-  const uint32_t z = blockIdx.y;
-  if (threadIdx.x == 0) {
-    double s = 0.0;
-    for (int i = 0; i < kParts; ++i) s += part[z * kParts + i];
-    inv = 1.0 / (sqrt(s) + a.eps);
-  }
-  __syncthreads();
-  const double f = inv * scale;
-  const uint64_t n = (uint64_t)a.rows * a.cols, groups = (uint64_t)rb * 64 * cb * 8;
-  for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < groups; t += 256ull * gridDim.x) {
-    const uint32_t i = (uint32_t)(t / (cb * 8)), c = (uint32_t)(t % (cb * 8));
-    uint32_t h[4] = {}, l[4] = {};
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t j = c * 8 + e;
-      v[e] = i < a.rows && j < a.cols ? (float)(direction(a, z * n + (uint64_t)i * a.cols + j) * f) : 0.f;
+  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += 256ull * gridDim.x) {
+    float g[V], m[V];
+    if constexpr (V == 4) {
+      *reinterpret_cast<float4*>(g) = reinterpret_cast<const float4*>(a.g)[base + i];
+      if (a.update) *reinterpret_cast<float4*>(m) = reinterpret_cast<const float4*>(a.m)[base + i];
+    } else {
+      g[0] = a.g[base + i];
+      if (a.update) m[0] = a.m[base + i];
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) split2(v[2 * e], v[2 * e + 1], h[e], l[e]);
+    for (int e = 0; e < V; ++e) {
+      m[e] = a.update ? updated(a, m[e], g[e]) : 0.f;
+      const float x = direction(a, m[e], g[e]);
+      s += (double)x * x;
+    }
+    if (!a.update) continue;
+    if constexpr (V == 4) reinterpret_cast<float4*>(a.m)[base + i] = *reinterpret_cast<const float4*>(m);
+    else a.m[base + i] = m[0];
+  }
+  s = block_sum(s, sh);
+  if (threadIdx.x == 0) part[blockIdx.y * gridDim.x + blockIdx.x] = s;
+}
+
+// 1 / (norm + eps) of the block's matrix, in every thread
+DCT_DEV double inverse_norm(const MuonArgs& a, const double* part, uint32_t parts) {
+  __shared__ double sh[32], inv;
+  const double s = block_sum(strided_sum(part + (uint64_t)blockIdx.y * parts, parts), sh);
+  if (threadIdx.x == 0) inv = 1.0 / (sqrt(s) + a.eps);
+  __syncthreads();
+  return inv;
+}
+
+// the chunks of X = direction / (norm + eps), a thread per 8 columns of a row
+template <int V>
+__global__ void __launch_bounds__(256) k_muon_split(const __grid_constant__ MuonArgs a, const double* part,
+                                                    uint32_t parts, uint8_t* x, uint32_t rb, uint32_t cb, float scale) {
+  const uint32_t z = blockIdx.y;
+  const double f = inverse_norm(a, part, parts) * scale;
+  const uint64_t base = (uint64_t)z * a.rows * a.cols, groups = (uint64_t)rb * 64 * cb * 8;
+  for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < groups; t += 256ull * gridDim.x) {
+    const uint32_t i = (uint32_t)(t / (cb * 8)), c = (uint32_t)(t % (cb * 8));
+    const uint64_t at = base + (uint64_t)i * a.cols + c * 8;
+    float g[8], m[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += V) {
+      const bool in = i < a.rows && c * 8 + e < a.cols;
+      if constexpr (V == 4) {
+        const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4*>(g + e) = in ? *reinterpret_cast<const float4*>(a.g + at + e) : none;
+        *reinterpret_cast<float4*>(m + e) = in && a.update ? *reinterpret_cast<const float4*>(a.m + at + e) : none;
+      } else {
+        g[e] = in ? a.g[at + e] : 0.f;
+        m[e] = in && a.update ? a.m[at + e] : 0.f;
+      }
+    }
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      split2((float)(direction(a, m[2 * e], g[2 * e]) * f), (float)(direction(a, m[2 * e + 1], g[2 * e + 1]) * f), h[e],
+             l[e]);
     uint8_t* o = x + (((uint64_t)z * rb + (i >> 6)) * cb + (c >> 3)) * kPairBytes + chunk_at(i & 63, c & 7);
     *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
     *reinterpret_cast<uint4*>(o + kChunkBytes) = make_uint4(l[0], l[1], l[2], l[3]);
@@ -491,14 +521,13 @@ __global__ void __launch_bounds__(256) k_muon_split(const __grid_constant__ Muon
 }
 
 // no steps: the result is X itself
-__global__ void __launch_bounds__(256) k_muon_apply(const __grid_constant__ MuonArgs a, const double* part) {
+__global__ void __launch_bounds__(256) k_muon_apply(const __grid_constant__ MuonArgs a, const double* part,
+                                                    uint32_t parts) {
   const uint64_t n = (uint64_t)a.rows * a.cols;
-  double s = 0.0;
-  for (int i = 0; i < kParts; ++i) s += part[blockIdx.y * kParts + i];
-  const double inv = 1.0 / (sqrt(s) + a.eps);
+  const double inv = inverse_norm(a, part, parts);
   for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < n; t += 256ull * gridDim.x) {
     const uint64_t i = blockIdx.y * n + t;
-    const float x = (float)(direction(a, i) * inv);
+    const float x = (float)(direction(a, a.update ? a.m[i] : 0.f, a.g[i]) * inv);
     if (a.update) a.w[i] = fmaf(-a.rate, x, a.keep * a.w[i]);
     else a.y[i] = x;
   }
@@ -520,7 +549,7 @@ struct Layout {
     x1 = take(x * a.batch);
     gram = take(s * a.batch);
     poly = take(s * a.batch);
-    part = take(8 * kParts * (size_t)a.batch);
+    part = take(8 * kMostParts * (size_t)a.batch);
     cut = take(2ull * dev_info().sm_count * kRows * 256 * sizeof(float));
     arrived = take(sizeof(uint32_t) * dev_info().sm_count);
     total = at;
@@ -618,18 +647,24 @@ cudaError_t launch_muon(const MuonArgs& a, void* ws, cudaStream_t st) {
   uint8_t *x = w + L.x0, *y = w + L.x1;
   double* part = reinterpret_cast<double*>(w + L.part);
   uint32_t* arrived = reinterpret_cast<uint32_t*>(w + L.arrived);
-  k_muon_momentum<<<dim3(kParts, a.batch), 256, 0, st>>>(a, part, arrived, dev_info().sm_count);
   const uint64_t n = (uint64_t)a.rows * a.cols;
-  const unsigned across = std::max(1u, grid_for(n, 256 * 8, 4) / std::max(1u, a.batch / 8));
+  const bool vec = a.cols % 4 == 0 && aligned16_h(a.g) && (!a.update || aligned16_h(a.m));
+  // blocks a matrix: a thread takes 16 elements or more, the batch eight blocks an SM
+  const uint32_t across = (uint32_t)std::max<uint64_t>(
+      1, std::min<uint64_t>(std::min<uint64_t>((n + 4095) / 4096, kMostParts), 8ull * dev_info().sm_count / a.batch));
+  const dim3 grid(across, a.batch);
+  if (vec) k_muon_momentum<4><<<grid, 256, 0, st>>>(a, part, arrived, dev_info().sm_count);
+  else k_muon_momentum<1><<<grid, 256, 0, st>>>(a, part, arrived, dev_info().sm_count);
   if (!a.steps) {
-    k_muon_apply<<<dim3(across, a.batch), 256, 0, st>>>(a, part);
+    k_muon_apply<<<grid, 256, 0, st>>>(a, part, across);
     return cudaGetLastError();
   }
   // no entry of X exceeds its largest singular value, none of A that squared, none of P
   // b t + c t^2 on those
   const double top = a.bound * a.bound, most = std::max(1e-30, fabs(a.b) * top + fabs(a.c) * top * top);
   const int ex = room(a.bound), eg = room(top), ep = room(most);
-  k_muon_split<<<dim3(across, a.batch), 256, 0, st>>>(a, part, x, L.rb, L.cb, pow2(ex));
+  if (vec) k_muon_split<4><<<grid, 256, 0, st>>>(a, part, across, x, L.rb, L.cb, pow2(ex));
+  else k_muon_split<1><<<grid, 256, 0, st>>>(a, part, across, x, L.rb, L.cb, pow2(ex));
   cudaError_t e = cudaGetLastError();
   const bool wide = a.rows <= a.cols;
   const uint32_t S = wide ? a.rows : a.cols;
