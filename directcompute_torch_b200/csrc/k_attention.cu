@@ -59,14 +59,6 @@ DCT_DEV float octet_sum(float s) {
 // 2^(x - top), with 0 for a place whose running maximum is still -inf
 DCT_DEV float weight(float x, float top) { return exp2f(x - (top == -INFINITY ? 0.f : top)); }
 
-struct RowAt {                 // a row's query position and head
-  int i, h;
-  DCT_DEV RowAt(const AttnArgs& a, int hk, int r) : i(r / a.group), h(hk * a.group + r % a.group) {}
-};
-
-// the address of (b, t, h) of a strided tensor
-DCT_DEV int64_t at(const int64_t* s, int b, int t, int h) { return b * s[0] + t * s[1] + h * s[2]; }
-
 // record of a split: [dim] outputs, then the maximum (base 2) and the sum
 DCT_DEV float* record(float* part, const AttnArgs& a, int64_t row, int splits, int split) {
   return part + (row * splits + split) * (a.dim + 2);
@@ -79,13 +71,13 @@ DCT_DEV void store_row(const AttnArgs& a, int b, const RowAt& w, int f, float ac
 }
 
 template <int NV, bool VEC, int R>
-__global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const __grid_constant__ AttnArgs a, int groups, int splits,
-                                                           float* part) {
+DCT_DEV void rows_forward(const AttnArgs& a, int item, int groups, int splits, float* part,
+                          float (&sh)[kWarps][R][32 * NV + 2]) {
   constexpr int F = 4 * NV;
-  __shared__ float sh[kWarps][R][32 * NV + 2];
   const int lane = threadIdx.x & 7, oct = threadIdx.x >> 3, warp = threadIdx.x >> 5;
-  const int split = blockIdx.x % splits, gi = (blockIdx.x / splits) % groups, bh = blockIdx.x / splits / groups;
+  const int split = item % splits, gi = (item / splits) % groups, bh = item / splits / groups;
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads, rows = a.q_len * a.group;
+  if (a.stats && scales_of(a.stats[bh], a.scale, a.dim, false).split) return;
   const AttnSpan span(a, b);
   const float scale = a.scale * kLog2e;
 
@@ -196,12 +188,26 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const __grid_constant
   }
 }
 
+// A block takes one item, or with `stats` items in turn: most heads then belong to the
+// tensor cores, and passing over them is cheaper than a block for each.
+template <int NV, bool VEC, int R>
+__global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const __grid_constant__ AttnArgs a, int groups, int splits,
+                                                           float* part, int items) {
+  __shared__ float sh[kWarps][R][32 * NV + 2];
+  for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    rows_forward<NV, VEC, R>(a, i, groups, splits, part, sh);
+    __syncthreads();
+  }
+}
+
 // joins a row's splits in order, a warp per row
-__global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ AttnArgs a, int splits, float* part) {
+__global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ AttnArgs a, int splits, float* part,
+                                                   bool tensor) {
   const int rows = a.q_len * a.group, lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= (int64_t)a.batch * a.kv_heads * rows) return;
   const int bh = (int)(row / rows);
+  if (a.stats && scales_of(a.stats[bh], a.scale, a.dim, false).split != tensor) return;
   const float* rec = record(part, a, row, splits, 0);
   const int step = a.dim + 2;
   float best = -INFINITY, s = 0.f;
@@ -225,7 +231,8 @@ __global__ void __launch_bounds__(128) k_attn_delta(const __grid_constant__ Attn
   if (i < AttnSpan(a, b).m)
     for (int f = threadIdx.x & 31; f < a.dim; f += 32) s = fmaf(a.dout[o + f], a.out[o + f], s);
   s = warp_sum_f(s);
-  if ((threadIdx.x & 31) == 0) a.delta[row] = s;
+  if ((threadIdx.x & 31) == 0)
+    a.delta[((int64_t)b * a.kv_heads + h / a.group) * padded_rows(a) + (int64_t)i * a.group + h % a.group] = s;
 }
 
 // sums x over the octets of a block into sh, then calls store(feature, total)
@@ -253,12 +260,12 @@ DCT_DEV void join_sums(float (&x)[4 * NV], float (&sh)[kWarps][32 * NV], int dim
 
 // dq of R rows: an octet per key
 template <int NV, bool VEC, int R>
-__global__ void __launch_bounds__(32 * kWarps) k_attn_rows_dq(const __grid_constant__ AttnArgs a, int groups) {
+DCT_DEV void rows_dq(const AttnArgs& a, int item, int groups, float (&sh)[kWarps][32 * NV]) {
   constexpr int F = 4 * NV;
-  __shared__ float sh[kWarps][32 * NV];
   const int lane = threadIdx.x & 7, oct = threadIdx.x >> 3;
-  const int gi = blockIdx.x % groups, bh = blockIdx.x / groups;
+  const int gi = item % groups, bh = item / groups;
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads, rows = a.q_len * a.group;
+  if (a.stats && scales_of(a.stats[bh], a.scale, a.dim, true).split) return;
   const AttnSpan span(a, b);
   const float scale = a.scale * kLog2e;
   float q[R][F], go[R][F], dq[R][F], lse[R], delta[R];
@@ -273,7 +280,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows_dq(const __grid_const
     if (row < rows && w.i < span.m) {
       const int64_t s = ((int64_t)b * a.q_heads + w.h) * a.q_len + w.i;
       lse[r] = a.lse[s] * kLog2e;
-      delta[r] = a.delta[s];
+      delta[r] = a.delta[(int64_t)bh * padded_rows(a) + row];
       if (lse[r] == -INFINITY) continue;                    // the row sees nothing
       lo[r] = span.lo(a, w.i);
       hi[r] = span.hi(a, w.i);
@@ -315,12 +322,12 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows_dq(const __grid_const
 
 // dk and dv of R keys: an octet per row
 template <int NV, bool VEC, int R>
-__global__ void __launch_bounds__(32 * kWarps) k_attn_rows_dkv(const __grid_constant__ AttnArgs a, int groups) {
+DCT_DEV void rows_dkv(const AttnArgs& a, int item, int groups, float (&sh)[kWarps][32 * NV]) {
   constexpr int F = 4 * NV;
-  __shared__ float sh[kWarps][32 * NV];
   const int lane = threadIdx.x & 7, oct = threadIdx.x >> 3;
-  const int gi = blockIdx.x % groups, bh = blockIdx.x / groups;
+  const int gi = item % groups, bh = item / groups;
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+  if (a.stats && scales_of(a.stats[bh], a.scale, a.dim, true).split) return;
   const AttnSpan span(a, b);
   const float scale = a.scale * kLog2e;
   float k[R][F], v[R][F], dk[R][F], dv[R][F];
@@ -346,7 +353,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows_dkv(const __grid_cons
     const int row = base + oct;
     const RowAt w(a, hk, min(row, r1 - 1));
     const int64_t s = ((int64_t)b * a.q_heads + w.h) * a.q_len + w.i;
-    const float lse = a.lse[s] * kLog2e, delta = a.delta[s];
+    const float lse = a.lse[s] * kLog2e, delta = a.delta[(int64_t)bh * padded_rows(a) + min(row, r1 - 1)];
     float q[F], go[F];
     load_row<NV, VEC>(q, a.q + at(a.qs, b, w.i, w.h), lane, a.dim);
     load_row<NV, VEC>(go, a.dout + at(a.os, b, w.i, w.h), lane, a.dim);
@@ -374,6 +381,21 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows_dkv(const __grid_cons
       if (j < a.kv_len) a.dv[ov + f] = s;
     });
   }
+}
+
+template <int NV, bool VEC, int R, bool KEYS>
+__global__ void __launch_bounds__(32 * kWarps) k_attn_rows_backward(const __grid_constant__ AttnArgs a, int groups,
+                                                                    int items) {
+  __shared__ float sh[kWarps][32 * NV];
+  for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    if constexpr (KEYS) rows_dkv<NV, VEC, R>(a, i, groups, sh);
+    else rows_dq<NV, VEC, R>(a, i, groups, sh);
+    __syncthreads();
+  }
+}
+
+unsigned blocks_for(const AttnArgs& a, int64_t items) {
+  return (unsigned)(a.stats ? std::min<int64_t>(items, 8ll * dev_info().sm_count) : items);
 }
 
 bool aligned(const float* p, const int64_t* s) {
@@ -425,13 +447,20 @@ cudaError_t launch_attn_rows_forward(const AttnArgs& a, void* ws, cudaStream_t s
   cudaError_t e = by_width(a.dim, vec, [&](auto nv, auto v) {
     constexpr int NV = decltype(nv)::value;
     constexpr bool V = decltype(v)::value;
-    if (R == 4) k_attn_rows<NV, V, 4><<<(unsigned)blocks, 32 * kWarps, 0, st>>>(a, (int)groups, splits, part);
-    else if (R == 2) k_attn_rows<NV, V, 2><<<(unsigned)blocks, 32 * kWarps, 0, st>>>(a, (int)groups, splits, part);
-    else k_attn_rows<NV, V, 1><<<(unsigned)blocks, 32 * kWarps, 0, st>>>(a, (int)groups, splits, part);
+    const unsigned n = blocks_for(a, blocks);
+    const int items = (int)blocks, g = (int)groups;
+    if (R == 4) k_attn_rows<NV, V, 4><<<n, 32 * kWarps, 0, st>>>(a, g, splits, part, items);
+    else if (R == 2) k_attn_rows<NV, V, 2><<<n, 32 * kWarps, 0, st>>>(a, g, splits, part, items);
+    else k_attn_rows<NV, V, 1><<<n, 32 * kWarps, 0, st>>>(a, g, splits, part, items);
     return cudaGetLastError();
   });
   if (e != cudaSuccess || splits == 1) return e;
-  k_attn_join<<<(unsigned)((rows * a.batch * a.kv_heads + 3) / 4), 128, 0, st>>>(a, splits, part);
+  return launch_attn_join(a, splits, part, false, st);
+}
+
+cudaError_t launch_attn_join(const AttnArgs& a, int splits, float* part, bool tensor, cudaStream_t st) {
+  const int64_t rows = (int64_t)a.batch * a.q_heads * a.q_len;
+  k_attn_join<<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(a, splits, part, tensor);
   return cudaGetLastError();
 }
 
@@ -452,8 +481,9 @@ cudaError_t launch_attn_rows_backward(const AttnArgs& a, cudaStream_t st) {
   return by_width(a.dim, vec, [&](auto nv, auto v) {
     constexpr int NV = decltype(nv)::value;
     constexpr bool V = decltype(v)::value;
-    if (gq * heads) k_attn_rows_dq<NV, V, R><<<(unsigned)(gq * heads), 32 * kWarps, 0, st>>>(a, (int)gq);
-    if (gk * heads) k_attn_rows_dkv<NV, V, R><<<(unsigned)(gk * heads), 32 * kWarps, 0, st>>>(a, (int)gk);
+    const int nq = (int)(gq * heads), nk = (int)(gk * heads);
+    if (nq) k_attn_rows_backward<NV, V, R, false><<<blocks_for(a, nq), 32 * kWarps, 0, st>>>(a, (int)gq, nq);
+    if (nk) k_attn_rows_backward<NV, V, R, true><<<blocks_for(a, nk), 32 * kWarps, 0, st>>>(a, (int)gk, nk);
     return cudaGetLastError();
   });
 }

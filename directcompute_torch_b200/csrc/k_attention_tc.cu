@@ -1,0 +1,549 @@
+// Attention on the fifth-generation tensor cores at float32 accuracy.
+//
+// A pass over the operands finds each key head's magnitudes (k_attn_scan), a second writes
+// them as split float16 tiles of 128 rows (k_attn_split; layout and arithmetic in
+// dct_umma.cuh), and the products run on those: three matrix instructions for each product
+// of float32 numbers, so the bound is a third of the float16 rate, about 540 TFLOP/s.
+//
+// A tile is [64 features][hi, lo][128 rows][64 float16], 32 KB for every 64 features, so
+// one bulk copy brings it and it serves as either operand: with its features as the
+// contraction (scores) or with its rows (the products with P, dS).
+//
+// Heads that the split cannot hold (infinities, NaN, rows of very different size) take the
+// kernels of k_attention.cu, which pick them by the same test on the device.
+#include <limits.h>
+
+#include <algorithm>
+
+#include "dct_attn.cuh"
+#include "dct_umma.cuh"
+
+namespace dct {
+namespace {
+
+constexpr int kTile = 128;
+constexpr uint32_t kBlockBytes = 2 * kTile * 128;      // 64 features of a tile, hi and lo
+
+// 2^x by the hardware (2 ulp; results below 2^-126 are 0)
+DCT_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+DCT_DEV uint32_t lane_bits(int warp) { return (uint32_t)(warp & 3) * 32u << 16; }
+
+struct Tiles {
+  uint8_t* p[4];               // q, k, v, dout
+  AttnStats* stats;            // [heads]
+  float *lse2, *delta;         // [heads][padded rows], backward: log2 units, 2^eds delta
+  int64_t tiles[4];            // of a head
+  int blocks;                  // of 64 features
+};
+
+// the rows of operand t of a head that are valid, and one of them
+DCT_DEV int rows_of(const AttnArgs& a, const AttnSpan& s, int t) { return t == 1 || t == 2 ? s.n : s.m * a.group; }
+DCT_DEV const float* row_of(const AttnArgs& a, int t, int b, int hk, int r) {
+  if (t == 1) return a.k + at(a.ks, b, r, hk);
+  if (t == 2) return a.v + at(a.vs, b, r, hk);
+  const RowAt w(a, hk, r);
+  return t == 0 ? a.q + at(a.qs, b, w.i, w.h) : a.dout + at(a.os, b, w.i, w.h);
+}
+
+// ---------------------------------------------------------------------------
+// magnitudes, splitting
+// ---------------------------------------------------------------------------
+constexpr int kScanRows = 64;
+
+// blocks [tensor][head][64 rows]; a warp takes every eighth row
+__global__ void __launch_bounds__(256) k_attn_scan(const __grid_constant__ AttnArgs a, AttnStats* stats, int per_q,
+                                                   int per_k, int backward) {
+  __shared__ uint32_t sh[3];
+  const int heads = a.batch * a.kv_heads, lane = threadIdx.x & 31;
+  int x = blockIdx.x, t = 0;
+  for (; t < 3; ++t) {                            // q, k, v, dout in turn
+    const int n = heads * (t == 0 ? per_q : per_k);
+    if (x < n) break;
+    x -= n;
+  }
+  const int per = t == 1 || t == 2 ? per_k : per_q, bh = x / per, r0 = (x - bh * per) * kScanRows;
+  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+  const int rows = min(rows_of(a, AttnSpan(a, b), t), r0 + kScanRows);
+  if (threadIdx.x < 3) sh[threadIdx.x] = 0;
+  __syncthreads();
+  uint32_t top = 0, low = 0, norm = 0;
+  for (int r = r0 + (threadIdx.x >> 5); r < rows; r += 8) {
+    const float* p = row_of(a, t, b, hk, r);
+    float v[4];
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = lane + 32 * e < a.dim ? p[lane + 32 * e] : 0.f;
+      m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    top = max(top, m);
+    if (m) low = max(low, ~m);
+    if (backward && t >= 2 && m && m < 0x7f800000u) {
+      // the norm through the row's own scale, so that squares neither vanish nor overflow
+      const float f = __uint_as_float(m);
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = fmaf(v[e] / f, v[e] / f, s);
+      norm = max(norm, __float_as_uint(1.001f * f * sqrtf(warp_sum_f(s))));
+    }
+  }
+  if (lane == 0) {
+    atomicMax(&sh[0], top);
+    atomicMax(&sh[1], low);
+    atomicMax(&sh[2], norm);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && sh[0]) {
+    atomicMax(&stats[bh].top[t], sh[0]);
+    atomicMax(&stats[bh].low[t], sh[1]);
+    if (sh[2]) atomicMax(&stats[bh].norm[t], sh[2]);
+  }
+}
+
+// blocks [tensor][head][tile][16 rows]; a thread takes 8 features of a row, 8 or 16
+// neighbouring ones a row.  With dout come delta = sum dout out and the log-sums.
+template <int BLOCKS>
+__global__ void __launch_bounds__(128 * BLOCKS) k_attn_split(const __grid_constant__ AttnArgs a,
+                                                             const __grid_constant__ Tiles w, int tq, int tk,
+                                                             int backward, bool vec) {
+  const int heads = a.batch * a.kv_heads;
+  int x = blockIdx.x, t = 0;
+  for (; t < 3; ++t) {
+    const int n = heads * (t == 0 ? tq : tk) * 8;
+    if (x < n) break;
+    x -= n;
+  }
+  const int per = (t == 1 || t == 2 ? tk : tq) * 8, bh = x / per, r = (x - bh * per) * 16 + threadIdx.x / (8 * BLOCKS);
+  const int g = threadIdx.x % (8 * BLOCKS), b = bh / a.kv_heads, hk = bh % a.kv_heads;
+  const AttnSpan span(a, b);
+  const bool in = r < rows_of(a, span, t);
+  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, backward);
+  if (!sc.split && t != 3) return;
+  float v[8] = {};
+  if (in) {
+    const float* p = row_of(a, t, b, hk, r);
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const int f = g * 8 + e;
+      if (vec) {
+        if (f < a.dim) *reinterpret_cast<float4*>(v + e) = *reinterpret_cast<const float4*>(p + f);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[e + q] = f + q < a.dim ? p[f + q] : 0.f;
+      }
+    }
+  }
+  if (t == 3) {
+    float d = 0.f;
+    if (in) {
+      const RowAt q(a, hk, r);
+      const float* o = a.out + at(a.os, b, q.i, q.h);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (g * 8 + e < a.dim) d = fmaf(v[e], o[g * 8 + e], d);
+    }
+#pragma unroll
+    for (int o = 1; o < 8 * BLOCKS; o <<= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (g == 0) {
+      const int64_t at_row = (int64_t)bh * padded_rows(a) + r;
+      float l = INFINITY;                         // a row that sees nothing: P = 2^(s - inf) = 0
+      if (in) {
+        const RowAt q(a, hk, r);
+        l = a.lse[((int64_t)b * a.q_heads + q.h) * a.q_len + q.i] * kLog2e;
+        if (l == -INFINITY) l = INFINITY;
+      }
+      w.lse2[at_row] = l;
+      w.delta[at_row] = sc.split ? ldexpf(d, sc.eds) : d;
+    }
+    if (!sc.split) return;
+  }
+  const float f = ldexpf(1.f, sc.e[t]);
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) split2(v[2 * e] * f, v[2 * e + 1] * f, h[e], l[e]);
+  uint8_t* o = w.p[t] + ((bh * w.tiles[t] + r / kTile) * BLOCKS + g / 8) * (int64_t)kBlockBytes +
+               chunk_at(r % kTile, g % 8);
+  *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
+  *reinterpret_cast<uint4*>(o + kBlockBytes / 2) = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+constexpr int kSoft = 8;                           // softmax warps: two threads a row
+constexpr int kThreads = 32 * (kSoft + 2);
+// P is held as 2^7 P: a weight is at most 1, and hi + lo reach 2^-32 of it
+constexpr float kUp = 7.f;
+
+template <int BLOCKS>
+struct Forward {
+  static constexpr int kD = 64 * BLOCKS;
+  static constexpr uint32_t kTileBytes = BLOCKS * kBlockBytes;
+  static constexpr int kSlots = BLOCKS == 1 ? 4 : 2;         // K and V tiles in turn
+  static constexpr size_t kSmem = 1024 + (1 + kSlots) * (size_t)kTileBytes;
+};
+
+DCT_DEV void pair_sync(int warp) {                 // warps w and w + 4, which share rows
+  asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
+}
+
+// One tile of 128 rows of a key head against its keys, 128 at a time.
+//
+// Warps 0..7 hold the softmax: thread (row, half) takes 64 of the 128 scores of its row and
+// half of its output features.  The scores of the next tile are formed while they work, and
+// each tile's P V is drained into registers, where the outputs are scaled when the running
+// maximum moves: no accumulator lives longer than one tile, so the tensor cores' rounding
+// toward zero does not build up.  P goes back into the scores' place in tensor memory as
+// the product's operand.  Warp 8 loads, warp 9 issues.
+template <int BLOCKS>
+__global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_constant__ AttnArgs a,
+                                                              const __grid_constant__ Tiles w, int row_tiles,
+                                                              int splits, float* part, uint32_t* err) {
+  using S = Forward<BLOCKS>;
+  constexpr int kO = S::kD / 2;                    // output features of a thread
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+  __shared__ uint64_t q_full, full[S::kSlots], empty[S::kSlots], s_full[2], p_full[2], o_full[2], o_empty[2];
+  __shared__ uint32_t tmem_base;
+  __shared__ float exch[2][2][kTile];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads;
+  const int split = blockIdx.x / heads % splits, tile = row_tiles - 1 - blockIdx.x / heads / splits;  // long rows first
+  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, false);
+  if (!sc.split) return;
+  const AttnSpan span(a, b);
+  const int rows = a.q_len * a.group, r0 = tile * kTile;
+  // keys of the tile's rows
+  const int i0 = r0 / a.group, i1 = min(min(r0 + kTile, rows) - 1, span.m * a.group - 1) / a.group;
+  int k0 = 0, k1 = 0;
+  if (i0 < span.m) {
+    k0 = span.lo(a, i0);
+    k1 = span.hi(a, i1);
+  }
+  int t0 = k0 / kTile, t1 = k1 > k0 ? (k1 + kTile - 1) / kTile : t0;
+  if (splits > 1) {
+    const int per = (t1 - t0 + splits - 1) / splits;
+    const int from = min(t1, t0 + split * per);
+    t1 = min(t1, from + per);
+    t0 = from;
+  }
+  const int n = t1 - t0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    for (int s = 0; s < S::kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 32 * kSoft);
+      mbar_init(&o_full[s], 1);
+      mbar_init(&o_empty[s], 32 * kSoft);
+    }
+    mbar_fence_init();
+  }
+  if (warp == kSoft + 1) tmem_alloc(&tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base, tmem_o = tmem + 256;
+
+  if (warp == kSoft) {
+    if (lane == 0 && n) {
+      auto load = [&](uint8_t* to, int t, int64_t index, uint64_t* bar) {
+        mbar_arrive_expect_tx(bar, S::kTileBytes);
+        const uint8_t* from = w.p[t] + (bh * w.tiles[t] + index) * (int64_t)S::kTileBytes;
+#pragma unroll
+        for (uint32_t o = 0; o < S::kTileBytes; o += kBlockBytes / 2)
+          bulk_load(to + o, from + o, kBlockBytes / 2, bar);
+      };
+      load(sm, 0, tile, &q_full);
+      bool ok = true;
+      int it = 0;
+      for (; it < 2 * n; ++it) {
+        const int s = it % S::kSlots;
+        ok = mbar_wait(&empty[s], ((it / S::kSlots) & 1) ^ 1, err);
+        if (!ok) break;
+        load(sm + (1 + s) * S::kTileBytes, 1 + (it & 1), t0 + it / 2, &full[s]);
+      }
+      mbar_wait(&q_full, 0, err);                  // every copy has landed before the block ends
+      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&full[u % S::kSlots], (u / S::kSlots) & 1, err);
+    }
+  } else if (warp == kSoft + 1) {
+    if (lane == 0 && n) {
+      constexpr uint32_t id_s = umma_idesc(kTile, kTile, false, false), id_o = umma_idesc(kTile, S::kD, false, true);
+      constexpr uint64_t lo = kBlockBytes / 32;    // from hi to lo, in descriptor units
+      bool ok = mbar_wait(&q_full, 0, err);
+      const uint64_t q = umma_desc(smem_addr(sm), kChunkBytes, 1024);
+      auto scores = [&](int j) {                   // S(j) = Q K(j)^T
+        const int it = 2 * j, s = it % S::kSlots;
+        ok = ok && mbar_wait(&full[s], (it / S::kSlots) & 1, err);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t k = umma_desc(smem_addr(sm + (1 + s) * S::kTileBytes), kChunkBytes, 1024);
+        const uint32_t d = tmem + (j & 1) * kTile;
+        auto step = [](int c) { return (uint64_t)((c >> 2) * (kBlockBytes / 16) + (c & 3) * 2); };
+#pragma unroll
+        for (int c = 0; c < 4 * BLOCKS; ++c) {     // the small products first
+          umma(d, q + lo + step(c), k + step(c), id_s, c != 0);
+          umma(d, q + step(c), k + lo + step(c), id_s, true);
+        }
+#pragma unroll
+        for (int c = 0; c < 4 * BLOCKS; ++c) umma(d, q + step(c), k + step(c), id_s, true);
+        umma_commit(&empty[s]);
+        umma_commit(&s_full[j & 1]);
+      };
+      scores(0);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) scores(j + 1);
+        const int it = 2 * j + 1, s = it % S::kSlots, buf = j & 1;
+        ok = ok && mbar_wait(&p_full[buf], (j >> 1) & 1, err);
+        ok = ok && mbar_wait(&o_empty[buf], ((j >> 1) & 1) ^ 1, err);
+        ok = ok && mbar_wait(&full[s], (it / S::kSlots) & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t v = umma_desc(smem_addr(sm + (1 + s) * S::kTileBytes), kBlockBytes, 1024);
+        const uint32_t p = tmem + buf * kTile, d = tmem_o + buf * S::kD;
+        // 16 keys: 8 columns of P, halves of 64 keys holding 32 columns hi, then 32 lo
+        auto pat = [&](int c) { return p + (c >> 2) * 64 + (c & 3) * 8; };
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          umma_ts(d, pat(c) + 32, v + c * 128, id_o, c != 0);
+          umma_ts(d, pat(c), v + lo + c * 128, id_o, true);
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) umma_ts(d, pat(c), v + c * 128, id_o, true);
+        umma_commit(&empty[s]);
+        umma_commit(&o_full[buf]);
+      }
+    }
+  } else {
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
+    const RowAt at_row(a, hk, min(r, rows - 1));
+    const bool in = r < rows && at_row.i < span.m;
+    const int lo = in ? span.lo(a, at_row.i) : 0, hi = in ? span.hi(a, at_row.i) : 0;
+    // (not 0: a masked score is infinite, and times 0 it would not be)
+    const float f = copysignf(fmaxf(fabsf(ldexpf(a.scale * kLog2e, -(sc.e[0] + sc.e[1]))), 1e-36f), a.scale);
+    float o[kO], top = -INFINITY, sum = 0.f, scale_o = 1.f;
+#pragma unroll
+    for (int e = 0; e < kO; ++e) o[e] = 0.f;
+    // once a wait has run out the loop goes on without waiting: the other warp of a row
+    // still counts on meeting this one
+    bool ok = true;
+    auto take = [&](int j) {                       // adds P V of tile j
+      const int buf = j & 1;
+      ok = ok && mbar_wait(&o_full[buf], (j >> 1) & 1, err);
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < kO; c += 32) {
+        uint32_t v[32];
+        tmem_load32(tmem_o + lane_bits(warp) + buf * S::kD + half * kO + c, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[c + e] = fmaf(o[c + e], scale_o, __uint_as_float(v[e]));
+      }
+      tc_fence_before();
+      mbar_arrive(&o_empty[buf]);
+    };
+    for (int j = 0; j < n; ++j) {
+      const int buf = j & 1, key = (t0 + j) * kTile + half * 64;
+      ok = ok && mbar_wait(&s_full[buf], (j >> 1) & 1, err);
+      tc_fence_after();
+      const uint32_t addr = tmem + lane_bits(warp) + buf * kTile + half * 64;
+      uint32_t x[64];
+      tmem_load32(addr, *reinterpret_cast<uint32_t(*)[32]>(x));
+      tmem_load32(addr + 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32));
+      tmem_wait_ld();
+      float best = -INFINITY;
+      if (__any_sync(0xffffffffu, key < lo || key + 64 > hi)) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (key + e < lo || key + e >= hi) x[e] = __float_as_uint(f < 0.f ? INFINITY : -INFINITY);
+      }
+      // the largest of f x: a negative scale turns the order
+      if (f >= 0.f) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e) best = fmaxf(best, __uint_as_float(x[e]));
+        best = best == -INFINITY ? best : best * f;
+      } else {
+        best = INFINITY;
+#pragma unroll
+        for (int e = 0; e < 64; ++e) best = fminf(best, __uint_as_float(x[e]));
+        best = best == INFINITY ? -INFINITY : best * f;
+      }
+      exch[j & 1][half][row] = best;
+      pair_sync(warp);
+      const float next = fmaxf(top, fmaxf(best, exch[j & 1][half ^ 1][row]));
+      const float base = next == -INFINITY ? 0.f : next;       // nothing seen yet: every weight is 0
+      const float move = ex2(top - base);
+      top = next;
+      sum *= move;
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t h[16], l[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p0 = ex2(fmaf(__uint_as_float(x[c + 2 * e]), f, kUp - base));
+          const float p1 = ex2(fmaf(__uint_as_float(x[c + 2 * e + 1]), f, kUp - base));
+          sum += p0 + p1;
+          split2(p0, p1, h[e], l[e]);
+        }
+        tmem_store16(addr + c / 2, h);
+        tmem_store16(addr + 32 + c / 2, l);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[buf]);
+      if (j) take(j - 1);
+      scale_o = move;
+    }
+    if (n) take(n - 1);
+    // the two halves of a row meet
+    pair_sync(warp);
+    exch[0][half][row] = sum;
+    pair_sync(warp);
+    sum += exch[0][half ^ 1][row];
+    if (ok && r < rows) {
+      float back = ldexpf(1.f, -sc.e[2]);
+      if (splits > 1) {
+        const float down = exp2f(-kUp);
+        back *= down;
+        float* rec = part + (((int64_t)bh * rows + r) * splits + split) * (a.dim + 2);
+#pragma unroll
+        for (int e = 0; e < kO; ++e)
+          if (half * kO + e < a.dim) rec[half * kO + e] = o[e] * back;
+        if (half == 0) {
+          rec[a.dim] = top;
+          rec[a.dim + 1] = sum * down;
+        }
+      } else {
+        float* out = a.out + at(a.os, b, at_row.i, at_row.h);
+        const float inv = sum == 0.f ? 0.f : back / sum;
+#pragma unroll
+        for (int e = 0; e < kO; ++e)
+          if (half * kO + e < a.dim) out[half * kO + e] = o[e] * inv;
+        if (half == 0 && a.lse)
+          a.lse[((int64_t)b * a.q_heads + at_row.h) * a.q_len + at_row.i] =
+              sum == 0.f ? -INFINITY : fmaf(top, kLn2, logf(sum * exp2f(-kUp)));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kSoft + 1) tmem_free(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct Layout {
+  int64_t heads, row_tiles, key_tiles, blocks;
+  size_t stats, tile[4], lse2, delta, part, total;
+  int splits;
+  Layout(const AttnArgs& a, bool backward) {
+    heads = (int64_t)a.batch * a.kv_heads;
+    row_tiles = padded_rows(a) / kTile;
+    key_tiles = (a.kv_len + kTile - 1) / kTile;
+    blocks = a.dim <= 64 ? 1 : 2;
+    splits = 1;
+    if (!backward && heads * row_tiles) {          // fill the SMs when there are few tiles of rows
+      const int64_t want = dev_info().sm_count / (heads * row_tiles);
+      splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, key_tiles / 2), 64));
+    }
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t o = at; at += (n + 1023) & ~size_t(1023); return o; };
+    stats = take(sizeof(AttnStats) * heads);
+    for (int t = 0; t < (backward ? 4 : 3); ++t)
+      tile[t] = take((size_t)heads * (t == 1 || t == 2 ? key_tiles : row_tiles) * blocks * kBlockBytes);
+    lse2 = delta = part = 0;
+    if (backward) {
+      lse2 = take(sizeof(float) * heads * row_tiles * kTile);
+      delta = take(sizeof(float) * heads * row_tiles * kTile);
+    } else {
+      part = take(std::max(attn_rows_ws_bytes(a),
+                           splits > 1 ? sizeof(float) * heads * a.group * a.q_len * splits * (size_t)(a.dim + 2) : 0));
+    }
+    total = at;
+  }
+};
+
+bool aligned(const float* p, const int64_t* s) {
+  return aligned16_h(p) && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0;
+}
+
+cudaError_t prepare(const AttnArgs& a, const Layout& L, uint8_t* w, bool backward, Tiles& t, cudaStream_t st) {
+  t = Tiles{};
+  t.stats = reinterpret_cast<AttnStats*>(w + L.stats);
+  for (int i = 0; i < (backward ? 4 : 3); ++i) {
+    t.p[i] = w + L.tile[i];
+    t.tiles[i] = i == 1 || i == 2 ? L.key_tiles : L.row_tiles;
+  }
+  t.lse2 = reinterpret_cast<float*>(w + L.lse2);
+  t.delta = reinterpret_cast<float*>(w + L.delta);
+  t.blocks = (int)L.blocks;
+  cudaError_t e = cudaMemsetAsync(t.stats, 0, sizeof(AttnStats) * L.heads, st);
+  if (e != cudaSuccess) return e;
+  const int per_q = (int)((int64_t)a.q_len * a.group + kScanRows - 1) / kScanRows, per_k = (a.kv_len + kScanRows - 1) / kScanRows;
+  const int64_t scan = L.heads * ((backward ? 2ll : 1ll) * per_q + 2ll * per_k);
+  const int64_t split = L.heads * 8 * ((backward ? 2 : 1) * L.row_tiles + 2 * L.key_tiles);
+  if (scan > INT_MAX || split > INT_MAX) return cudaErrorInvalidConfiguration;
+  if (!scan) return cudaSuccess;
+  k_attn_scan<<<(unsigned)scan, 256, 0, st>>>(a, t.stats, per_q, per_k, backward);
+  const bool vec = a.dim % 4 == 0 && aligned(a.q, a.qs) && aligned(a.k, a.ks) && aligned(a.v, a.vs) &&
+                   (!backward || aligned(a.dout, a.os));
+  if (L.blocks == 1)
+    k_attn_split<1><<<(unsigned)split, 128, 0, st>>>(a, t, (int)L.row_tiles, (int)L.key_tiles, backward, vec);
+  else
+    k_attn_split<2><<<(unsigned)split, 256, 0, st>>>(a, t, (int)L.row_tiles, (int)L.key_tiles, backward, vec);
+  return cudaGetLastError();
+}
+
+template <int BLOCKS>
+cudaError_t forward(const AttnArgs& a, const Layout& L, const Tiles& t, float* part, cudaStream_t st) {
+  using S = Forward<BLOCKS>;
+  static const cudaError_t set = cudaFuncSetAttribute(k_attn_forward<BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                      (int)S::kSmem);
+  if (set != cudaSuccess) return set;
+  const int64_t blocks = L.heads * L.row_tiles * L.splits;
+  if (blocks > INT_MAX) return cudaErrorInvalidConfiguration;
+  k_attn_forward<BLOCKS><<<(unsigned)blocks, kThreads, S::kSmem, st>>>(a, t, (int)L.row_tiles, L.splits, part,
+                                                                       device_error_word());
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+bool attn_tensor_fits(const AttnArgs& a, bool backward) {
+  return !backward && a.batch && a.kv_len && (int64_t)a.q_len * a.group >= 32;
+}
+
+size_t attn_tensor_ws_bytes(const AttnArgs& a, bool backward) { return Layout(a, backward).total; }
+
+cudaError_t launch_attn_tensor_forward(const AttnArgs& args, void* ws, cudaStream_t st) {
+  AttnArgs a = args;
+  const Layout L(a, false);
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  Tiles t;
+  cudaError_t e = prepare(a, L, w, false, t, st);
+  if (e != cudaSuccess) return e;
+  a.stats = t.stats;
+  float* part = reinterpret_cast<float*>(w + L.part);
+  e = L.blocks == 1 ? forward<1>(a, L, t, part, st) : forward<2>(a, L, t, part, st);
+  if (e == cudaSuccess && L.splits > 1) e = launch_attn_join(a, L.splits, part, true, st);
+  if (e == cudaSuccess) e = launch_attn_rows_forward(a, part, st);
+  return e;
+}
+
+cudaError_t launch_attn_tensor_backward(const AttnArgs& args, void* ws, cudaStream_t st) {
+  return cudaErrorNotSupported;
+}
+
+}  // namespace dct

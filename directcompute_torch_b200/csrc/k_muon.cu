@@ -275,14 +275,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
     const uint32_t side = warp >> 2;
     uint8_t* stage = sm + S::kStages * S::kStage + warp * kStaging;
     uint32_t part = 0;
+    // once a wait has run out the loop goes on without waiting: the other warps still count
+    // on meeting this one
     bool ok = true;
-    while (ok && run.next(sg)) {
+    while (run.next(sg)) {
       float acc[W];
 #pragma unroll
       for (int c = 0; c < W; ++c) acc[c] = 0.f;
-      for (uint32_t k0 = sg.k0; k0 < sg.k1 && ok; k0 += kDrain, ++part) {
+      for (uint32_t k0 = sg.k0; k0 < sg.k1; k0 += kDrain, ++part) {
         const uint32_t buf = part % S::kBufs;
-        ok = mbar_wait(&done[buf], (part / S::kBufs) & 1, err);
+        ok = ok && mbar_wait(&done[buf], (part / S::kBufs) & 1, err);
         tc_fence_after();
         if (ok) {
 #pragma unroll
@@ -301,7 +303,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
           else mbar_arrive_at(&freed[buf], 0);
         }
       }
-      if (!ok) break;
       if (sg.count > 1) {                         // the tile is cut
         auto slot = [&](uint32_t w) {
           return g.parts + (size_t)(2 * (PAIR ? 2 * w + rank : w) + (w == sg.first)) * (kRows * BN) + threadIdx.x;

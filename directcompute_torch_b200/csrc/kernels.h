@@ -271,13 +271,25 @@ struct AttnArgs {
   int batch, q_heads, kv_heads, group, q_len, kv_len, dim;
   int causal, window;                    // window 0: none
   float scale;
-  float* delta;                          // scratch [batch, q_heads, q_len]: sum_d dout out
+  float* delta;                          // scratch [batch * kv_heads, padded_rows]: sum_d dout out
+  const struct AttnStats* stats;         // [batch * kv_heads] or null: every head on the CUDA cores
 };
+// rows of a key head in scratch: whole tiles of 128
+__host__ __device__ inline int64_t padded_rows(const AttnArgs& a) {
+  return ((int64_t)a.q_len * a.group + 127) / 128 * 128;
+}
 // Float32 arithmetic on the CUDA cores, any finite or non-finite input.
 size_t attn_rows_ws_bytes(const AttnArgs& a);
 cudaError_t launch_attn_rows_forward(const AttnArgs& a, void* ws, cudaStream_t st);
+cudaError_t launch_attn_join(const AttnArgs& a, int splits, float* part, bool tensor, cudaStream_t st);
 cudaError_t launch_attn_delta(const AttnArgs& a, cudaStream_t st);
 cudaError_t launch_attn_rows_backward(const AttnArgs& a, cudaStream_t st);
+
+// On the tensor cores, with the CUDA cores for heads that those cannot hold (k_attention_tc.cu).
+bool attn_tensor_fits(const AttnArgs& a, bool backward);      // whether it is the faster way
+size_t attn_tensor_ws_bytes(const AttnArgs& a, bool backward);
+cudaError_t launch_attn_tensor_forward(const AttnArgs& a, void* ws, cudaStream_t st);
+cudaError_t launch_attn_tensor_backward(const AttnArgs& a, void* ws, cudaStream_t st);
 
 // ---- orthogonalised update (k_muon.cu) -----------------------------------------
 struct MuonArgs {

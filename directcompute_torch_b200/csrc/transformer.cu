@@ -171,16 +171,24 @@ int attention(const char* what, const DctAttention* p, void* q, void* k, void* v
   a.window = (int)std::min<uint32_t>(p->window, (uint32_t)kMost);
   a.scale = p->scale != 0.f ? p->scale : (float)(1.0 / sqrt((double)p->head_dim));
   OnDevice guard;
-  if (!backward) {
-    if (!rt_ensure_ws(attn_rows_ws_bytes(a))) return DCT_ERR_CUDA;
-    return rt_cuda_ok(launch_attn_rows_forward(a, rt_ws(), rt_stream()), what) ? DCT_OK : DCT_ERR_CUDA;
+  cudaStream_t st = rt_stream();
+  if (backward) {
+    a.dout = args[4].buf->d; a.dq = args[5].buf->d; a.dk = args[6].buf->d; a.dv = args[7].buf->d;
+    copy3(a.dqs, p->dq_stride); copy3(a.dks, p->dk_stride); copy3(a.dvs, p->dv_stride);
   }
-  a.dout = args[4].buf->d; a.dq = args[5].buf->d; a.dk = args[6].buf->d; a.dv = args[7].buf->d;
-  copy3(a.dqs, p->dq_stride); copy3(a.dks, p->dk_stride); copy3(a.dvs, p->dv_stride);
-  if (!rt_ensure_ws(sizeof(float) * B * p->q_heads * p->q_len)) return DCT_ERR_CUDA;
-  a.delta = static_cast<float*>(rt_ws());
-  cudaError_t e = launch_attn_delta(a, rt_stream());
-  if (e == cudaSuccess) e = launch_attn_rows_backward(a, rt_stream());
+  cudaError_t e;
+  if (attn_tensor_fits(a, backward)) {
+    if (!rt_ensure_ws(attn_tensor_ws_bytes(a, backward))) return DCT_ERR_CUDA;
+    e = backward ? launch_attn_tensor_backward(a, rt_ws(), st) : launch_attn_tensor_forward(a, rt_ws(), st);
+  } else if (!backward) {
+    if (!rt_ensure_ws(attn_rows_ws_bytes(a))) return DCT_ERR_CUDA;
+    e = launch_attn_rows_forward(a, rt_ws(), st);
+  } else {
+    if (!rt_ensure_ws(sizeof(float) * B * p->kv_heads * padded_rows(a))) return DCT_ERR_CUDA;
+    a.delta = static_cast<float*>(rt_ws());
+    e = launch_attn_delta(a, st);
+    if (e == cudaSuccess) e = launch_attn_rows_backward(a, st);
+  }
   return rt_cuda_ok(e, what) ? DCT_OK : DCT_ERR_CUDA;
 }
 
