@@ -49,6 +49,21 @@ DCT_DEV const float* row_of(const AttnArgs& a, int t, int b, int hk, int r) {
   return t == 0 ? a.q + at(a.qs, b, w.i, w.h) : a.dout + at(a.os, b, w.i, w.h);
 }
 
+// features [first, first + N) of a row, as far as it has them
+template <int N>
+DCT_DEV void store_features(float* row, int first, int dim, bool vec, const float (&x)[N]) {
+  if (vec) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4)
+      if (first + e < dim)
+        *reinterpret_cast<float4*>(row + first + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (first + e < dim) row[first + e] = x[e];
+  }
+}
+
 // ---------------------------------------------------------------------------
 // magnitudes, splitting
 // ---------------------------------------------------------------------------
@@ -203,7 +218,7 @@ DCT_DEV void pair_sync(int warp) {                 // warps w and w + 4, which s
 template <int BLOCKS>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_constant__ AttnArgs a,
                                                               const __grid_constant__ Tiles w, int row_tiles,
-                                                              int splits, float* part, uint32_t* err) {
+                                                              int splits, float* part, bool vec_out, uint32_t* err) {
   using S = Forward<BLOCKS>;
   constexpr int kO = S::kD / 2;                    // output features of a thread
   extern __shared__ uint8_t raw[];
@@ -427,8 +442,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
         float* out = a.out + at(a.os, b, at_row.i, at_row.h);
         const float inv = sum == 0.f ? 0.f : back / sum;
 #pragma unroll
-        for (int e = 0; e < kO; ++e)
-          if (half * kO + e < a.dim) out[half * kO + e] = o[e] * inv;
+        for (int e = 0; e < kO; ++e) o[e] *= inv;
+        store_features<kO>(out, half * kO, a.dim, vec_out, o);
         if (half == 0 && a.lse)
           a.lse[((int64_t)b * a.q_heads + at_row.h) * a.q_len + at_row.i] =
               sum == 0.f ? -INFINITY : fmaf(top, kLn2, logf(sum * exp2f(-kUp)));
@@ -439,6 +454,491 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
   __syncthreads();
   tc_fence_after();
   if (warp == kSoft + 1) tmem_free(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+// Two kernels that each form the scores and dP = dout V^T again, one for dq (a tile of rows
+// against its keys) and one for dk and dv (a tile of keys against the rows that see them):
+// seven products instead of five, but every gradient has one owner, no atomics and one
+// order.  The inner side goes in half tiles of 64, since the resident operands take most of
+// shared memory; one of them lives in tensor memory instead, where the matrix instructions
+// read it beside shared memory's 128 bytes a cycle, which bound them otherwise.
+constexpr int kHalf = 64;
+constexpr float kUpP = 14.f;                       // P <= 1 is held as 2^14 P
+
+template <int BLOCKS>
+struct Backward {
+  static constexpr int kD = 64 * BLOCKS, kF = kD / 2;              // features, of them a thread's
+  static constexpr uint32_t kTileBytes = BLOCKS * kBlockBytes, kSlotBytes = kTileBytes / 2;
+  static constexpr int kSlots = BLOCKS == 1 ? 8 : 5;
+  static constexpr size_t kSmem = 1024 + kTileBytes + (size_t)kSlots * kSlotBytes;
+};
+
+// half tile `h` (64 rows) of operand t: [64 features][hi, lo][64 rows][64 float16]
+template <int BLOCKS>
+DCT_DEV void load_half(const Tiles& w, int bh, int t, int64_t h, uint8_t* to, uint64_t* bar) {
+  const uint8_t* from = w.p[t] + (bh * w.tiles[t] + h / 2) * (int64_t)(BLOCKS * kBlockBytes) + (h & 1) * kChunkBytes;
+#pragma unroll
+  for (int i = 0; i < 2 * BLOCKS; ++i) bulk_load(to + i * kChunkBytes, from + i * 2 * kChunkBytes, kChunkBytes, bar);
+}
+
+// A thread's row of a whole tile into tensor memory as an operand: columns of hi, then of lo.
+// Warps w and w + 4 take the halves of the features.
+template <int BLOCKS>
+DCT_DEV void tile_to_tmem(const uint8_t* tile, uint32_t addr, int warp, int row) {
+  constexpr int kGroups = 4 * BLOCKS;              // of 8 features, a thread's
+  const int g0 = (warp >> 2) * kGroups;
+#pragma unroll
+  for (int low = 0; low < 2; ++low)
+#pragma unroll
+    for (int g = 0; g < kGroups; g += 4) {
+      uint32_t r[16];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int f = g0 + g + e;
+        const uint4 v = *reinterpret_cast<const uint4*>(tile + (f >> 3) * kBlockBytes + low * (kBlockBytes / 2) +
+                                                        chunk_at(row, f & 7));
+        r[4 * e] = v.x; r[4 * e + 1] = v.y; r[4 * e + 2] = v.z; r[4 * e + 3] = v.w;
+      }
+      tmem_store16(addr + lane_bits(warp) + low * 32 * BLOCKS + (g0 + g) * 4, r);
+    }
+}
+
+// D = A B^T over the features: A a whole tile in shared memory, B a half tile
+template <int BLOCKS>
+DCT_DEV void mma_features_ss(uint32_t d, uint64_t a, uint64_t b) {
+  constexpr uint32_t id = umma_idesc(kTile, kHalf, false, false);
+  constexpr uint64_t lo_a = kBlockBytes / 32, lo_b = kChunkBytes / 16;
+  auto sa = [](int c) { return (uint64_t)((c >> 2) * (kBlockBytes / 16) + (c & 3) * 2); };
+  auto sb = [](int c) { return (uint64_t)((c >> 2) * (2 * kChunkBytes / 16) + (c & 3) * 2); };
+#pragma unroll
+  for (int c = 0; c < 4 * BLOCKS; ++c) {
+    umma(d, a + lo_a + sa(c), b + sb(c), id, c != 0);
+    umma(d, a + sa(c), b + lo_b + sb(c), id, true);
+  }
+#pragma unroll
+  for (int c = 0; c < 4 * BLOCKS; ++c) umma(d, a + sa(c), b + sb(c), id, true);
+}
+// the same with A in tensor memory
+template <int BLOCKS>
+DCT_DEV void mma_features_ts(uint32_t d, uint32_t a, uint64_t b) {
+  constexpr uint32_t id = umma_idesc(kTile, kHalf, false, false);
+  constexpr uint64_t lo_b = kChunkBytes / 16;
+  auto sb = [](int c) { return (uint64_t)((c >> 2) * (2 * kChunkBytes / 16) + (c & 3) * 2); };
+#pragma unroll
+  for (int c = 0; c < 4 * BLOCKS; ++c) {
+    umma_ts(d, a + 32 * BLOCKS + 8 * c, b + sb(c), id, c != 0);
+    umma_ts(d, a + 8 * c, b + lo_b + sb(c), id, true);
+  }
+#pragma unroll
+  for (int c = 0; c < 4 * BLOCKS; ++c) umma_ts(d, a + 8 * c, b + sb(c), id, true);
+}
+// D (+)= A B over 64 rows: A in tensor memory (for each 32 of them 16 columns hi, 16 lo), B
+// a half tile with its rows as the contraction
+template <int BLOCKS>
+DCT_DEV void mma_rows(uint32_t d, uint32_t a, uint64_t b, bool add) {
+  constexpr uint32_t id = umma_idesc(kTile, 64 * BLOCKS, false, true);
+  constexpr uint64_t lo_b = kChunkBytes / 16;
+  auto sa = [](int c) { return (uint32_t)((c >> 1) * 32 + (c & 1) * 8); };
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    umma_ts(d, a + 16 + sa(c), b + c * 128, id, add || c != 0);
+    umma_ts(d, a + sa(c), b + lo_b + c * 128, id, true);
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) umma_ts(d, a + sa(c), b + c * 128, id, true);
+}
+
+// 32 values as an operand's columns, 16 of hi and 16 of lo
+DCT_DEV void store_operand(uint32_t addr, const float (&x)[32]) {
+  uint32_t h[16], l[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) split2(x[2 * e], x[2 * e + 1], h[e], l[e]);
+  tmem_store16(addr, h);
+  tmem_store16(addr + 16, l);
+}
+
+// acc += 32 columns at a time
+template <int N>
+DCT_DEV void drain(uint32_t addr, float (&acc)[N]) {
+#pragma unroll
+  for (int c = 0; c < N; c += 32) {
+    uint32_t v[32];
+    tmem_load32(addr + c, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) acc[c + e] += __uint_as_float(v[e]);
+  }
+}
+
+constexpr int kGroup = 2;                          // half tiles between drains of an accumulator
+
+// dq of a tile of 128 rows: dS = P (dP - delta), dq = scale dS K.  Q rests in shared memory,
+// dout in tensor memory; V and K come in half tiles of 64 keys.
+template <int BLOCKS>
+__global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__ AttnArgs a,
+                                                         const __grid_constant__ Tiles w, int row_tiles, bool vec_out,
+                                                         uint32_t* err) {
+  using S = Backward<BLOCKS>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+  __shared__ uint64_t q_full, go_full, full[S::kSlots], empty[S::kSlots], s_full[2], ds_full[2], acc_full, acc_empty;
+  __shared__ uint32_t tmem_base;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = row_tiles - 1 - blockIdx.x / heads;
+  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, true);
+  if (!sc.split) return;
+  const AttnSpan span(a, b);
+  const int rows = a.q_len * a.group, r0 = tile * kTile;
+  const int i0 = r0 / a.group, i1 = min(min(r0 + kTile, rows) - 1, span.m * a.group - 1) / a.group;
+  int t0 = 0, n = 0;
+  if (i0 < span.m) {
+    const int k0 = span.lo(a, i0), k1 = span.hi(a, i1);
+    t0 = k0 / kHalf;
+    n = k1 > k0 ? (k1 + kHalf - 1) / kHalf - t0 : 0;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    mbar_init(&go_full, 32 * kSoft);
+    for (int s = 0; s < S::kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&ds_full[s], 32 * kSoft);
+    }
+    mbar_init(&acc_full, 1);
+    mbar_init(&acc_empty, 32 * kSoft);
+    mbar_fence_init();
+  }
+  if (warp == kSoft + 1) tmem_alloc(&tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // S and dP twice, the operand dout, the accumulator
+  const uint32_t tm_s = tmem_base, tm_dp = tm_s + 128, tm_go = tm_s + 256, tm_acc = tm_s + 384;
+
+  if (warp == kSoft) {
+    if (lane == 0 && n) {
+      mbar_arrive_expect_tx(&q_full, S::kTileBytes);
+      const uint8_t* q = w.p[0] + (bh * w.tiles[0] + tile) * (int64_t)S::kTileBytes;
+#pragma unroll
+      for (uint32_t o = 0; o < S::kTileBytes; o += kBlockBytes / 2)
+        bulk_load(sm + o, q + o, kBlockBytes / 2, &q_full);
+      int it = 0;
+      for (; it < 2 * n; ++it) {                   // V, K, V, K ...
+        const int s = it % S::kSlots;
+        if (!mbar_wait(&empty[s], ((it / S::kSlots) & 1) ^ 1, err)) break;
+        mbar_arrive_expect_tx(&full[s], S::kSlotBytes);
+        load_half<BLOCKS>(w, bh, it & 1 ? 1 : 2, t0 + it / 2, sm + S::kTileBytes + s * S::kSlotBytes, &full[s]);
+      }
+      mbar_wait(&q_full, 0, err);                  // every copy has landed before the block ends
+      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&full[u % S::kSlots], (u / S::kSlots) & 1, err);
+    }
+  } else if (warp == kSoft + 1) {
+    if (lane == 0 && n) {
+      bool ok = mbar_wait(&q_full, 0, err) && mbar_wait(&go_full, 0, err);
+      tc_fence_after();
+      const uint64_t q = umma_desc(smem_addr(sm), kChunkBytes, 1024);
+      auto slot = [&](int it) { return smem_addr(sm + S::kTileBytes + it % S::kSlots * S::kSlotBytes); };
+      auto await = [&](int it) {
+        ok = ok && mbar_wait(&full[it % S::kSlots], (it / S::kSlots) & 1, err);
+        tc_fence_after();
+      };
+      auto scores = [&](int j) {                   // S(j) = Q K^T, dP(j) = dout V^T
+        await(2 * j + 1);
+        if (!ok) return;
+        mma_features_ss<BLOCKS>(tm_s + (j & 1) * kHalf, q, umma_desc(slot(2 * j + 1), kChunkBytes, 1024));
+        await(2 * j);
+        if (!ok) return;
+        mma_features_ts<BLOCKS>(tm_dp + (j & 1) * kHalf, tm_go, umma_desc(slot(2 * j), kChunkBytes, 1024));
+        umma_commit(&empty[2 * j % S::kSlots]);
+        umma_commit(&s_full[j & 1]);
+      };
+      scores(0);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) scores(j + 1);
+        const int group = j / kGroup;
+        ok = ok && mbar_wait(&ds_full[j & 1], (j >> 1) & 1, err);
+        if (j % kGroup == 0) ok = ok && mbar_wait(&acc_empty, (group & 1) ^ 1, err);
+        if (!ok) break;
+        tc_fence_after();
+        mma_rows<BLOCKS>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(slot(2 * j + 1), 2 * kChunkBytes, 1024),
+                         j % kGroup != 0);
+        umma_commit(&empty[(2 * j + 1) % S::kSlots]);
+        if (j % kGroup == kGroup - 1 || j == n - 1) umma_commit(&acc_full);
+      }
+    }
+  } else {
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
+    const RowAt at_row(a, hk, min(r, rows - 1));
+    const bool in = r < rows && at_row.i < span.m;
+    const int lo = in ? span.lo(a, at_row.i) : 0, hi = in ? span.hi(a, at_row.i) : 0;
+    const float f = ldexpf(a.scale * kLog2e, -(sc.e[0] + sc.e[1])), fd = ldexpf(1.f, sc.eds - sc.e[3] - sc.e[2]);
+    float acc[S::kF];
+#pragma unroll
+    for (int e = 0; e < S::kF; ++e) acc[e] = 0.f;
+    if (n) {
+      const int64_t at_stat = (int64_t)bh * row_tiles * kTile + r;
+      const float lse2 = w.lse2[at_stat], delta = w.delta[at_stat];
+      tile_to_tmem<BLOCKS>(w.p[3] + (bh * w.tiles[3] + tile) * (int64_t)S::kTileBytes, tm_go, warp, row);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&go_full);
+      bool ok = true;
+      auto take = [&](int group) {
+        ok = ok && mbar_wait(&acc_full, group & 1, err);
+        tc_fence_after();
+        drain(tm_acc + lane_bits(warp) + half * S::kF, acc);
+        tc_fence_before();
+        mbar_arrive(&acc_empty);
+      };
+      for (int j = 0; j < n; ++j) {
+        const int key = (t0 + j) * kHalf + half * 32;
+        ok = ok && mbar_wait(&s_full[j & 1], (j >> 1) & 1, err);
+        tc_fence_after();
+        const uint32_t off = lane_bits(warp) + (j & 1) * kHalf + half * 32;
+        uint32_t x[32], y[32];
+        tmem_load32(tm_s + off, x);
+        tmem_load32(tm_dp + off, y);
+        tmem_wait_ld();
+        float ds[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          ds[e] = ex2(fmaf(__uint_as_float(x[e]), f, -lse2)) * fmaf(__uint_as_float(y[e]), fd, -delta);
+        if (__any_sync(0xffffffffu, key < lo || key + 32 > hi)) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (key + e < lo || key + e >= hi) ds[e] = 0.f;
+        }
+        store_operand(tm_s + off, ds);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&ds_full[j & 1]);
+        if (j && j % kGroup == 0) take(j / kGroup - 1);
+      }
+      take((n - 1) / kGroup);
+    }
+    if (r < rows) {
+      const float back = ldexpf(a.scale, -(sc.eds + sc.e[1]));
+#pragma unroll
+      for (int e = 0; e < S::kF; ++e) acc[e] *= back;
+      store_features<S::kF>(a.dq + at(a.dqs, b, at_row.i, at_row.h), half * S::kF, a.dim, vec_out, acc);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kSoft + 1) tmem_free(tmem_base, 512);
+}
+
+// dk and dv of a tile of 128 keys: dv = P^T dout, dk = scale dS^T Q.  K rests in shared
+// memory, V in tensor memory; Q and dout come in half tiles of 64 rows with their log-sums
+// and deltas.  A thread holds (key, half): 32 rows of the scores and half the features of
+// both gradients, 128 registers of sums, so the loading warps give registers up.
+template <int BLOCKS>
+__global__ void __launch_bounds__(384, 1) k_attn_dkv(const __grid_constant__ AttnArgs a,
+                                                     const __grid_constant__ Tiles w, int row_tiles, bool vec_out,
+                                                     uint32_t* err) {
+  using S = Backward<BLOCKS>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+  __shared__ uint64_t k_full, v_full, full[S::kSlots], empty[S::kSlots], s_full, dp_full, p_full, ds_full, acc_full,
+      acc_empty;
+  // Log-sums and deltas come with Q(j) but outlive its neighbours' slots: with five slots
+  // Q(j + 3) may come in after dv(j), when the log-sums of j are used, and Q(j + 4) after
+  // dv(j + 1), when the deltas are; with eight, both stay until dk(j).
+  constexpr int kLse = BLOCKS == 1 ? 5 : 3, kDelta = BLOCKS == 1 ? 5 : 4;
+  __shared__ __align__(16) float vec_lse[kLse][kHalf], vec_delta[kDelta][kHalf];
+  __shared__ uint32_t tmem_base;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = blockIdx.x / heads;    // long ones first
+  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, true);
+  if (!sc.split) return;
+  const AttnSpan span(a, b);
+  const int j0 = tile * kTile, j1 = min(j0 + kTile, span.n) - 1;
+  int t0 = 0, n = 0;
+  if (j0 < span.n) {
+    const int first = span.first(a, j0) * a.group, last = span.last(a, j1) * a.group;
+    t0 = first / kHalf;
+    n = last > first ? (last + kHalf - 1) / kHalf - t0 : 0;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(&k_full, 1);
+    mbar_init(&v_full, 32 * kSoft);
+    for (int s = 0; s < S::kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&s_full, 1);
+    mbar_init(&dp_full, 1);
+    mbar_init(&p_full, 32 * kSoft);
+    mbar_init(&ds_full, 32 * kSoft);
+    mbar_init(&acc_full, 1);
+    mbar_init(&acc_empty, 32 * kSoft);
+    mbar_fence_init();
+  }
+  if (warp == kSoft + 1) tmem_alloc(&tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // the accumulators, the operand V, S and dP (each also P's and dS's place)
+  const uint32_t tm_dk = tmem_base, tm_dv = tm_dk + 128, tm_v = tm_dk + 256, tm_s = tm_dk + 384, tm_dp = tm_dk + 448;
+
+  if (warp >= kSoft) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == kSoft && lane == 0 && n) {
+      mbar_arrive_expect_tx(&k_full, S::kTileBytes);
+      const uint8_t* k = w.p[1] + (bh * w.tiles[1] + tile) * (int64_t)S::kTileBytes;
+#pragma unroll
+      for (uint32_t o = 0; o < S::kTileBytes; o += kBlockBytes / 2)
+        bulk_load(sm + o, k + o, kBlockBytes / 2, &k_full);
+      int it = 0;
+      for (; it < 2 * n; ++it) {                   // Q, dout, Q, dout ...
+        const int s = it % S::kSlots, j = it / 2;
+        if (!mbar_wait(&empty[s], ((it / S::kSlots) & 1) ^ 1, err)) break;
+        mbar_arrive_expect_tx(&full[s], S::kSlotBytes + (it & 1 ? 0 : 2 * kHalf * 4));
+        load_half<BLOCKS>(w, bh, it & 1 ? 3 : 0, t0 + j, sm + S::kTileBytes + s * S::kSlotBytes, &full[s]);
+        if (!(it & 1)) {
+          const int64_t at_stat = (int64_t)bh * row_tiles * kTile + (int64_t)(t0 + j) * kHalf;
+          bulk_load(vec_lse[j % kLse], w.lse2 + at_stat, kHalf * 4, &full[s]);
+          bulk_load(vec_delta[j % kDelta], w.delta + at_stat, kHalf * 4, &full[s]);
+        }
+      }
+      mbar_wait(&k_full, 0, err);                  // every copy has landed before the block ends
+      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&full[u % S::kSlots], (u / S::kSlots) & 1, err);
+    }
+    if (warp == kSoft + 1 && lane == 0 && n) {
+      bool ok = mbar_wait(&k_full, 0, err) && mbar_wait(&v_full, 0, err);
+      tc_fence_after();
+      const uint64_t k = umma_desc(smem_addr(sm), kChunkBytes, 1024);
+      auto slot = [&](int it) { return smem_addr(sm + S::kTileBytes + it % S::kSlots * S::kSlotBytes); };
+      auto await = [&](uint64_t* bar, int parity) {
+        ok = ok && mbar_wait(bar, parity & 1, err);
+        tc_fence_after();
+      };
+      auto scores = [&](int j) {                   // S^T(j) = K Q^T
+        await(&full[2 * j % S::kSlots], 2 * j / S::kSlots);
+        if (!ok) return;
+        mma_features_ss<BLOCKS>(tm_s, k, umma_desc(slot(2 * j), kChunkBytes, 1024));
+        umma_commit(&s_full);
+      };
+      auto dps = [&](int j) {                      // dP^T(j) = V dout^T
+        await(&full[(2 * j + 1) % S::kSlots], (2 * j + 1) / S::kSlots);
+        if (!ok) return;
+        mma_features_ts<BLOCKS>(tm_dp, tm_v, umma_desc(slot(2 * j + 1), kChunkBytes, 1024));
+        umma_commit(&dp_full);
+      };
+      scores(0);
+      dps(0);
+      for (int j = 0; j < n && ok; ++j) {
+        await(&p_full, j);
+        if (j % kGroup == 0) await(&acc_empty, (j / kGroup & 1) ^ 1);
+        if (!ok) break;
+        mma_rows<BLOCKS>(tm_dv, tm_s, umma_desc(slot(2 * j + 1), 2 * kChunkBytes, 1024), j % kGroup != 0);
+        umma_commit(&empty[(2 * j + 1) % S::kSlots]);
+        if (j + 1 < n) scores(j + 1);
+        await(&ds_full, j);
+        if (!ok) break;
+        mma_rows<BLOCKS>(tm_dk, tm_dp, umma_desc(slot(2 * j), 2 * kChunkBytes, 1024), j % kGroup != 0);
+        umma_commit(&empty[2 * j % S::kSlots]);
+        if (j % kGroup == kGroup - 1 || j == n - 1) umma_commit(&acc_full);
+        if (j + 1 < n) dps(j + 1);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane, key = j0 + row;
+    // rows that see the thread's key
+    const int lo = key < span.n ? span.first(a, key) * a.group : 0, hi = key < span.n ? span.last(a, key) * a.group : 0;
+    const float f = ldexpf(a.scale * kLog2e, -(sc.e[0] + sc.e[1])), fd = ldexpf(1.f, sc.eds - sc.e[3] - sc.e[2]);
+    float dk[S::kF], dv[S::kF];
+#pragma unroll
+    for (int e = 0; e < S::kF; ++e) dk[e] = dv[e] = 0.f;
+    if (n) {
+      tile_to_tmem<BLOCKS>(w.p[2] + (bh * w.tiles[2] + tile) * (int64_t)S::kTileBytes, tm_v, warp, row);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&v_full);
+      bool ok = true;
+      auto take = [&](int group) {
+        ok = ok && mbar_wait(&acc_full, group & 1, err);
+        tc_fence_after();
+        drain(tm_dv + lane_bits(warp) + half * S::kF, dv);
+        drain(tm_dk + lane_bits(warp) + half * S::kF, dk);
+        tc_fence_before();
+        mbar_arrive(&acc_empty);
+      };
+      const uint32_t off = lane_bits(warp) + half * 32;
+      for (int j = 0; j < n; ++j) {
+        const int r = (t0 + j) * kHalf + half * 32, s = 2 * j % S::kSlots;
+        ok = ok && mbar_wait(&full[s], (2 * j / S::kSlots) & 1, err);      // the log-sums and deltas
+        ok = ok && mbar_wait(&s_full, j & 1, err);
+        tc_fence_after();
+        const float4* lse = reinterpret_cast<const float4*>(vec_lse[j % kLse] + half * 32);
+        const float4* del = reinterpret_cast<const float4*>(vec_delta[j % kDelta] + half * 32);
+        uint32_t x[32];
+        float p[32];
+        tmem_load32(tm_s + off, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 l = lse[e / 4];
+          p[e] = ex2(fmaf(__uint_as_float(x[e]), f, kUpP - l.x));
+          p[e + 1] = ex2(fmaf(__uint_as_float(x[e + 1]), f, kUpP - l.y));
+          p[e + 2] = ex2(fmaf(__uint_as_float(x[e + 2]), f, kUpP - l.z));
+          p[e + 3] = ex2(fmaf(__uint_as_float(x[e + 3]), f, kUpP - l.w));
+        }
+        if (__any_sync(0xffffffffu, r < lo || r + 32 > hi)) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (r + e < lo || r + e >= hi) p[e] = 0.f;
+        }
+        store_operand(tm_s + off, p);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full);
+        if (j && j % kGroup == 0) take(j / kGroup - 1);
+        ok = ok && mbar_wait(&dp_full, j & 1, err);
+        tc_fence_after();
+        tmem_load32(tm_dp + off, x);
+        tmem_wait_ld();
+        constexpr float down = 1.f / 16384.f;      // 2^-14: P itself
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 d = del[e / 4];
+          p[e] *= down * fmaf(__uint_as_float(x[e]), fd, -d.x);
+          p[e + 1] *= down * fmaf(__uint_as_float(x[e + 1]), fd, -d.y);
+          p[e + 2] *= down * fmaf(__uint_as_float(x[e + 2]), fd, -d.z);
+          p[e + 3] *= down * fmaf(__uint_as_float(x[e + 3]), fd, -d.w);
+        }
+        store_operand(tm_dp + off, p);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&ds_full);
+      }
+      take((n - 1) / kGroup);
+    }
+    if (key < a.kv_len) {
+      const float bk = ldexpf(a.scale, -(sc.eds + sc.e[0])), bv = ldexpf(1.f, -(int)kUpP - sc.e[3]);
+#pragma unroll
+      for (int e = 0; e < S::kF; ++e) {
+        dk[e] *= bk;
+        dv[e] *= bv;
+      }
+      store_features<S::kF>(a.dk + at(a.dks, b, key, hk), half * S::kF, a.dim, vec_out, dk);
+      store_features<S::kF>(a.dv + at(a.dvs, b, key, hk), half * S::kF, a.dim, vec_out, dv);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kSoft + 1) tmem_free(tmem_base, 512);
 }
 
 // ---------------------------------------------------------------------------
@@ -514,15 +1014,36 @@ cudaError_t forward(const AttnArgs& a, const Layout& L, const Tiles& t, float* p
   if (set != cudaSuccess) return set;
   const int64_t blocks = L.heads * L.row_tiles * L.splits;
   if (blocks > INT_MAX) return cudaErrorInvalidConfiguration;
-  k_attn_forward<BLOCKS><<<(unsigned)blocks, kThreads, S::kSmem, st>>>(a, t, (int)L.row_tiles, L.splits, part,
-                                                                       device_error_word());
+  k_attn_forward<BLOCKS><<<(unsigned)blocks, kThreads, S::kSmem, st>>>(
+      a, t, (int)L.row_tiles, L.splits, part, a.dim % 4 == 0 && aligned(a.out, a.os), device_error_word());
+  return cudaGetLastError();
+}
+
+template <int BLOCKS>
+cudaError_t backward(const AttnArgs& a, const Layout& L, const Tiles& t, cudaStream_t st) {
+  using S = Backward<BLOCKS>;
+  static const cudaError_t set_q = cudaFuncSetAttribute(k_attn_dq<BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                        (int)S::kSmem);
+  static const cudaError_t set_kv = cudaFuncSetAttribute(k_attn_dkv<BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                         (int)S::kSmem);
+  if (set_q != cudaSuccess) return set_q;
+  if (set_kv != cudaSuccess) return set_kv;
+  const int64_t nq = L.heads * L.row_tiles, nk = L.heads * L.key_tiles;
+  if (nq > INT_MAX || nk > INT_MAX) return cudaErrorInvalidConfiguration;
+  const bool vec = a.dim % 4 == 0;
+  if (nk)
+    k_attn_dkv<BLOCKS><<<(unsigned)nk, 384, S::kSmem, st>>>(
+        a, t, (int)L.row_tiles, vec && aligned(a.dk, a.dks) && aligned(a.dv, a.dvs), device_error_word());
+  if (nq)
+    k_attn_dq<BLOCKS><<<(unsigned)nq, kThreads, S::kSmem, st>>>(a, t, (int)L.row_tiles, vec && aligned(a.dq, a.dqs),
+                                                                device_error_word());
   return cudaGetLastError();
 }
 
 }  // namespace
 
 bool attn_tensor_fits(const AttnArgs& a, bool backward) {
-  return !backward && a.batch && a.kv_len && (int64_t)a.q_len * a.group >= 32;
+  return a.batch && a.kv_len && (int64_t)a.q_len * a.group >= 32;
 }
 
 size_t attn_tensor_ws_bytes(const AttnArgs& a, bool backward) { return Layout(a, backward).total; }
@@ -543,7 +1064,16 @@ cudaError_t launch_attn_tensor_forward(const AttnArgs& args, void* ws, cudaStrea
 }
 
 cudaError_t launch_attn_tensor_backward(const AttnArgs& args, void* ws, cudaStream_t st) {
-  return cudaErrorNotSupported;
+  AttnArgs a = args;
+  const Layout L(a, true);
+  Tiles t;
+  cudaError_t e = prepare(a, L, static_cast<uint8_t*>(ws), true, t, st);
+  if (e != cudaSuccess) return e;
+  a.stats = t.stats;
+  a.delta = t.delta;
+  e = L.blocks == 1 ? backward<1>(a, L, t, st) : backward<2>(a, L, t, st);
+  if (e == cudaSuccess) e = launch_attn_rows_backward(a, st);
+  return e;
 }
 
 }  // namespace dct
