@@ -88,6 +88,24 @@ DCT_DEV void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
       : "memory");
 }
 
+DCT_DEV void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+DCT_DEV void tmem_store8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+DCT_DEV void tmem_load(uint32_t addr, uint32_t (&r)[32]) { tmem_load32(addr, r); }
+DCT_DEV void tmem_load(uint32_t addr, uint32_t (&r)[16]) { tmem_load16(addr, r); }
+DCT_DEV void tmem_store(uint32_t addr, const uint32_t (&r)[16]) { tmem_store16(addr, r); }
+DCT_DEV void tmem_store(uint32_t addr, const uint32_t (&r)[8]) { tmem_store8(addr, r); }
+
 // ---- matrix instructions ---------------------------------------------------------
 // Shared memory descriptor of a 128-byte swizzled operand (start address, leading and
 // stride byte offsets in units of 16; version 1; swizzle mode 2).

@@ -194,6 +194,8 @@ template <int NV, bool VEC, int R>
 __global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const __grid_constant__ AttnArgs a, int groups, int splits,
                                                            float* part, int items) {
   __shared__ float sh[kWarps][R][32 * NV + 2];
+  pdl_entry();
+  if (a.any && !*a.any) return;
   for (int i = blockIdx.x; i < items; i += gridDim.x) {
     rows_forward<NV, VEC, R>(a, i, groups, splits, part, sh);
     __syncthreads();
@@ -383,19 +385,21 @@ DCT_DEV void rows_dkv(const AttnArgs& a, int item, int groups, float (&sh)[kWarp
   }
 }
 
-template <int NV, bool VEC, int R, bool KEYS>
-__global__ void __launch_bounds__(32 * kWarps) k_attn_rows_backward(const __grid_constant__ AttnArgs a, int groups,
-                                                                    int items) {
+template <int NV, bool VEC, int R>
+__global__ void __launch_bounds__(32 * kWarps) k_attn_rows_backward(const __grid_constant__ AttnArgs a, int groups_q,
+                                                                    int items_q, int groups_k, int items_k) {
   __shared__ float sh[kWarps][32 * NV];
-  for (int i = blockIdx.x; i < items; i += gridDim.x) {
-    if constexpr (KEYS) rows_dkv<NV, VEC, R>(a, i, groups, sh);
-    else rows_dq<NV, VEC, R>(a, i, groups, sh);
+  pdl_entry();
+  if (a.any && !*a.any) return;
+  for (int64_t i = blockIdx.x; i < (int64_t)items_q + items_k; i += gridDim.x) {
+    if (i < items_q) rows_dq<NV, VEC, R>(a, (int)i, groups_q, sh);
+    else rows_dkv<NV, VEC, R>(a, (int)(i - items_q), groups_k, sh);
     __syncthreads();
   }
 }
 
 unsigned blocks_for(const AttnArgs& a, int64_t items) {
-  return (unsigned)(a.stats ? std::min<int64_t>(items, 8ll * dev_info().sm_count) : items);
+  return (unsigned)(a.stats ? std::min<int64_t>(items, 8ll * dev_info().sm_count) : std::min<int64_t>(items, INT_MAX));
 }
 
 bool aligned(const float* p, const int64_t* s) {
@@ -449,10 +453,8 @@ cudaError_t launch_attn_rows_forward(const AttnArgs& a, void* ws, cudaStream_t s
     constexpr bool V = decltype(v)::value;
     const unsigned n = blocks_for(a, blocks);
     const int items = (int)blocks, g = (int)groups;
-    if (R == 4) k_attn_rows<NV, V, 4><<<n, 32 * kWarps, 0, st>>>(a, g, splits, part, items);
-    else if (R == 2) k_attn_rows<NV, V, 2><<<n, 32 * kWarps, 0, st>>>(a, g, splits, part, items);
-    else k_attn_rows<NV, V, 1><<<n, 32 * kWarps, 0, st>>>(a, g, splits, part, items);
-    return cudaGetLastError();
+    const auto kernel = R == 4 ? k_attn_rows<NV, V, 4> : R == 2 ? k_attn_rows<NV, V, 2> : k_attn_rows<NV, V, 1>;
+    return launch_pdl(kernel, dim3(n), dim3(32 * kWarps), 0, st, a, g, splits, part, items);
   });
   if (e != cudaSuccess || splits == 1) return e;
   return launch_attn_join(a, splits, part, false, st);
@@ -482,9 +484,9 @@ cudaError_t launch_attn_rows_backward(const AttnArgs& a, cudaStream_t st) {
     constexpr int NV = decltype(nv)::value;
     constexpr bool V = decltype(v)::value;
     const int nq = (int)(gq * heads), nk = (int)(gk * heads);
-    if (nq) k_attn_rows_backward<NV, V, R, false><<<blocks_for(a, nq), 32 * kWarps, 0, st>>>(a, (int)gq, nq);
-    if (nk) k_attn_rows_backward<NV, V, R, true><<<blocks_for(a, nk), 32 * kWarps, 0, st>>>(a, (int)gk, nk);
-    return cudaGetLastError();
+    if (!(nq + (int64_t)nk)) return cudaSuccess;
+    return launch_pdl(k_attn_rows_backward<NV, V, R>, dim3(blocks_for(a, nq + (int64_t)nk)), dim3(32 * kWarps), 0, st, a,
+                      (int)gq, nq, (int)gk, nk);
   });
 }
 

@@ -35,6 +35,7 @@ DCT_DEV uint32_t lane_bits(int warp) { return (uint32_t)(warp & 3) * 32u << 16; 
 struct Tiles {
   uint8_t* p[4];               // q, k, v, dout
   AttnStats* stats;            // [heads]
+  uint32_t* any;               // set where a head cannot be split
   float *lse2, *delta;         // [heads][padded rows], backward: log2 units, 2^eds delta
   int64_t tiles[4];            // of a head
   int blocks;                  // of 64 features
@@ -69,7 +70,8 @@ DCT_DEV void store_features(float* row, int first, int dim, bool vec, const floa
 // ---------------------------------------------------------------------------
 constexpr int kScanRows = 64;
 
-// blocks [tensor][head][64 rows]; a warp takes every eighth row
+// blocks [tensor][head][64 rows]; a warp takes four rows at a time, a lane four features
+template <bool VEC>
 __global__ void __launch_bounds__(256) k_attn_scan(const __grid_constant__ AttnArgs a, AttnStats* stats, int per_q,
                                                    int per_k, int backward) {
   __shared__ uint32_t sh[3];
@@ -86,25 +88,35 @@ __global__ void __launch_bounds__(256) k_attn_scan(const __grid_constant__ AttnA
   if (threadIdx.x < 3) sh[threadIdx.x] = 0;
   __syncthreads();
   uint32_t top = 0, low = 0, norm = 0;
-  for (int r = r0 + (threadIdx.x >> 5); r < rows; r += 8) {
-    const float* p = row_of(a, t, b, hk, r);
-    float v[4];
-    uint32_t m = 0;
+  for (int r = r0 + (threadIdx.x >> 5) * 4; r < rows; r += 32) {
+    float v[4][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = lane + 32 * e < a.dim ? p[lane + 32 * e] : 0.f;
-      m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
+    for (int u = 0; u < 4; ++u) {
+      const float* p = row_of(a, t, b, hk, min(r + u, rows - 1)) + 4 * lane;
+      if constexpr (VEC) {
+        *reinterpret_cast<float4*>(v[u]) =
+            4 * lane < a.dim ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[u][e] = 4 * lane + e < a.dim ? p[e] : 0.f;
+      }
     }
-    m = __reduce_max_sync(0xffffffffu, m);
-    top = max(top, m);
-    if (m) low = max(low, ~m);
-    if (backward && t >= 2 && m && m < 0x7f800000u) {
-      // the norm through the row's own scale, so that squares neither vanish nor overflow
-      const float f = __uint_as_float(m);
-      float s = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s = fmaf(v[e] / f, v[e] / f, s);
-      norm = max(norm, __float_as_uint(1.001f * f * sqrtf(warp_sum_f(s))));
+    for (int u = 0; u < 4; ++u) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(v[u][e]) & 0x7fffffffu);
+      m = __reduce_max_sync(0xffffffffu, m);
+      top = max(top, m);
+      if (m) low = max(low, ~m);
+      if (backward && t >= 2 && m && m < 0x7f800000u) {
+        // the norm through the row's own scale, so that squares neither vanish nor overflow
+        const float f = __uint_as_float(m), g = 1.f / f;
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = fmaf(v[u][e] * g, v[u][e] * g, s);
+        norm = max(norm, __float_as_uint(1.001f * f * sqrtf(warp_sum_f(s))));
+      }
     }
   }
   if (lane == 0) {
@@ -126,6 +138,7 @@ template <int BLOCKS>
 __global__ void __launch_bounds__(128 * BLOCKS) k_attn_split(const __grid_constant__ AttnArgs a,
                                                              const __grid_constant__ Tiles w, int tq, int tk,
                                                              int backward, bool vec) {
+  pdl_entry();
   const int heads = a.batch * a.kv_heads;
   int x = blockIdx.x, t = 0;
   for (; t < 3; ++t) {
@@ -138,6 +151,7 @@ __global__ void __launch_bounds__(128 * BLOCKS) k_attn_split(const __grid_consta
   const AttnSpan span(a, b);
   const bool in = r < rows_of(a, span, t);
   const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, backward);
+  if (!sc.split && threadIdx.x == 0) *w.any = 1;  // work for the float32 kernels
   if (!sc.split && t != 3) return;
   float v[8] = {};
   if (in) {
@@ -188,292 +202,22 @@ __global__ void __launch_bounds__(128 * BLOCKS) k_attn_split(const __grid_consta
 }
 
 // ---------------------------------------------------------------------------
-// forward
+// what the three kernels share
 // ---------------------------------------------------------------------------
-constexpr int kSoft = 8;                           // softmax warps: two threads a row
+// 16 warps compute, four threads a row of 128 (warp w holds rows 32 (w & 3) .. and quarter
+// w >> 2 of the columns); warp 16 loads, warp 17 issues the matrix instructions.  Four warps
+// a scheduler hide the latencies that one phase after the other has (two a scheduler left
+// the tensor cores busy 38 to 47% of the time).  The inner side comes in half tiles of 64
+// rows, so that the next ones arrive while these are used.  The operand that rests lies in
+// tensor memory where there is room, which spares shared memory its bandwidth.
+constexpr int kSoft = 16;
 constexpr int kThreads = 32 * (kSoft + 2);
-// P is held as 2^7 P: a weight is at most 1, and hi + lo reach 2^-32 of it
-constexpr float kUp = 7.f;
-
-template <int BLOCKS>
-struct Forward {
-  static constexpr int kD = 64 * BLOCKS;
-  static constexpr uint32_t kTileBytes = BLOCKS * kBlockBytes;
-  static constexpr int kSlots = BLOCKS == 1 ? 4 : 2;         // K and V tiles in turn
-  static constexpr size_t kSmem = 1024 + (1 + kSlots) * (size_t)kTileBytes;
-};
-
-DCT_DEV void pair_sync(int warp) {                 // warps w and w + 4, which share rows
-  asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
-}
-
-// One tile of 128 rows of a key head against its keys, 128 at a time.
-//
-// Warps 0..7 hold the softmax: thread (row, half) takes 64 of the 128 scores of its row and
-// half of its output features.  The scores of the next tile are formed while they work, and
-// each tile's P V is drained into registers, where the outputs are scaled when the running
-// maximum moves: no accumulator lives longer than one tile, so the tensor cores' rounding
-// toward zero does not build up.  P goes back into the scores' place in tensor memory as
-// the product's operand.  Warp 8 loads, warp 9 issues.
-template <int BLOCKS>
-__global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_constant__ AttnArgs a,
-                                                              const __grid_constant__ Tiles w, int row_tiles,
-                                                              int splits, float* part, bool vec_out, uint32_t* err) {
-  using S = Forward<BLOCKS>;
-  constexpr int kO = S::kD / 2;                    // output features of a thread
-  extern __shared__ uint8_t raw[];
-  uint8_t* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-  __shared__ uint64_t q_full, full[S::kSlots], empty[S::kSlots], s_full[2], p_full[2], o_full[2], o_empty[2];
-  __shared__ uint32_t tmem_base;
-  __shared__ float exch[2][2][kTile];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads;
-  const int split = blockIdx.x / heads % splits, tile = row_tiles - 1 - blockIdx.x / heads / splits;  // long rows first
-  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, false);
-  if (!sc.split) return;
-  const AttnSpan span(a, b);
-  const int rows = a.q_len * a.group, r0 = tile * kTile;
-  // keys of the tile's rows
-  const int i0 = r0 / a.group, i1 = min(min(r0 + kTile, rows) - 1, span.m * a.group - 1) / a.group;
-  int k0 = 0, k1 = 0;
-  if (i0 < span.m) {
-    k0 = span.lo(a, i0);
-    k1 = span.hi(a, i1);
-  }
-  int t0 = k0 / kTile, t1 = k1 > k0 ? (k1 + kTile - 1) / kTile : t0;
-  if (splits > 1) {
-    const int per = (t1 - t0 + splits - 1) / splits;
-    const int from = min(t1, t0 + split * per);
-    t1 = min(t1, from + per);
-    t0 = from;
-  }
-  const int n = t1 - t0;
-
-  if (threadIdx.x == 0) {
-    mbar_init(&q_full, 1);
-    for (int s = 0; s < S::kSlots; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 32 * kSoft);
-      mbar_init(&o_full[s], 1);
-      mbar_init(&o_empty[s], 32 * kSoft);
-    }
-    mbar_fence_init();
-  }
-  if (warp == kSoft + 1) tmem_alloc(&tmem_base, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = tmem_base, tmem_o = tmem + 256;
-
-  if (warp == kSoft) {
-    if (lane == 0 && n) {
-      auto load = [&](uint8_t* to, int t, int64_t index, uint64_t* bar) {
-        mbar_arrive_expect_tx(bar, S::kTileBytes);
-        const uint8_t* from = w.p[t] + (bh * w.tiles[t] + index) * (int64_t)S::kTileBytes;
-#pragma unroll
-        for (uint32_t o = 0; o < S::kTileBytes; o += kBlockBytes / 2)
-          bulk_load(to + o, from + o, kBlockBytes / 2, bar);
-      };
-      load(sm, 0, tile, &q_full);
-      bool ok = true;
-      int it = 0;
-      for (; it < 2 * n; ++it) {
-        const int s = it % S::kSlots;
-        ok = mbar_wait(&empty[s], ((it / S::kSlots) & 1) ^ 1, err);
-        if (!ok) break;
-        load(sm + (1 + s) * S::kTileBytes, 1 + (it & 1), t0 + it / 2, &full[s]);
-      }
-      mbar_wait(&q_full, 0, err);                  // every copy has landed before the block ends
-      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&full[u % S::kSlots], (u / S::kSlots) & 1, err);
-    }
-  } else if (warp == kSoft + 1) {
-    if (lane == 0 && n) {
-      constexpr uint32_t id_s = umma_idesc(kTile, kTile, false, false), id_o = umma_idesc(kTile, S::kD, false, true);
-      constexpr uint64_t lo = kBlockBytes / 32;    // from hi to lo, in descriptor units
-      bool ok = mbar_wait(&q_full, 0, err);
-      const uint64_t q = umma_desc(smem_addr(sm), kChunkBytes, 1024);
-      auto scores = [&](int j) {                   // S(j) = Q K(j)^T
-        const int it = 2 * j, s = it % S::kSlots;
-        ok = ok && mbar_wait(&full[s], (it / S::kSlots) & 1, err);
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t k = umma_desc(smem_addr(sm + (1 + s) * S::kTileBytes), kChunkBytes, 1024);
-        const uint32_t d = tmem + (j & 1) * kTile;
-        auto step = [](int c) { return (uint64_t)((c >> 2) * (kBlockBytes / 16) + (c & 3) * 2); };
-#pragma unroll
-        for (int c = 0; c < 4 * BLOCKS; ++c) {     // the small products first
-          umma(d, q + lo + step(c), k + step(c), id_s, c != 0);
-          umma(d, q + step(c), k + lo + step(c), id_s, true);
-        }
-#pragma unroll
-        for (int c = 0; c < 4 * BLOCKS; ++c) umma(d, q + step(c), k + step(c), id_s, true);
-        umma_commit(&empty[s]);
-        umma_commit(&s_full[j & 1]);
-      };
-      scores(0);
-      for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n) scores(j + 1);
-        const int it = 2 * j + 1, s = it % S::kSlots, buf = j & 1;
-        ok = ok && mbar_wait(&p_full[buf], (j >> 1) & 1, err);
-        ok = ok && mbar_wait(&o_empty[buf], ((j >> 1) & 1) ^ 1, err);
-        ok = ok && mbar_wait(&full[s], (it / S::kSlots) & 1, err);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t v = umma_desc(smem_addr(sm + (1 + s) * S::kTileBytes), kBlockBytes, 1024);
-        const uint32_t p = tmem + buf * kTile, d = tmem_o + buf * S::kD;
-        // 16 keys: 8 columns of P, halves of 64 keys holding 32 columns hi, then 32 lo
-        auto pat = [&](int c) { return p + (c >> 2) * 64 + (c & 3) * 8; };
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          umma_ts(d, pat(c) + 32, v + c * 128, id_o, c != 0);
-          umma_ts(d, pat(c), v + lo + c * 128, id_o, true);
-        }
-#pragma unroll
-        for (int c = 0; c < 8; ++c) umma_ts(d, pat(c), v + c * 128, id_o, true);
-        umma_commit(&empty[s]);
-        umma_commit(&o_full[buf]);
-      }
-    }
-  } else {
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
-    const RowAt at_row(a, hk, min(r, rows - 1));
-    const bool in = r < rows && at_row.i < span.m;
-    const int lo = in ? span.lo(a, at_row.i) : 0, hi = in ? span.hi(a, at_row.i) : 0;
-    // (not 0: a masked score is infinite, and times 0 it would not be)
-    const float f = copysignf(fmaxf(fabsf(ldexpf(a.scale * kLog2e, -(sc.e[0] + sc.e[1]))), 1e-36f), a.scale);
-    float o[kO], top = -INFINITY, sum = 0.f, scale_o = 1.f;
-#pragma unroll
-    for (int e = 0; e < kO; ++e) o[e] = 0.f;
-    // once a wait has run out the loop goes on without waiting: the other warp of a row
-    // still counts on meeting this one
-    bool ok = true;
-    auto take = [&](int j) {                       // adds P V of tile j
-      const int buf = j & 1;
-      ok = ok && mbar_wait(&o_full[buf], (j >> 1) & 1, err);
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < kO; c += 32) {
-        uint32_t v[32];
-        tmem_load32(tmem_o + lane_bits(warp) + buf * S::kD + half * kO + c, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[c + e] = fmaf(o[c + e], scale_o, __uint_as_float(v[e]));
-      }
-      tc_fence_before();
-      mbar_arrive(&o_empty[buf]);
-    };
-    for (int j = 0; j < n; ++j) {
-      const int buf = j & 1, key = (t0 + j) * kTile + half * 64;
-      ok = ok && mbar_wait(&s_full[buf], (j >> 1) & 1, err);
-      tc_fence_after();
-      const uint32_t addr = tmem + lane_bits(warp) + buf * kTile + half * 64;
-      uint32_t x[64];
-      tmem_load32(addr, *reinterpret_cast<uint32_t(*)[32]>(x));
-      tmem_load32(addr + 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32));
-      tmem_wait_ld();
-      float best = -INFINITY;
-      if (__any_sync(0xffffffffu, key < lo || key + 64 > hi)) {
-#pragma unroll
-        for (int e = 0; e < 64; ++e)
-          if (key + e < lo || key + e >= hi) x[e] = __float_as_uint(f < 0.f ? INFINITY : -INFINITY);
-      }
-      // the largest of f x: a negative scale turns the order
-      if (f >= 0.f) {
-#pragma unroll
-        for (int e = 0; e < 64; ++e) best = fmaxf(best, __uint_as_float(x[e]));
-        best = best == -INFINITY ? best : best * f;
-      } else {
-        best = INFINITY;
-#pragma unroll
-        for (int e = 0; e < 64; ++e) best = fminf(best, __uint_as_float(x[e]));
-        best = best == INFINITY ? -INFINITY : best * f;
-      }
-      exch[j & 1][half][row] = best;
-      pair_sync(warp);
-      const float next = fmaxf(top, fmaxf(best, exch[j & 1][half ^ 1][row]));
-      const float base = next == -INFINITY ? 0.f : next;       // nothing seen yet: every weight is 0
-      const float move = ex2(top - base);
-      top = next;
-      sum *= move;
-#pragma unroll
-      for (int c = 0; c < 64; c += 32) {
-        uint32_t h[16], l[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p0 = ex2(fmaf(__uint_as_float(x[c + 2 * e]), f, kUp - base));
-          const float p1 = ex2(fmaf(__uint_as_float(x[c + 2 * e + 1]), f, kUp - base));
-          sum += p0 + p1;
-          split2(p0, p1, h[e], l[e]);
-        }
-        tmem_store16(addr + c / 2, h);
-        tmem_store16(addr + 32 + c / 2, l);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&p_full[buf]);
-      if (j) take(j - 1);
-      scale_o = move;
-    }
-    if (n) take(n - 1);
-    // the two halves of a row meet
-    pair_sync(warp);
-    exch[0][half][row] = sum;
-    pair_sync(warp);
-    sum += exch[0][half ^ 1][row];
-    if (ok && r < rows) {
-      float back = ldexpf(1.f, -sc.e[2]);
-      if (splits > 1) {
-        const float down = exp2f(-kUp);
-        back *= down;
-        float* rec = part + (((int64_t)bh * rows + r) * splits + split) * (a.dim + 2);
-#pragma unroll
-        for (int e = 0; e < kO; ++e)
-          if (half * kO + e < a.dim) rec[half * kO + e] = o[e] * back;
-        if (half == 0) {
-          rec[a.dim] = top;
-          rec[a.dim + 1] = sum * down;
-        }
-      } else {
-        float* out = a.out + at(a.os, b, at_row.i, at_row.h);
-        const float inv = sum == 0.f ? 0.f : back / sum;
-#pragma unroll
-        for (int e = 0; e < kO; ++e) o[e] *= inv;
-        store_features<kO>(out, half * kO, a.dim, vec_out, o);
-        if (half == 0 && a.lse)
-          a.lse[((int64_t)b * a.q_heads + at_row.h) * a.q_len + at_row.i] =
-              sum == 0.f ? -INFINITY : fmaf(top, kLn2, logf(sum * exp2f(-kUp)));
-      }
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  if (warp == kSoft + 1) tmem_free(tmem, 512);
-}
-
-// ---------------------------------------------------------------------------
-// backward
-// ---------------------------------------------------------------------------
-// Two kernels that each form the scores and dP = dout V^T again, one for dq (a tile of rows
-// against its keys) and one for dk and dv (a tile of keys against the rows that see them):
-// seven products instead of five, but every gradient has one owner, no atomics and one
-// order.  The inner side goes in half tiles of 64, since the resident operands take most of
-// shared memory; one of them lives in tensor memory instead, where the matrix instructions
-// read it beside shared memory's 128 bytes a cycle, which bound them otherwise.
 constexpr int kHalf = 64;
-constexpr float kUpP = 14.f;                       // P <= 1 is held as 2^14 P
 
 template <int BLOCKS>
-struct Backward {
-  static constexpr int kD = 64 * BLOCKS, kF = kD / 2;              // features, of them a thread's
+struct Sizes {
+  static constexpr int kD = 64 * BLOCKS, kF = kD / 4;              // features, of them a thread's
   static constexpr uint32_t kTileBytes = BLOCKS * kBlockBytes, kSlotBytes = kTileBytes / 2;
-  static constexpr int kSlots = BLOCKS == 1 ? 8 : 5;
-  static constexpr size_t kSmem = 1024 + kTileBytes + (size_t)kSlots * kSlotBytes;
 };
 
 // half tile `h` (64 rows) of operand t: [64 features][hi, lo][64 rows][64 float16]
@@ -483,30 +227,37 @@ DCT_DEV void load_half(const Tiles& w, int bh, int t, int64_t h, uint8_t* to, ui
 #pragma unroll
   for (int i = 0; i < 2 * BLOCKS; ++i) bulk_load(to + i * kChunkBytes, from + i * 2 * kChunkBytes, kChunkBytes, bar);
 }
-
-// A thread's row of a whole tile into tensor memory as an operand: columns of hi, then of lo.
-// Warps w and w + 4 take the halves of the features.
+// a whole tile as it lies
 template <int BLOCKS>
-DCT_DEV void tile_to_tmem(const uint8_t* tile, uint32_t addr, int warp, int row) {
-  constexpr int kGroups = 4 * BLOCKS;              // of 8 features, a thread's
-  const int g0 = (warp >> 2) * kGroups;
+DCT_DEV void load_tile(const Tiles& w, int bh, int t, int64_t tile, uint8_t* to, uint64_t* bar) {
+  const uint8_t* from = w.p[t] + (bh * w.tiles[t] + tile) * (int64_t)(BLOCKS * kBlockBytes);
 #pragma unroll
-  for (int low = 0; low < 2; ++low)
-#pragma unroll
-    for (int g = 0; g < kGroups; g += 4) {
-      uint32_t r[16];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int f = g0 + g + e;
-        const uint4 v = *reinterpret_cast<const uint4*>(tile + (f >> 3) * kBlockBytes + low * (kBlockBytes / 2) +
-                                                        chunk_at(row, f & 7));
-        r[4 * e] = v.x; r[4 * e + 1] = v.y; r[4 * e + 2] = v.z; r[4 * e + 3] = v.w;
-      }
-      tmem_store16(addr + lane_bits(warp) + low * 32 * BLOCKS + (g0 + g) * 4, r);
-    }
+  for (uint32_t o = 0; o < BLOCKS * kBlockBytes; o += kBlockBytes / 2)
+    bulk_load(to + o, from + o, kBlockBytes / 2, bar);
 }
 
-// D = A B^T over the features: A a whole tile in shared memory, B a half tile
+// A thread's quarter of its row of a whole tile into tensor memory as an operand: columns of
+// hi, then of lo.
+template <int BLOCKS>
+DCT_DEV void tile_to_tmem(const uint8_t* tile, uint32_t addr, int warp, int row) {
+  constexpr int kGroups = 2 * BLOCKS;              // of 8 features, a thread's
+  const int g0 = (warp >> 2) * kGroups;
+#pragma unroll
+  for (int low = 0; low < 2; ++low) {
+    uint32_t r[4 * kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int f = g0 + g;
+      const uint4 v = *reinterpret_cast<const uint4*>(tile + (f >> 3) * kBlockBytes + low * (kBlockBytes / 2) +
+                                                      chunk_at(row, f & 7));
+      r[4 * g] = v.x; r[4 * g + 1] = v.y; r[4 * g + 2] = v.z; r[4 * g + 3] = v.w;
+    }
+    tmem_store(addr + lane_bits(warp) + low * 32 * BLOCKS + g0 * 4, r);
+  }
+}
+
+// D = A B^T over the features: A a whole tile in shared memory, B a half tile.  The small
+// products come first: every matrix instruction rounds its sum toward zero.
 template <int BLOCKS>
 DCT_DEV void mma_features_ss(uint32_t d, uint64_t a, uint64_t b) {
   constexpr uint32_t id = umma_idesc(kTile, kHalf, false, false);
@@ -535,45 +286,309 @@ DCT_DEV void mma_features_ts(uint32_t d, uint32_t a, uint64_t b) {
 #pragma unroll
   for (int c = 0; c < 4 * BLOCKS; ++c) umma_ts(d, a + 8 * c, b + sb(c), id, true);
 }
-// D (+)= A B over 64 rows: A in tensor memory (for each 32 of them 16 columns hi, 16 lo), B
-// a half tile with its rows as the contraction
-template <int BLOCKS>
+// D (+)= A B over 64 rows: A in tensor memory, for each Q rows Q/2 columns of hi and Q/2 of
+// lo (store_operand); B a half tile with its rows as the contraction
+template <int BLOCKS, int Q>
 DCT_DEV void mma_rows(uint32_t d, uint32_t a, uint64_t b, bool add) {
   constexpr uint32_t id = umma_idesc(kTile, 64 * BLOCKS, false, true);
   constexpr uint64_t lo_b = kChunkBytes / 16;
-  auto sa = [](int c) { return (uint32_t)((c >> 1) * 32 + (c & 1) * 8); };
+  auto sa = [](int c) { return (uint32_t)(16 * c / Q * Q + 16 * c % Q / 2); };
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    umma_ts(d, a + 16 + sa(c), b + c * 128, id, add || c != 0);
+    umma_ts(d, a + Q / 2 + sa(c), b + c * 128, id, add || c != 0);
     umma_ts(d, a + sa(c), b + lo_b + c * 128, id, true);
   }
 #pragma unroll
   for (int c = 0; c < 4; ++c) umma_ts(d, a + sa(c), b + c * 128, id, true);
 }
 
-// 32 values as an operand's columns, 16 of hi and 16 of lo
-DCT_DEV void store_operand(uint32_t addr, const float (&x)[32]) {
-  uint32_t h[16], l[16];
+// Q values as an operand's columns
+template <int Q>
+DCT_DEV void store_operand(uint32_t addr, const float (&x)[Q]) {
+  uint32_t h[Q / 2], l[Q / 2];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) split2(x[2 * e], x[2 * e + 1], h[e], l[e]);
-  tmem_store16(addr, h);
-  tmem_store16(addr + 16, l);
+  for (int e = 0; e < Q / 2; ++e) split2(x[2 * e], x[2 * e + 1], h[e], l[e]);
+  tmem_store(addr, h);
+  tmem_store(addr + Q / 2, l);
 }
 
-// acc += 32 columns at a time
+// a warp's arrival after its accesses to tensor memory
+DCT_DEV void arrive_warp(uint64_t* bar) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// Bounded waits of one warp or thread.  After one has run out the others are passed over, and
+// the loops go on to their ends: whoever still counts on meeting this one must not wait.
+struct Waits {
+  uint32_t* err;
+  bool ok = true;
+  DCT_DEV bool operator()(uint64_t* bar, int phase) {
+    ok = ok && mbar_wait(bar, phase & 1, err);
+    tc_fence_after();
+    return ok;
+  }
+};
+
+// shared memory: tiles first (1024-byte aligned), then the kernel's barriers and vectors
+DCT_DEV bool misaligned(const uint8_t* sm, uint32_t* err) {
+  if ((smem_addr(sm) & 1023) == 0) return false;
+  if (err && threadIdx.x == 0) atomicOr(err, DCT_DEVERR_WAIT_TIMEOUT);
+  return true;
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+// P is held as 2^7 P: a weight is at most 1, and hi + lo reach 2^-32 of it
+constexpr float kUp = 7.f;
+
+template <int BLOCKS>
+struct Forward : Sizes<BLOCKS> {
+  static constexpr int kSlots = BLOCKS == 1 ? 12 : 7;
+  struct Control {
+    uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], o_full, o_empty;
+    uint32_t tmem;
+    float exch[4][kTile];
+  };
+  static constexpr size_t kSmem = (size_t)kSlots * Sizes<BLOCKS>::kSlotBytes + sizeof(Control);
+};
+
+DCT_DEV void rows_sync(int warp) {                 // the four warps that share rows
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + (warp & 3)) : "memory");
+}
+
+// One tile of 128 rows of a key head against its keys, 128 at a time: softmax(Q K^T) V with
+// the running maximum and sum.  The next scores are formed while the warps work on these;
+// each tile's P V is drained into registers, where the outputs are scaled when the maximum
+// moves, so no accumulator lives longer than one tile and the tensor cores' rounding toward
+// zero does not build up.  P goes back into the scores' place as the product's operand.
+template <int BLOCKS>
+__global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_constant__ AttnArgs a,
+                                                              const __grid_constant__ Tiles w, int row_tiles,
+                                                              int splits, float* part, bool vec_out, uint32_t* err) {
+  using S = Forward<BLOCKS>;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  auto& ctl = *reinterpret_cast<typename S::Control*>(sm + S::kSlots * S::kSlotBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (misaligned(sm, err)) return;
+  if (threadIdx.x == 0) {
+    mbar_init(&ctl.q_full, kSoft);
+    for (int s = 0; s < S::kSlots; ++s) {
+      mbar_init(&ctl.full[s], 1);
+      mbar_init(&ctl.empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&ctl.s_full[s], 1);
+      mbar_init(&ctl.p_full[s], kSoft);
+    }
+    mbar_init(&ctl.o_full, 1);
+    mbar_init(&ctl.o_empty, kSoft);
+    mbar_fence_init();
+  }
+  if (warp == kSoft + 1) tmem_alloc(&ctl.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // S twice, P V, the operand Q
+  const uint32_t tm_s = ctl.tmem, tm_o = tm_s + 256, tm_q = tm_s + 384;
+  pdl_entry();
+  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads;
+  const int split = blockIdx.x / heads % splits, tile = row_tiles - 1 - blockIdx.x / heads / splits;  // long rows first
+  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, false);
+  const AttnSpan span(a, b);
+  const int rows = a.q_len * a.group, r0 = tile * kTile;
+  // keys of the tile's rows
+  const int i0 = r0 / a.group, i1 = min(min(r0 + kTile, rows) - 1, span.m * a.group - 1) / a.group;
+  int t0 = 0, n = 0;
+  if (sc.split && i0 < span.m) {
+    const int k0 = span.lo(a, i0), k1 = span.hi(a, i1);
+    t0 = k0 / kTile;
+    int t1 = k1 > k0 ? (k1 + kTile - 1) / kTile : t0;
+    if (splits > 1) {
+      const int per = (t1 - t0 + splits - 1) / splits;
+      const int from = min(t1, t0 + split * per);
+      t1 = min(t1, from + per);
+      t0 = from;
+    }
+    n = t1 - t0;
+  }
+  Waits wait{err};
+
+  if (warp == kSoft) {
+    if (lane == 0) {
+      int it = 0;
+      for (; it < 4 * n; ++it) {                   // K in halves, V in halves
+        const int s = it % S::kSlots;
+        if (!wait(&ctl.empty[s], (it / S::kSlots) ^ 1)) break;
+        mbar_arrive_expect_tx(&ctl.full[s], S::kSlotBytes);
+        load_half<BLOCKS>(w, bh, 1 + ((it >> 1) & 1), 2 * (t0 + it / 4) + (it & 1), sm + s * S::kSlotBytes,
+                          &ctl.full[s]);
+      }
+      // every copy has landed before the block ends
+      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&ctl.full[u % S::kSlots], (u / S::kSlots) & 1, err);
+    }
+  } else if (warp == kSoft + 1) {
+    if (lane == 0 && n) {
+      wait(&ctl.q_full, 0);
+      auto slot = [&](int it) { return smem_addr(sm + it % S::kSlots * S::kSlotBytes); };
+      auto scores = [&](int j) {                   // S(j) = Q K(j)^T
+        for (int h = 0; h < 2; ++h) {
+          const int it = 4 * j + h;
+          if (!wait(&ctl.full[it % S::kSlots], it / S::kSlots)) return;
+          mma_features_ts<BLOCKS>(tm_s + (j & 1) * kTile + h * kHalf, tm_q, umma_desc(slot(it), kChunkBytes, 1024));
+          umma_commit(&ctl.empty[it % S::kSlots]);
+        }
+        umma_commit(&ctl.s_full[j & 1]);
+      };
+      scores(0);
+      for (int j = 0; j < n && wait.ok; ++j) {
+        if (j + 1 < n) scores(j + 1);
+        wait(&ctl.p_full[j & 1], j >> 1);
+        wait(&ctl.o_empty, j ^ 1);
+        for (int h = 0; h < 2; ++h) {
+          const int it = 4 * j + 2 + h;
+          if (!wait(&ctl.full[it % S::kSlots], it / S::kSlots)) break;
+          mma_rows<BLOCKS, 32>(tm_o, tm_s + (j & 1) * kTile + h * kHalf, umma_desc(slot(it), 2 * kChunkBytes, 1024), h);
+          umma_commit(&ctl.empty[it % S::kSlots]);
+        }
+        umma_commit(&ctl.o_full);
+      }
+    }
+  } else if (sc.split) {
+    const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
+    const RowAt at_row(a, hk, min(r, rows - 1));
+    const bool in = r < rows && at_row.i < span.m;
+    const int lo = in ? span.lo(a, at_row.i) : 0, hi = in ? span.hi(a, at_row.i) : 0;
+    // (not 0: a masked score is infinite, and times 0 it would not be)
+    const float f = copysignf(fmaxf(fabsf(ldexpf(a.scale * kLog2e, -(sc.e[0] + sc.e[1]))), 1e-36f), a.scale);
+    const float hidden = f < 0.f ? INFINITY : -INFINITY;
+    float o[S::kF], top = -INFINITY, sum = 0.f, scale_o = 1.f;
+#pragma unroll
+    for (int e = 0; e < S::kF; ++e) o[e] = 0.f;
+    if (n) {
+      tile_to_tmem<BLOCKS>(w.p[0] + (bh * w.tiles[0] + tile) * (int64_t)S::kTileBytes, tm_q, warp, row);
+      tmem_wait_st();
+      arrive_warp(&ctl.q_full);
+    }
+    auto take = [&](int j) {                       // adds P V of tile j
+      wait(&ctl.o_full, j);
+      uint32_t v[S::kF];
+      tmem_load(tm_o + lane_bits(warp) + quarter * S::kF, v);
+      tmem_wait_ld();
+      arrive_warp(&ctl.o_empty);
+#pragma unroll
+      for (int e = 0; e < S::kF; ++e) o[e] = fmaf(o[e], scale_o, __uint_as_float(v[e]));
+    };
+    for (int j = 0; j < n; ++j) {
+      const int key = (t0 + j) * kTile + quarter * 32;
+      wait(&ctl.s_full[j & 1], j >> 1);
+      const uint32_t addr = tm_s + lane_bits(warp) + (j & 1) * kTile + quarter * 32;
+      uint32_t x[32];
+      tmem_load32(addr, x);
+      tmem_wait_ld();
+      if (__any_sync(0xffffffffu, key < lo || key + 32 > hi)) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (key + e < lo || key + e >= hi) x[e] = __float_as_uint(hidden);
+      }
+      // the largest of f x: a negative scale turns the order
+      float best = __uint_as_float(x[0]);
+      if (f >= 0.f) {
+#pragma unroll
+        for (int e = 1; e < 32; ++e) best = fmaxf(best, __uint_as_float(x[e]));
+      } else {
+#pragma unroll
+        for (int e = 1; e < 32; ++e) best = fminf(best, __uint_as_float(x[e]));
+      }
+      ctl.exch[quarter][row] = best * f;
+      rows_sync(warp);
+      float next = fmaxf(fmaxf(ctl.exch[0][row], ctl.exch[1][row]), fmaxf(ctl.exch[2][row], ctl.exch[3][row]));
+      rows_sync(warp);
+      next = fmaxf(top, next);
+      const float base = next == -INFINITY ? 0.f : next;       // nothing seen yet: every weight is 0
+      const float move = ex2(top - base), up = kUp - base;
+      top = next;
+      float p[32], s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        p[e] = ex2(fmaf(__uint_as_float(x[e]), f, up));
+        p[e + 1] = ex2(fmaf(__uint_as_float(x[e + 1]), f, up));
+        s0 += p[e];
+        s1 += p[e + 1];
+      }
+      store_operand<32>(addr, p);
+      sum = fmaf(sum, move, s0 + s1);
+      tmem_wait_st();
+      arrive_warp(&ctl.p_full[j & 1]);
+      if (j) take(j - 1);
+      scale_o = move;
+    }
+    if (n) take(n - 1);
+    // the four quarters of a row meet
+    ctl.exch[quarter][row] = sum;
+    rows_sync(warp);
+    sum = (ctl.exch[0][row] + ctl.exch[1][row]) + (ctl.exch[2][row] + ctl.exch[3][row]);
+    if (wait.ok && r < rows) {
+      float back = ldexpf(1.f, -sc.e[2]);
+      const float down = exp2f(-kUp);
+      if (splits > 1) {
+        float* rec = part + (((int64_t)bh * rows + r) * splits + split) * (a.dim + 2);
+        back *= down;
+#pragma unroll
+        for (int e = 0; e < S::kF; ++e)
+          if (quarter * S::kF + e < a.dim) rec[quarter * S::kF + e] = o[e] * back;
+        if (quarter == 0) {
+          rec[a.dim] = top;
+          rec[a.dim + 1] = sum * down;
+        }
+      } else {
+        const float inv = sum == 0.f ? 0.f : back / sum;
+#pragma unroll
+        for (int e = 0; e < S::kF; ++e) o[e] *= inv;
+        store_features<S::kF>(a.out + at(a.os, b, at_row.i, at_row.h), quarter * S::kF, a.dim, vec_out, o);
+        if (quarter == 0 && a.lse)
+          a.lse[((int64_t)b * a.q_heads + at_row.h) * a.q_len + at_row.i] =
+              sum == 0.f ? -INFINITY : fmaf(top, kLn2, logf(sum * down));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kSoft + 1) tmem_free(tm_s, 512);
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+// Two kernels that each form the scores and dP = dout V^T again, one for dq (a tile of rows
+// against its keys) and one for dk and dv (a tile of keys against the rows that see them):
+// seven products instead of five, but every gradient has one owner, no atomics and one
+// order.
+constexpr float kUpP = 14.f;                       // P <= 1 is held as 2^14 P
+constexpr int kGroup = 2;                          // half tiles between drains of an accumulator
+
 template <int N>
 DCT_DEV void drain(uint32_t addr, float (&acc)[N]) {
+  uint32_t v[N];
+  tmem_load(addr, v);
+  tmem_wait_ld();
 #pragma unroll
-  for (int c = 0; c < N; c += 32) {
-    uint32_t v[32];
-    tmem_load32(addr + c, v);
-    tmem_wait_ld();
-#pragma unroll
-    for (int e = 0; e < 32; ++e) acc[c + e] += __uint_as_float(v[e]);
-  }
+  for (int e = 0; e < N; ++e) acc[e] += __uint_as_float(v[e]);
 }
 
-constexpr int kGroup = 2;                          // half tiles between drains of an accumulator
+template <int BLOCKS>
+struct Dq : Sizes<BLOCKS> {
+  static constexpr int kSlots = BLOCKS == 1 ? 8 : 5;
+  struct Control {
+    uint64_t q_full, go_full, full[kSlots], empty[kSlots], s_full[2], ds_full[2], acc_full, acc_empty;
+    uint32_t tmem;
+  };
+  static constexpr size_t kSmem = Sizes<BLOCKS>::kTileBytes + (size_t)kSlots * Sizes<BLOCKS>::kSlotBytes + sizeof(Control);
+};
 
 // dq of a tile of 128 rows: dS = P (dP - delta), dq = scale dS K.  Q rests in shared memory,
 // dout in tensor memory; V and K come in half tiles of 64 keys.
@@ -581,100 +596,91 @@ template <int BLOCKS>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__ AttnArgs a,
                                                          const __grid_constant__ Tiles w, int row_tiles, bool vec_out,
                                                          uint32_t* err) {
-  using S = Backward<BLOCKS>;
-  extern __shared__ uint8_t raw[];
-  uint8_t* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-  __shared__ uint64_t q_full, go_full, full[S::kSlots], empty[S::kSlots], s_full[2], ds_full[2], acc_full, acc_empty;
-  __shared__ uint32_t tmem_base;
+  using S = Dq<BLOCKS>;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  uint8_t* slots = sm + S::kTileBytes;
+  auto& ctl = *reinterpret_cast<typename S::Control*>(slots + S::kSlots * S::kSlotBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = row_tiles - 1 - blockIdx.x / heads;
-  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, true);
-  if (!sc.split) return;
-  const AttnSpan span(a, b);
-  const int rows = a.q_len * a.group, r0 = tile * kTile;
-  const int i0 = r0 / a.group, i1 = min(min(r0 + kTile, rows) - 1, span.m * a.group - 1) / a.group;
-  int t0 = 0, n = 0;
-  if (i0 < span.m) {
-    const int k0 = span.lo(a, i0), k1 = span.hi(a, i1);
-    t0 = k0 / kHalf;
-    n = k1 > k0 ? (k1 + kHalf - 1) / kHalf - t0 : 0;
-  }
+  if (misaligned(sm, err)) return;
   if (threadIdx.x == 0) {
-    mbar_init(&q_full, 1);
-    mbar_init(&go_full, 32 * kSoft);
+    mbar_init(&ctl.q_full, 1);
+    mbar_init(&ctl.go_full, kSoft);
     for (int s = 0; s < S::kSlots; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&ctl.full[s], 1);
+      mbar_init(&ctl.empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&s_full[s], 1);
-      mbar_init(&ds_full[s], 32 * kSoft);
+      mbar_init(&ctl.s_full[s], 1);
+      mbar_init(&ctl.ds_full[s], kSoft);
     }
-    mbar_init(&acc_full, 1);
-    mbar_init(&acc_empty, 32 * kSoft);
+    mbar_init(&ctl.acc_full, 1);
+    mbar_init(&ctl.acc_empty, kSoft);
     mbar_fence_init();
   }
-  if (warp == kSoft + 1) tmem_alloc(&tmem_base, 512);
+  if (warp == kSoft + 1) tmem_alloc(&ctl.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   // S and dP twice, the operand dout, the accumulator
-  const uint32_t tm_s = tmem_base, tm_dp = tm_s + 128, tm_go = tm_s + 256, tm_acc = tm_s + 384;
+  const uint32_t tm_s = ctl.tmem, tm_dp = tm_s + 128, tm_go = tm_s + 256, tm_acc = tm_s + 384;
+  pdl_entry();
+  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = row_tiles - 1 - blockIdx.x / heads;
+  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, true);
+  const AttnSpan span(a, b);
+  const int rows = a.q_len * a.group, r0 = tile * kTile;
+  const int i0 = r0 / a.group, i1 = min(min(r0 + kTile, rows) - 1, span.m * a.group - 1) / a.group;
+  int t0 = 0, n = 0;
+  if (sc.split && i0 < span.m) {
+    const int k0 = span.lo(a, i0), k1 = span.hi(a, i1);
+    t0 = k0 / kHalf;
+    n = k1 > k0 ? (k1 + kHalf - 1) / kHalf - t0 : 0;
+  }
+  Waits wait{err};
 
   if (warp == kSoft) {
     if (lane == 0 && n) {
-      mbar_arrive_expect_tx(&q_full, S::kTileBytes);
-      const uint8_t* q = w.p[0] + (bh * w.tiles[0] + tile) * (int64_t)S::kTileBytes;
-#pragma unroll
-      for (uint32_t o = 0; o < S::kTileBytes; o += kBlockBytes / 2)
-        bulk_load(sm + o, q + o, kBlockBytes / 2, &q_full);
+      mbar_arrive_expect_tx(&ctl.q_full, S::kTileBytes);
+      load_tile<BLOCKS>(w, bh, 0, tile, sm, &ctl.q_full);
       int it = 0;
-      for (; it < 2 * n; ++it) {                   // V, K, V, K ...
+      for (; it < 2 * n; ++it) {                   // K, V, K, V ...
         const int s = it % S::kSlots;
-        if (!mbar_wait(&empty[s], ((it / S::kSlots) & 1) ^ 1, err)) break;
-        mbar_arrive_expect_tx(&full[s], S::kSlotBytes);
-        load_half<BLOCKS>(w, bh, it & 1 ? 1 : 2, t0 + it / 2, sm + S::kTileBytes + s * S::kSlotBytes, &full[s]);
+        if (!wait(&ctl.empty[s], (it / S::kSlots) ^ 1)) break;
+        mbar_arrive_expect_tx(&ctl.full[s], S::kSlotBytes);
+        load_half<BLOCKS>(w, bh, it & 1 ? 2 : 1, t0 + it / 2, slots + s * S::kSlotBytes, &ctl.full[s]);
       }
-      mbar_wait(&q_full, 0, err);                  // every copy has landed before the block ends
-      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&full[u % S::kSlots], (u / S::kSlots) & 1, err);
+      mbar_wait(&ctl.q_full, 0, err);              // every copy has landed before the block ends
+      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&ctl.full[u % S::kSlots], (u / S::kSlots) & 1, err);
     }
   } else if (warp == kSoft + 1) {
     if (lane == 0 && n) {
-      bool ok = mbar_wait(&q_full, 0, err) && mbar_wait(&go_full, 0, err);
-      tc_fence_after();
+      wait(&ctl.q_full, 0);
+      wait(&ctl.go_full, 0);
       const uint64_t q = umma_desc(smem_addr(sm), kChunkBytes, 1024);
-      auto slot = [&](int it) { return smem_addr(sm + S::kTileBytes + it % S::kSlots * S::kSlotBytes); };
-      auto await = [&](int it) {
-        ok = ok && mbar_wait(&full[it % S::kSlots], (it / S::kSlots) & 1, err);
-        tc_fence_after();
-      };
+      auto slot = [&](int it) { return smem_addr(slots + it % S::kSlots * S::kSlotBytes); };
       auto scores = [&](int j) {                   // S(j) = Q K^T, dP(j) = dout V^T
-        await(2 * j + 1);
-        if (!ok) return;
-        mma_features_ss<BLOCKS>(tm_s + (j & 1) * kHalf, q, umma_desc(slot(2 * j + 1), kChunkBytes, 1024));
-        await(2 * j);
-        if (!ok) return;
-        mma_features_ts<BLOCKS>(tm_dp + (j & 1) * kHalf, tm_go, umma_desc(slot(2 * j), kChunkBytes, 1024));
-        umma_commit(&empty[2 * j % S::kSlots]);
-        umma_commit(&s_full[j & 1]);
+        const int k = 2 * j, v = k + 1;
+        if (!wait(&ctl.full[k % S::kSlots], k / S::kSlots)) return;
+        mma_features_ss<BLOCKS>(tm_s + (j & 1) * kHalf, q, umma_desc(slot(k), kChunkBytes, 1024));
+        if (!wait(&ctl.full[v % S::kSlots], v / S::kSlots)) return;
+        mma_features_ts<BLOCKS>(tm_dp + (j & 1) * kHalf, tm_go, umma_desc(slot(v), kChunkBytes, 1024));
+        umma_commit(&ctl.empty[v % S::kSlots]);
+        umma_commit(&ctl.s_full[j & 1]);
       };
       scores(0);
-      for (int j = 0; j < n && ok; ++j) {
+      for (int j = 0; j < n && wait.ok; ++j) {
         if (j + 1 < n) scores(j + 1);
-        const int group = j / kGroup;
-        ok = ok && mbar_wait(&ds_full[j & 1], (j >> 1) & 1, err);
-        if (j % kGroup == 0) ok = ok && mbar_wait(&acc_empty, (group & 1) ^ 1, err);
-        if (!ok) break;
-        tc_fence_after();
-        mma_rows<BLOCKS>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(slot(2 * j + 1), 2 * kChunkBytes, 1024),
-                         j % kGroup != 0);
-        umma_commit(&empty[(2 * j + 1) % S::kSlots]);
-        if (j % kGroup == kGroup - 1 || j == n - 1) umma_commit(&acc_full);
+        wait(&ctl.ds_full[j & 1], j >> 1);
+        if (j % kGroup == 0) wait(&ctl.acc_empty, (j / kGroup) ^ 1);
+        if (!wait.ok) break;
+        mma_rows<BLOCKS, 16>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(slot(2 * j), 2 * kChunkBytes, 1024),
+                             j % kGroup != 0);
+        umma_commit(&ctl.empty[2 * j % S::kSlots]);
+        if (j % kGroup == kGroup - 1 || j == n - 1) umma_commit(&ctl.acc_full);
       }
     }
-  } else {
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
+  } else if (sc.split) {
+    const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
     const RowAt at_row(a, hk, min(r, rows - 1));
     const bool in = r < rows && at_row.i < span.m;
     const int lo = in ? span.lo(a, at_row.i) : 0, hi = in ? span.hi(a, at_row.i) : 0;
@@ -687,38 +693,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       const float lse2 = w.lse2[at_stat], delta = w.delta[at_stat];
       tile_to_tmem<BLOCKS>(w.p[3] + (bh * w.tiles[3] + tile) * (int64_t)S::kTileBytes, tm_go, warp, row);
       tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&go_full);
-      bool ok = true;
+      arrive_warp(&ctl.go_full);
       auto take = [&](int group) {
-        ok = ok && mbar_wait(&acc_full, group & 1, err);
-        tc_fence_after();
-        drain(tm_acc + lane_bits(warp) + half * S::kF, acc);
-        tc_fence_before();
-        mbar_arrive(&acc_empty);
+        wait(&ctl.acc_full, group);
+        drain(tm_acc + lane_bits(warp) + quarter * S::kF, acc);
+        arrive_warp(&ctl.acc_empty);
       };
       for (int j = 0; j < n; ++j) {
-        const int key = (t0 + j) * kHalf + half * 32;
-        ok = ok && mbar_wait(&s_full[j & 1], (j >> 1) & 1, err);
-        tc_fence_after();
-        const uint32_t off = lane_bits(warp) + (j & 1) * kHalf + half * 32;
-        uint32_t x[32], y[32];
-        tmem_load32(tm_s + off, x);
-        tmem_load32(tm_dp + off, y);
+        const int key = (t0 + j) * kHalf + quarter * 16;
+        wait(&ctl.s_full[j & 1], j >> 1);
+        const uint32_t off = lane_bits(warp) + (j & 1) * kHalf + quarter * 16;
+        uint32_t x[16], y[16];
+        tmem_load16(tm_s + off, x);
+        tmem_load16(tm_dp + off, y);
         tmem_wait_ld();
-        float ds[32];
+        float ds[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
+        for (int e = 0; e < 16; ++e)
           ds[e] = ex2(fmaf(__uint_as_float(x[e]), f, -lse2)) * fmaf(__uint_as_float(y[e]), fd, -delta);
-        if (__any_sync(0xffffffffu, key < lo || key + 32 > hi)) {
+        if (__any_sync(0xffffffffu, key < lo || key + 16 > hi)) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
+          for (int e = 0; e < 16; ++e)
             if (key + e < lo || key + e >= hi) ds[e] = 0.f;
         }
-        store_operand(tm_s + off, ds);
+        store_operand<16>(tm_s + off, ds);
         tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&ds_full[j & 1]);
+        arrive_warp(&ctl.ds_full[j & 1]);
         if (j && j % kGroup == 0) take(j / kGroup - 1);
       }
       take((n - 1) / kGroup);
@@ -727,133 +727,134 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       const float back = ldexpf(a.scale, -(sc.eds + sc.e[1]));
 #pragma unroll
       for (int e = 0; e < S::kF; ++e) acc[e] *= back;
-      store_features<S::kF>(a.dq + at(a.dqs, b, at_row.i, at_row.h), half * S::kF, a.dim, vec_out, acc);
+      store_features<S::kF>(a.dq + at(a.dqs, b, at_row.i, at_row.h), quarter * S::kF, a.dim, vec_out, acc);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kSoft + 1) tmem_free(tmem_base, 512);
+  if (warp == kSoft + 1) tmem_free(tm_s, 512);
 }
 
-// dk and dv of a tile of 128 keys: dv = P^T dout, dk = scale dS^T Q.  K rests in shared
-// memory, V in tensor memory; Q and dout come in half tiles of 64 rows with their log-sums
-// and deltas.  A thread holds (key, half): 32 rows of the scores and half the features of
-// both gradients, 128 registers of sums, so the loading warps give registers up.
 template <int BLOCKS>
-__global__ void __launch_bounds__(384, 1) k_attn_dkv(const __grid_constant__ AttnArgs a,
-                                                     const __grid_constant__ Tiles w, int row_tiles, bool vec_out,
-                                                     uint32_t* err) {
-  using S = Backward<BLOCKS>;
-  extern __shared__ uint8_t raw[];
-  uint8_t* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-  __shared__ uint64_t k_full, v_full, full[S::kSlots], empty[S::kSlots], s_full, dp_full, p_full, ds_full, acc_full,
-      acc_empty;
+struct Dkv : Sizes<BLOCKS> {
+  static constexpr int kSlots = BLOCKS == 1 ? 8 : 5;
   // Log-sums and deltas come with Q(j) but outlive its neighbours' slots: with five slots
   // Q(j + 3) may come in after dv(j), when the log-sums of j are used, and Q(j + 4) after
   // dv(j + 1), when the deltas are; with eight, both stay until dk(j).
-  constexpr int kLse = BLOCKS == 1 ? 5 : 3, kDelta = BLOCKS == 1 ? 5 : 4;
-  __shared__ __align__(16) float vec_lse[kLse][kHalf], vec_delta[kDelta][kHalf];
-  __shared__ uint32_t tmem_base;
+  static constexpr int kLse = BLOCKS == 1 ? 5 : 3, kDelta = BLOCKS == 1 ? 5 : 4;
+  struct Control {
+    float lse[kLse][kHalf], delta[kDelta][kHalf];  // 16-byte aligned: the bulk copies' targets
+    uint64_t k_full, v_full, full[kSlots], empty[kSlots], s_full, dp_full, p_full, ds_full, acc_full, acc_empty;
+    uint32_t tmem;
+  };
+  static constexpr size_t kSmem = Sizes<BLOCKS>::kTileBytes + (size_t)kSlots * Sizes<BLOCKS>::kSlotBytes + sizeof(Control);
+};
+
+// dk and dv of a tile of 128 keys: dv = P^T dout, dk = scale dS^T Q.  K rests in shared
+// memory, V in tensor memory; Q and dout come in half tiles of 64 rows with their log-sums
+// and deltas.  A thread holds (key, quarter): 16 rows of the scores and a quarter of the
+// features of both gradients.
+template <int BLOCKS>
+__global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant__ AttnArgs a,
+                                                          const __grid_constant__ Tiles w, int row_tiles, bool vec_out,
+                                                          uint32_t* err) {
+  using S = Dkv<BLOCKS>;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  uint8_t* slots = sm + S::kTileBytes;
+  auto& ctl = *reinterpret_cast<typename S::Control*>(slots + S::kSlots * S::kSlotBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = blockIdx.x / heads;    // long ones first
-  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, true);
-  if (!sc.split) return;
-  const AttnSpan span(a, b);
-  const int j0 = tile * kTile, j1 = min(j0 + kTile, span.n) - 1;
-  int t0 = 0, n = 0;
-  if (j0 < span.n) {
-    const int first = span.first(a, j0) * a.group, last = span.last(a, j1) * a.group;
-    t0 = first / kHalf;
-    n = last > first ? (last + kHalf - 1) / kHalf - t0 : 0;
-  }
+  if (misaligned(sm, err)) return;
   if (threadIdx.x == 0) {
-    mbar_init(&k_full, 1);
-    mbar_init(&v_full, 32 * kSoft);
+    mbar_init(&ctl.k_full, 1);
+    mbar_init(&ctl.v_full, kSoft);
     for (int s = 0; s < S::kSlots; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&ctl.full[s], 1);
+      mbar_init(&ctl.empty[s], 1);
     }
-    mbar_init(&s_full, 1);
-    mbar_init(&dp_full, 1);
-    mbar_init(&p_full, 32 * kSoft);
-    mbar_init(&ds_full, 32 * kSoft);
-    mbar_init(&acc_full, 1);
-    mbar_init(&acc_empty, 32 * kSoft);
+    mbar_init(&ctl.s_full, 1);
+    mbar_init(&ctl.dp_full, 1);
+    mbar_init(&ctl.p_full, kSoft);
+    mbar_init(&ctl.ds_full, kSoft);
+    mbar_init(&ctl.acc_full, 1);
+    mbar_init(&ctl.acc_empty, kSoft);
     mbar_fence_init();
   }
-  if (warp == kSoft + 1) tmem_alloc(&tmem_base, 512);
+  if (warp == kSoft + 1) tmem_alloc(&ctl.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   // the accumulators, the operand V, S and dP (each also P's and dS's place)
-  const uint32_t tm_dk = tmem_base, tm_dv = tm_dk + 128, tm_v = tm_dk + 256, tm_s = tm_dk + 384, tm_dp = tm_dk + 448;
+  const uint32_t tm_dk = ctl.tmem, tm_dv = tm_dk + 128, tm_v = tm_dk + 256, tm_s = tm_dk + 384, tm_dp = tm_dk + 448;
+  pdl_entry();
+  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = blockIdx.x / heads;    // long ones first
+  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, true);
+  const AttnSpan span(a, b);
+  const int j0 = tile * kTile, j1 = min(j0 + kTile, span.n) - 1;
+  int t0 = 0, n = 0;
+  if (sc.split && j0 < span.n) {
+    const int first = span.first(a, j0) * a.group, last = span.last(a, j1) * a.group;
+    t0 = first / kHalf;
+    n = last > first ? (last + kHalf - 1) / kHalf - t0 : 0;
+  }
+  Waits wait{err};
 
-  if (warp >= kSoft) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == kSoft && lane == 0 && n) {
-      mbar_arrive_expect_tx(&k_full, S::kTileBytes);
-      const uint8_t* k = w.p[1] + (bh * w.tiles[1] + tile) * (int64_t)S::kTileBytes;
-#pragma unroll
-      for (uint32_t o = 0; o < S::kTileBytes; o += kBlockBytes / 2)
-        bulk_load(sm + o, k + o, kBlockBytes / 2, &k_full);
+  if (warp == kSoft) {
+    if (lane == 0 && n) {
+      mbar_arrive_expect_tx(&ctl.k_full, S::kTileBytes);
+      load_tile<BLOCKS>(w, bh, 1, tile, sm, &ctl.k_full);
       int it = 0;
       for (; it < 2 * n; ++it) {                   // Q, dout, Q, dout ...
         const int s = it % S::kSlots, j = it / 2;
-        if (!mbar_wait(&empty[s], ((it / S::kSlots) & 1) ^ 1, err)) break;
-        mbar_arrive_expect_tx(&full[s], S::kSlotBytes + (it & 1 ? 0 : 2 * kHalf * 4));
-        load_half<BLOCKS>(w, bh, it & 1 ? 3 : 0, t0 + j, sm + S::kTileBytes + s * S::kSlotBytes, &full[s]);
+        if (!wait(&ctl.empty[s], (it / S::kSlots) ^ 1)) break;
+        mbar_arrive_expect_tx(&ctl.full[s], S::kSlotBytes + (it & 1 ? 0 : 2 * kHalf * 4));
+        load_half<BLOCKS>(w, bh, it & 1 ? 3 : 0, t0 + j, slots + s * S::kSlotBytes, &ctl.full[s]);
         if (!(it & 1)) {
           const int64_t at_stat = (int64_t)bh * row_tiles * kTile + (int64_t)(t0 + j) * kHalf;
-          bulk_load(vec_lse[j % kLse], w.lse2 + at_stat, kHalf * 4, &full[s]);
-          bulk_load(vec_delta[j % kDelta], w.delta + at_stat, kHalf * 4, &full[s]);
+          bulk_load(ctl.lse[j % S::kLse], w.lse2 + at_stat, kHalf * 4, &ctl.full[s]);
+          bulk_load(ctl.delta[j % S::kDelta], w.delta + at_stat, kHalf * 4, &ctl.full[s]);
         }
       }
-      mbar_wait(&k_full, 0, err);                  // every copy has landed before the block ends
-      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&full[u % S::kSlots], (u / S::kSlots) & 1, err);
+      mbar_wait(&ctl.k_full, 0, err);              // every copy has landed before the block ends
+      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&ctl.full[u % S::kSlots], (u / S::kSlots) & 1, err);
     }
-    if (warp == kSoft + 1 && lane == 0 && n) {
-      bool ok = mbar_wait(&k_full, 0, err) && mbar_wait(&v_full, 0, err);
-      tc_fence_after();
+  } else if (warp == kSoft + 1) {
+    if (lane == 0 && n) {
+      wait(&ctl.k_full, 0);
+      wait(&ctl.v_full, 0);
       const uint64_t k = umma_desc(smem_addr(sm), kChunkBytes, 1024);
-      auto slot = [&](int it) { return smem_addr(sm + S::kTileBytes + it % S::kSlots * S::kSlotBytes); };
-      auto await = [&](uint64_t* bar, int parity) {
-        ok = ok && mbar_wait(bar, parity & 1, err);
-        tc_fence_after();
-      };
+      auto slot = [&](int it) { return smem_addr(slots + it % S::kSlots * S::kSlotBytes); };
       auto scores = [&](int j) {                   // S^T(j) = K Q^T
-        await(&full[2 * j % S::kSlots], 2 * j / S::kSlots);
-        if (!ok) return;
-        mma_features_ss<BLOCKS>(tm_s, k, umma_desc(slot(2 * j), kChunkBytes, 1024));
-        umma_commit(&s_full);
+        const int it = 2 * j;
+        if (!wait(&ctl.full[it % S::kSlots], it / S::kSlots)) return;
+        mma_features_ss<BLOCKS>(tm_s, k, umma_desc(slot(it), kChunkBytes, 1024));
+        umma_commit(&ctl.s_full);
       };
       auto dps = [&](int j) {                      // dP^T(j) = V dout^T
-        await(&full[(2 * j + 1) % S::kSlots], (2 * j + 1) / S::kSlots);
-        if (!ok) return;
-        mma_features_ts<BLOCKS>(tm_dp, tm_v, umma_desc(slot(2 * j + 1), kChunkBytes, 1024));
-        umma_commit(&dp_full);
+        const int it = 2 * j + 1;
+        if (!wait(&ctl.full[it % S::kSlots], it / S::kSlots)) return;
+        mma_features_ts<BLOCKS>(tm_dp, tm_v, umma_desc(slot(it), kChunkBytes, 1024));
+        umma_commit(&ctl.dp_full);
       };
       scores(0);
       dps(0);
-      for (int j = 0; j < n && ok; ++j) {
-        await(&p_full, j);
-        if (j % kGroup == 0) await(&acc_empty, (j / kGroup & 1) ^ 1);
-        if (!ok) break;
-        mma_rows<BLOCKS>(tm_dv, tm_s, umma_desc(slot(2 * j + 1), 2 * kChunkBytes, 1024), j % kGroup != 0);
-        umma_commit(&empty[(2 * j + 1) % S::kSlots]);
+      for (int j = 0; j < n && wait.ok; ++j) {
+        wait(&ctl.p_full, j);
+        if (j % kGroup == 0) wait(&ctl.acc_empty, (j / kGroup) ^ 1);
+        if (!wait.ok) break;
+        mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(slot(2 * j + 1), 2 * kChunkBytes, 1024), j % kGroup != 0);
+        umma_commit(&ctl.empty[(2 * j + 1) % S::kSlots]);
         if (j + 1 < n) scores(j + 1);
-        await(&ds_full, j);
-        if (!ok) break;
-        mma_rows<BLOCKS>(tm_dk, tm_dp, umma_desc(slot(2 * j), 2 * kChunkBytes, 1024), j % kGroup != 0);
-        umma_commit(&empty[2 * j % S::kSlots]);
-        if (j % kGroup == kGroup - 1 || j == n - 1) umma_commit(&acc_full);
+        if (!wait(&ctl.ds_full, j)) break;
+        mma_rows<BLOCKS, 16>(tm_dk, tm_dp, umma_desc(slot(2 * j), 2 * kChunkBytes, 1024), j % kGroup != 0);
+        umma_commit(&ctl.empty[2 * j % S::kSlots]);
+        if (j % kGroup == kGroup - 1 || j == n - 1) umma_commit(&ctl.acc_full);
         if (j + 1 < n) dps(j + 1);
       }
     }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane, key = j0 + row;
+  } else if (sc.split) {
+    const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, key = j0 + row;
     // rows that see the thread's key
     const int lo = key < span.n ? span.first(a, key) * a.group : 0, hi = key < span.n ? span.last(a, key) * a.group : 0;
     const float f = ldexpf(a.scale * kLog2e, -(sc.e[0] + sc.e[1])), fd = ldexpf(1.f, sc.eds - sc.e[3] - sc.e[2]);
@@ -863,64 +864,56 @@ __global__ void __launch_bounds__(384, 1) k_attn_dkv(const __grid_constant__ Att
     if (n) {
       tile_to_tmem<BLOCKS>(w.p[2] + (bh * w.tiles[2] + tile) * (int64_t)S::kTileBytes, tm_v, warp, row);
       tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&v_full);
-      bool ok = true;
+      arrive_warp(&ctl.v_full);
       auto take = [&](int group) {
-        ok = ok && mbar_wait(&acc_full, group & 1, err);
-        tc_fence_after();
-        drain(tm_dv + lane_bits(warp) + half * S::kF, dv);
-        drain(tm_dk + lane_bits(warp) + half * S::kF, dk);
-        tc_fence_before();
-        mbar_arrive(&acc_empty);
+        wait(&ctl.acc_full, group);
+        drain(tm_dv + lane_bits(warp) + quarter * S::kF, dv);
+        drain(tm_dk + lane_bits(warp) + quarter * S::kF, dk);
+        arrive_warp(&ctl.acc_empty);
       };
-      const uint32_t off = lane_bits(warp) + half * 32;
+      const uint32_t off = lane_bits(warp) + quarter * 16;
       for (int j = 0; j < n; ++j) {
-        const int r = (t0 + j) * kHalf + half * 32, s = 2 * j % S::kSlots;
-        ok = ok && mbar_wait(&full[s], (2 * j / S::kSlots) & 1, err);      // the log-sums and deltas
-        ok = ok && mbar_wait(&s_full, j & 1, err);
-        tc_fence_after();
-        const float4* lse = reinterpret_cast<const float4*>(vec_lse[j % kLse] + half * 32);
-        const float4* del = reinterpret_cast<const float4*>(vec_delta[j % kDelta] + half * 32);
-        uint32_t x[32];
-        float p[32];
-        tmem_load32(tm_s + off, x);
+        const int r = (t0 + j) * kHalf + quarter * 16;
+        wait(&ctl.full[2 * j % S::kSlots], 2 * j / S::kSlots);             // the log-sums and deltas
+        wait(&ctl.s_full, j);
+        const float4* lse = reinterpret_cast<const float4*>(ctl.lse[j % S::kLse] + quarter * 16);
+        const float4* del = reinterpret_cast<const float4*>(ctl.delta[j % S::kDelta] + quarter * 16);
+        uint32_t x[16];
+        float p[16];
+        tmem_load16(tm_s + off, x);
         tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
+        for (int e = 0; e < 16; e += 4) {
           const float4 l = lse[e / 4];
           p[e] = ex2(fmaf(__uint_as_float(x[e]), f, kUpP - l.x));
           p[e + 1] = ex2(fmaf(__uint_as_float(x[e + 1]), f, kUpP - l.y));
           p[e + 2] = ex2(fmaf(__uint_as_float(x[e + 2]), f, kUpP - l.z));
           p[e + 3] = ex2(fmaf(__uint_as_float(x[e + 3]), f, kUpP - l.w));
         }
-        if (__any_sync(0xffffffffu, r < lo || r + 32 > hi)) {
+        if (__any_sync(0xffffffffu, r < lo || r + 16 > hi)) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
+          for (int e = 0; e < 16; ++e)
             if (r + e < lo || r + e >= hi) p[e] = 0.f;
         }
-        store_operand(tm_s + off, p);
+        store_operand<16>(tm_s + off, p);
         tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&p_full);
+        arrive_warp(&ctl.p_full);
         if (j && j % kGroup == 0) take(j / kGroup - 1);
-        ok = ok && mbar_wait(&dp_full, j & 1, err);
-        tc_fence_after();
-        tmem_load32(tm_dp + off, x);
+        wait(&ctl.dp_full, j);
+        tmem_load16(tm_dp + off, x);
         tmem_wait_ld();
         constexpr float down = 1.f / 16384.f;      // 2^-14: P itself
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
+        for (int e = 0; e < 16; e += 4) {
           const float4 d = del[e / 4];
           p[e] *= down * fmaf(__uint_as_float(x[e]), fd, -d.x);
           p[e + 1] *= down * fmaf(__uint_as_float(x[e + 1]), fd, -d.y);
           p[e + 2] *= down * fmaf(__uint_as_float(x[e + 2]), fd, -d.z);
           p[e + 3] *= down * fmaf(__uint_as_float(x[e + 3]), fd, -d.w);
         }
-        store_operand(tm_dp + off, p);
+        store_operand<16>(tm_dp + off, p);
         tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&ds_full);
+        arrive_warp(&ctl.ds_full);
       }
       take((n - 1) / kGroup);
     }
@@ -931,14 +924,14 @@ __global__ void __launch_bounds__(384, 1) k_attn_dkv(const __grid_constant__ Att
         dk[e] *= bk;
         dv[e] *= bv;
       }
-      store_features<S::kF>(a.dk + at(a.dks, b, key, hk), half * S::kF, a.dim, vec_out, dk);
-      store_features<S::kF>(a.dv + at(a.dvs, b, key, hk), half * S::kF, a.dim, vec_out, dv);
+      store_features<S::kF>(a.dk + at(a.dks, b, key, hk), quarter * S::kF, a.dim, vec_out, dk);
+      store_features<S::kF>(a.dv + at(a.dvs, b, key, hk), quarter * S::kF, a.dim, vec_out, dv);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kSoft + 1) tmem_free(tmem_base, 512);
+  if (warp == kSoft + 1) tmem_free(tm_dk, 512);
 }
 
 // ---------------------------------------------------------------------------
@@ -960,7 +953,7 @@ struct Layout {
     }
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 1023) & ~size_t(1023); return o; };
-    stats = take(sizeof(AttnStats) * heads);
+    stats = take(sizeof(AttnStats) * heads + sizeof(uint32_t));     // and the word `any`
     for (int t = 0; t < (backward ? 4 : 3); ++t)
       tile[t] = take((size_t)heads * (t == 1 || t == 2 ? key_tiles : row_tiles) * blocks * kBlockBytes);
     lse2 = delta = part = 0;
@@ -982,6 +975,7 @@ bool aligned(const float* p, const int64_t* s) {
 cudaError_t prepare(const AttnArgs& a, const Layout& L, uint8_t* w, bool backward, Tiles& t, cudaStream_t st) {
   t = Tiles{};
   t.stats = reinterpret_cast<AttnStats*>(w + L.stats);
+  t.any = reinterpret_cast<uint32_t*>(t.stats + L.heads);
   for (int i = 0; i < (backward ? 4 : 3); ++i) {
     t.p[i] = w + L.tile[i];
     t.tiles[i] = i == 1 || i == 2 ? L.key_tiles : L.row_tiles;
@@ -989,21 +983,22 @@ cudaError_t prepare(const AttnArgs& a, const Layout& L, uint8_t* w, bool backwar
   t.lse2 = reinterpret_cast<float*>(w + L.lse2);
   t.delta = reinterpret_cast<float*>(w + L.delta);
   t.blocks = (int)L.blocks;
-  cudaError_t e = cudaMemsetAsync(t.stats, 0, sizeof(AttnStats) * L.heads, st);
+  cudaError_t e = cudaMemsetAsync(t.stats, 0, sizeof(AttnStats) * L.heads + sizeof(uint32_t), st);
   if (e != cudaSuccess) return e;
   const int per_q = (int)((int64_t)a.q_len * a.group + kScanRows - 1) / kScanRows, per_k = (a.kv_len + kScanRows - 1) / kScanRows;
   const int64_t scan = L.heads * ((backward ? 2ll : 1ll) * per_q + 2ll * per_k);
   const int64_t split = L.heads * 8 * ((backward ? 2 : 1) * L.row_tiles + 2 * L.key_tiles);
   if (scan > INT_MAX || split > INT_MAX) return cudaErrorInvalidConfiguration;
   if (!scan) return cudaSuccess;
-  k_attn_scan<<<(unsigned)scan, 256, 0, st>>>(a, t.stats, per_q, per_k, backward);
   const bool vec = a.dim % 4 == 0 && aligned(a.q, a.qs) && aligned(a.k, a.ks) && aligned(a.v, a.vs) &&
                    (!backward || aligned(a.dout, a.os));
-  if (L.blocks == 1)
-    k_attn_split<1><<<(unsigned)split, 128, 0, st>>>(a, t, (int)L.row_tiles, (int)L.key_tiles, backward, vec);
-  else
-    k_attn_split<2><<<(unsigned)split, 256, 0, st>>>(a, t, (int)L.row_tiles, (int)L.key_tiles, backward, vec);
-  return cudaGetLastError();
+  const int back = backward, tq = (int)L.row_tiles, tk = (int)L.key_tiles;
+  if (vec) k_attn_scan<true><<<(unsigned)scan, 256, 0, st>>>(a, t.stats, per_q, per_k, back);
+  else k_attn_scan<false><<<(unsigned)scan, 256, 0, st>>>(a, t.stats, per_q, per_k, back);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return L.blocks == 1 ? launch_pdl(k_attn_split<1>, dim3((unsigned)split), dim3(128), 0, st, a, t, tq, tk, back, vec)
+                       : launch_pdl(k_attn_split<2>, dim3((unsigned)split), dim3(256), 0, st, a, t, tq, tk, back, vec);
 }
 
 template <int BLOCKS>
@@ -1014,30 +1009,26 @@ cudaError_t forward(const AttnArgs& a, const Layout& L, const Tiles& t, float* p
   if (set != cudaSuccess) return set;
   const int64_t blocks = L.heads * L.row_tiles * L.splits;
   if (blocks > INT_MAX) return cudaErrorInvalidConfiguration;
-  k_attn_forward<BLOCKS><<<(unsigned)blocks, kThreads, S::kSmem, st>>>(
-      a, t, (int)L.row_tiles, L.splits, part, a.dim % 4 == 0 && aligned(a.out, a.os), device_error_word());
-  return cudaGetLastError();
+  return launch_pdl(k_attn_forward<BLOCKS>, dim3((unsigned)blocks), dim3(kThreads), S::kSmem, st, a, t,
+                    (int)L.row_tiles, L.splits, part, a.dim % 4 == 0 && aligned(a.out, a.os), device_error_word());
 }
 
 template <int BLOCKS>
 cudaError_t backward(const AttnArgs& a, const Layout& L, const Tiles& t, cudaStream_t st) {
-  using S = Backward<BLOCKS>;
   static const cudaError_t set_q = cudaFuncSetAttribute(k_attn_dq<BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                        (int)S::kSmem);
+                                                        (int)Dq<BLOCKS>::kSmem);
   static const cudaError_t set_kv = cudaFuncSetAttribute(k_attn_dkv<BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                         (int)S::kSmem);
+                                                         (int)Dkv<BLOCKS>::kSmem);
   if (set_q != cudaSuccess) return set_q;
   if (set_kv != cudaSuccess) return set_kv;
   const int64_t nq = L.heads * L.row_tiles, nk = L.heads * L.key_tiles;
   if (nq > INT_MAX || nk > INT_MAX) return cudaErrorInvalidConfiguration;
-  const bool vec = a.dim % 4 == 0;
-  if (nk)
-    k_attn_dkv<BLOCKS><<<(unsigned)nk, 384, S::kSmem, st>>>(
-        a, t, (int)L.row_tiles, vec && aligned(a.dk, a.dks) && aligned(a.dv, a.dvs), device_error_word());
-  if (nq)
-    k_attn_dq<BLOCKS><<<(unsigned)nq, kThreads, S::kSmem, st>>>(a, t, (int)L.row_tiles, vec && aligned(a.dq, a.dqs),
-                                                                device_error_word());
-  return cudaGetLastError();
+  const bool vec = a.dim % 4 == 0, vec_kv = vec && aligned(a.dk, a.dks) && aligned(a.dv, a.dvs);
+  cudaError_t e = launch_pdl(k_attn_dkv<BLOCKS>, dim3((unsigned)nk), dim3(kThreads), Dkv<BLOCKS>::kSmem, st, a, t,
+                             (int)L.row_tiles, vec_kv, device_error_word());
+  if (e != cudaSuccess) return e;
+  return launch_pdl(k_attn_dq<BLOCKS>, dim3((unsigned)nq), dim3(kThreads), Dq<BLOCKS>::kSmem, st, a, t,
+                    (int)L.row_tiles, vec && aligned(a.dq, a.dqs), device_error_word());
 }
 
 }  // namespace
@@ -1056,6 +1047,7 @@ cudaError_t launch_attn_tensor_forward(const AttnArgs& args, void* ws, cudaStrea
   cudaError_t e = prepare(a, L, w, false, t, st);
   if (e != cudaSuccess) return e;
   a.stats = t.stats;
+  a.any = t.any;
   float* part = reinterpret_cast<float*>(w + L.part);
   e = L.blocks == 1 ? forward<1>(a, L, t, part, st) : forward<2>(a, L, t, part, st);
   if (e == cudaSuccess && L.splits > 1) e = launch_attn_join(a, L.splits, part, true, st);
@@ -1070,6 +1062,7 @@ cudaError_t launch_attn_tensor_backward(const AttnArgs& args, void* ws, cudaStre
   cudaError_t e = prepare(a, L, static_cast<uint8_t*>(ws), true, t, st);
   if (e != cudaSuccess) return e;
   a.stats = t.stats;
+  a.any = t.any;
   a.delta = t.delta;
   e = L.blocks == 1 ? backward<1>(a, L, t, st) : backward<2>(a, L, t, st);
   if (e == cudaSuccess) e = launch_attn_rows_backward(a, st);

@@ -414,10 +414,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
           if (j < g.N) {
             float* o = g.out + ((uint64_t)z * g.M + i0) * g.N + j;
             const uint32_t rows = i0 < g.M ? min(32u, g.M - i0) : 0;
-#pragma unroll 8
-            for (uint32_t r = 0; r < rows; ++r) {
-              const float v = t[r * 32 + ((lane + r) & 31)];
-              o[(uint64_t)r * g.N] = g.update ? fmaf(-g.rate, v, g.keep * o[(uint64_t)r * g.N]) : v;
+#pragma unroll
+            for (uint32_t r = 0; r < 32; r += 16) {          // 16 rows of w in flight
+              float old[16];
+              if (g.update) {
+#pragma unroll
+                for (uint32_t e = 0; e < 16; ++e)
+                  if (r + e < rows) old[e] = o[(uint64_t)(r + e) * g.N];
+              }
+#pragma unroll
+              for (uint32_t e = 0; e < 16; ++e) {
+                const float v = t[(r + e) * 32 + ((lane + r + e) & 31)];
+                if (r + e < rows) o[(uint64_t)(r + e) * g.N] = g.update ? fmaf(-g.rate, v, g.keep * old[e]) : v;
+              }
             }
           }
         }

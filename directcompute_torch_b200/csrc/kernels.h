@@ -273,6 +273,7 @@ struct AttnArgs {
   float scale;
   float* delta;                          // scratch [batch * kv_heads, padded_rows]: sum_d dout out
   const struct AttnStats* stats;         // [batch * kv_heads] or null: every head on the CUDA cores
+  const uint32_t* any;                   // with stats: 0 where no head is left to the CUDA cores
 };
 // rows of a key head in scratch: whole tiles of 128
 __host__ __device__ inline int64_t padded_rows(const AttnArgs& a) {
