@@ -205,13 +205,15 @@ __global__ void __launch_bounds__(128 * BLOCKS) k_attn_split(const __grid_consta
 // what the three kernels share
 // ---------------------------------------------------------------------------
 // 16 warps compute, four threads a row of 128 (warp w holds rows 32 (w & 3) .. and quarter
-// w >> 2 of the columns); warp 16 loads, warp 17 issues the matrix instructions.  Four warps
-// a scheduler hide the latencies that one phase after the other has (two a scheduler left
-// the tensor cores busy 38 to 47% of the time).  The inner side comes in half tiles of 64
-// rows, so that the next ones arrive while these are used.  The operand that rests lies in
-// tensor memory where there is room, which spares shared memory its bandwidth.
+// w >> 2 of the columns); warp 17 issues the matrix instructions, warps 16 and 18 load, each
+// its own ring of slots: the two inner operands are used up in different orders, and in one
+// ring each would wait for the other's slots.  Four warps a scheduler hide the latencies
+// that one phase after the other has.  The operand that rests lies in tensor memory where
+// there is room; the inner side comes in half tiles of 64 rows where there is not enough
+// shared memory for whole ones (a matrix instruction 64 columns wide takes 45 or 48 cycles,
+// one of 128 takes 64: measured).
 constexpr int kSoft = 16;
-constexpr int kThreads = 32 * (kSoft + 2);
+constexpr int kThreads = 32 * (kSoft + 3);
 constexpr int kHalf = 64;
 
 template <int BLOCKS>
@@ -256,6 +258,33 @@ DCT_DEV void tile_to_tmem(const uint8_t* tile, uint32_t addr, int warp, int row)
   }
 }
 
+// A ring of slots: loads fill them in turn, matrix instructions empty them.
+template <int N>
+struct Ring {
+  uint64_t full[N], empty[N];
+  DCT_DEV void init() {
+    for (int s = 0; s < N; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+  }
+  // fills `count` slots: load(number, slot, barrier)
+  template <typename Wait, typename Load>
+  DCT_DEV void fill(int count, uint32_t bytes, Wait& wait, Load load) {
+    int it = 0;
+    for (; it < count; ++it) {
+      if (!wait(&empty[it % N], (it / N) ^ 1)) break;
+      mbar_arrive_expect_tx(&full[it % N], bytes);
+      load(it, it % N, &full[it % N]);
+    }
+    // every copy has landed before the block ends
+    for (int u = max(0, it - N); u < it; ++u) mbar_wait(&full[u % N], (u / N) & 1, wait.err);
+  }
+  template <typename Wait>
+  DCT_DEV bool ready(int it, Wait& wait) { return wait(&full[it % N], it / N); }
+  DCT_DEV void release(int it) { umma_commit(&empty[it % N]); }
+};
+
 // D = A B^T over the features: A a whole tile in shared memory, B a half tile.  The small
 // products come first: every matrix instruction rounds its sum toward zero.
 template <int BLOCKS>
@@ -272,12 +301,12 @@ DCT_DEV void mma_features_ss(uint32_t d, uint64_t a, uint64_t b) {
 #pragma unroll
   for (int c = 0; c < 4 * BLOCKS; ++c) umma(d, a + sa(c), b + sb(c), id, true);
 }
-// the same with A in tensor memory
-template <int BLOCKS>
+// the same with A in tensor memory, B a tile of ROWS rows
+template <int BLOCKS, int ROWS>
 DCT_DEV void mma_features_ts(uint32_t d, uint32_t a, uint64_t b) {
-  constexpr uint32_t id = umma_idesc(kTile, kHalf, false, false);
-  constexpr uint64_t lo_b = kChunkBytes / 16;
-  auto sb = [](int c) { return (uint64_t)((c >> 2) * (2 * kChunkBytes / 16) + (c & 3) * 2); };
+  constexpr uint32_t id = umma_idesc(kTile, ROWS, false, false);
+  constexpr uint64_t lo_b = ROWS * 128 / 16;
+  auto sb = [](int c) { return (uint64_t)((c >> 2) * (2 * ROWS * 128 / 16) + (c & 3) * 2); };
 #pragma unroll
   for (int c = 0; c < 4 * BLOCKS; ++c) {
     umma_ts(d, a + 32 * BLOCKS + 8 * c, b + sb(c), id, c != 0);
@@ -346,13 +375,17 @@ constexpr float kUp = 7.f;
 
 template <int BLOCKS>
 struct Forward : Sizes<BLOCKS> {
-  static constexpr int kSlots = BLOCKS == 1 ? 12 : 7;
+  static constexpr int kKeys = BLOCKS == 1 ? 3 : 2, kValues = BLOCKS == 1 ? 6 : 3;   // tiles of K, halves of V
   struct Control {
-    uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], o_full, o_empty;
+    Ring<kKeys> k;
+    Ring<kValues> v;
+    uint64_t q_full, s_full[2], p_full[2], o_full, o_empty;
     uint32_t tmem;
     float exch[4][kTile];
   };
-  static constexpr size_t kSmem = (size_t)kSlots * Sizes<BLOCKS>::kSlotBytes + sizeof(Control);
+  static constexpr uint32_t kV = kKeys * Sizes<BLOCKS>::kTileBytes;          // where the halves of V begin
+  static constexpr uint32_t kEnd = kV + kValues * Sizes<BLOCKS>::kSlotBytes;
+  static constexpr size_t kSmem = kEnd + sizeof(Control);
 };
 
 DCT_DEV void rows_sync(int warp) {                 // the four warps that share rows
@@ -370,15 +403,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
                                                               int splits, float* part, bool vec_out, uint32_t* err) {
   using S = Forward<BLOCKS>;
   extern __shared__ __align__(1024) uint8_t sm[];
-  auto& ctl = *reinterpret_cast<typename S::Control*>(sm + S::kSlots * S::kSlotBytes);
+  auto& ctl = *reinterpret_cast<typename S::Control*>(sm + S::kEnd);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (misaligned(sm, err)) return;
   if (threadIdx.x == 0) {
+    ctl.k.init();
+    ctl.v.init();
     mbar_init(&ctl.q_full, kSoft);
-    for (int s = 0; s < S::kSlots; ++s) {
-      mbar_init(&ctl.full[s], 1);
-      mbar_init(&ctl.empty[s], 1);
-    }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&ctl.s_full[s], 1);
       mbar_init(&ctl.p_full[s], kSoft);
@@ -418,29 +449,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
   Waits wait{err};
 
   if (warp == kSoft) {
-    if (lane == 0) {
-      int it = 0;
-      for (; it < 4 * n; ++it) {                   // K in halves, V in halves
-        const int s = it % S::kSlots;
-        if (!wait(&ctl.empty[s], (it / S::kSlots) ^ 1)) break;
-        mbar_arrive_expect_tx(&ctl.full[s], S::kSlotBytes);
-        load_half<BLOCKS>(w, bh, 1 + ((it >> 1) & 1), 2 * (t0 + it / 4) + (it & 1), sm + s * S::kSlotBytes,
-                          &ctl.full[s]);
-      }
-      // every copy has landed before the block ends
-      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&ctl.full[u % S::kSlots], (u / S::kSlots) & 1, err);
-    }
+    if (lane == 0)
+      ctl.k.fill(n, S::kTileBytes, wait, [&](int it, int s, uint64_t* bar) {
+        load_tile<BLOCKS>(w, bh, 1, t0 + it, sm + s * S::kTileBytes, bar);
+      });
+  } else if (warp == kSoft + 2) {
+    if (lane == 0)
+      ctl.v.fill(2 * n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
+        load_half<BLOCKS>(w, bh, 2, 2 * t0 + it, sm + S::kV + s * S::kSlotBytes, bar);
+      });
   } else if (warp == kSoft + 1) {
     if (lane == 0 && n) {
       wait(&ctl.q_full, 0);
-      auto slot = [&](int it) { return smem_addr(sm + it % S::kSlots * S::kSlotBytes); };
       auto scores = [&](int j) {                   // S(j) = Q K(j)^T
-        for (int h = 0; h < 2; ++h) {
-          const int it = 4 * j + h;
-          if (!wait(&ctl.full[it % S::kSlots], it / S::kSlots)) return;
-          mma_features_ts<BLOCKS>(tm_s + (j & 1) * kTile + h * kHalf, tm_q, umma_desc(slot(it), kChunkBytes, 1024));
-          umma_commit(&ctl.empty[it % S::kSlots]);
-        }
+        if (!ctl.k.ready(j, wait)) return;
+        mma_features_ts<BLOCKS, kTile>(tm_s + (j & 1) * kTile, tm_q,
+                                       umma_desc(smem_addr(sm + j % S::kKeys * S::kTileBytes), kChunkBytes, 1024));
+        ctl.k.release(j);
         umma_commit(&ctl.s_full[j & 1]);
       };
       scores(0);
@@ -449,10 +474,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
         wait(&ctl.p_full[j & 1], j >> 1);
         wait(&ctl.o_empty, j ^ 1);
         for (int h = 0; h < 2; ++h) {
-          const int it = 4 * j + 2 + h;
-          if (!wait(&ctl.full[it % S::kSlots], it / S::kSlots)) break;
-          mma_rows<BLOCKS, 32>(tm_o, tm_s + (j & 1) * kTile + h * kHalf, umma_desc(slot(it), 2 * kChunkBytes, 1024), h);
-          umma_commit(&ctl.empty[it % S::kSlots]);
+          const int it = 2 * j + h;
+          if (!ctl.v.ready(it, wait)) break;
+          mma_rows<BLOCKS, 32>(tm_o, tm_s + (j & 1) * kTile + h * kHalf,
+                               umma_desc(smem_addr(sm + S::kV + it % S::kValues * S::kSlotBytes), 2 * kChunkBytes, 1024), h);
+          ctl.v.release(it);
         }
         umma_commit(&ctl.o_full);
       }
@@ -582,12 +608,16 @@ DCT_DEV void drain(uint32_t addr, float (&acc)[N]) {
 
 template <int BLOCKS>
 struct Dq : Sizes<BLOCKS> {
-  static constexpr int kSlots = BLOCKS == 1 ? 8 : 5;
+  static constexpr int kKeys = BLOCKS == 1 ? 5 : 3, kValues = BLOCKS == 1 ? 4 : 2;   // halves of K, of V
   struct Control {
-    uint64_t q_full, go_full, full[kSlots], empty[kSlots], s_full[2], ds_full[2], acc_full, acc_empty;
+    Ring<kKeys> k;
+    Ring<kValues> v;
+    uint64_t q_full, go_full, s_full[2], ds_full[2], acc_full, acc_empty;
     uint32_t tmem;
   };
-  static constexpr size_t kSmem = Sizes<BLOCKS>::kTileBytes + (size_t)kSlots * Sizes<BLOCKS>::kSlotBytes + sizeof(Control);
+  static constexpr uint32_t kK = Sizes<BLOCKS>::kTileBytes, kV = kK + kKeys * Sizes<BLOCKS>::kSlotBytes;
+  static constexpr uint32_t kEnd = kV + kValues * Sizes<BLOCKS>::kSlotBytes;
+  static constexpr size_t kSmem = kEnd + sizeof(Control);
 };
 
 // dq of a tile of 128 rows: dS = P (dP - delta), dq = scale dS K.  Q rests in shared memory,
@@ -598,17 +628,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
                                                          uint32_t* err) {
   using S = Dq<BLOCKS>;
   extern __shared__ __align__(1024) uint8_t sm[];
-  uint8_t* slots = sm + S::kTileBytes;
-  auto& ctl = *reinterpret_cast<typename S::Control*>(slots + S::kSlots * S::kSlotBytes);
+  auto& ctl = *reinterpret_cast<typename S::Control*>(sm + S::kEnd);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (misaligned(sm, err)) return;
   if (threadIdx.x == 0) {
     mbar_init(&ctl.q_full, 1);
     mbar_init(&ctl.go_full, kSoft);
-    for (int s = 0; s < S::kSlots; ++s) {
-      mbar_init(&ctl.full[s], 1);
-      mbar_init(&ctl.empty[s], 1);
-    }
+    ctl.k.init();
+    ctl.v.init();
     for (int s = 0; s < 2; ++s) {
       mbar_init(&ctl.s_full[s], 1);
       mbar_init(&ctl.ds_full[s], kSoft);
@@ -642,29 +669,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
     if (lane == 0 && n) {
       mbar_arrive_expect_tx(&ctl.q_full, S::kTileBytes);
       load_tile<BLOCKS>(w, bh, 0, tile, sm, &ctl.q_full);
-      int it = 0;
-      for (; it < 2 * n; ++it) {                   // K, V, K, V ...
-        const int s = it % S::kSlots;
-        if (!wait(&ctl.empty[s], (it / S::kSlots) ^ 1)) break;
-        mbar_arrive_expect_tx(&ctl.full[s], S::kSlotBytes);
-        load_half<BLOCKS>(w, bh, it & 1 ? 2 : 1, t0 + it / 2, slots + s * S::kSlotBytes, &ctl.full[s]);
-      }
-      mbar_wait(&ctl.q_full, 0, err);              // every copy has landed before the block ends
-      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&ctl.full[u % S::kSlots], (u / S::kSlots) & 1, err);
+      ctl.k.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
+        load_half<BLOCKS>(w, bh, 1, t0 + it, sm + S::kK + s * S::kSlotBytes, bar);
+      });
+      mbar_wait(&ctl.q_full, 0, err);
     }
+  } else if (warp == kSoft + 2) {
+    if (lane == 0)
+      ctl.v.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
+        load_half<BLOCKS>(w, bh, 2, t0 + it, sm + S::kV + s * S::kSlotBytes, bar);
+      });
   } else if (warp == kSoft + 1) {
     if (lane == 0 && n) {
       wait(&ctl.q_full, 0);
       wait(&ctl.go_full, 0);
       const uint64_t q = umma_desc(smem_addr(sm), kChunkBytes, 1024);
-      auto slot = [&](int it) { return smem_addr(slots + it % S::kSlots * S::kSlotBytes); };
+      auto key = [&](int j) { return smem_addr(sm + S::kK + j % S::kKeys * S::kSlotBytes); };
+      auto value = [&](int j) { return smem_addr(sm + S::kV + j % S::kValues * S::kSlotBytes); };
       auto scores = [&](int j) {                   // S(j) = Q K^T, dP(j) = dout V^T
-        const int k = 2 * j, v = k + 1;
-        if (!wait(&ctl.full[k % S::kSlots], k / S::kSlots)) return;
-        mma_features_ss<BLOCKS>(tm_s + (j & 1) * kHalf, q, umma_desc(slot(k), kChunkBytes, 1024));
-        if (!wait(&ctl.full[v % S::kSlots], v / S::kSlots)) return;
-        mma_features_ts<BLOCKS>(tm_dp + (j & 1) * kHalf, tm_go, umma_desc(slot(v), kChunkBytes, 1024));
-        umma_commit(&ctl.empty[v % S::kSlots]);
+        if (!ctl.k.ready(j, wait)) return;
+        mma_features_ss<BLOCKS>(tm_s + (j & 1) * kHalf, q, umma_desc(key(j), kChunkBytes, 1024));
+        if (!ctl.v.ready(j, wait)) return;
+        mma_features_ts<BLOCKS, kHalf>(tm_dp + (j & 1) * kHalf, tm_go, umma_desc(value(j), kChunkBytes, 1024));
+        ctl.v.release(j);
         umma_commit(&ctl.s_full[j & 1]);
       };
       scores(0);
@@ -673,9 +700,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         wait(&ctl.ds_full[j & 1], j >> 1);
         if (j % kGroup == 0) wait(&ctl.acc_empty, (j / kGroup) ^ 1);
         if (!wait.ok) break;
-        mma_rows<BLOCKS, 16>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(slot(2 * j), 2 * kChunkBytes, 1024),
-                             j % kGroup != 0);
-        umma_commit(&ctl.empty[2 * j % S::kSlots]);
+        mma_rows<BLOCKS, 16>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(key(j), 2 * kChunkBytes, 1024), j % kGroup != 0);
+        ctl.k.release(j);
         if (j % kGroup == kGroup - 1 || j == n - 1) umma_commit(&ctl.acc_full);
       }
     }
@@ -738,17 +764,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
 
 template <int BLOCKS>
 struct Dkv : Sizes<BLOCKS> {
-  static constexpr int kSlots = BLOCKS == 1 ? 8 : 5;
-  // Log-sums and deltas come with Q(j) but outlive its neighbours' slots: with five slots
-  // Q(j + 3) may come in after dv(j), when the log-sums of j are used, and Q(j + 4) after
-  // dv(j + 1), when the deltas are; with eight, both stay until dk(j).
-  static constexpr int kLse = BLOCKS == 1 ? 5 : 3, kDelta = BLOCKS == 1 ? 5 : 4;
+  static constexpr int kRowsQ = BLOCKS == 1 ? 5 : 3, kRowsGo = BLOCKS == 1 ? 4 : 2;  // halves of Q, of dout
   struct Control {
-    float lse[kLse][kHalf], delta[kDelta][kHalf];  // 16-byte aligned: the bulk copies' targets
-    uint64_t k_full, v_full, full[kSlots], empty[kSlots], s_full, dp_full, p_full, ds_full, acc_full, acc_empty;
+    float lse[kRowsQ][kHalf], delta[kRowsQ][kHalf];  // with Q; 16-byte aligned: the bulk copies' targets
+    Ring<kRowsQ> q;
+    Ring<kRowsGo> go;
+    uint64_t k_full, v_full, s_full, dp_full, p_full, ds_full, acc_full, acc_empty;
     uint32_t tmem;
   };
-  static constexpr size_t kSmem = Sizes<BLOCKS>::kTileBytes + (size_t)kSlots * Sizes<BLOCKS>::kSlotBytes + sizeof(Control);
+  static constexpr uint32_t kQ = Sizes<BLOCKS>::kTileBytes, kGo = kQ + kRowsQ * Sizes<BLOCKS>::kSlotBytes;
+  static constexpr uint32_t kEnd = kGo + kRowsGo * Sizes<BLOCKS>::kSlotBytes;
+  static constexpr size_t kSmem = kEnd + sizeof(Control);
 };
 
 // dk and dv of a tile of 128 keys: dv = P^T dout, dk = scale dS^T Q.  K rests in shared
@@ -761,17 +787,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
                                                           uint32_t* err) {
   using S = Dkv<BLOCKS>;
   extern __shared__ __align__(1024) uint8_t sm[];
-  uint8_t* slots = sm + S::kTileBytes;
-  auto& ctl = *reinterpret_cast<typename S::Control*>(slots + S::kSlots * S::kSlotBytes);
+  auto& ctl = *reinterpret_cast<typename S::Control*>(sm + S::kEnd);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (misaligned(sm, err)) return;
   if (threadIdx.x == 0) {
     mbar_init(&ctl.k_full, 1);
     mbar_init(&ctl.v_full, kSoft);
-    for (int s = 0; s < S::kSlots; ++s) {
-      mbar_init(&ctl.full[s], 1);
-      mbar_init(&ctl.empty[s], 1);
-    }
+    ctl.q.init();
+    ctl.go.init();
     mbar_init(&ctl.s_full, 1);
     mbar_init(&ctl.dp_full, 1);
     mbar_init(&ctl.p_full, kSoft);
@@ -804,37 +827,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     if (lane == 0 && n) {
       mbar_arrive_expect_tx(&ctl.k_full, S::kTileBytes);
       load_tile<BLOCKS>(w, bh, 1, tile, sm, &ctl.k_full);
-      int it = 0;
-      for (; it < 2 * n; ++it) {                   // Q, dout, Q, dout ...
-        const int s = it % S::kSlots, j = it / 2;
-        if (!wait(&ctl.empty[s], (it / S::kSlots) ^ 1)) break;
-        mbar_arrive_expect_tx(&ctl.full[s], S::kSlotBytes + (it & 1 ? 0 : 2 * kHalf * 4));
-        load_half<BLOCKS>(w, bh, it & 1 ? 3 : 0, t0 + j, slots + s * S::kSlotBytes, &ctl.full[s]);
-        if (!(it & 1)) {
-          const int64_t at_stat = (int64_t)bh * row_tiles * kTile + (int64_t)(t0 + j) * kHalf;
-          bulk_load(ctl.lse[j % S::kLse], w.lse2 + at_stat, kHalf * 4, &ctl.full[s]);
-          bulk_load(ctl.delta[j % S::kDelta], w.delta + at_stat, kHalf * 4, &ctl.full[s]);
-        }
-      }
-      mbar_wait(&ctl.k_full, 0, err);              // every copy has landed before the block ends
-      for (int u = max(0, it - S::kSlots); u < it; ++u) mbar_wait(&ctl.full[u % S::kSlots], (u / S::kSlots) & 1, err);
+      ctl.q.fill(n, S::kSlotBytes + 2 * kHalf * 4, wait, [&](int it, int s, uint64_t* bar) {
+        const int64_t at_stat = (int64_t)bh * row_tiles * kTile + (int64_t)(t0 + it) * kHalf;
+        load_half<BLOCKS>(w, bh, 0, t0 + it, sm + S::kQ + s * S::kSlotBytes, bar);
+        bulk_load(ctl.lse[s], w.lse2 + at_stat, kHalf * 4, bar);
+        bulk_load(ctl.delta[s], w.delta + at_stat, kHalf * 4, bar);
+      });
+      mbar_wait(&ctl.k_full, 0, err);
     }
+  } else if (warp == kSoft + 2) {
+    if (lane == 0)
+      ctl.go.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
+        load_half<BLOCKS>(w, bh, 3, t0 + it, sm + S::kGo + s * S::kSlotBytes, bar);
+      });
   } else if (warp == kSoft + 1) {
     if (lane == 0 && n) {
       wait(&ctl.k_full, 0);
       wait(&ctl.v_full, 0);
       const uint64_t k = umma_desc(smem_addr(sm), kChunkBytes, 1024);
-      auto slot = [&](int it) { return smem_addr(slots + it % S::kSlots * S::kSlotBytes); };
+      auto query = [&](int j) { return smem_addr(sm + S::kQ + j % S::kRowsQ * S::kSlotBytes); };
+      auto grad = [&](int j) { return smem_addr(sm + S::kGo + j % S::kRowsGo * S::kSlotBytes); };
       auto scores = [&](int j) {                   // S^T(j) = K Q^T
-        const int it = 2 * j;
-        if (!wait(&ctl.full[it % S::kSlots], it / S::kSlots)) return;
-        mma_features_ss<BLOCKS>(tm_s, k, umma_desc(slot(it), kChunkBytes, 1024));
+        if (!ctl.q.ready(j, wait)) return;
+        mma_features_ss<BLOCKS>(tm_s, k, umma_desc(query(j), kChunkBytes, 1024));
         umma_commit(&ctl.s_full);
       };
       auto dps = [&](int j) {                      // dP^T(j) = V dout^T
-        const int it = 2 * j + 1;
-        if (!wait(&ctl.full[it % S::kSlots], it / S::kSlots)) return;
-        mma_features_ts<BLOCKS>(tm_dp, tm_v, umma_desc(slot(it), kChunkBytes, 1024));
+        if (!ctl.go.ready(j, wait)) return;
+        mma_features_ts<BLOCKS, kHalf>(tm_dp, tm_v, umma_desc(grad(j), kChunkBytes, 1024));
         umma_commit(&ctl.dp_full);
       };
       scores(0);
@@ -843,12 +863,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
         wait(&ctl.p_full, j);
         if (j % kGroup == 0) wait(&ctl.acc_empty, (j / kGroup) ^ 1);
         if (!wait.ok) break;
-        mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(slot(2 * j + 1), 2 * kChunkBytes, 1024), j % kGroup != 0);
-        umma_commit(&ctl.empty[(2 * j + 1) % S::kSlots]);
+        mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(grad(j), 2 * kChunkBytes, 1024), j % kGroup != 0);
+        ctl.go.release(j);
         if (j + 1 < n) scores(j + 1);
         if (!wait(&ctl.ds_full, j)) break;
-        mma_rows<BLOCKS, 16>(tm_dk, tm_dp, umma_desc(slot(2 * j), 2 * kChunkBytes, 1024), j % kGroup != 0);
-        umma_commit(&ctl.empty[2 * j % S::kSlots]);
+        mma_rows<BLOCKS, 16>(tm_dk, tm_dp, umma_desc(query(j), 2 * kChunkBytes, 1024), j % kGroup != 0);
+        ctl.q.release(j);
         if (j % kGroup == kGroup - 1 || j == n - 1) umma_commit(&ctl.acc_full);
         if (j + 1 < n) dps(j + 1);
       }
@@ -874,10 +894,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       const uint32_t off = lane_bits(warp) + quarter * 16;
       for (int j = 0; j < n; ++j) {
         const int r = (t0 + j) * kHalf + quarter * 16;
-        wait(&ctl.full[2 * j % S::kSlots], 2 * j / S::kSlots);             // the log-sums and deltas
+        ctl.q.ready(j, wait);                      // the log-sums and deltas
         wait(&ctl.s_full, j);
-        const float4* lse = reinterpret_cast<const float4*>(ctl.lse[j % S::kLse] + quarter * 16);
-        const float4* del = reinterpret_cast<const float4*>(ctl.delta[j % S::kDelta] + quarter * 16);
+        const float4* lse = reinterpret_cast<const float4*>(ctl.lse[j % S::kRowsQ] + quarter * 16);
+        const float4* del = reinterpret_cast<const float4*>(ctl.delta[j % S::kRowsQ] + quarter * 16);
         uint32_t x[16];
         float p[16];
         tmem_load16(tm_s + off, x);
