@@ -106,6 +106,16 @@ DCT_DEV void tmem_load(uint32_t addr, uint32_t (&r)[16]) { tmem_load16(addr, r);
 DCT_DEV void tmem_store(uint32_t addr, const uint32_t (&r)[16]) { tmem_store16(addr, r); }
 DCT_DEV void tmem_store(uint32_t addr, const uint32_t (&r)[8]) { tmem_store8(addr, r); }
 
+// One thread of a converged warp.  The compiler knows that a branch on it has one thread, and
+// forms the operands of the instructions inside in uniform registers; behind `lane == 0` it
+// moves each there, and with busy warps beside it the issuing warp then took 550 cycles for
+// a matrix instruction of 64 (72 with this).
+DCT_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // ---- matrix instructions ---------------------------------------------------------
 // Shared memory descriptor of a 128-byte swizzled operand (start address, leading and
 // stride byte offsets in units of 16; version 1; swizzle mode 2).

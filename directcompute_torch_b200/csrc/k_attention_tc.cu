@@ -449,17 +449,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
   Waits wait{err};
 
   if (warp == kSoft) {
-    if (lane == 0)
+    if (elect_one())
       ctl.k.fill(n, S::kTileBytes, wait, [&](int it, int s, uint64_t* bar) {
         load_tile<BLOCKS>(w, bh, 1, t0 + it, sm + s * S::kTileBytes, bar);
       });
   } else if (warp == kSoft + 2) {
-    if (lane == 0)
+    if (elect_one())
       ctl.v.fill(2 * n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
         load_half<BLOCKS>(w, bh, 2, 2 * t0 + it, sm + S::kV + s * S::kSlotBytes, bar);
       });
   } else if (warp == kSoft + 1) {
-    if (lane == 0 && n) {
+    if (n && elect_one()) {
       wait(&ctl.q_full, 0);
       auto scores = [&](int j) {                   // S(j) = Q K(j)^T
         if (!ctl.k.ready(j, wait)) return;
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
   Waits wait{err};
 
   if (warp == kSoft) {
-    if (lane == 0 && n) {
+    if (n && elect_one()) {
       mbar_arrive_expect_tx(&ctl.q_full, S::kTileBytes);
       load_tile<BLOCKS>(w, bh, 0, tile, sm, &ctl.q_full);
       ctl.k.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
@@ -675,12 +675,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       mbar_wait(&ctl.q_full, 0, err);
     }
   } else if (warp == kSoft + 2) {
-    if (lane == 0)
+    if (elect_one())
       ctl.v.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
         load_half<BLOCKS>(w, bh, 2, t0 + it, sm + S::kV + s * S::kSlotBytes, bar);
       });
   } else if (warp == kSoft + 1) {
-    if (lane == 0 && n) {
+    if (n && elect_one()) {
       wait(&ctl.q_full, 0);
       wait(&ctl.go_full, 0);
       const uint64_t q = umma_desc(smem_addr(sm), kChunkBytes, 1024);
@@ -824,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
   Waits wait{err};
 
   if (warp == kSoft) {
-    if (lane == 0 && n) {
+    if (n && elect_one()) {
       mbar_arrive_expect_tx(&ctl.k_full, S::kTileBytes);
       load_tile<BLOCKS>(w, bh, 1, tile, sm, &ctl.k_full);
       ctl.q.fill(n, S::kSlotBytes + 2 * kHalf * 4, wait, [&](int it, int s, uint64_t* bar) {
@@ -836,12 +836,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       mbar_wait(&ctl.k_full, 0, err);
     }
   } else if (warp == kSoft + 2) {
-    if (lane == 0)
+    if (elect_one())
       ctl.go.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
         load_half<BLOCKS>(w, bh, 3, t0 + it, sm + S::kGo + s * S::kSlotBytes, bar);
       });
   } else if (warp == kSoft + 1) {
-    if (lane == 0 && n) {
+    if (n && elect_one()) {
       wait(&ctl.k_full, 0);
       wait(&ctl.v_full, 0);
       const uint64_t k = umma_desc(smem_addr(sm), kChunkBytes, 1024);

@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
   };
 
   if (warp == kEpi) {
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t it = 0;
       bool ok = true;
       while (ok && run.next(sg)) {
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
         mbar_wait(&full[u % S::kStages], (u / S::kStages) & 1, err);
     }
   } else if (warp == kEpi + 1 && rank != 0) {
-    if (lane == 0) {                              // tells the even block of each chunk that has come in
+    if (elect_one()) {                              // tells the even block of each chunk that has come in
       uint32_t it = 0;
       bool ok = true;
       while (ok && run.next(sg))
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
         }
     }
   } else if (warp == kEpi + 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       auto mma = [](uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
         if constexpr (PAIR) umma_pair(d, a, b, idesc, add);
         else umma(d, a, b, idesc, add);
