@@ -44,45 +44,35 @@ struct RowAt {                 // a row's query position and head
 DCT_DEV int64_t at(const int64_t* s, int b, int t, int h) { return b * s[0] + t * s[1] + h * s[2]; }
 
 // ---------------------------------------------------------------------------
-// what the tensor-core kernels know about a key head's operands (q, k, v, dout)
+// what the tensor-core kernels know about their operands (q, k, v, dout)
 // ---------------------------------------------------------------------------
-// Magnitudes over the valid rows as float bits, which order like integers, so that they
-// meet by atomic maximum from 0 (the same in any order).
-struct AttnStats {
-  uint32_t top[4];             // the largest |x|; from 0x7f800000 on: infinity or NaN
-  uint32_t low[4];             // ~ the smallest row maximum that is not 0
-  uint32_t norm[4];            // the largest row norm
-};
-// Each operand is held as 2^e x = hi + lo in float16 with its largest magnitude in
+// A tile of 128 rows is held as 2^e x = hi + lo in float16 with its largest magnitude in
 // [2^14, 2^15); an element is then off by 2^-23 of itself or 2^-40 of that largest one.
-// dS is scaled by 2^eds, from |dS / (P scale)| <= 2 max|dout row| max|v row|.
-struct AttnScales {
-  int e[4], eds;
-  bool split;                  // false: the head goes to the float32 kernels
+struct AttnTile {
+  int32_t e;
+  float norm;                  // of v and dout: a bound on its rows' norms
 };
-DCT_DEV AttnScales scales_of(const AttnStats& st, float scale, int dim, bool backward) {
-  AttnScales s;
-  s.split = true;
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    if (t == 3 && !backward) { s.e[t] = 0; break; }
-    const int top = (int)(st.top[t] >> 23) - 127, low = st.low[t] ? (int)(~st.low[t] >> 23) - 127 : top;
-    s.e[t] = st.top[t] ? 14 - top : 0;
-    // infinities and NaN; sizes whose scaling leaves float32; rows so far apart that the
-    // small ones would lose their own accuracy to the common scale
-    if (st.top[t] && (top < -100 || top > 100 || low < top - 14)) s.split = false;
-  }
-  // scores beyond 2^18 amplify the common scale's 2^-40 past float32's own error
-  const float most = __uint_as_float(st.top[0]) * __uint_as_float(st.top[1]);
-  if (!(fabsf(scale) * dim * most < 262144.f)) s.split = false;
-  s.eds = 0;
-  if (backward) {
-    const float n = __uint_as_float(st.norm[2]) * __uint_as_float(st.norm[3]);
-    if (!(n < 1e30f)) s.split = false;
-    else if (n > 0.f) s.eds = 13 - ((int)(__float_as_uint(n) >> 23) - 127);
-    if (n > 0.f && n < 1e-30f) s.split = false;
-  }
-  return s;
+// Of a key head: magnitudes as float bits, which order like integers, so that they meet by
+// atomic maximum from 0 (the same in any order).
+struct AttnStats {
+  uint32_t top_q, top_k;       // the largest |q|, |k|
+  uint32_t bad;                // some tile cannot be split
+  uint32_t top_v, low_v;       // the largest |v| of a tile, and ~ the smallest that is not 0
+  uint32_t pad[3];
+};
+// Tiles of infinities or NaN, of sizes whose scaling could leave float32, or with rows so far
+// apart that the small ones would lose their own accuracy to the common scale, cannot be
+// split.  `low` is the smallest row maximum that is not 0.
+DCT_DEV bool tile_splits(uint32_t top, uint32_t low) {
+  const int t = (int)(top >> 23) - 127, l = (int)(low >> 23) - 127;
+  return top == 0 || (t >= -60 && t <= 44 && l >= t - 14);
+}
+// Whether a head takes the tensor cores: scores beyond 2^18 would amplify a tile's 2^-40 past
+// float32's own error; tiles of v further than 2^60 apart could overflow the running outputs,
+// which carry the scale of the tile added last.
+DCT_DEV bool head_splits(const AttnStats& st, float scale, int dim) {
+  if (st.low_v && (int)(st.top_v >> 23) - (int)(~st.low_v >> 23) > 60) return false;
+  return !st.bad && fabsf(scale) * dim * __uint_as_float(st.top_q) * __uint_as_float(st.top_k) < 262144.f;
 }
 
 }  // namespace dct

@@ -77,7 +77,7 @@ DCT_DEV void rows_forward(const AttnArgs& a, int item, int groups, int splits, f
   const int lane = threadIdx.x & 7, oct = threadIdx.x >> 3, warp = threadIdx.x >> 5;
   const int split = item % splits, gi = (item / splits) % groups, bh = item / splits / groups;
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads, rows = a.q_len * a.group;
-  if (a.stats && scales_of(a.stats[bh], a.scale, a.dim, false).split) return;
+  if (a.stats && head_splits(a.stats[bh], a.scale, a.dim)) return;
   const AttnSpan span(a, b);
   const float scale = a.scale * kLog2e;
 
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ AttnA
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= (int64_t)a.batch * a.kv_heads * rows) return;
   const int bh = (int)(row / rows);
-  if (a.stats && scales_of(a.stats[bh], a.scale, a.dim, false).split != tensor) return;
+  if (a.stats && head_splits(a.stats[bh], a.scale, a.dim) != tensor) return;
   const float* rec = record(part, a, row, splits, 0);
   const int step = a.dim + 2;
   float best = -INFINITY, s = 0.f;
@@ -267,7 +267,7 @@ DCT_DEV void rows_dq(const AttnArgs& a, int item, int groups, float (&sh)[kWarps
   const int lane = threadIdx.x & 7, oct = threadIdx.x >> 3;
   const int gi = item % groups, bh = item / groups;
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads, rows = a.q_len * a.group;
-  if (a.stats && scales_of(a.stats[bh], a.scale, a.dim, true).split) return;
+  if (a.stats && head_splits(a.stats[bh], a.scale, a.dim)) return;
   const AttnSpan span(a, b);
   const float scale = a.scale * kLog2e;
   float q[R][F], go[R][F], dq[R][F], lse[R], delta[R];
@@ -329,7 +329,7 @@ DCT_DEV void rows_dkv(const AttnArgs& a, int item, int groups, float (&sh)[kWarp
   const int lane = threadIdx.x & 7, oct = threadIdx.x >> 3;
   const int gi = item % groups, bh = item / groups;
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  if (a.stats && scales_of(a.stats[bh], a.scale, a.dim, true).split) return;
+  if (a.stats && head_splits(a.stats[bh], a.scale, a.dim)) return;
   const AttnSpan span(a, b);
   const float scale = a.scale * kLog2e;
   float k[R][F], v[R][F], dk[R][F], dv[R][F];

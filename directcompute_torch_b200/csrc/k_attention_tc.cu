@@ -1,9 +1,9 @@
 // Attention on the fifth-generation tensor cores at float32 accuracy.
 //
-// A pass over the operands finds each key head's magnitudes (k_attn_scan), a second writes
-// them as split float16 tiles of 128 rows (k_attn_split; layout and arithmetic in
-// dct_umma.cuh), and the products run on those: three matrix instructions for each product
-// of float32 numbers, so the bound is a third of the float16 rate, about 540 TFLOP/s.
+// A pass over the operands writes them as split float16 tiles of 128 rows, each with a power
+// of two of its own (k_attn_split; arithmetic and layout in dct_umma.cuh), and the products
+// run on those: three matrix instructions for each product of float32 numbers, so the bound
+// is a third of the float16 rate, about 540 TFLOP/s.
 //
 // A tile is [64 features][hi, lo][128 rows][64 float16], 32 KB for every 64 features, so
 // one bulk copy brings it and it serves as either operand: with its features as the
@@ -30,13 +30,16 @@ DCT_DEV float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// 2^e for -126 <= e <= 127; the tiles' exponents and their sums are clamped to that
+DCT_DEV float pow2(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
 DCT_DEV uint32_t lane_bits(int warp) { return (uint32_t)(warp & 3) * 32u << 16; }
 
 struct Tiles {
   uint8_t* p[4];               // q, k, v, dout
+  AttnTile* info[4];           // [heads][tiles]
   AttnStats* stats;            // [heads]
-  uint32_t* any;               // set where a head cannot be split
-  float *lse2, *delta;         // [heads][padded rows], backward: log2 units, 2^eds delta
+  uint32_t* any;               // set where a head does not take the tensor cores
+  float *lse2, *delta;         // [heads][padded rows], backward: log-sums in log2 units, sum dout out
   int64_t tiles[4];            // of a head
   int blocks;                  // of 64 features
 };
@@ -66,139 +69,126 @@ DCT_DEV void store_features(float* row, int first, int dim, bool vec, const floa
 }
 
 // ---------------------------------------------------------------------------
-// magnitudes, splitting
+// splitting
 // ---------------------------------------------------------------------------
-constexpr int kScanRows = 64;
-
-// blocks [tensor][head][64 rows]; a warp takes four rows at a time, a lane four features
-template <bool VEC>
-__global__ void __launch_bounds__(256) k_attn_scan(const __grid_constant__ AttnArgs a, AttnStats* stats, int per_q,
-                                                   int per_k, int backward) {
+// blocks [tensor][head][tile] of 512 threads; a thread takes 8 features of every 32nd (64th)
+// row and holds them while the block finds the tile's magnitude, so each operand is read
+// once.  With dout come delta = sum dout out and the log-sums.  Bound by memory: 8 bytes a
+// feature (12 for dout).
+template <int BLOCKS>
+__global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ AttnArgs a, const __grid_constant__ Tiles w,
+                                                    int tq, int tk, bool vec) {
+  constexpr int kGroups = 8 * BLOCKS, kStep = 512 / kGroups, kPasses = kTile / kStep;
   __shared__ uint32_t sh[3];
-  const int heads = a.batch * a.kv_heads, lane = threadIdx.x & 31;
+  const int heads = a.batch * a.kv_heads;
   int x = blockIdx.x, t = 0;
-  for (; t < 3; ++t) {                            // q, k, v, dout in turn
-    const int n = heads * (t == 0 ? per_q : per_k);
+  for (; t < 3; ++t) {                             // q, k, v, dout in turn
+    const int n = heads * (t == 0 ? tq : tk);
     if (x < n) break;
     x -= n;
   }
-  const int per = t == 1 || t == 2 ? per_k : per_q, bh = x / per, r0 = (x - bh * per) * kScanRows;
-  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const int rows = min(rows_of(a, AttnSpan(a, b), t), r0 + kScanRows);
+  const int per = t == 1 || t == 2 ? tk : tq, bh = x / per, tile = x - bh * per;
+  const int g = threadIdx.x % kGroups, row0 = threadIdx.x / kGroups, b = bh / a.kv_heads, hk = bh % a.kv_heads;
+  const AttnSpan span(a, b);
+  const int rows = rows_of(a, span, t);
   if (threadIdx.x < 3) sh[threadIdx.x] = 0;
   __syncthreads();
+  float v[kPasses][8];
   uint32_t top = 0, low = 0, norm = 0;
-  for (int r = r0 + (threadIdx.x >> 5) * 4; r < rows; r += 32) {
-    float v[4][4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float* p = row_of(a, t, b, hk, min(r + u, rows - 1)) + 4 * lane;
-      if constexpr (VEC) {
-        *reinterpret_cast<float4*>(v[u]) =
-            4 * lane < a.dim ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p = 0; p < kPasses; ++p) {
+    const int r = tile * kTile + row0 + p * kStep;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[p][e] = 0.f;
+    if (r >= rows) continue;
+    const float* src = row_of(a, t, b, hk, r) + g * 8;
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      if (vec) {
+        if (g * 8 + e < a.dim) *reinterpret_cast<float4*>(v[p] + e) = *reinterpret_cast<const float4*>(src + e);
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[u][e] = 4 * lane + e < a.dim ? p[e] : 0.f;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(v[u][e]) & 0x7fffffffu);
-      m = __reduce_max_sync(0xffffffffu, m);
-      top = max(top, m);
-      if (m) low = max(low, ~m);
-      if (backward && t >= 2 && m && m < 0x7f800000u) {
-        // the norm through the row's own scale, so that squares neither vanish nor overflow
-        const float f = __uint_as_float(m), g = 1.f / f;
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s = fmaf(v[u][e] * g, v[u][e] * g, s);
-        norm = max(norm, __float_as_uint(1.001f * f * sqrtf(warp_sum_f(s))));
+        for (int q = 0; q < 4; ++q)
+          if (g * 8 + e + q < a.dim) v[p][e + q] = src[e + q];
       }
     }
   }
-  if (lane == 0) {
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[p][e]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < kGroups; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    top = max(top, m);
+    if (m) low = max(low, ~m);
+    if (t >= 2) {
+      // the row's norm through its own scale, so that squares neither vanish nor overflow
+      const float f = __uint_as_float(m), i = m ? 1.f / f : 0.f;
+      float s = 0.f, d = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = fmaf(v[p][e] * i, v[p][e] * i, s);
+      const int r = tile * kTile + row0 + p * kStep;
+      if (t == 3 && r < rows) {
+        const RowAt q(a, hk, r);
+        const float* o = a.out + at(a.os, b, q.i, q.h) + g * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (g * 8 + e < a.dim) d = fmaf(v[p][e], o[e], d);
+      }
+#pragma unroll
+      for (int o = 1; o < kGroups; o <<= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        d += __shfl_xor_sync(0xffffffffu, d, o);
+      }
+      if (m < 0x7f800000u) norm = max(norm, __float_as_uint(1.001f * f * sqrtf(s)));
+      if (t == 3 && g == 0) {
+        const int64_t at_row = (int64_t)bh * padded_rows(a) + r;
+        float l = INFINITY;                        // a row that sees nothing: P = 2^(s - inf) = 0
+        if (r < rows) {
+          const RowAt q(a, hk, r);
+          l = a.lse[((int64_t)b * a.q_heads + q.h) * a.q_len + q.i] * kLog2e;
+          if (l == -INFINITY) l = INFINITY;
+        }
+        w.lse2[at_row] = l;
+        w.delta[at_row] = d;
+      }
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  low = __reduce_max_sync(0xffffffffu, low);
+  norm = __reduce_max_sync(0xffffffffu, norm);
+  if ((threadIdx.x & 31) == 0) {
     atomicMax(&sh[0], top);
     atomicMax(&sh[1], low);
     atomicMax(&sh[2], norm);
   }
   __syncthreads();
-  if (threadIdx.x == 0 && sh[0]) {
-    atomicMax(&stats[bh].top[t], sh[0]);
-    atomicMax(&stats[bh].low[t], sh[1]);
-    if (sh[2]) atomicMax(&stats[bh].norm[t], sh[2]);
-  }
-}
-
-// blocks [tensor][head][tile][16 rows]; a thread takes 8 features of a row, 8 or 16
-// neighbouring ones a row.  With dout come delta = sum dout out and the log-sums.
-template <int BLOCKS>
-__global__ void __launch_bounds__(128 * BLOCKS) k_attn_split(const __grid_constant__ AttnArgs a,
-                                                             const __grid_constant__ Tiles w, int tq, int tk,
-                                                             int backward, bool vec) {
-  pdl_entry();
-  const int heads = a.batch * a.kv_heads;
-  int x = blockIdx.x, t = 0;
-  for (; t < 3; ++t) {
-    const int n = heads * (t == 0 ? tq : tk) * 8;
-    if (x < n) break;
-    x -= n;
-  }
-  const int per = (t == 1 || t == 2 ? tk : tq) * 8, bh = x / per, r = (x - bh * per) * 16 + threadIdx.x / (8 * BLOCKS);
-  const int g = threadIdx.x % (8 * BLOCKS), b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const AttnSpan span(a, b);
-  const bool in = r < rows_of(a, span, t);
-  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, backward);
-  if (!sc.split && threadIdx.x == 0) *w.any = 1;  // work for the float32 kernels
-  if (!sc.split && t != 3) return;
-  float v[8] = {};
-  if (in) {
-    const float* p = row_of(a, t, b, hk, r);
-#pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      const int f = g * 8 + e;
-      if (vec) {
-        if (f < a.dim) *reinterpret_cast<float4*>(v + e) = *reinterpret_cast<const float4*>(p + f);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[e + q] = f + q < a.dim ? p[f + q] : 0.f;
-      }
+  top = sh[0];
+  const bool splits = tile_splits(top, ~sh[1]);
+  const int e = top && splits ? 14 - ((int)(top >> 23) - 127) : 0;
+  if (threadIdx.x == 0) {
+    w.info[t][bh * w.tiles[t] + tile] = AttnTile{e, __uint_as_float(sh[2])};
+    if (t == 0) atomicMax(&w.stats[bh].top_q, top);
+    if (t == 1) atomicMax(&w.stats[bh].top_k, top);
+    if (t == 2 && top) {
+      atomicMax(&w.stats[bh].top_v, top);
+      atomicMax(&w.stats[bh].low_v, ~top);
     }
+    if (!splits) w.stats[bh].bad = 1;
   }
-  if (t == 3) {
-    float d = 0.f;
-    if (in) {
-      const RowAt q(a, hk, r);
-      const float* o = a.out + at(a.os, b, q.i, q.h);
+  if (!splits) return;
+  const float f = pow2(e);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (g * 8 + e < a.dim) d = fmaf(v[e], o[g * 8 + e], d);
-    }
+  for (int p = 0; p < kPasses; ++p) {
+    uint32_t h[4], l[4];
 #pragma unroll
-    for (int o = 1; o < 8 * BLOCKS; o <<= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (g == 0) {
-      const int64_t at_row = (int64_t)bh * padded_rows(a) + r;
-      float l = INFINITY;                         // a row that sees nothing: P = 2^(s - inf) = 0
-      if (in) {
-        const RowAt q(a, hk, r);
-        l = a.lse[((int64_t)b * a.q_heads + q.h) * a.q_len + q.i] * kLog2e;
-        if (l == -INFINITY) l = INFINITY;
-      }
-      w.lse2[at_row] = l;
-      w.delta[at_row] = sc.split ? ldexpf(d, sc.eds) : d;
-    }
-    if (!sc.split) return;
+    for (int q = 0; q < 4; ++q) split2(v[p][2 * q] * f, v[p][2 * q + 1] * f, h[q], l[q]);
+    uint8_t* o = w.p[t] + ((bh * w.tiles[t] + tile) * BLOCKS + g / 8) * (int64_t)kBlockBytes +
+                 chunk_at(row0 + p * kStep, g % 8);
+    *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(o + kBlockBytes / 2) = make_uint4(l[0], l[1], l[2], l[3]);
   }
-  const float f = ldexpf(1.f, sc.e[t]);
-  uint32_t h[4], l[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) split2(v[2 * e] * f, v[2 * e + 1] * f, h[e], l[e]);
-  uint8_t* o = w.p[t] + ((bh * w.tiles[t] + r / kTile) * BLOCKS + g / 8) * (int64_t)kBlockBytes +
-               chunk_at(r % kTile, g % 8);
-  *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
-  *reinterpret_cast<uint4*>(o + kBlockBytes / 2) = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
 // ---------------------------------------------------------------------------
@@ -428,13 +418,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
   const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads;
   const int split = blockIdx.x / heads % splits, tile = row_tiles - 1 - blockIdx.x / heads / splits;  // long rows first
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, false);
+  const bool splits_head = head_splits(w.stats[bh], a.scale, a.dim);
+  if (!splits_head && threadIdx.x == 0) *w.any = 1;          // work for the float32 kernels
   const AttnSpan span(a, b);
   const int rows = a.q_len * a.group, r0 = tile * kTile;
   // keys of the tile's rows
   const int i0 = r0 / a.group, i1 = min(min(r0 + kTile, rows) - 1, span.m * a.group - 1) / a.group;
   int t0 = 0, n = 0;
-  if (sc.split && i0 < span.m) {
+  if (splits_head && i0 < span.m) {
     const int k0 = span.lo(a, i0), k1 = span.hi(a, i1);
     t0 = k0 / kTile;
     int t1 = k1 > k0 ? (k1 + kTile - 1) / kTile : t0;
@@ -483,14 +474,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
         umma_commit(&ctl.o_full);
       }
     }
-  } else if (sc.split) {
+  } else if (splits_head) {
     const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
     const RowAt at_row(a, hk, min(r, rows - 1));
     const bool in = r < rows && at_row.i < span.m;
     const int lo = in ? span.lo(a, at_row.i) : 0, hi = in ? span.hi(a, at_row.i) : 0;
-    // (not 0: a masked score is infinite, and times 0 it would not be)
-    const float f = copysignf(fmaxf(fabsf(ldexpf(a.scale * kLog2e, -(sc.e[0] + sc.e[1]))), 1e-36f), a.scale);
-    const float hidden = f < 0.f ? INFINITY : -INFINITY;
+    const AttnTile *ki = w.info[1] + bh * w.tiles[1] + t0, *vi = w.info[2] + bh * w.tiles[2] + t0;
+    const int eq = w.info[0][bh * w.tiles[0] + tile].e;
+    const float scale = a.scale * kLog2e, hidden = scale < 0.f ? INFINITY : -INFINITY;
+    int ek = n ? ki[0].e : 0, ev = n ? vi[0].e : 0, ev_last = ev;    // of the tile at hand, of the one before
     float o[S::kF], top = -INFINITY, sum = 0.f, scale_o = 1.f;
 #pragma unroll
     for (int e = 0; e < S::kF; ++e) o[e] = 0.f;
@@ -510,6 +502,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
     };
     for (int j = 0; j < n; ++j) {
       const int key = (t0 + j) * kTile + quarter * 32;
+      // (f is not 0: a masked score is infinite, and times 0 it would not be)
+      const float f = copysignf(fmaxf(fabsf(scale * pow2(-eq - ek)), 1e-36f), scale);
+      const int ek_next = j + 1 < n ? ki[j + 1].e : 0, ev_next = j + 1 < n ? vi[j + 1].e : 0;
       wait(&ctl.s_full[j & 1], j >> 1);
       const uint32_t addr = tm_s + lane_bits(warp) + (j & 1) * kTile + quarter * 32;
       uint32_t x[32];
@@ -550,7 +545,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
       tmem_wait_st();
       arrive_warp(&ctl.p_full[j & 1]);
       if (j) take(j - 1);
-      scale_o = move;
+      // the outputs are held as 2^ev of the tile that was added last
+      scale_o = move * pow2(ev - ev_last);
+      ev_last = ev;
+      ek = ek_next;
+      ev = ev_next;
     }
     if (n) take(n - 1);
     // the four quarters of a row meet
@@ -558,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
     rows_sync(warp);
     sum = (ctl.exch[0][row] + ctl.exch[1][row]) + (ctl.exch[2][row] + ctl.exch[3][row]);
     if (wait.ok && r < rows) {
-      float back = ldexpf(1.f, -sc.e[2]);
+      float back = pow2(-ev_last);
       const float down = exp2f(-kUp);
       if (splits > 1) {
         float* rec = part + (((int64_t)bh * rows + r) * splits + split) * (a.dim + 2);
@@ -595,15 +594,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
 // seven products instead of five, but every gradient has one owner, no atomics and one
 // order.
 constexpr float kUpP = 14.f;                       // P <= 1 is held as 2^14 P
-constexpr int kGroup = 2;                          // half tiles between drains of an accumulator
 
+// The accumulators are drained after every tile of the inner side, whose scales they carry.
 template <int N>
-DCT_DEV void drain(uint32_t addr, float (&acc)[N]) {
-  uint32_t v[N];
-  tmem_load(addr, v);
-  tmem_wait_ld();
+DCT_DEV void drain(uint32_t addr, float f, float (&acc)[N]) {
 #pragma unroll
-  for (int e = 0; e < N; ++e) acc[e] += __uint_as_float(v[e]);
+  for (int c = 0; c < N; c += 16) {                // by 16: registers are short
+    uint32_t v[16];
+    tmem_load16(addr + c, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(__uint_as_float(v[e]), f, acc[c + e]);
+  }
+}
+
+// dS is held as 2^eds dS / scale, from |dS / (P scale)| <= 2 max|dout row| max|v row|
+DCT_DEV int scale_of_ds(float norm_do, float norm_v) {
+  const float n = norm_do * norm_v;
+  return n > 0.f ? min(13 - ((int)(__float_as_uint(n) >> 23) - 127), 120) : 0;
 }
 
 template <int BLOCKS>
@@ -653,12 +661,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
   pdl_entry();
   const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = row_tiles - 1 - blockIdx.x / heads;
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, true);
+  const bool splits_head = head_splits(w.stats[bh], a.scale, a.dim);
+  if (!splits_head && threadIdx.x == 0) *w.any = 1;          // work for the float32 kernels
   const AttnSpan span(a, b);
   const int rows = a.q_len * a.group, r0 = tile * kTile;
   const int i0 = r0 / a.group, i1 = min(min(r0 + kTile, rows) - 1, span.m * a.group - 1) / a.group;
   int t0 = 0, n = 0;
-  if (sc.split && i0 < span.m) {
+  if (splits_head && i0 < span.m) {
     const int k0 = span.lo(a, i0), k1 = span.hi(a, i1);
     t0 = k0 / kHalf;
     n = k1 > k0 ? (k1 + kHalf - 1) / kHalf - t0 : 0;
@@ -694,23 +703,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         ctl.v.release(j);
         umma_commit(&ctl.s_full[j & 1]);
       };
+      int group = 0;
       scores(0);
       for (int j = 0; j < n && wait.ok; ++j) {
         if (j + 1 < n) scores(j + 1);
         wait(&ctl.ds_full[j & 1], j >> 1);
-        if (j % kGroup == 0) wait(&ctl.acc_empty, (j / kGroup) ^ 1);
+        const bool first = j == 0 || !((t0 + j) & 1), last = j == n - 1 || ((t0 + j) & 1);   // of its tile
+        if (first) wait(&ctl.acc_empty, group++ ^ 1);
         if (!wait.ok) break;
-        mma_rows<BLOCKS, 16>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(key(j), 2 * kChunkBytes, 1024), j % kGroup != 0);
+        mma_rows<BLOCKS, 16>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(key(j), 2 * kChunkBytes, 1024), !first);
         ctl.k.release(j);
-        if (j % kGroup == kGroup - 1 || j == n - 1) umma_commit(&ctl.acc_full);
+        if (last) umma_commit(&ctl.acc_full);
       }
     }
-  } else if (sc.split) {
+  } else if (splits_head) {
     const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
     const RowAt at_row(a, hk, min(r, rows - 1));
     const bool in = r < rows && at_row.i < span.m;
     const int lo = in ? span.lo(a, at_row.i) : 0, hi = in ? span.hi(a, at_row.i) : 0;
-    const float f = ldexpf(a.scale * kLog2e, -(sc.e[0] + sc.e[1])), fd = ldexpf(1.f, sc.eds - sc.e[3] - sc.e[2]);
+    const AttnTile *ki = w.info[1] + bh * w.tiles[1], *vi = w.info[2] + bh * w.tiles[2];
+    const int eq = w.info[0][bh * w.tiles[0] + tile].e;
+    const AttnTile go = w.info[3][bh * w.tiles[3] + tile];
     float acc[S::kF];
 #pragma unroll
     for (int e = 0; e < S::kF; ++e) acc[e] = 0.f;
@@ -720,13 +733,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       tile_to_tmem<BLOCKS>(w.p[3] + (bh * w.tiles[3] + tile) * (int64_t)S::kTileBytes, tm_go, warp, row);
       tmem_wait_st();
       arrive_warp(&ctl.go_full);
+      float f = 0.f, fd = 0.f, ds_delta = 0.f, back = 0.f;
+      int group = 0;
       auto take = [&](int group) {
         wait(&ctl.acc_full, group);
-        drain(tm_acc + lane_bits(warp) + quarter * S::kF, acc);
+        drain(tm_acc + lane_bits(warp) + quarter * S::kF, back, acc);
         arrive_warp(&ctl.acc_empty);
       };
+      AttnTile kt = ki[t0 >> 1], vt = vi[t0 >> 1];
       for (int j = 0; j < n; ++j) {
         const int key = (t0 + j) * kHalf + quarter * 16;
+        float back_next = back;
+        if (j == 0 || !((t0 + j) & 1)) {           // another tile of K and V
+          const int eds = scale_of_ds(go.norm, vt.norm);
+          f = a.scale * kLog2e * pow2(-eq - kt.e);
+          fd = pow2(eds - go.e - vt.e);
+          ds_delta = delta * pow2(eds);
+          back_next = ldexpf(a.scale, -eds - kt.e);
+          const int next = ((t0 + j) >> 1) + 1;
+          if (next <= (t0 + n - 1) >> 1) {
+            kt = ki[next];
+            vt = vi[next];
+          }
+        }
         wait(&ctl.s_full[j & 1], j >> 1);
         const uint32_t off = lane_bits(warp) + (j & 1) * kHalf + quarter * 16;
         uint32_t x[16], y[16];
@@ -736,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         float ds[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          ds[e] = ex2(fmaf(__uint_as_float(x[e]), f, -lse2)) * fmaf(__uint_as_float(y[e]), fd, -delta);
+          ds[e] = ex2(fmaf(__uint_as_float(x[e]), f, -lse2)) * fmaf(__uint_as_float(y[e]), fd, -ds_delta);
         if (__any_sync(0xffffffffu, key < lo || key + 16 > hi)) {
 #pragma unroll
           for (int e = 0; e < 16; ++e)
@@ -745,14 +774,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         store_operand<16>(tm_s + off, ds);
         tmem_wait_st();
         arrive_warp(&ctl.ds_full[j & 1]);
-        if (j && j % kGroup == 0) take(j / kGroup - 1);
+        if (j && !((t0 + j) & 1)) take(group++);
+        back = back_next;
       }
-      take((n - 1) / kGroup);
+      take(group);
     }
     if (r < rows) {
-      const float back = ldexpf(a.scale, -(sc.eds + sc.e[1]));
-#pragma unroll
-      for (int e = 0; e < S::kF; ++e) acc[e] *= back;
       store_features<S::kF>(a.dq + at(a.dqs, b, at_row.i, at_row.h), quarter * S::kF, a.dim, vec_out, acc);
     }
   }
@@ -769,7 +796,7 @@ struct Dkv : Sizes<BLOCKS> {
     float lse[kRowsQ][kHalf], delta[kRowsQ][kHalf];  // with Q; 16-byte aligned: the bulk copies' targets
     Ring<kRowsQ> q;
     Ring<kRowsGo> go;
-    uint64_t k_full, v_full, s_full, dp_full, p_full, ds_full, acc_full, acc_empty;
+    uint64_t k_full, v_full, s_full, dp_full, p_full, ds_full, dv_full, dv_empty, dk_full, dk_empty;
     uint32_t tmem;
   };
   static constexpr uint32_t kQ = Sizes<BLOCKS>::kTileBytes, kGo = kQ + kRowsQ * Sizes<BLOCKS>::kSlotBytes;
@@ -799,8 +826,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     mbar_init(&ctl.dp_full, 1);
     mbar_init(&ctl.p_full, kSoft);
     mbar_init(&ctl.ds_full, kSoft);
-    mbar_init(&ctl.acc_full, 1);
-    mbar_init(&ctl.acc_empty, kSoft);
+    mbar_init(&ctl.dv_full, 1);
+    mbar_init(&ctl.dv_empty, kSoft);
+    mbar_init(&ctl.dk_full, 1);
+    mbar_init(&ctl.dk_empty, kSoft);
     mbar_fence_init();
   }
   if (warp == kSoft + 1) tmem_alloc(&ctl.tmem, 512);
@@ -812,11 +841,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
   pdl_entry();
   const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = blockIdx.x / heads;    // long ones first
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const AttnScales sc = scales_of(w.stats[bh], a.scale, a.dim, true);
+  const bool splits_head = head_splits(w.stats[bh], a.scale, a.dim);
+  if (!splits_head && threadIdx.x == 0) *w.any = 1;          // work for the float32 kernels
   const AttnSpan span(a, b);
   const int j0 = tile * kTile, j1 = min(j0 + kTile, span.n) - 1;
   int t0 = 0, n = 0;
-  if (sc.split && j0 < span.n) {
+  if (splits_head && j0 < span.n) {
     const int first = span.first(a, j0) * a.group, last = span.last(a, j1) * a.group;
     t0 = first / kHalf;
     n = last > first ? (last + kHalf - 1) / kHalf - t0 : 0;
@@ -859,25 +889,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       };
       scores(0);
       dps(0);
+      int group = 0;
       for (int j = 0; j < n && wait.ok; ++j) {
+        const bool first = j == 0 || !((t0 + j) & 1), last = j == n - 1 || ((t0 + j) & 1);   // of its tile
         wait(&ctl.p_full, j);
-        if (j % kGroup == 0) wait(&ctl.acc_empty, (j / kGroup) ^ 1);
+        if (first) wait(&ctl.dv_empty, group ^ 1);
         if (!wait.ok) break;
-        mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(grad(j), 2 * kChunkBytes, 1024), j % kGroup != 0);
+        mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(grad(j), 2 * kChunkBytes, 1024), !first);
         ctl.go.release(j);
+        if (last) umma_commit(&ctl.dv_full);
         if (j + 1 < n) scores(j + 1);
-        if (!wait(&ctl.ds_full, j)) break;
-        mma_rows<BLOCKS, 16>(tm_dk, tm_dp, umma_desc(query(j), 2 * kChunkBytes, 1024), j % kGroup != 0);
+        wait(&ctl.ds_full, j);
+        if (first) wait(&ctl.dk_empty, group++ ^ 1);
+        if (!wait.ok) break;
+        mma_rows<BLOCKS, 16>(tm_dk, tm_dp, umma_desc(query(j), 2 * kChunkBytes, 1024), !first);
         ctl.q.release(j);
-        if (j % kGroup == kGroup - 1 || j == n - 1) umma_commit(&ctl.acc_full);
+        if (last) umma_commit(&ctl.dk_full);
         if (j + 1 < n) dps(j + 1);
       }
     }
-  } else if (sc.split) {
+  } else if (splits_head) {
     const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, key = j0 + row;
     // rows that see the thread's key
     const int lo = key < span.n ? span.first(a, key) * a.group : 0, hi = key < span.n ? span.last(a, key) * a.group : 0;
-    const float f = ldexpf(a.scale * kLog2e, -(sc.e[0] + sc.e[1])), fd = ldexpf(1.f, sc.eds - sc.e[3] - sc.e[2]);
+    const AttnTile *qi = w.info[0] + bh * w.tiles[0], *gi = w.info[3] + bh * w.tiles[3];
+    const int ek = w.info[1][bh * w.tiles[1] + tile].e;
+    const AttnTile vt = w.info[2][bh * w.tiles[2] + tile];
     float dk[S::kF], dv[S::kF];
 #pragma unroll
     for (int e = 0; e < S::kF; ++e) dk[e] = dv[e] = 0.f;
@@ -885,15 +922,40 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       tile_to_tmem<BLOCKS>(w.p[2] + (bh * w.tiles[2] + tile) * (int64_t)S::kTileBytes, tm_v, warp, row);
       tmem_wait_st();
       arrive_warp(&ctl.v_full);
-      auto take = [&](int group) {
-        wait(&ctl.acc_full, group);
-        drain(tm_dv + lane_bits(warp) + quarter * S::kF, dv);
-        drain(tm_dk + lane_bits(warp) + quarter * S::kF, dk);
-        arrive_warp(&ctl.acc_empty);
+      // The gradients of a tile of rows are drained at the end of it (dv) and after the next
+      // tile's first P (dk), when their last products are done and no matrix instruction yet
+      // waits for the accumulator.
+      float f = 0.f, fd = 0.f, fp = 0.f, back_v = 0.f, back_k = 0.f;
+      int group = 0;
+      auto take_dv = [&]() {
+        wait(&ctl.dv_full, group);
+        drain(tm_dv + lane_bits(warp) + quarter * S::kF, back_v, dv);
+        arrive_warp(&ctl.dv_empty);
       };
+      auto take_dk = [&]() {
+        wait(&ctl.dk_full, group++);
+        drain(tm_dk + lane_bits(warp) + quarter * S::kF, back_k, dk);
+        arrive_warp(&ctl.dk_empty);
+      };
+      AttnTile qt = qi[t0 >> 1], gt = gi[t0 >> 1];
       const uint32_t off = lane_bits(warp) + quarter * 16;
       for (int j = 0; j < n; ++j) {
         const int r = (t0 + j) * kHalf + quarter * 16;
+        const bool first = j == 0 || !((t0 + j) & 1);      // of another tile of Q and dout
+        float back_k_next = back_k;
+        if (first) {
+          const int eds = scale_of_ds(gt.norm, vt.norm);
+          f = a.scale * kLog2e * pow2(-qt.e - ek);
+          fd = pow2(-gt.e - vt.e);
+          fp = pow2(eds - (int)kUpP);                      // P from 2^14 P, and dS's scale
+          back_v = pow2(-(int)kUpP - gt.e);
+          back_k_next = ldexpf(a.scale, -eds - qt.e);
+          const int next = ((t0 + j) >> 1) + 1;
+          if (next <= (t0 + n - 1) >> 1) {
+            qt = qi[next];
+            gt = gi[next];
+          }
+        }
         ctl.q.ready(j, wait);                      // the log-sums and deltas
         wait(&ctl.s_full, j);
         const float4* lse = reinterpret_cast<const float4*>(ctl.lse[j % S::kRowsQ] + quarter * 16);
@@ -918,32 +980,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
         store_operand<16>(tm_s + off, p);
         tmem_wait_st();
         arrive_warp(&ctl.p_full);
-        if (j && j % kGroup == 0) take(j / kGroup - 1);
+        if (j && first) take_dk();
+        back_k = back_k_next;
         wait(&ctl.dp_full, j);
         tmem_load16(tm_dp + off, x);
         tmem_wait_ld();
-        constexpr float down = 1.f / 16384.f;      // 2^-14: P itself
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const float4 d = del[e / 4];
-          p[e] *= down * fmaf(__uint_as_float(x[e]), fd, -d.x);
-          p[e + 1] *= down * fmaf(__uint_as_float(x[e + 1]), fd, -d.y);
-          p[e + 2] *= down * fmaf(__uint_as_float(x[e + 2]), fd, -d.z);
-          p[e + 3] *= down * fmaf(__uint_as_float(x[e + 3]), fd, -d.w);
+          p[e] = p[e] * fp * fmaf(__uint_as_float(x[e]), fd, -d.x);
+          p[e + 1] = p[e + 1] * fp * fmaf(__uint_as_float(x[e + 1]), fd, -d.y);
+          p[e + 2] = p[e + 2] * fp * fmaf(__uint_as_float(x[e + 2]), fd, -d.z);
+          p[e + 3] = p[e + 3] * fp * fmaf(__uint_as_float(x[e + 3]), fd, -d.w);
         }
         store_operand<16>(tm_dp + off, p);
         tmem_wait_st();
         arrive_warp(&ctl.ds_full);
+        if (j == n - 1 || ((t0 + j) & 1)) take_dv();
       }
-      take((n - 1) / kGroup);
+      take_dk();
     }
     if (key < a.kv_len) {
-      const float bk = ldexpf(a.scale, -(sc.eds + sc.e[0])), bv = ldexpf(1.f, -(int)kUpP - sc.e[3]);
-#pragma unroll
-      for (int e = 0; e < S::kF; ++e) {
-        dk[e] *= bk;
-        dv[e] *= bv;
-      }
       store_features<S::kF>(a.dk + at(a.dks, b, key, hk), quarter * S::kF, a.dim, vec_out, dk);
       store_features<S::kF>(a.dv + at(a.dvs, b, key, hk), quarter * S::kF, a.dim, vec_out, dv);
     }
@@ -959,7 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
 // ---------------------------------------------------------------------------
 struct Layout {
   int64_t heads, row_tiles, key_tiles, blocks;
-  size_t stats, tile[4], lse2, delta, part, total;
+  size_t stats, tile[4], info[4], lse2, delta, part, total;
   int splits;
   Layout(const AttnArgs& a, bool backward) {
     heads = (int64_t)a.batch * a.kv_heads;
@@ -974,8 +1031,11 @@ struct Layout {
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 1023) & ~size_t(1023); return o; };
     stats = take(sizeof(AttnStats) * heads + sizeof(uint32_t));     // and the word `any`
-    for (int t = 0; t < (backward ? 4 : 3); ++t)
-      tile[t] = take((size_t)heads * (t == 1 || t == 2 ? key_tiles : row_tiles) * blocks * kBlockBytes);
+    for (int t = 0; t < (backward ? 4 : 3); ++t) {
+      const size_t tiles = (size_t)heads * (t == 1 || t == 2 ? key_tiles : row_tiles);
+      tile[t] = take(tiles * blocks * kBlockBytes);
+      info[t] = take(tiles * sizeof(AttnTile));
+    }
     lse2 = delta = part = 0;
     if (backward) {
       lse2 = take(sizeof(float) * heads * row_tiles * kTile);
@@ -998,6 +1058,7 @@ cudaError_t prepare(const AttnArgs& a, const Layout& L, uint8_t* w, bool backwar
   t.any = reinterpret_cast<uint32_t*>(t.stats + L.heads);
   for (int i = 0; i < (backward ? 4 : 3); ++i) {
     t.p[i] = w + L.tile[i];
+    t.info[i] = reinterpret_cast<AttnTile*>(w + L.info[i]);
     t.tiles[i] = i == 1 || i == 2 ? L.key_tiles : L.row_tiles;
   }
   t.lse2 = reinterpret_cast<float*>(w + L.lse2);
@@ -1005,20 +1066,15 @@ cudaError_t prepare(const AttnArgs& a, const Layout& L, uint8_t* w, bool backwar
   t.blocks = (int)L.blocks;
   cudaError_t e = cudaMemsetAsync(t.stats, 0, sizeof(AttnStats) * L.heads + sizeof(uint32_t), st);
   if (e != cudaSuccess) return e;
-  const int per_q = (int)((int64_t)a.q_len * a.group + kScanRows - 1) / kScanRows, per_k = (a.kv_len + kScanRows - 1) / kScanRows;
-  const int64_t scan = L.heads * ((backward ? 2ll : 1ll) * per_q + 2ll * per_k);
-  const int64_t split = L.heads * 8 * ((backward ? 2 : 1) * L.row_tiles + 2 * L.key_tiles);
-  if (scan > INT_MAX || split > INT_MAX) return cudaErrorInvalidConfiguration;
-  if (!scan) return cudaSuccess;
+  const int64_t split = L.heads * ((backward ? 2 : 1) * L.row_tiles + 2 * L.key_tiles);
+  if (split > INT_MAX) return cudaErrorInvalidConfiguration;
+  if (!split) return cudaSuccess;
   const bool vec = a.dim % 4 == 0 && aligned(a.q, a.qs) && aligned(a.k, a.ks) && aligned(a.v, a.vs) &&
                    (!backward || aligned(a.dout, a.os));
-  const int back = backward, tq = (int)L.row_tiles, tk = (int)L.key_tiles;
-  if (vec) k_attn_scan<true><<<(unsigned)scan, 256, 0, st>>>(a, t.stats, per_q, per_k, back);
-  else k_attn_scan<false><<<(unsigned)scan, 256, 0, st>>>(a, t.stats, per_q, per_k, back);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  return L.blocks == 1 ? launch_pdl(k_attn_split<1>, dim3((unsigned)split), dim3(128), 0, st, a, t, tq, tk, back, vec)
-                       : launch_pdl(k_attn_split<2>, dim3((unsigned)split), dim3(256), 0, st, a, t, tq, tk, back, vec);
+  const int tq = (int)L.row_tiles, tk = (int)L.key_tiles;
+  if (L.blocks == 1) k_attn_split<1><<<(unsigned)split, 512, 0, st>>>(a, t, tq, tk, vec);
+  else k_attn_split<2><<<(unsigned)split, 512, 0, st>>>(a, t, tq, tk, vec);
+  return cudaGetLastError();
 }
 
 template <int BLOCKS>
