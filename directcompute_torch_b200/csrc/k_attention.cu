@@ -21,6 +21,18 @@ namespace {
 
 constexpr int kWarps = 4, kOctets = 4 * kWarps;
 constexpr unsigned kFull = 0xffffffffu;
+constexpr int kMostSplits = 64;
+constexpr int kAhead = 3;                // steps of the key ring
+
+// 16 bytes (or zeros, for `bytes` 0) into shared memory, behind the thread's back
+DCT_DEV void copy_async(void* to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from),
+               "r"(bytes)
+               : "memory");
+}
+DCT_DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+DCT_DEV void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // feature of element e of chunk c for lane l of an octet
 template <int NV, bool VEC>
@@ -113,34 +125,79 @@ DCT_DEV void rows_forward(const AttnArgs& a, int item, int groups, int splits, f
   }
   const float* kp = a.k + at(a.ks, b, 0, hk);
   const float* vp = a.v + at(a.vs, b, 0, hk);
-  for (int base = k0; base < k1; base += 2 * kOctets) {     // two keys an octet, loaded together
-    float k[2][F], v[2][F];
+  auto add = [&](int j, const float (&x)[R], const float (&v)[F]) {      // key j, its scores and value
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int j = min(base + u * kOctets + oct, k1 - 1);
-      load_row<NV, VEC>(k[u], kp + (int64_t)j * a.ks[1], lane, a.dim);
-      load_row<NV, VEC>(v[u], vp + (int64_t)j * a.vs[1], lane, a.dim);
-    }
+    for (int r = 0; r < R; ++r)
+      if (j >= lo[r] && j < hi[r] && j < k1) {            // uniform in the octet
+        if (x[r] > top[r]) {
+          const float c = weight(top[r], x[r]);
+          sum[r] *= c;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int j = base + u * kOctets + oct;
+          for (int e = 0; e < F; ++e) acc[r][e] *= c;
+          top[r] = x[r];
+        }
+        const float p = weight(x[r], top[r]);
+        sum[r] += p;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float x = octet_sum(dot(q[r], k[u])) * scale;
-        if (j >= lo[r] && j < hi[r] && j < k1) {            // uniform in the octet
-          if (x > top[r]) {
-            const float c = weight(top[r], x);
-            sum[r] *= c;
+        for (int e = 0; e < F; ++e) acc[r][e] = fmaf(p, v[e], acc[r][e]);
+      }
+  };
+  if constexpr (VEC) {
+    // Two keys an octet at a time, two such steps ahead of their use in shared memory.  A
+    // thread copies just what it reads itself, so nothing but its own copies is waited for.
+    extern __shared__ float4 ring[];
+    auto place = [&](int step, int u, int value) { return ring + (((step % kAhead * 2 + u) * 2 + value) * NV) * (32 * kWarps) + threadIdx.x; };
+    auto fetch = [&](int step) {
 #pragma unroll
-            for (int e = 0; e < F; ++e) acc[r][e] *= c;
-            top[r] = x;
-          }
-          const float p = weight(x, top[r]);
-          sum[r] += p;
+      for (int u = 0; u < 2; ++u) {
+        const int64_t j = min(k0 + (step * 2 + u) * kOctets + oct, k1 - 1);
 #pragma unroll
-          for (int e = 0; e < F; ++e) acc[r][e] = fmaf(p, v[u][e], acc[r][e]);
+        for (int c = 0; c < NV; ++c) {
+          const int f = (c * 8 + lane) * 4, bytes = f < a.dim ? 16 : 0;    // 0: zeros are written
+          copy_async(place(step, u, 0) + c * 32 * kWarps, kp + j * a.ks[1] + (bytes ? f : 0), bytes);
+          copy_async(place(step, u, 1) + c * 32 * kWarps, vp + j * a.vs[1] + (bytes ? f : 0), bytes);
         }
       }
+    };
+    auto read = [&](float (&x)[F], const float4* from) {
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        const float4 v = from[c * 32 * kWarps];
+        x[4 * c] = v.x; x[4 * c + 1] = v.y; x[4 * c + 2] = v.z; x[4 * c + 3] = v.w;
+      }
+    };
+    const int steps = k0 < k1 ? (k1 - k0 + 2 * kOctets - 1) / (2 * kOctets) : 0;
+#pragma unroll
+    for (int i = 0; i < kAhead - 1; ++i) {
+      if (i < steps) fetch(i);
+      copy_commit();
+    }
+    for (int i = 0; i < steps; ++i) {
+      if (i + kAhead - 1 < steps) fetch(i + kAhead - 1);
+      copy_commit();
+      copy_wait<kAhead - 1>();
+      float x[2][R], k[F];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        read(k, place(i, u, 0));
+#pragma unroll
+        for (int r = 0; r < R; ++r) x[u][r] = octet_sum(dot(q[r], k)) * scale;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        read(k, place(i, u, 1));
+        add(k0 + (i * 2 + u) * kOctets + oct, x[u], k);
+      }
+    }
+  } else {
+    for (int base = k0; base < k1; base += kOctets) {
+      const int j = min(base + oct, k1 - 1);
+      float k[F], v[F], x[R];
+      load_row<NV, VEC>(k, kp + (int64_t)j * a.ks[1], lane, a.dim);
+      load_row<NV, VEC>(v, vp + (int64_t)j * a.vs[1], lane, a.dim);
+#pragma unroll
+      for (int r = 0; r < R; ++r) x[r] = octet_sum(dot(q[r], k)) * scale;
+      add(base + oct, x, v);
     }
   }
   // join the octets of a warp, then the warps
@@ -202,25 +259,46 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const __grid_constant
   }
 }
 
-// joins a row's splits in order, a warp per row
+// joins a row's splits in order, a block per row
 __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ AttnArgs a, int splits, float* part,
                                                    bool tensor) {
-  const int rows = a.q_len * a.group, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (int64_t)a.batch * a.kv_heads * rows) return;
+  __shared__ float share[kMostSplits], best, sum;
+  pdl_entry();
+  const int rows = a.q_len * a.group;
+  const int64_t row = blockIdx.x;
   const int bh = (int)(row / rows);
   if (a.stats && head_splits(a.stats[bh], a.scale, a.dim) != tensor) return;
   const float* rec = record(part, a, row, splits, 0);
   const int step = a.dim + 2;
-  float best = -INFINITY, s = 0.f;
-  for (int i = lane; i < splits; i += 32) best = fmaxf(best, rec[(int64_t)i * step + a.dim]);
-  best = warp_max_f(best);
-  for (int i = 0; i < splits; ++i) s += rec[(int64_t)i * step + a.dim + 1] * weight(rec[(int64_t)i * step + a.dim], best);
-  for (int f = lane; f < a.dim; f += 32) {
-    float o = 0.f;
-    for (int i = 0; i < splits; ++i) o += rec[(int64_t)i * step + f] * weight(rec[(int64_t)i * step + a.dim], best);
-    store_row(a, bh / a.kv_heads, RowAt(a, bh % a.kv_heads, (int)(row % rows)), f, o, best, s);
+  if (threadIdx.x < 32) {
+    float t[kMostSplits / 32], m = -INFINITY, s = 0.f;
+#pragma unroll
+    for (int u = 0; u < kMostSplits / 32; ++u) {
+      const int i = threadIdx.x + 32 * u;
+      t[u] = i < splits ? rec[i * step + a.dim] : -INFINITY;
+      m = fmaxf(m, t[u]);
+    }
+    m = warp_max_f(m);
+#pragma unroll
+    for (int u = 0; u < kMostSplits / 32; ++u) {
+      const int i = threadIdx.x + 32 * u;
+      if (i >= splits) continue;
+      share[i] = weight(t[u], m);
+      s = fmaf(rec[i * step + a.dim + 1], share[i], s);
+    }
+    s = warp_sum_f(s);
+    if (threadIdx.x == 0) {
+      best = m;
+      sum = s;
+    }
   }
+  __syncthreads();
+  const int f = threadIdx.x;
+  if (f >= a.dim) return;
+  float o = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < splits; ++i) o = fmaf(rec[i * step + f], share[i], o);
+  store_row(a, bh / a.kv_heads, RowAt(a, bh % a.kv_heads, (int)(row % rows)), f, o, best, sum);
 }
 
 // delta = sum_d dout out, a warp per (batch, head, position)
@@ -430,7 +508,7 @@ int rows_splits(const AttnArgs& a) {
   const int64_t blocks = (int64_t)a.batch * a.kv_heads * (((int64_t)a.q_len * a.group + R - 1) / R);
   if (!blocks) return 1;
   const int64_t want = (8ll * dev_info().sm_count + blocks - 1) / blocks, most = (a.kv_len + 127) / 128;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(64, std::min(want, most)));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, std::min(want, most)));
 }
 
 }  // namespace
@@ -454,16 +532,18 @@ cudaError_t launch_attn_rows_forward(const AttnArgs& a, void* ws, cudaStream_t s
     const unsigned n = blocks_for(a, blocks);
     const int items = (int)blocks, g = (int)groups;
     const auto kernel = R == 4 ? k_attn_rows<NV, V, 4> : R == 2 ? k_attn_rows<NV, V, 2> : k_attn_rows<NV, V, 1>;
-    return launch_pdl(kernel, dim3(n), dim3(32 * kWarps), 0, st, a, g, splits, part, items);
+    const size_t smem = V ? sizeof(float4) * kAhead * 4 * NV * 32 * kWarps : 0;      // 96 KB at 128 features
+    const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (set != cudaSuccess) return set;
+    return launch_pdl(kernel, dim3(n), dim3(32 * kWarps), smem, st, a, g, splits, part, items);
   });
   if (e != cudaSuccess || splits == 1) return e;
   return launch_attn_join(a, splits, part, false, st);
 }
 
 cudaError_t launch_attn_join(const AttnArgs& a, int splits, float* part, bool tensor, cudaStream_t st) {
-  const int64_t rows = (int64_t)a.batch * a.q_heads * a.q_len;
-  k_attn_join<<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(a, splits, part, tensor);
-  return cudaGetLastError();
+  return launch_pdl(k_attn_join, dim3((unsigned)((int64_t)a.batch * a.q_heads * a.q_len)), dim3(128), 0, st, a, splits,
+                    part, tensor);
 }
 
 cudaError_t launch_attn_delta(const AttnArgs& a, cudaStream_t st) {

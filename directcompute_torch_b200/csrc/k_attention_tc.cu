@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
   const int g = threadIdx.x % kGroups, row0 = threadIdx.x / kGroups, b = bh / a.kv_heads, hk = bh % a.kv_heads;
   const AttnSpan span(a, b);
   const int rows = rows_of(a, span, t);
+  if (tile * kTile >= rows && t != 3) return;      // nothing reads it (dout's log-sums are read by whole tiles)
   if (threadIdx.x < 3) sh[threadIdx.x] = 0;
   __syncthreads();
   float v[kPasses][8];

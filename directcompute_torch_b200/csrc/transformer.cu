@@ -275,15 +275,18 @@ DCT_API int dct_rotary(const DctRotary* p, void* x, void* positions, void* y) {
   a.start = p->start; a.magnitude = (float)p->magnitude;
   a.interleaved = p->interleaved != 0; a.inverse = p->inverse != 0; a.in_place = same;
   RotaryTurns f;
+  // powers by products in long double: 2^-64 a factor, at most 128 factors
   const double two_pi = 6.283185307179586476925286766559;
-  for (uint32_t j = 0; j < p->rotated / 2; ++j) {
-    double w = pow(p->base, -2.0 * j / p->rotated);
+  const long double ratio = p->rotated ? powl((long double)p->base, -2.0L / p->rotated) : 1.0L;
+  long double w = 1.0L;
+  for (uint32_t j = 0; j < p->rotated / 2; ++j, w *= ratio) {
+    double t = (double)(w / two_pi);             // turns a position
     if (p->factor != 1.0) {
       double keep = 0.0;
-      if (p->original > 0) keep = std::min(1.0, std::max(0.0, (p->original * w / two_pi - p->low) / (p->high - p->low)));
-      w *= keep + (1.0 - keep) / p->factor;
+      if (p->original > 0) keep = std::min(1.0, std::max(0.0, (p->original * t - p->low) / (p->high - p->low)));
+      t *= keep + (1.0 - keep) / p->factor;
     }
-    f.turns[j] = w / two_pi;
+    f.turns[j] = t;
   }
   OnDevice guard;
   return rt_cuda_ok(launch_rotary(a, f, rt_stream()), what) ? DCT_OK : DCT_ERR_CUDA;
