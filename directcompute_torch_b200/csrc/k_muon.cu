@@ -543,6 +543,308 @@ __global__ void __launch_bounds__(256) k_muon_apply(const __grid_constant__ Muon
   }
 }
 
+// ---------------------------------------------------------------------------
+// short matrices: everything in one launch
+// ---------------------------------------------------------------------------
+// With a shorter side of 128 or less, what bounds the products above is not their work but
+// their number: each is a launch of one or a few tiles, about 9 us from its first load to
+// its last store.  Here a cluster holds a matrix: X^T or X as [shorter side][longer side],
+// `chunks` columns of 64 a block in shared memory, from the first read of the gradient to
+// the last step, and A and P in another 64 KB.  Only the blocks' sums of A meet through
+// memory, added by every block in the same order.
+constexpr int kMostChunks = 5;
+struct Small {
+  MuonArgs a;
+  uint32_t side, length;         // the shorter and the longer side
+  bool tall;                     // the matrix is [longer][shorter]
+  int chunks;                    // of this cluster's blocks
+  float *sums;                   // [matrix][block][128][128]
+  float first;                   // scale of the first X
+  float gram, poly_a, poly_b, next_p, next_x, last_p, last_x;    // powers of two and coefficients
+};
+
+DCT_DEV uint64_t at_small(const Small& g, uint32_t s, uint32_t t) {
+  return g.tall ? (uint64_t)t * g.a.cols + s : (uint64_t)s * g.a.cols + t;
+}
+
+// 16 warps: a thread holds a quarter (32 columns) of a row of A and P, and of every 64 columns
+// of X.  The steps alternate between all threads and one that issues matrix instructions.
+constexpr int kSmallThreads = 512;
+__global__ void __launch_bounds__(kSmallThreads) k_muon_small(const __grid_constant__ Small g, uint32_t* err) {
+  extern __shared__ __align__(1024) uint8_t sm[];
+  __shared__ uint64_t bar, ready[kMostChunks];
+  __shared__ uint32_t tmem_base;
+  __shared__ double sh[32], square;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, C = g.chunks;
+  uint8_t* ap = sm + C * 4 * kChunkBytes;         // A, then P: [64 columns][hi, lo][128 rows]
+  const uint32_t rank = cluster_rank();
+  uint32_t blocks;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
+  const uint32_t z = blockIdx.x / blocks, t0 = rank * C * 64;
+  const uint64_t base = (uint64_t)z * g.a.rows * g.a.cols;
+  if ((smem_addr(sm) & 1023) != 0) {              // uniform over the cluster
+    if (err && threadIdx.x == 0) atomicOr(err, DCT_DEVERR_WAIT_TIMEOUT);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    for (int k = 0; k < kMostChunks; ++k) mbar_init(&ready[k], 1);
+    mbar_fence_init();
+  }
+  if (warp == 0) tmem_alloc(&tmem_base, 512);
+  for (uint32_t i = threadIdx.x; i < C * 4 * kChunkBytes / 16; i += kSmallThreads)
+    reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+
+  // Momentum and norm.  The direction waits for its scale where the first X will lie, its
+  // upper and lower 16 bits in the places of hi and lo.  A warp takes lines of memory.
+  const uint32_t lines = g.tall ? min((uint32_t)C * 64, g.length > t0 ? g.length - t0 : 0) : g.side;
+  const uint32_t across = g.tall ? g.side : min((uint32_t)C * 64, g.length > t0 ? g.length - t0 : 0);
+  double part = 0.0;
+  for (uint32_t line = warp; line < lines; line += kSmallThreads / 32) {
+    const uint64_t from = base + (g.tall ? at_small(g, 0, t0 + line) : at_small(g, line, t0));
+    for (uint32_t c0 = lane; c0 < across; c0 += 128) {
+      float x[4], m[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t c = c0 + e * 32;
+        x[e] = c < across ? g.a.g[from + c] : 0.f;
+        m[e] = g.a.update && c < across ? g.a.m[from + c] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t c = c0 + e * 32;
+        if (c >= across) break;
+        if (g.a.update) g.a.m[from + c] = m[e] = updated(g.a, m[e], x[e]);
+        const float u = direction(g.a, m[e], x[e]);
+        part += (double)u * u;
+        const uint32_t s = g.tall ? c : line, k = g.tall ? line : c, bits = __float_as_uint(u);
+        uint8_t* p = sm + (k >> 6) * 4 * kChunkBytes + chunk_at(s, (k & 63) >> 3) + 2 * (k & 7);
+        *reinterpret_cast<uint16_t*>(p) = (uint16_t)(bits >> 16);
+        *reinterpret_cast<uint16_t*>(p + 2 * kChunkBytes) = (uint16_t)bits;
+      }
+    }
+  }
+  part = block_sum(part, sh);
+  if (threadIdx.x == 0) square = part;
+  cluster_sync();
+  double all = 0.0;
+  for (uint32_t b = 0; b < blocks; ++b) {
+    uint32_t addr;
+    double v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_addr(&square)), "r"(b));
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
+    all += v;
+  }
+  const double f = (double)g.first / (sqrt(all) + g.a.eps);
+  for (uint32_t i = threadIdx.x; i < C * 2 * kChunkBytes / 16; i += kSmallThreads) {
+    uint4* h = reinterpret_cast<uint4*>(sm + i / (2 * kChunkBytes / 16) * 4 * kChunkBytes) + i % (2 * kChunkBytes / 16);
+    uint4* l = h + 2 * kChunkBytes / 16;
+    const uint32_t hh[4] = {h->x, h->y, h->z, h->w}, ll[4] = {l->x, l->y, l->z, l->w};
+    uint32_t u[4], v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      split2((float)(__uint_as_float(hh[e] << 16 | (ll[e] & 0xffff)) * f),
+             (float)(__uint_as_float((hh[e] & 0xffff0000u) | ll[e] >> 16) * f), u[e], v[e]);
+    *h = make_uint4(u[0], u[1], u[2], u[3]);
+    *l = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+
+  const uint32_t row = (warp & 3) * 32 + lane, quarter = warp >> 2, lanes = (uint32_t)(warp & 3) * 32u << 16;
+  bool ok = true;
+  uint32_t phase = 0;
+  auto to_tensor = [&]() {
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  };
+  auto from_tensor = [&]() {
+    ok = ok && mbar_wait(&bar, phase & 1, err);
+    ++phase;
+    tc_fence_after();
+  };
+  auto three = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t step_a, uint32_t step_b, uint64_t lo, uint32_t idesc,
+                   bool add, int deep) {          // 16 `deep` of the contraction
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (q >= deep) break;
+      umma(d, a + lo + q * step_a, b + q * step_b, idesc, add || q != 0);
+      umma(d, a + q * step_a, b + lo + q * step_b, idesc, true);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < deep) umma(d, a + q * step_a, b + q * step_b, idesc, true);
+  };
+  // rows of the shorter side in 16s: all the columns of A and P, and the contraction with them
+  const int wide = (int)(g.side + 15) / 16, deep0 = min(wide, 4), deep1 = wide - deep0;
+  const int cols = min(max(16 * wide - (int)quarter * 32, 0), 32);     // of the thread's columns (the rest stays 0)
+  constexpr uint64_t kLow = 2 * kChunkBytes / 16;                 // from hi to lo of 128 rows
+  constexpr uint32_t kBlock = 4 * kChunkBytes / 16;               // from 64 columns to the next
+  const uint64_t x = umma_desc(smem_addr(sm), kChunkBytes, 1024), p = umma_desc(smem_addr(ap), kChunkBytes, 1024);
+  for (uint32_t it = 0; it < g.a.steps; ++it) {
+    const bool last = it + 1 == g.a.steps;
+    // A = X X^T: every 64 columns an accumulator of their own (the fifth joins the first)
+    to_tensor();
+    if (warp == 0 && elect_one()) {
+      const uint32_t id = umma_idesc(128, 16 * wide, false, false);
+      for (int k = 0; k < C; ++k) three(tmem + (k & 3) * 128, x + k * kBlock, x + k * kBlock, 2, 2, kLow, id, k > 3, 4);
+      umma_commit(&bar);
+    }
+    from_tensor();
+    float acc[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) acc[e] = 0.f;
+    for (int k = 0; k < min(C, 4) && cols > 0; ++k) {
+      uint32_t v[32];
+      tmem_load32(tmem + lanes + k * 128 + quarter * 32, v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (e < cols) acc[e] += __uint_as_float(v[e]);
+    }
+    if (blocks > 1) {
+      const uint32_t at = quarter * 32 * 128 + row;
+      float* mine = g.sums + ((uint64_t)z * blocks + rank) * 16384 + at;
+      if (cols > 0) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          __stcg(mine + e * 128, acc[e]);
+          acc[e] = 0.f;
+        }
+      }
+      __threadfence();
+      cluster_sync();
+      for (uint32_t b = 0; b < blocks && cols > 0; ++b) {
+        const float* from = g.sums + ((uint64_t)z * blocks + b) * 16384 + at;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) acc[e] += __ldcg(from + e * 128);
+      }
+      cluster_sync();                             // before the next step's sums
+    }
+    auto store = [&](const float (&v)[32]) {      // the thread's columns of A or P
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) split2(v[e + 2 * q], v[e + 2 * q + 1], h[q], l[q]);
+        uint8_t* o = ap + (quarter >> 1) * 4 * kChunkBytes + chunk_at(row, (quarter & 1) * 4 + (e >> 3));
+        *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(o + 2 * kChunkBytes) = make_uint4(l[0], l[1], l[2], l[3]);
+      }
+    };
+#pragma unroll
+    for (int e = 0; e < 32; ++e) acc[e] *= g.gram;
+    store(acc);
+    // P = c A A + b A
+    to_tensor();
+    if (warp == 0 && elect_one()) {
+      const uint32_t id = umma_idesc(128, 16 * wide, false, false);
+      three(tmem, p, p, 2, 2, kLow, id, false, deep0);
+      if (deep1) three(tmem + 128, p + kBlock, p + kBlock, 2, 2, kLow, id, false, deep1);
+      umma_commit(&bar);
+    }
+    from_tensor();
+    if (cols > 0) {
+      uint32_t v[32], w[32];
+      tmem_load32(tmem + lanes + quarter * 32, v);
+      if (deep1) tmem_load32(tmem + lanes + 128 + quarter * 32, w);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        if (e >= cols) continue;
+        const float s = deep1 ? __uint_as_float(v[e]) + __uint_as_float(w[e]) : __uint_as_float(v[e]);
+        acc[e] = fmaf(g.poly_b, acc[e], g.poly_a * s);
+      }
+    }
+    store(acc);
+    // X = P X + a X, the two halves of the contraction apart where tensor memory has room
+    to_tensor();
+    const bool apart = C <= 4 && deep1;
+    if (warp == 0 && elect_one()) {
+      constexpr uint32_t id = umma_idesc(128, 64, false, true);
+      for (int k = 0; k < C; ++k) {
+        for (int h = 0; h < (deep1 ? 2 : 1); ++h)
+          three(tmem + (apart ? 2 * k + h : k) * 64, p + h * kBlock, x + k * kBlock + h * (kChunkBytes / 16), 2, 128, kLow, id,
+                !apart && h, h ? deep1 : deep0);
+        umma_commit(&ready[k]);
+      }
+    }
+    const float sp = last ? g.last_p : g.next_p, sx = last ? g.last_x : g.next_x;
+    for (int k = 0; k < C; ++k) {
+      ok = ok && mbar_wait(&ready[k], it & 1, err);
+      tc_fence_after();
+      uint32_t v[16];
+      float y[16];
+      tmem_load16(tmem + lanes + (apart ? 2 * k : k) * 64 + quarter * 16, v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[e] = __uint_as_float(v[e]);
+      if (apart) {
+        tmem_load16(tmem + lanes + (2 * k + 1) * 64 + quarter * 16, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] += __uint_as_float(v[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e += 8) {
+        uint8_t* o = sm + k * 4 * kChunkBytes + chunk_at(row, quarter * 2 + (e >> 3));
+        const uint4 h = *reinterpret_cast<const uint4*>(o), l = *reinterpret_cast<const uint4*>(o + 2 * kChunkBytes);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) y[e + q] *= sp;
+        add8(y, e, sx, h);
+        add8(y, e, sx, l);
+        if (!last) {
+          uint32_t hh[4], ll[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) split2(y[e + 2 * q], y[e + 2 * q + 1], hh[q], ll[q]);
+          *reinterpret_cast<uint4*>(o) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
+          *reinterpret_cast<uint4*>(o + 2 * kChunkBytes) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
+        }
+      }
+      if (last && row < g.side) {
+        const uint32_t t = t0 + k * 64 + quarter * 16;
+        const uint64_t first = base + at_small(g, row, t), step = g.tall ? g.a.cols : 1;
+        float old[16];
+        if (g.a.update) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (t + e < g.length) old[e] = g.a.w[first + e * step];
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if (t + e >= g.length) break;
+          if (g.a.update) g.a.w[first + e * step] = fmaf(-g.a.rate, y[e], g.a.keep * old[e]);
+          else g.a.y[first + e * step] = y[e];
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  cluster_sync();                                 // the others have read this block's square
+  tc_fence_after();
+  if (warp == 0) tmem_free(tmem, 512);
+}
+
+// Blocks of a matrix's cluster, or 0 where the general way takes it.  More blocks have fewer
+// chunks each (about 2800 cycles a step) but more sums to meet (1100, and 1500 for meeting).
+int small_blocks(const MuonArgs& a) {
+  const uint32_t s = std::min(a.rows, a.cols), chunks = (std::max(a.rows, a.cols) + 63) / 64;
+  if (s > 128 || !a.steps || chunks > 8 * kMostChunks) return 0;
+  int best = 0;
+  uint32_t cost = ~0u;
+  for (uint32_t n = 1; n <= 8; ++n) {
+    const uint32_t c = (chunks + n - 1) / n, want = c * 2800 + (n > 1 ? 1500 + 1100 * n : 0);
+    if (c > kMostChunks || (n - 1) * c >= chunks || want >= cost) continue;
+    cost = want;
+    best = (int)n;
+  }
+  return best;
+}
+
 struct Layout {
   uint32_t rb, cb, sb;              // chunks of rows, columns, the shorter side
   uint64_t x, s;                    // bytes of X's and of a Gram matrix's chunks
@@ -645,14 +947,64 @@ int room(double most) {
   return 15 - e;
 }
 float pow2(int e) { return (float)ldexp(1.0, e); }
+// exponents at which X, A and P are held: no entry of X exceeds its largest singular value,
+// none of A that squared, none of P b t + c t^2 on those
+struct Powers {
+  int x, g, p;
+  explicit Powers(const MuonArgs& a) {
+    const double top = a.bound * a.bound, most = std::max(1e-30, fabs(a.b) * top + fabs(a.c) * top * top);
+    x = room(a.bound);
+    g = room(top);
+    p = room(most);
+  }
+};
 
 }  // namespace
 
-size_t muon_ws_bytes(const MuonArgs& a) { return Layout(a).total; }
+size_t muon_ws_bytes(const MuonArgs& a) {
+  if (const int n = small_blocks(a)) return (size_t)a.batch * n * 16384 * sizeof(float);
+  return Layout(a).total;
+}
+
+cudaError_t launch_small(const MuonArgs& a, int blocks, void* ws, cudaStream_t st) {
+  Small g{};
+  g.a = a;
+  g.tall = a.rows > a.cols;
+  g.side = std::min(a.rows, a.cols);
+  g.length = std::max(a.rows, a.cols);
+  g.chunks = (int)(((g.length + 63) / 64 + blocks - 1) / blocks);
+  g.sums = static_cast<float*>(ws);
+  const Powers w(a);
+  g.first = pow2(w.x);
+  g.gram = pow2(w.g - 2 * w.x);
+  g.poly_a = (float)(a.c * pow2(w.p - 2 * w.g));
+  g.poly_b = (float)(a.b * pow2(w.p - w.g));
+  g.next_p = pow2(-w.p);
+  g.next_x = (float)a.a;
+  g.last_p = pow2(-w.x - w.p);
+  g.last_x = (float)(a.a * pow2(-w.x));
+  const size_t smem = (size_t)(g.chunks + 2) * 4 * kChunkBytes;
+  static const cudaError_t set = cudaFuncSetAttribute(k_muon_small, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                      (kMostChunks + 2) * 4 * kChunkBytes);
+  if (set != cudaSuccess) return set;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(a.batch * blocks);
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_muon_small, g, device_error_word());
+}
 
 cudaError_t launch_muon(const MuonArgs& a, void* ws, cudaStream_t st) {
-  const Layout L(a);
   if (!a.rows || !a.cols || !a.batch) return cudaSuccess;
+  if (const int n = small_blocks(a)) return launch_small(a, n, ws, st);
+  const Layout L(a);
   uint8_t* w = static_cast<uint8_t*>(ws);
   uint8_t *x = w + L.x0, *y = w + L.x1;
   double* part = reinterpret_cast<double*>(w + L.part);
@@ -669,10 +1021,8 @@ cudaError_t launch_muon(const MuonArgs& a, void* ws, cudaStream_t st) {
     k_muon_apply<<<grid, 256, 0, st>>>(a, part, across);
     return cudaGetLastError();
   }
-  // no entry of X exceeds its largest singular value, none of A that squared, none of P
-  // b t + c t^2 on those
-  const double top = a.bound * a.bound, most = std::max(1e-30, fabs(a.b) * top + fabs(a.c) * top * top);
-  const int ex = room(a.bound), eg = room(top), ep = room(most);
+  const Powers powers(a);
+  const int ex = powers.x, eg = powers.g, ep = powers.p;
   if (vec) k_muon_split<4><<<grid, 256, 0, st>>>(a, part, across, x, L.rb, L.cb, pow2(ex));
   else k_muon_split<1><<<grid, 256, 0, st>>>(a, part, across, x, L.rb, L.cb, pow2(ex));
   cudaError_t e = cudaGetLastError();
