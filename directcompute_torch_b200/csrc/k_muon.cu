@@ -550,8 +550,8 @@ __global__ void __launch_bounds__(256) k_muon_apply(const __grid_constant__ Muon
 // their number: each is a launch of one or a few tiles, about 9 us from its first load to
 // its last store.  Here a cluster holds a matrix: X^T or X as [shorter side][longer side],
 // `chunks` columns of 64 a block in shared memory, from the first read of the gradient to
-// the last step, and A and P in another 64 KB.  Only the blocks' sums of A meet through
-// memory, added by every block in the same order.
+// the last step, and A and P in another 64 KB.  Only the blocks' sums of A meet, through L2
+// (the cluster's shared memory measured slower: 81 us against 69 for 333 x 127).
 constexpr int kMostChunks = 5;
 struct Small {
   MuonArgs a;
@@ -565,6 +565,13 @@ struct Small {
 
 DCT_DEV uint64_t at_small(const Small& g, uint32_t s, uint32_t t) {
   return g.tall ? (uint64_t)t * g.a.cols + s : (uint64_t)s * g.a.cols + t;
+}
+
+// a shared memory address in another block of the cluster
+DCT_DEV uint32_t at_block(uint32_t addr, uint32_t block) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(block));
+  return r;
 }
 
 // 16 warps: a thread holds a quarter (32 columns) of a row of A and P, and of every 64 columns
@@ -604,39 +611,48 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const __grid_const
   const uint32_t lines = g.tall ? min((uint32_t)C * 64, g.length > t0 ? g.length - t0 : 0) : g.side;
   const uint32_t across = g.tall ? g.side : min((uint32_t)C * 64, g.length > t0 ? g.length - t0 : 0);
   double part = 0.0;
-  for (uint32_t line = warp; line < lines; line += kSmallThreads / 32) {
-    const uint64_t from = base + (g.tall ? at_small(g, 0, t0 + line) : at_small(g, line, t0));
+  constexpr int kW = kSmallThreads / 32, kL = 4;  // lines in flight
+  for (uint32_t l0 = warp; l0 < lines; l0 += kW * kL)
     for (uint32_t c0 = lane; c0 < across; c0 += 128) {
-      float x[4], m[4];
+      float x[kL][4], m[kL][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t c = c0 + e * 32;
-        x[e] = c < across ? g.a.g[from + c] : 0.f;
-        m[e] = g.a.update && c < across ? g.a.m[from + c] : 0.f;
+      for (int j = 0; j < kL; ++j) {
+        const uint32_t line = l0 + j * kW;
+        const uint64_t from = base + (g.tall ? at_small(g, 0, t0 + line) : at_small(g, line, t0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t c = c0 + e * 32;
+          const bool in = line < lines && c < across;
+          x[j][e] = in ? g.a.g[from + c] : 0.f;
+          m[j][e] = g.a.update && in ? g.a.m[from + c] : 0.f;
+        }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t c = c0 + e * 32;
-        if (c >= across) break;
-        if (g.a.update) g.a.m[from + c] = m[e] = updated(g.a, m[e], x[e]);
-        const float u = direction(g.a, m[e], x[e]);
-        part += (double)u * u;
-        const uint32_t s = g.tall ? c : line, k = g.tall ? line : c, bits = __float_as_uint(u);
-        uint8_t* p = sm + (k >> 6) * 4 * kChunkBytes + chunk_at(s, (k & 63) >> 3) + 2 * (k & 7);
-        *reinterpret_cast<uint16_t*>(p) = (uint16_t)(bits >> 16);
-        *reinterpret_cast<uint16_t*>(p + 2 * kChunkBytes) = (uint16_t)bits;
+      for (int j = 0; j < kL; ++j) {
+        const uint32_t line = l0 + j * kW;
+        if (line >= lines) break;
+        const uint64_t from = base + (g.tall ? at_small(g, 0, t0 + line) : at_small(g, line, t0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t c = c0 + e * 32;
+          if (c >= across) break;
+          if (g.a.update) g.a.m[from + c] = m[j][e] = updated(g.a, m[j][e], x[j][e]);
+          const float u = direction(g.a, m[j][e], x[j][e]);
+          part += (double)u * u;
+          const uint32_t s = g.tall ? c : line, k = g.tall ? line : c, bits = __float_as_uint(u);
+          uint8_t* p = sm + (k >> 6) * 4 * kChunkBytes + chunk_at(s, (k & 63) >> 3) + 2 * (k & 7);
+          *reinterpret_cast<uint16_t*>(p) = (uint16_t)(bits >> 16);
+          *reinterpret_cast<uint16_t*>(p + 2 * kChunkBytes) = (uint16_t)bits;
+        }
       }
     }
-  }
   part = block_sum(part, sh);
   if (threadIdx.x == 0) square = part;
   cluster_sync();
   double all = 0.0;
   for (uint32_t b = 0; b < blocks; ++b) {
-    uint32_t addr;
     double v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_addr(&square)), "r"(b));
-    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at_block(smem_addr(&square), b)) : "memory");
     all += v;
   }
   const double f = (double)g.first / (sqrt(all) + g.a.eps);
@@ -706,22 +722,22 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const __grid_const
       for (int e = 0; e < 32; ++e)
         if (e < cols) acc[e] += __uint_as_float(v[e]);
     }
-    if (blocks > 1) {
-      const uint32_t at = quarter * 32 * 128 + row;
-      float* mine = g.sums + ((uint64_t)z * blocks + rank) * 16384 + at;
+    if (blocks > 1) {                             // the blocks' sums meet, added in the blocks' order
+      float* mine = g.sums + ((uint64_t)z * blocks + rank) * 16384 + quarter * 32 * 128 + row;
       if (cols > 0) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          __stcg(mine + e * 128, acc[e]);
-          acc[e] = 0.f;
-        }
+        for (int e = 0; e < 32; ++e) __stcg(mine + e * 128, acc[e]);
       }
       __threadfence();
       cluster_sync();
-      for (uint32_t b = 0; b < blocks && cols > 0; ++b) {
-        const float* from = g.sums + ((uint64_t)z * blocks + b) * 16384 + at;
+      if (cols > 0) {
+        const float* from = g.sums + (uint64_t)z * blocks * 16384 + quarter * 32 * 128 + row;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) acc[e] += __ldcg(from + e * 128);
+        for (int e = 0; e < 32; ++e) acc[e] = 0.f;
+        for (uint32_t b = 0; b < blocks; ++b) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) acc[e] += __ldcg(from + b * 16384 + e * 128);
+        }
       }
       cluster_sync();                             // before the next step's sums
     }
@@ -829,15 +845,15 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const __grid_const
   if (warp == 0) tmem_free(tmem, 512);
 }
 
-// Blocks of a matrix's cluster, or 0 where the general way takes it.  More blocks have fewer
-// chunks each (about 2800 cycles a step) but more sums to meet (1100, and 1500 for meeting).
+// Blocks of a matrix's cluster, or 0 where the general way takes it.  A chunk costs a block
+// about 2300 cycles a step, the meeting of several blocks' sums 6800.
 int small_blocks(const MuonArgs& a) {
   const uint32_t s = std::min(a.rows, a.cols), chunks = (std::max(a.rows, a.cols) + 63) / 64;
   if (s > 128 || !a.steps || chunks > 8 * kMostChunks) return 0;
   int best = 0;
   uint32_t cost = ~0u;
   for (uint32_t n = 1; n <= 8; ++n) {
-    const uint32_t c = (chunks + n - 1) / n, want = c * 2800 + (n > 1 ? 1500 + 1100 * n : 0);
+    const uint32_t c = (chunks + n - 1) / n, want = c * 2300 + (n > 1 ? 6800 : 0);
     if (c > kMostChunks || (n - 1) * c >= chunks || want >= cost) continue;
     cost = want;
     best = (int)n;
@@ -962,7 +978,7 @@ struct Powers {
 }  // namespace
 
 size_t muon_ws_bytes(const MuonArgs& a) {
-  if (const int n = small_blocks(a)) return (size_t)a.batch * n * 16384 * sizeof(float);
+  if (const int n = small_blocks(a)) return n > 1 ? (size_t)a.batch * n * 16384 * sizeof(float) : 0;
   return Layout(a).total;
 }
 
