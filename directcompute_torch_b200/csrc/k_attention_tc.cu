@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
                                                     int tq, int tk, bool vec) {
   constexpr int kGroups = 8 * BLOCKS, kStep = 512 / kGroups, kPasses = kTile / kStep;
   __shared__ uint32_t sh[3];
+  pdl_entry();
   const int heads = a.batch * a.kv_heads;
   int x = blockIdx.x, t = 0;
   for (; t < 3; ++t) {                             // q, k, v, dout in turn
@@ -180,6 +181,7 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
   }
   if (!splits) return;
   const float f = pow2(e);
+  if (g >= (a.dim + 15) / 16 * 2) return;          // features that no product reads
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
     uint32_t h[4], l[4];
@@ -278,39 +280,45 @@ struct Ring {
 
 // D = A B^T over the features: A a whole tile in shared memory, B a half tile.  The small
 // products come first: every matrix instruction rounds its sum toward zero.
+// `steps`: 16 features each; what lies behind is neither written nor read.  (FULL: a constant
+// number of them, 3% faster at 128 features than asking for each step.)
 template <int BLOCKS>
-DCT_DEV void mma_features_ss(uint32_t d, uint64_t a, uint64_t b) {
+DCT_DEV void mma_features_ss(uint32_t d, uint64_t a, uint64_t b, int steps) {
   constexpr uint32_t id = umma_idesc(kTile, kHalf, false, false);
   constexpr uint64_t lo_a = kBlockBytes / 32, lo_b = kChunkBytes / 16;
   auto sa = [](int c) { return (uint64_t)((c >> 2) * (kBlockBytes / 16) + (c & 3) * 2); };
   auto sb = [](int c) { return (uint64_t)((c >> 2) * (2 * kChunkBytes / 16) + (c & 3) * 2); };
 #pragma unroll
   for (int c = 0; c < 4 * BLOCKS; ++c) {
+    if (c >= steps) break;
     umma(d, a + lo_a + sa(c), b + sb(c), id, c != 0);
     umma(d, a + sa(c), b + lo_b + sb(c), id, true);
   }
 #pragma unroll
-  for (int c = 0; c < 4 * BLOCKS; ++c) umma(d, a + sa(c), b + sb(c), id, true);
+  for (int c = 0; c < 4 * BLOCKS; ++c)
+    if (c < steps) umma(d, a + sa(c), b + sb(c), id, true);
 }
 // the same with A in tensor memory, B a tile of ROWS rows
 template <int BLOCKS, int ROWS>
-DCT_DEV void mma_features_ts(uint32_t d, uint32_t a, uint64_t b) {
+DCT_DEV void mma_features_ts(uint32_t d, uint32_t a, uint64_t b, int steps) {
   constexpr uint32_t id = umma_idesc(kTile, ROWS, false, false);
   constexpr uint64_t lo_b = ROWS * 128 / 16;
   auto sb = [](int c) { return (uint64_t)((c >> 2) * (2 * ROWS * 128 / 16) + (c & 3) * 2); };
 #pragma unroll
   for (int c = 0; c < 4 * BLOCKS; ++c) {
+    if (c >= steps) break;
     umma_ts(d, a + 32 * BLOCKS + 8 * c, b + sb(c), id, c != 0);
     umma_ts(d, a + 8 * c, b + lo_b + sb(c), id, true);
   }
 #pragma unroll
-  for (int c = 0; c < 4 * BLOCKS; ++c) umma_ts(d, a + 8 * c, b + sb(c), id, true);
+  for (int c = 0; c < 4 * BLOCKS; ++c)
+    if (c < steps) umma_ts(d, a + 8 * c, b + sb(c), id, true);
 }
 // D (+)= A B over 64 rows: A in tensor memory, for each Q rows Q/2 columns of hi and Q/2 of
 // lo (store_operand); B a half tile with its rows as the contraction
 template <int BLOCKS, int Q>
-DCT_DEV void mma_rows(uint32_t d, uint32_t a, uint64_t b, bool add) {
-  constexpr uint32_t id = umma_idesc(kTile, 64 * BLOCKS, false, true);
+DCT_DEV void mma_rows(uint32_t d, uint32_t a, uint64_t b, bool add, int steps) {
+  const uint32_t id = umma_idesc(kTile, 16 * steps, false, true);
   constexpr uint64_t lo_b = kChunkBytes / 16;
   auto sa = [](int c) { return (uint32_t)(16 * c / Q * Q + 16 * c % Q / 2); };
 #pragma unroll
@@ -388,7 +396,7 @@ DCT_DEV void rows_sync(int warp) {                 // the four warps that share 
 // each tile's P V is drained into registers, where the outputs are scaled when the maximum
 // moves, so no accumulator lives longer than one tile and the tensor cores' rounding toward
 // zero does not build up.  P goes back into the scores' place as the product's operand.
-template <int BLOCKS>
+template <int BLOCKS, bool FULL>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_constant__ AttnArgs a,
                                                               const __grid_constant__ Tiles w, int row_tiles,
                                                               int splits, float* part, bool vec_out, uint32_t* err) {
@@ -439,6 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
     n = t1 - t0;
   }
   Waits wait{err};
+  const int steps = FULL ? 4 * BLOCKS : (a.dim + 15) / 16;
 
   if (warp == kSoft) {
     if (elect_one())
@@ -456,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
       auto scores = [&](int j) {                   // S(j) = Q K(j)^T
         if (!ctl.k.ready(j, wait)) return;
         mma_features_ts<BLOCKS, kTile>(tm_s + (j & 1) * kTile, tm_q,
-                                       umma_desc(smem_addr(sm + j % S::kKeys * S::kTileBytes), kChunkBytes, 1024));
+                                       umma_desc(smem_addr(sm + j % S::kKeys * S::kTileBytes), kChunkBytes, 1024), steps);
         ctl.k.release(j);
         umma_commit(&ctl.s_full[j & 1]);
       };
@@ -469,7 +478,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
           const int it = 2 * j + h;
           if (!ctl.v.ready(it, wait)) break;
           mma_rows<BLOCKS, 32>(tm_o, tm_s + (j & 1) * kTile + h * kHalf,
-                               umma_desc(smem_addr(sm + S::kV + it % S::kValues * S::kSlotBytes), 2 * kChunkBytes, 1024), h);
+                               umma_desc(smem_addr(sm + S::kV + it % S::kValues * S::kSlotBytes), 2 * kChunkBytes, 1024), h,
+                               steps);
           ctl.v.release(it);
         }
         umma_commit(&ctl.o_full);
@@ -590,10 +600,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
-// Two kernels that each form the scores and dP = dout V^T again, one for dq (a tile of rows
-// against its keys) and one for dk and dv (a tile of keys against the rows that see them):
-// seven products instead of five, but every gradient has one owner, no atomics and one
-// order.
+// Two kinds of blocks that each form the scores and dP = dout V^T again, for dq (a tile of rows
+// against its keys) and for dk and dv (a tile of keys against the rows that see them): seven
+// products instead of five, but every gradient has one owner, no atomics and one order.
 constexpr float kUpP = 14.f;                       // P <= 1 is held as 2^14 P
 
 // The accumulators are drained after every tile of the inner side, whose scales they carry.
@@ -631,10 +640,8 @@ struct Dq : Sizes<BLOCKS> {
 
 // dq of a tile of 128 rows: dS = P (dP - delta), dq = scale dS K.  Q rests in shared memory,
 // dout in tensor memory; V and K come in half tiles of 64 keys.
-template <int BLOCKS>
-__global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__ AttnArgs a,
-                                                         const __grid_constant__ Tiles w, int row_tiles, bool vec_out,
-                                                         uint32_t* err) {
+template <int BLOCKS, bool FULL>
+DCT_DEV void attn_dq(const AttnArgs& a, const Tiles& w, int block, int row_tiles, bool vec_out, uint32_t* err) {
   using S = Dq<BLOCKS>;
   extern __shared__ __align__(1024) uint8_t sm[];
   auto& ctl = *reinterpret_cast<typename S::Control*>(sm + S::kEnd);
@@ -660,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
   // S and dP twice, the operand dout, the accumulator
   const uint32_t tm_s = ctl.tmem, tm_dp = tm_s + 128, tm_go = tm_s + 256, tm_acc = tm_s + 384;
   pdl_entry();
-  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = row_tiles - 1 - blockIdx.x / heads;
+  const int heads = a.batch * a.kv_heads, bh = block % heads, tile = row_tiles - 1 - block / heads;
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
   const bool splits_head = head_splits(w.stats[bh], a.scale, a.dim);
   if (!splits_head && threadIdx.x == 0) *w.any = 1;          // work for the float32 kernels
@@ -674,6 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
     n = k1 > k0 ? (k1 + kHalf - 1) / kHalf - t0 : 0;
   }
   Waits wait{err};
+  const int steps = FULL ? 4 * BLOCKS : (a.dim + 15) / 16;
 
   if (warp == kSoft) {
     if (n && elect_one()) {
@@ -698,9 +706,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       auto value = [&](int j) { return smem_addr(sm + S::kV + j % S::kValues * S::kSlotBytes); };
       auto scores = [&](int j) {                   // S(j) = Q K^T, dP(j) = dout V^T
         if (!ctl.k.ready(j, wait)) return;
-        mma_features_ss<BLOCKS>(tm_s + (j & 1) * kHalf, q, umma_desc(key(j), kChunkBytes, 1024));
+        mma_features_ss<BLOCKS>(tm_s + (j & 1) * kHalf, q, umma_desc(key(j), kChunkBytes, 1024), steps);
         if (!ctl.v.ready(j, wait)) return;
-        mma_features_ts<BLOCKS, kHalf>(tm_dp + (j & 1) * kHalf, tm_go, umma_desc(value(j), kChunkBytes, 1024));
+        mma_features_ts<BLOCKS, kHalf>(tm_dp + (j & 1) * kHalf, tm_go, umma_desc(value(j), kChunkBytes, 1024), steps);
         ctl.v.release(j);
         umma_commit(&ctl.s_full[j & 1]);
       };
@@ -712,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         const bool first = j == 0 || !((t0 + j) & 1), last = j == n - 1 || ((t0 + j) & 1);   // of its tile
         if (first) wait(&ctl.acc_empty, group++ ^ 1);
         if (!wait.ok) break;
-        mma_rows<BLOCKS, 16>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(key(j), 2 * kChunkBytes, 1024), !first);
+        mma_rows<BLOCKS, 16>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(key(j), 2 * kChunkBytes, 1024), !first, steps);
         ctl.k.release(j);
         if (last) umma_commit(&ctl.acc_full);
       }
@@ -809,10 +817,8 @@ struct Dkv : Sizes<BLOCKS> {
 // memory, V in tensor memory; Q and dout come in half tiles of 64 rows with their log-sums
 // and deltas.  A thread holds (key, quarter): 16 rows of the scores and a quarter of the
 // features of both gradients.
-template <int BLOCKS>
-__global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant__ AttnArgs a,
-                                                          const __grid_constant__ Tiles w, int row_tiles, bool vec_out,
-                                                          uint32_t* err) {
+template <int BLOCKS, bool FULL>
+DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tiles, bool vec_out, uint32_t* err) {
   using S = Dkv<BLOCKS>;
   extern __shared__ __align__(1024) uint8_t sm[];
   auto& ctl = *reinterpret_cast<typename S::Control*>(sm + S::kEnd);
@@ -840,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
   // the accumulators, the operand V, S and dP (each also P's and dS's place)
   const uint32_t tm_dk = ctl.tmem, tm_dv = tm_dk + 128, tm_v = tm_dk + 256, tm_s = tm_dk + 384, tm_dp = tm_dk + 448;
   pdl_entry();
-  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = blockIdx.x / heads;    // long ones first
+  const int heads = a.batch * a.kv_heads, bh = block % heads, tile = block / heads;    // long ones first
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
   const bool splits_head = head_splits(w.stats[bh], a.scale, a.dim);
   if (!splits_head && threadIdx.x == 0) *w.any = 1;          // work for the float32 kernels
@@ -853,6 +859,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     n = last > first ? (last + kHalf - 1) / kHalf - t0 : 0;
   }
   Waits wait{err};
+  const int steps = FULL ? 4 * BLOCKS : (a.dim + 15) / 16;
 
   if (warp == kSoft) {
     if (n && elect_one()) {
@@ -880,12 +887,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       auto grad = [&](int j) { return smem_addr(sm + S::kGo + j % S::kRowsGo * S::kSlotBytes); };
       auto scores = [&](int j) {                   // S^T(j) = K Q^T
         if (!ctl.q.ready(j, wait)) return;
-        mma_features_ss<BLOCKS>(tm_s, k, umma_desc(query(j), kChunkBytes, 1024));
+        mma_features_ss<BLOCKS>(tm_s, k, umma_desc(query(j), kChunkBytes, 1024), steps);
         umma_commit(&ctl.s_full);
       };
       auto dps = [&](int j) {                      // dP^T(j) = V dout^T
         if (!ctl.go.ready(j, wait)) return;
-        mma_features_ts<BLOCKS, kHalf>(tm_dp, tm_v, umma_desc(grad(j), kChunkBytes, 1024));
+        mma_features_ts<BLOCKS, kHalf>(tm_dp, tm_v, umma_desc(grad(j), kChunkBytes, 1024), steps);
         umma_commit(&ctl.dp_full);
       };
       scores(0);
@@ -896,14 +903,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
         wait(&ctl.p_full, j);
         if (first) wait(&ctl.dv_empty, group ^ 1);
         if (!wait.ok) break;
-        mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(grad(j), 2 * kChunkBytes, 1024), !first);
+        mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(grad(j), 2 * kChunkBytes, 1024), !first, steps);
         ctl.go.release(j);
         if (last) umma_commit(&ctl.dv_full);
         if (j + 1 < n) scores(j + 1);
         wait(&ctl.ds_full, j);
         if (first) wait(&ctl.dk_empty, group++ ^ 1);
         if (!wait.ok) break;
-        mma_rows<BLOCKS, 16>(tm_dk, tm_dp, umma_desc(query(j), 2 * kChunkBytes, 1024), !first);
+        mma_rows<BLOCKS, 16>(tm_dk, tm_dp, umma_desc(query(j), 2 * kChunkBytes, 1024), !first, steps);
         ctl.q.release(j);
         if (last) umma_commit(&ctl.dk_full);
         if (j + 1 < n) dps(j + 1);
@@ -1012,6 +1019,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
   if (warp == kSoft + 1) tmem_free(tm_dk, 512);
 }
 
+// Both in one launch: the long tiles of keys first, then the tiles of rows, which fill the
+// SMs that the last tiles of keys leave idle.
+template <int BLOCKS, bool FULL>
+__global__ void __launch_bounds__(kThreads, 1) k_attn_backward(const __grid_constant__ AttnArgs a,
+                                                               const __grid_constant__ Tiles w, int row_tiles,
+                                                               int key_blocks, bool vec_q, bool vec_kv, uint32_t* err) {
+  if ((int)blockIdx.x < key_blocks) attn_dkv<BLOCKS, FULL>(a, w, blockIdx.x, row_tiles, vec_kv, err);
+  else attn_dq<BLOCKS, FULL>(a, w, blockIdx.x - key_blocks, row_tiles, vec_q, err);
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -1073,39 +1090,34 @@ cudaError_t prepare(const AttnArgs& a, const Layout& L, uint8_t* w, bool backwar
   const bool vec = a.dim % 4 == 0 && aligned(a.q, a.qs) && aligned(a.k, a.ks) && aligned(a.v, a.vs) &&
                    (!backward || aligned(a.dout, a.os));
   const int tq = (int)L.row_tiles, tk = (int)L.key_tiles;
-  if (L.blocks == 1) k_attn_split<1><<<(unsigned)split, 512, 0, st>>>(a, t, tq, tk, vec);
-  else k_attn_split<2><<<(unsigned)split, 512, 0, st>>>(a, t, tq, tk, vec);
-  return cudaGetLastError();
+  return launch_pdl(L.blocks == 1 ? k_attn_split<1> : k_attn_split<2>, dim3((unsigned)split), dim3(512), 0, st, a, t, tq,
+                    tk, vec);
 }
 
-template <int BLOCKS>
+template <int BLOCKS, bool FULL>
 cudaError_t forward(const AttnArgs& a, const Layout& L, const Tiles& t, float* part, cudaStream_t st) {
   using S = Forward<BLOCKS>;
-  static const cudaError_t set = cudaFuncSetAttribute(k_attn_forward<BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  static const cudaError_t set = cudaFuncSetAttribute(k_attn_forward<BLOCKS, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                       (int)S::kSmem);
   if (set != cudaSuccess) return set;
   const int64_t blocks = L.heads * L.row_tiles * L.splits;
   if (blocks > INT_MAX) return cudaErrorInvalidConfiguration;
-  return launch_pdl(k_attn_forward<BLOCKS>, dim3((unsigned)blocks), dim3(kThreads), S::kSmem, st, a, t,
+  return launch_pdl(k_attn_forward<BLOCKS, FULL>, dim3((unsigned)blocks), dim3(kThreads), S::kSmem, st, a, t,
                     (int)L.row_tiles, L.splits, part, a.dim % 4 == 0 && aligned(a.out, a.os), device_error_word());
 }
 
-template <int BLOCKS>
+template <int BLOCKS, bool FULL>
 cudaError_t backward(const AttnArgs& a, const Layout& L, const Tiles& t, cudaStream_t st) {
-  static const cudaError_t set_q = cudaFuncSetAttribute(k_attn_dq<BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                        (int)Dq<BLOCKS>::kSmem);
-  static const cudaError_t set_kv = cudaFuncSetAttribute(k_attn_dkv<BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                         (int)Dkv<BLOCKS>::kSmem);
-  if (set_q != cudaSuccess) return set_q;
-  if (set_kv != cudaSuccess) return set_kv;
+  constexpr size_t kSmem = std::max(Dq<BLOCKS>::kSmem, Dkv<BLOCKS>::kSmem);
+  static const cudaError_t set = cudaFuncSetAttribute(k_attn_backward<BLOCKS, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                      (int)kSmem);
+  if (set != cudaSuccess) return set;
   const int64_t nq = L.heads * L.row_tiles, nk = L.heads * L.key_tiles;
-  if (nq > INT_MAX || nk > INT_MAX) return cudaErrorInvalidConfiguration;
-  const bool vec = a.dim % 4 == 0, vec_kv = vec && aligned(a.dk, a.dks) && aligned(a.dv, a.dvs);
-  cudaError_t e = launch_pdl(k_attn_dkv<BLOCKS>, dim3((unsigned)nk), dim3(kThreads), Dkv<BLOCKS>::kSmem, st, a, t,
-                             (int)L.row_tiles, vec_kv, device_error_word());
-  if (e != cudaSuccess) return e;
-  return launch_pdl(k_attn_dq<BLOCKS>, dim3((unsigned)nq), dim3(kThreads), Dq<BLOCKS>::kSmem, st, a, t,
-                    (int)L.row_tiles, vec && aligned(a.dq, a.dqs), device_error_word());
+  if (nq + nk > INT_MAX) return cudaErrorInvalidConfiguration;
+  const bool vec = a.dim % 4 == 0;
+  return launch_pdl(k_attn_backward<BLOCKS, FULL>, dim3((unsigned)(nq + nk)), dim3(kThreads), kSmem, st, a, t, (int)L.row_tiles,
+                    (int)nk, vec && aligned(a.dq, a.dqs), vec && aligned(a.dk, a.dks) && aligned(a.dv, a.dvs),
+                    device_error_word());
 }
 
 }  // namespace
@@ -1126,7 +1138,9 @@ cudaError_t launch_attn_tensor_forward(const AttnArgs& args, void* ws, cudaStrea
   a.stats = t.stats;
   a.any = t.any;
   float* part = reinterpret_cast<float*>(w + L.part);
-  e = L.blocks == 1 ? forward<1>(a, L, t, part, st) : forward<2>(a, L, t, part, st);
+  const auto run = L.blocks == 1 ? (a.dim == 64 ? forward<1, true> : forward<1, false>)
+                                 : (a.dim == 128 ? forward<2, true> : forward<2, false>);
+  e = run(a, L, t, part, st);
   if (e == cudaSuccess && L.splits > 1) e = launch_attn_join(a, L.splits, part, true, st);
   if (e == cudaSuccess) e = launch_attn_rows_forward(a, part, st);
   return e;
@@ -1141,7 +1155,9 @@ cudaError_t launch_attn_tensor_backward(const AttnArgs& args, void* ws, cudaStre
   a.stats = t.stats;
   a.any = t.any;
   a.delta = t.delta;
-  e = L.blocks == 1 ? backward<1>(a, L, t, st) : backward<2>(a, L, t, st);
+  const auto run = L.blocks == 1 ? (a.dim == 64 ? backward<1, true> : backward<1, false>)
+                                 : (a.dim == 128 ? backward<2, true> : backward<2, false>);
+  e = run(a, L, t, st);
   if (e == cudaSuccess) e = launch_attn_rows_backward(a, st);
   return e;
 }
