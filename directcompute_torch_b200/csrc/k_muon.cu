@@ -51,7 +51,7 @@ struct Product {
 };
 
 constexpr int kRows = 128, kEpi = 8;            // tile rows of a block, epilogue warps
-constexpr int kThreads = 32 * (kEpi + 2);
+constexpr int kThreads = 32 * (kEpi + 4);     // and a warp that loads, one that issues, two that give up their registers
 
 constexpr uint32_t kStaging = 4096;              // of an epilogue warp: its 32 rows of a chunk
 
@@ -78,28 +78,39 @@ DCT_DEV void tile_at(const Product& g, uint32_t t, uint32_t& z, uint32_t& i, uin
   j = r;
 }
 
-// The chunks of all tiles in a row are dealt to the workers (blocks, or pairs of blocks) in
-// equal runs of whole units: one chunk, so that every worker is busy to the end whatever the
-// number of tiles, or a whole tile.  A worker's share of one tile is a segment.
+// A worker (a block, or a pair of blocks) takes every workers-th tile as far as they go
+// around, so that the tiles at work at one time are neighbours and share their operands in
+// L2.  The tiles that are left go whole to some workers, or their chunks are dealt to all in
+// equal runs.  A worker's share of one tile is a segment.
 struct Segment {
   uint32_t tile, k0, k1;     // chunks [k0, k1) of the tile
   uint32_t first, count;     // the worker with the tile's first segment, the tile's segments
 };
 struct Run {
-  uint64_t at, end, units;
-  uint32_t kb, unit, workers;
-  DCT_DEV Run(uint32_t tiles, uint32_t kb_, uint32_t unit_, uint32_t worker, uint32_t workers_)
-      : units((uint64_t)tiles * (kb_ / unit_)), kb(kb_), unit(unit_), workers(workers_) {
-    at = worker * units / workers * unit;
-    end = (worker + 1) * units / workers * unit;
+  uint64_t at, end, units;   // of the tiles that are left
+  uint32_t kb, unit, worker, workers, round, rounds, used;
+  DCT_DEV Run(uint32_t tiles, uint32_t kb_, uint32_t unit_, uint32_t used_, uint32_t worker_, uint32_t workers_)
+      : units((uint64_t)(tiles % workers_) * (kb_ / unit_)), kb(kb_), unit(unit_), worker(worker_), workers(workers_),
+        round(0), rounds(tiles / workers_), used(used_) {
+    at = end = 0;
+    if (worker < used) {
+      at = worker * units / used * unit;
+      end = (worker + 1) * units / used * unit;
+    }
   }
-  DCT_DEV uint32_t worker_of(uint64_t chunk) const {
-    return (uint32_t)(((chunk / unit + 1) * workers - 1) / units);
-  }
+  DCT_DEV uint32_t worker_of(uint64_t chunk) const { return (uint32_t)(((chunk / unit + 1) * used - 1) / units); }
   DCT_DEV bool next(Segment& s) {
+    if (round < rounds) {
+      s.tile = round++ * workers + worker;
+      s.k0 = 0;
+      s.k1 = kb;
+      s.count = 1;
+      return true;
+    }
     if (at >= end) return false;
-    s.tile = (uint32_t)(at / kb);
-    const uint64_t base = (uint64_t)s.tile * kb;
+    const uint32_t t = (uint32_t)(at / kb);
+    const uint64_t base = (uint64_t)t * kb;
+    s.tile = rounds * workers + t;
     s.k0 = (uint32_t)(at - base);
     s.k1 = (uint32_t)min((uint64_t)kb, end - base);
     s.first = worker_of(base);
@@ -121,6 +132,7 @@ DCT_DEV void add8(float (&acc)[N], int at, float f, uint4 v) {
   }
 }
 
+DCT_DEV void prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 DCT_DEV void epilogue_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // Warps 0..7 drain and store, warp 8 loads, warp 9 issues the matrix instructions.
@@ -141,7 +153,7 @@ DCT_DEV void epilogue_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 // bounds the large products: 6.4 TB/s out of L2 at 2048 x 8192 without pairs.
 template <bool PAIR, int BN>
 __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__ Product g, uint32_t total,
-                                                         uint32_t unit, uint32_t* err) {
+                                                         uint32_t unit, uint32_t used, uint32_t* err) {
   using S = Shape<PAIR, BN>;
   constexpr uint32_t kDrain = PAIR ? 2 : 1;
   extern __shared__ uint8_t raw[];
@@ -173,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
   const uint32_t tmem = tmem_base;
   pdl_entry();
   const uint32_t mchunks = (g.M + 63) / 64, nchunks = (g.N + 63) / 64;
-  Run run(total, g.kb, unit, worker, PAIR ? gridDim.x / 2 : gridDim.x);
+  Run run(total, g.kb, unit, used, worker, PAIR ? gridDim.x / 2 : gridDim.x);
   Segment sg;
   // whether chunk k of an operand's tile is read with its rows as the contraction: its own
   // layout, or the mirror image of a chunk above the diagonal
@@ -181,6 +193,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
     return o.half ? tile < k / (S::kTileRows / 64) : o.mn;
   };
 
+  // 384 threads start with 168 registers, 64512 in all; 256 * 232 + 128 * 40 is as many
+  if (warp >= kEpi) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   if (warp == kEpi) {
     if (elect_one()) {
       uint32_t it = 0;
@@ -270,7 +285,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
         }
       }
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     constexpr int W = BN / 2;                     // columns of a thread's row
     const uint32_t side = warp >> 2;
     uint8_t* stage = sm + S::kStages * S::kStage + warp * kStaging;
@@ -279,6 +296,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
     // on meeting this one
     bool ok = true;
     while (run.next(sg)) {
+      uint32_t z, ti, tj;
+      tile_at(g, sg.tile, z, ti, tj);
+      // the warp's 32 rows from i0, the thread's columns from j0
+      const uint32_t i0 = ti * S::kTileRows + rank * kRows + (warp & 3) * 32, j0 = tj * BN + side * W;
+      // what the end of the tile reads, into L2 by then
+      if (g.D.p && i0 < mchunks * 64)
+        for (uint32_t c = 0; c < W && j0 + c < nchunks * 64; c += 64) {
+          const uint8_t* d = chunk_of(g.D, z, i0 >> 6, (j0 + c) >> 6) + (i0 & 32) * 128 + lane * 128;
+          prefetch(d);
+          prefetch(d + kChunkBytes);
+        }
+      if (g.update && i0 + lane < g.M)
+        for (uint32_t c = 0; c < W && j0 + c < g.N; c += 32) prefetch(g.out + ((uint64_t)z * g.M + i0 + lane) * g.N + j0 + c);
       float acc[W];
 #pragma unroll
       for (int c = 0; c < W; ++c) acc[c] = 0.f;
@@ -305,12 +335,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
       }
       if (sg.count > 1) {                         // the tile is cut
         auto slot = [&](uint32_t w) {
-          return g.parts + (size_t)(2 * (PAIR ? 2 * w + rank : w) + (w == sg.first)) * (kRows * BN) + threadIdx.x;
+          return reinterpret_cast<float4*>(
+                     g.parts + (size_t)(2 * (PAIR ? 2 * w + rank : w) + (w == sg.first)) * (kRows * BN)) + threadIdx.x;
         };
         uint32_t* arrived = g.arrived + (PAIR ? 2 * sg.first + rank : sg.first);
-        float* mine = slot(worker);
+        float4* mine = slot(worker);
 #pragma unroll
-        for (int c = 0; c < W; ++c) __stcg(mine + c * 256, acc[c]);
+        for (int c = 0; c < W / 4; ++c)
+          __stcg(mine + c * 256, make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]));
         __threadfence();
         epilogue_sync();
         if (threadIdx.x == 0) order = atomicAdd(arrived, 1u);
@@ -319,18 +351,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
         if (!last) continue;
         __threadfence();
         if (threadIdx.x == 0) *arrived = 0;
+        auto add = [&](uint32_t w) {
+          const float4* p = slot(w);
 #pragma unroll
-        for (int c = 0; c < W; ++c) acc[c] = 0.f;
-        for (uint32_t b = sg.first; b < sg.first + sg.count; ++b) {
-          const float* p = slot(b);
+          for (int c = 0; c < W / 4; ++c) {
+            const float4 v = __ldcg(p + c * 256);
+            acc[4 * c] += v.x;
+            acc[4 * c + 1] += v.y;
+            acc[4 * c + 2] += v.z;
+            acc[4 * c + 3] += v.w;
+          }
+        };
+        if (sg.count == 2) {                      // two sums: either order gives the same
+          add(worker == sg.first ? sg.first + 1 : sg.first);
+        } else {
 #pragma unroll
-          for (int c = 0; c < W; ++c) acc[c] += __ldcg(p + c * 256);
+          for (int c = 0; c < W; ++c) acc[c] = 0.f;
+          for (uint32_t w = sg.first; w < sg.first + sg.count; ++w) add(w);
         }
       }
-      uint32_t z, ti, tj;
-      tile_at(g, sg.tile, z, ti, tj);
-      // the warp's 32 rows from i0, the thread's row i, its columns from j0
-      const uint32_t i0 = ti * S::kTileRows + rank * kRows + (warp & 3) * 32, i = i0 + lane, j0 = tj * BN + side * W;
+      const uint32_t i = i0 + lane;
 #pragma unroll
       for (int c = 0; c < W; ++c) acc[c] *= g.sa;
       if (g.D.p && i0 < mchunks * 64) {
@@ -917,14 +957,14 @@ cudaError_t product_as(Product g, uint32_t batch, cudaStream_t st) {
   if (g.half) g.tiles = g.mt * (g.mt + 1) / 2;
   const uint64_t total = (uint64_t)g.tiles * batch, work = total * g.kb;
   if (total >= (1ull << 31)) return cudaErrorInvalidConfiguration;
-  // Whole tiles, or cut ones: whichever has the shorter longest run.  A cut tile's meeting in
-  // memory costs about as much as 6 chunks (one matrix of 1024 x 8192: 700 us cut, 1079 us
-  // whole; twelve of 768 x 768: 552 and 550 us), and runs below 4 chunks gain nothing.
+  // The tiles that do not go around: whole, or cut in runs of 4 chunks or more, whichever ends
+  // first.  A cut tile's meeting in memory costs about as much as 6 chunks (one matrix of
+  // 1024 x 8192: 700 us cut, 1079 us whole; twelve of 768 x 768: 552 and 550 us).
   constexpr uint64_t kShortest = 4, kMeeting = 6;
-  const uint64_t whole = (total + most - 1) / most * g.kb;
-  const uint64_t cut = std::max<uint64_t>(kShortest, (work + most - 1) / most) + kMeeting;
-  const uint32_t unit = whole <= cut ? g.kb : 1;
-  const uint64_t runs = std::min<uint64_t>(unit == 1 ? (work + kShortest - 1) / kShortest : total, most);
+  const uint64_t workers = std::min<uint64_t>(work / kShortest + 1, most), left = total % workers;
+  const uint64_t cut = std::max<uint64_t>(kShortest, (left * g.kb + workers - 1) / workers) + kMeeting;
+  const uint32_t unit = g.kb <= cut ? g.kb : 1;
+  const uint64_t used = std::min<uint64_t>(unit == 1 ? (left * g.kb + kShortest - 1) / kShortest : left, workers);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -932,13 +972,13 @@ cudaError_t product_as(Product g, uint32_t batch, cudaStream_t st) {
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = PAIR ? 2 : 1;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)runs * (PAIR ? 2 : 1));
+  cfg.gridDim = dim3((unsigned)workers * (PAIR ? 2 : 1));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, g, (uint32_t)total, unit, device_error_word());
+  return cudaLaunchKernelEx(&cfg, kernel, g, (uint32_t)total, unit, (uint32_t)used, device_error_word());
 }
 
 // The tile of a call's products: its rows and columns, of which symmetric results store
