@@ -206,8 +206,14 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
 // shared memory for whole ones (a matrix instruction 64 columns wide takes 45 or 48 cycles,
 // one of 128 takes 64: measured).
 constexpr int kSoft = 16;
-constexpr int kThreads = 32 * (kSoft + 3);
+constexpr int kThreads = 32 * (kSoft + 4);
 constexpr int kHalf = 64;
+
+// Registers move from the four helping warps (one idle) to the computing ones: 640 threads
+// start with 96 each, 61440 in all, and 512 * 104 + 128 * 56 is 60416.  (Inside the roles'
+// branches, where the compiler sees which code has how many.)
+DCT_DEV void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
+DCT_DEV void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
 
 template <int BLOCKS>
 struct Sizes {
@@ -449,6 +455,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
   Waits wait{err};
   const int steps = FULL ? 4 * BLOCKS : (a.dim + 15) / 16;
 
+  if (warp >= kSoft) {
+    registers_down();
   if (warp == kSoft) {
     if (elect_one())
       ctl.k.fill(n, S::kTileBytes, wait, [&](int it, int s, uint64_t* bar) {
@@ -485,7 +493,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
         umma_commit(&ctl.o_full);
       }
     }
+  }
   } else if (splits_head) {
+    registers_up();
     const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
     const RowAt at_row(a, hk, min(r, rows - 1));
     const bool in = r < rows && at_row.i < span.m;
@@ -683,6 +693,8 @@ DCT_DEV void attn_dq(const AttnArgs& a, const Tiles& w, int block, int row_tiles
   Waits wait{err};
   const int steps = FULL ? 4 * BLOCKS : (a.dim + 15) / 16;
 
+  if (warp >= kSoft) {
+    registers_down();
   if (warp == kSoft) {
     if (n && elect_one()) {
       mbar_arrive_expect_tx(&ctl.q_full, S::kTileBytes);
@@ -725,7 +737,9 @@ DCT_DEV void attn_dq(const AttnArgs& a, const Tiles& w, int block, int row_tiles
         if (last) umma_commit(&ctl.acc_full);
       }
     }
+  }
   } else if (splits_head) {
+    registers_up();
     const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
     const RowAt at_row(a, hk, min(r, rows - 1));
     const bool in = r < rows && at_row.i < span.m;
@@ -861,6 +875,8 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
   Waits wait{err};
   const int steps = FULL ? 4 * BLOCKS : (a.dim + 15) / 16;
 
+  if (warp >= kSoft) {
+    registers_down();
   if (warp == kSoft) {
     if (n && elect_one()) {
       mbar_arrive_expect_tx(&ctl.k_full, S::kTileBytes);
@@ -916,7 +932,9 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
         if (j + 1 < n) dps(j + 1);
       }
     }
+  }
   } else if (splits_head) {
+    registers_up();
     const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, key = j0 + row;
     // rows that see the thread's key
     const int lo = key < span.n ? span.first(a, key) * a.group : 0, hi = key < span.n ? span.last(a, key) * a.group : 0;

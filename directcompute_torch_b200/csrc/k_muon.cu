@@ -989,11 +989,12 @@ cudaError_t product(int tile, const Product& g, uint32_t batch, cudaStream_t st)
   return product_as<true, 256>(g, batch, st);
 }
 
-// Pairs with tiles of 256 for large matrices, where the loads bound (4096 x 4096: 3.91 ms,
-// 4.94 with 128); below, smaller tiles divide better (1024 x 8192: 700 us, 962 with 256).
+// Pairs with tiles of 256 where these fill a fifth of the SMs or more with one symmetric
+// product (twelve of 768 x 768: 479 us, 509 with tiles of 128; 4096 x 4096: 3.3 ms, 4.9);
+// below, smaller tiles divide better (1500 x 1500: 519 us, 419 with 128).
 int tile_of(const MuonArgs& a) {
-  const uint32_t s = std::min(a.rows, a.cols);
-  return s <= 64 ? 64 : s < 2048 ? 128 : 256;
+  const uint64_t s = std::min(a.rows, a.cols), n = (s + 255) / 256;
+  return s <= 64 ? 64 : n * (n + 1) / 2 * a.batch * 5 >= (uint64_t)dev_info().sm_count ? 256 : 128;
 }
 
 // the power of two that brings `most` to at most 2^15
