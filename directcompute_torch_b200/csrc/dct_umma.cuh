@@ -45,9 +45,11 @@ DCT_DEV float2 join2(uint32_t hi, uint32_t lo) {
 // bulk copy of shared memory to global memory (addresses and size multiples of 16), and the
 // wait until the copies of this thread have been read out of shared memory / have landed
 DCT_DEV void bulk_store(void* gmem_dst, const void* smem_src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;" ::"l"(gmem_dst),
-               "r"(smem_addr(smem_src)), "r"(bytes)
-               : "memory");
+  asm volatile(
+      "cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\t"
+      "cp.async.bulk.commit_group;" ::"l"(gmem_dst),
+      "r"(smem_addr(smem_src)), "r"(bytes)
+      : "memory");
 }
 DCT_DEV void bulk_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 DCT_DEV void bulk_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
@@ -114,6 +116,16 @@ DCT_DEV bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
   return p != 0;
+}
+
+// Whether a block of `kernel` is launched with at least `need` registers in all: what its
+// warps take (setmaxnreg) from what they give up must be there, or they would wait for ever.
+template <typename K>
+inline cudaError_t launched_with(K kernel, int threads, int need) {
+  cudaFuncAttributes a{};
+  const cudaError_t e = cudaFuncGetAttributes(&a, kernel);
+  if (e != cudaSuccess) return e;
+  return (a.numRegs + 7) / 8 * 8 * threads >= need ? cudaSuccess : cudaErrorInvalidConfiguration;
 }
 
 // ---- matrix instructions ---------------------------------------------------------

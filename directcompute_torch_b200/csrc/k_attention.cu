@@ -146,7 +146,9 @@ DCT_DEV void rows_forward(const AttnArgs& a, int item, int groups, int splits, f
     // Two keys an octet at a time, two such steps ahead of their use in shared memory.  A
     // thread copies just what it reads itself, so nothing but its own copies is waited for.
     extern __shared__ float4 ring[];
-    auto place = [&](int step, int u, int value) { return ring + (((step % kAhead * 2 + u) * 2 + value) * NV) * (32 * kWarps) + threadIdx.x; };
+    auto place = [&](int step, int u, int value) {
+      return ring + ((step % kAhead * 2 + u) * 2 + value) * NV * (32 * kWarps) + threadIdx.x;
+    };
     auto fetch = [&](int step) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -565,8 +567,8 @@ cudaError_t launch_attn_rows_backward(const AttnArgs& a, cudaStream_t st) {
     constexpr bool V = decltype(v)::value;
     const int nq = (int)(gq * heads), nk = (int)(gk * heads);
     if (!(nq + (int64_t)nk)) return cudaSuccess;
-    return launch_pdl(k_attn_rows_backward<NV, V, R>, dim3(blocks_for(a, nq + (int64_t)nk)), dim3(32 * kWarps), 0, st, a,
-                      (int)gq, nq, (int)gk, nk);
+    return launch_pdl(k_attn_rows_backward<NV, V, R>, dim3(blocks_for(a, nq + (int64_t)nk)), dim3(32 * kWarps), 0, st,
+                      a, (int)gq, nq, (int)gk, nk);
   });
 }
 

@@ -210,10 +210,12 @@ constexpr int kThreads = 32 * (kSoft + 4);
 constexpr int kHalf = 64;
 
 // Registers move from the four helping warps (one idle) to the computing ones: 640 threads
-// start with 96 each, 61440 in all, and 512 * 104 + 128 * 56 is 60416.  (Inside the roles'
-// branches, where the compiler sees which code has how many.)
-DCT_DEV void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
-DCT_DEV void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
+// start with 96 each, 61440 in all, of which 60416 are taken.  (Inside the roles' branches,
+// where the compiler sees which code has how many.)
+constexpr int kUpRegs = 104, kDownRegs = 56;
+constexpr int kRegs = 32 * (kSoft * kUpRegs + 4 * kDownRegs);
+DCT_DEV void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kUpRegs)); }
+DCT_DEV void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDownRegs)); }
 
 template <int BLOCKS>
 struct Sizes {
@@ -457,43 +459,43 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
 
   if (warp >= kSoft) {
     registers_down();
-  if (warp == kSoft) {
-    if (elect_one())
-      ctl.k.fill(n, S::kTileBytes, wait, [&](int it, int s, uint64_t* bar) {
-        load_tile<BLOCKS>(w, bh, 1, t0 + it, sm + s * S::kTileBytes, bar);
-      });
-  } else if (warp == kSoft + 2) {
-    if (elect_one())
-      ctl.v.fill(2 * n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
-        load_half<BLOCKS>(w, bh, 2, 2 * t0 + it, sm + S::kV + s * S::kSlotBytes, bar);
-      });
-  } else if (warp == kSoft + 1) {
-    if (n && elect_one()) {
-      wait(&ctl.q_full, 0);
-      auto scores = [&](int j) {                   // S(j) = Q K(j)^T
-        if (!ctl.k.ready(j, wait)) return;
-        mma_features_ts<BLOCKS, kTile>(tm_s + (j & 1) * kTile, tm_q,
-                                       umma_desc(smem_addr(sm + j % S::kKeys * S::kTileBytes), kChunkBytes, 1024), steps);
-        ctl.k.release(j);
-        umma_commit(&ctl.s_full[j & 1]);
-      };
-      scores(0);
-      for (int j = 0; j < n && wait.ok; ++j) {
-        if (j + 1 < n) scores(j + 1);
-        wait(&ctl.p_full[j & 1], j >> 1);
-        wait(&ctl.o_empty, j ^ 1);
-        for (int h = 0; h < 2; ++h) {
-          const int it = 2 * j + h;
-          if (!ctl.v.ready(it, wait)) break;
-          mma_rows<BLOCKS, 32>(tm_o, tm_s + (j & 1) * kTile + h * kHalf,
-                               umma_desc(smem_addr(sm + S::kV + it % S::kValues * S::kSlotBytes), 2 * kChunkBytes, 1024), h,
-                               steps);
-          ctl.v.release(it);
+    if (warp == kSoft) {
+      if (elect_one())
+        ctl.k.fill(n, S::kTileBytes, wait, [&](int it, int s, uint64_t* bar) {
+          load_tile<BLOCKS>(w, bh, 1, t0 + it, sm + s * S::kTileBytes, bar);
+        });
+    } else if (warp == kSoft + 2) {
+      if (elect_one())
+        ctl.v.fill(2 * n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
+          load_half<BLOCKS>(w, bh, 2, 2 * t0 + it, sm + S::kV + s * S::kSlotBytes, bar);
+        });
+    } else if (warp == kSoft + 1) {
+      if (n && elect_one()) {
+        wait(&ctl.q_full, 0);
+        auto key = [&](int j) { return smem_addr(sm + j % S::kKeys * S::kTileBytes); };
+        auto value = [&](int it) { return smem_addr(sm + S::kV + it % S::kValues * S::kSlotBytes); };
+        auto scores = [&](int j) {                 // S(j) = Q K(j)^T
+          if (!ctl.k.ready(j, wait)) return;
+          mma_features_ts<BLOCKS, kTile>(tm_s + (j & 1) * kTile, tm_q, umma_desc(key(j), kChunkBytes, 1024), steps);
+          ctl.k.release(j);
+          umma_commit(&ctl.s_full[j & 1]);
+        };
+        scores(0);
+        for (int j = 0; j < n && wait.ok; ++j) {
+          if (j + 1 < n) scores(j + 1);
+          wait(&ctl.p_full[j & 1], j >> 1);
+          wait(&ctl.o_empty, j ^ 1);
+          for (int h = 0; h < 2; ++h) {
+            const int it = 2 * j + h;
+            if (!ctl.v.ready(it, wait)) break;
+            mma_rows<BLOCKS, 32>(tm_o, tm_s + (j & 1) * kTile + h * kHalf, umma_desc(value(it), 2 * kChunkBytes, 1024),
+                                 h, steps);
+            ctl.v.release(it);
+          }
+          umma_commit(&ctl.o_full);
         }
-        umma_commit(&ctl.o_full);
       }
     }
-  }
   } else if (splits_head) {
     registers_up();
     const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
@@ -695,49 +697,49 @@ DCT_DEV void attn_dq(const AttnArgs& a, const Tiles& w, int block, int row_tiles
 
   if (warp >= kSoft) {
     registers_down();
-  if (warp == kSoft) {
-    if (n && elect_one()) {
-      mbar_arrive_expect_tx(&ctl.q_full, S::kTileBytes);
-      load_tile<BLOCKS>(w, bh, 0, tile, sm, &ctl.q_full);
-      ctl.k.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
-        load_half<BLOCKS>(w, bh, 1, t0 + it, sm + S::kK + s * S::kSlotBytes, bar);
-      });
-      mbar_wait(&ctl.q_full, 0, err);
-    }
-  } else if (warp == kSoft + 2) {
-    if (elect_one())
-      ctl.v.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
-        load_half<BLOCKS>(w, bh, 2, t0 + it, sm + S::kV + s * S::kSlotBytes, bar);
-      });
-  } else if (warp == kSoft + 1) {
-    if (n && elect_one()) {
-      wait(&ctl.q_full, 0);
-      wait(&ctl.go_full, 0);
-      const uint64_t q = umma_desc(smem_addr(sm), kChunkBytes, 1024);
-      auto key = [&](int j) { return smem_addr(sm + S::kK + j % S::kKeys * S::kSlotBytes); };
-      auto value = [&](int j) { return smem_addr(sm + S::kV + j % S::kValues * S::kSlotBytes); };
-      auto scores = [&](int j) {                   // S(j) = Q K^T, dP(j) = dout V^T
-        if (!ctl.k.ready(j, wait)) return;
-        mma_features_ss<BLOCKS>(tm_s + (j & 1) * kHalf, q, umma_desc(key(j), kChunkBytes, 1024), steps);
-        if (!ctl.v.ready(j, wait)) return;
-        mma_features_ts<BLOCKS, kHalf>(tm_dp + (j & 1) * kHalf, tm_go, umma_desc(value(j), kChunkBytes, 1024), steps);
-        ctl.v.release(j);
-        umma_commit(&ctl.s_full[j & 1]);
-      };
-      int group = 0;
-      scores(0);
-      for (int j = 0; j < n && wait.ok; ++j) {
-        if (j + 1 < n) scores(j + 1);
-        wait(&ctl.ds_full[j & 1], j >> 1);
-        const bool first = j == 0 || !((t0 + j) & 1), last = j == n - 1 || ((t0 + j) & 1);   // of its tile
-        if (first) wait(&ctl.acc_empty, group++ ^ 1);
-        if (!wait.ok) break;
-        mma_rows<BLOCKS, 16>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(key(j), 2 * kChunkBytes, 1024), !first, steps);
-        ctl.k.release(j);
-        if (last) umma_commit(&ctl.acc_full);
+    if (warp == kSoft) {
+      if (n && elect_one()) {
+        mbar_arrive_expect_tx(&ctl.q_full, S::kTileBytes);
+        load_tile<BLOCKS>(w, bh, 0, tile, sm, &ctl.q_full);
+        ctl.k.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
+          load_half<BLOCKS>(w, bh, 1, t0 + it, sm + S::kK + s * S::kSlotBytes, bar);
+        });
+        mbar_wait(&ctl.q_full, 0, err);
+      }
+    } else if (warp == kSoft + 2) {
+      if (elect_one())
+        ctl.v.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
+          load_half<BLOCKS>(w, bh, 2, t0 + it, sm + S::kV + s * S::kSlotBytes, bar);
+        });
+    } else if (warp == kSoft + 1) {
+      if (n && elect_one()) {
+        wait(&ctl.q_full, 0);
+        wait(&ctl.go_full, 0);
+        const uint64_t q = umma_desc(smem_addr(sm), kChunkBytes, 1024);
+        auto key = [&](int j) { return smem_addr(sm + S::kK + j % S::kKeys * S::kSlotBytes); };
+        auto value = [&](int j) { return smem_addr(sm + S::kV + j % S::kValues * S::kSlotBytes); };
+        auto scores = [&](int j) {                   // S(j) = Q K^T, dP(j) = dout V^T
+          if (!ctl.k.ready(j, wait)) return;
+          mma_features_ss<BLOCKS>(tm_s + (j & 1) * kHalf, q, umma_desc(key(j), kChunkBytes, 1024), steps);
+          if (!ctl.v.ready(j, wait)) return;
+          mma_features_ts<BLOCKS, kHalf>(tm_dp + (j & 1) * kHalf, tm_go, umma_desc(value(j), kChunkBytes, 1024), steps);
+          ctl.v.release(j);
+          umma_commit(&ctl.s_full[j & 1]);
+        };
+        int group = 0;
+        scores(0);
+        for (int j = 0; j < n && wait.ok; ++j) {
+          if (j + 1 < n) scores(j + 1);
+          wait(&ctl.ds_full[j & 1], j >> 1);
+          const bool first = j == 0 || !((t0 + j) & 1), last = j == n - 1 || ((t0 + j) & 1);   // of its tile
+          if (first) wait(&ctl.acc_empty, group++ ^ 1);
+          if (!wait.ok) break;
+          mma_rows<BLOCKS, 16>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(key(j), 2 * kChunkBytes, 1024), !first, steps);
+          ctl.k.release(j);
+          if (last) umma_commit(&ctl.acc_full);
+        }
       }
     }
-  }
   } else if (splits_head) {
     registers_up();
     const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
@@ -877,62 +879,62 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
 
   if (warp >= kSoft) {
     registers_down();
-  if (warp == kSoft) {
-    if (n && elect_one()) {
-      mbar_arrive_expect_tx(&ctl.k_full, S::kTileBytes);
-      load_tile<BLOCKS>(w, bh, 1, tile, sm, &ctl.k_full);
-      ctl.q.fill(n, S::kSlotBytes + 2 * kHalf * 4, wait, [&](int it, int s, uint64_t* bar) {
-        const int64_t at_stat = (int64_t)bh * row_tiles * kTile + (int64_t)(t0 + it) * kHalf;
-        load_half<BLOCKS>(w, bh, 0, t0 + it, sm + S::kQ + s * S::kSlotBytes, bar);
-        bulk_load(ctl.lse[s], w.lse2 + at_stat, kHalf * 4, bar);
-        bulk_load(ctl.delta[s], w.delta + at_stat, kHalf * 4, bar);
-      });
-      mbar_wait(&ctl.k_full, 0, err);
-    }
-  } else if (warp == kSoft + 2) {
-    if (elect_one())
-      ctl.go.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
-        load_half<BLOCKS>(w, bh, 3, t0 + it, sm + S::kGo + s * S::kSlotBytes, bar);
-      });
-  } else if (warp == kSoft + 1) {
-    if (n && elect_one()) {
-      wait(&ctl.k_full, 0);
-      wait(&ctl.v_full, 0);
-      const uint64_t k = umma_desc(smem_addr(sm), kChunkBytes, 1024);
-      auto query = [&](int j) { return smem_addr(sm + S::kQ + j % S::kRowsQ * S::kSlotBytes); };
-      auto grad = [&](int j) { return smem_addr(sm + S::kGo + j % S::kRowsGo * S::kSlotBytes); };
-      auto scores = [&](int j) {                   // S^T(j) = K Q^T
-        if (!ctl.q.ready(j, wait)) return;
-        mma_features_ss<BLOCKS>(tm_s, k, umma_desc(query(j), kChunkBytes, 1024), steps);
-        umma_commit(&ctl.s_full);
-      };
-      auto dps = [&](int j) {                      // dP^T(j) = V dout^T
-        if (!ctl.go.ready(j, wait)) return;
-        mma_features_ts<BLOCKS, kHalf>(tm_dp, tm_v, umma_desc(grad(j), kChunkBytes, 1024), steps);
-        umma_commit(&ctl.dp_full);
-      };
-      scores(0);
-      dps(0);
-      int group = 0;
-      for (int j = 0; j < n && wait.ok; ++j) {
-        const bool first = j == 0 || !((t0 + j) & 1), last = j == n - 1 || ((t0 + j) & 1);   // of its tile
-        wait(&ctl.p_full, j);
-        if (first) wait(&ctl.dv_empty, group ^ 1);
-        if (!wait.ok) break;
-        mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(grad(j), 2 * kChunkBytes, 1024), !first, steps);
-        ctl.go.release(j);
-        if (last) umma_commit(&ctl.dv_full);
-        if (j + 1 < n) scores(j + 1);
-        wait(&ctl.ds_full, j);
-        if (first) wait(&ctl.dk_empty, group++ ^ 1);
-        if (!wait.ok) break;
-        mma_rows<BLOCKS, 16>(tm_dk, tm_dp, umma_desc(query(j), 2 * kChunkBytes, 1024), !first, steps);
-        ctl.q.release(j);
-        if (last) umma_commit(&ctl.dk_full);
-        if (j + 1 < n) dps(j + 1);
+    if (warp == kSoft) {
+      if (n && elect_one()) {
+        mbar_arrive_expect_tx(&ctl.k_full, S::kTileBytes);
+        load_tile<BLOCKS>(w, bh, 1, tile, sm, &ctl.k_full);
+        ctl.q.fill(n, S::kSlotBytes + 2 * kHalf * 4, wait, [&](int it, int s, uint64_t* bar) {
+          const int64_t at_stat = (int64_t)bh * row_tiles * kTile + (int64_t)(t0 + it) * kHalf;
+          load_half<BLOCKS>(w, bh, 0, t0 + it, sm + S::kQ + s * S::kSlotBytes, bar);
+          bulk_load(ctl.lse[s], w.lse2 + at_stat, kHalf * 4, bar);
+          bulk_load(ctl.delta[s], w.delta + at_stat, kHalf * 4, bar);
+        });
+        mbar_wait(&ctl.k_full, 0, err);
+      }
+    } else if (warp == kSoft + 2) {
+      if (elect_one())
+        ctl.go.fill(n, S::kSlotBytes, wait, [&](int it, int s, uint64_t* bar) {
+          load_half<BLOCKS>(w, bh, 3, t0 + it, sm + S::kGo + s * S::kSlotBytes, bar);
+        });
+    } else if (warp == kSoft + 1) {
+      if (n && elect_one()) {
+        wait(&ctl.k_full, 0);
+        wait(&ctl.v_full, 0);
+        const uint64_t k = umma_desc(smem_addr(sm), kChunkBytes, 1024);
+        auto query = [&](int j) { return smem_addr(sm + S::kQ + j % S::kRowsQ * S::kSlotBytes); };
+        auto grad = [&](int j) { return smem_addr(sm + S::kGo + j % S::kRowsGo * S::kSlotBytes); };
+        auto scores = [&](int j) {                   // S^T(j) = K Q^T
+          if (!ctl.q.ready(j, wait)) return;
+          mma_features_ss<BLOCKS>(tm_s, k, umma_desc(query(j), kChunkBytes, 1024), steps);
+          umma_commit(&ctl.s_full);
+        };
+        auto dps = [&](int j) {                      // dP^T(j) = V dout^T
+          if (!ctl.go.ready(j, wait)) return;
+          mma_features_ts<BLOCKS, kHalf>(tm_dp, tm_v, umma_desc(grad(j), kChunkBytes, 1024), steps);
+          umma_commit(&ctl.dp_full);
+        };
+        scores(0);
+        dps(0);
+        int group = 0;
+        for (int j = 0; j < n && wait.ok; ++j) {
+          const bool first = j == 0 || !((t0 + j) & 1), last = j == n - 1 || ((t0 + j) & 1);   // of its tile
+          wait(&ctl.p_full, j);
+          if (first) wait(&ctl.dv_empty, group ^ 1);
+          if (!wait.ok) break;
+          mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(grad(j), 2 * kChunkBytes, 1024), !first, steps);
+          ctl.go.release(j);
+          if (last) umma_commit(&ctl.dv_full);
+          if (j + 1 < n) scores(j + 1);
+          wait(&ctl.ds_full, j);
+          if (first) wait(&ctl.dk_empty, group++ ^ 1);
+          if (!wait.ok) break;
+          mma_rows<BLOCKS, 16>(tm_dk, tm_dp, umma_desc(query(j), 2 * kChunkBytes, 1024), !first, steps);
+          ctl.q.release(j);
+          if (last) umma_commit(&ctl.dk_full);
+          if (j + 1 < n) dps(j + 1);
+        }
       }
     }
-  }
   } else if (splits_head) {
     registers_up();
     const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, key = j0 + row;
@@ -1108,15 +1110,20 @@ cudaError_t prepare(const AttnArgs& a, const Layout& L, uint8_t* w, bool backwar
   const bool vec = a.dim % 4 == 0 && aligned(a.q, a.qs) && aligned(a.k, a.ks) && aligned(a.v, a.vs) &&
                    (!backward || aligned(a.dout, a.os));
   const int tq = (int)L.row_tiles, tk = (int)L.key_tiles;
-  return launch_pdl(L.blocks == 1 ? k_attn_split<1> : k_attn_split<2>, dim3((unsigned)split), dim3(512), 0, st, a, t, tq,
-                    tk, vec);
+  return launch_pdl(L.blocks == 1 ? k_attn_split<1> : k_attn_split<2>, dim3((unsigned)split), dim3(512), 0, st, a, t,
+                    tq, tk, vec);
+}
+
+template <typename K>
+cudaError_t prepared(K kernel, size_t smem) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  return e == cudaSuccess ? launched_with(kernel, kThreads, kRegs) : e;
 }
 
 template <int BLOCKS, bool FULL>
 cudaError_t forward(const AttnArgs& a, const Layout& L, const Tiles& t, float* part, cudaStream_t st) {
   using S = Forward<BLOCKS>;
-  static const cudaError_t set = cudaFuncSetAttribute(k_attn_forward<BLOCKS, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                      (int)S::kSmem);
+  static const cudaError_t set = prepared(k_attn_forward<BLOCKS, FULL>, S::kSmem);
   if (set != cudaSuccess) return set;
   const int64_t blocks = L.heads * L.row_tiles * L.splits;
   if (blocks > INT_MAX) return cudaErrorInvalidConfiguration;
@@ -1127,14 +1134,13 @@ cudaError_t forward(const AttnArgs& a, const Layout& L, const Tiles& t, float* p
 template <int BLOCKS, bool FULL>
 cudaError_t backward(const AttnArgs& a, const Layout& L, const Tiles& t, cudaStream_t st) {
   constexpr size_t kSmem = std::max(Dq<BLOCKS>::kSmem, Dkv<BLOCKS>::kSmem);
-  static const cudaError_t set = cudaFuncSetAttribute(k_attn_backward<BLOCKS, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                      (int)kSmem);
+  static const cudaError_t set = prepared(k_attn_backward<BLOCKS, FULL>, kSmem);
   if (set != cudaSuccess) return set;
   const int64_t nq = L.heads * L.row_tiles, nk = L.heads * L.key_tiles;
   if (nq + nk > INT_MAX) return cudaErrorInvalidConfiguration;
   const bool vec = a.dim % 4 == 0;
-  return launch_pdl(k_attn_backward<BLOCKS, FULL>, dim3((unsigned)(nq + nk)), dim3(kThreads), kSmem, st, a, t, (int)L.row_tiles,
-                    (int)nk, vec && aligned(a.dq, a.dqs), vec && aligned(a.dk, a.dks) && aligned(a.dv, a.dvs),
+  return launch_pdl(k_attn_backward<BLOCKS, FULL>, dim3((unsigned)(nq + nk)), dim3(kThreads), kSmem, st, a, t,
+                    (int)L.row_tiles, (int)nk, vec && aligned(a.dq, a.dqs), vec && aligned(a.dk, a.dks) && aligned(a.dv, a.dvs),
                     device_error_word());
 }
 

@@ -51,7 +51,9 @@ struct Product {
 };
 
 constexpr int kRows = 128, kEpi = 8;            // tile rows of a block, epilogue warps
-constexpr int kThreads = 32 * (kEpi + 4);     // and a warp that loads, one that issues, two that give up their registers
+constexpr int kThreads = 32 * (kEpi + 4);     // and warps that load, issue, and give up registers (two)
+// 384 threads start with 168 registers, 64512 in all, and as many are taken
+constexpr int kUpRegs = 232, kDownRegs = 40, kRegs = 32 * (kEpi * kUpRegs + 4 * kDownRegs);
 
 constexpr uint32_t kStaging = 4096;              // of an epilogue warp: its 32 rows of a chunk
 
@@ -193,101 +195,101 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
     return o.half ? tile < k / (S::kTileRows / 64) : o.mn;
   };
 
-  // 384 threads start with 168 registers, 64512 in all; 256 * 232 + 128 * 40 is as many
   if (warp >= kEpi) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-  if (warp == kEpi) {
-    if (elect_one()) {
-      uint32_t it = 0;
-      bool ok = true;
-      while (ok && run.next(sg)) {
-        uint32_t z, ti, tj;
-        tile_at(g, sg.tile, z, ti, tj);
-        const uint32_t m0 = ti * (S::kTileRows / 64) + rank * 2, n0 = tj * (BN / 64) + rank * S::kBChunks;
-        const uint32_t mc = m0 < mchunks ? min(2u, mchunks - m0) : 0;
-        const uint32_t nc = n0 < nchunks ? min(S::kBChunks, nchunks - n0) : 0;
-        for (uint32_t k = sg.k0; k < sg.k1; ++k, ++it) {
-          const uint32_t s = it % S::kStages;
-          ok = mbar_wait(&empty[s], ((it / S::kStages) & 1) ^ 1, err);
-          if (!ok) break;
-          mbar_arrive_expect_tx(&full[s], (mc + nc) * kPairBytes);
-          const bool a_mn = transposed(g.A, ti, k), b_mn = transposed(g.B, tj, k);
-          uint8_t* a = sm + s * S::kStage;
-          for (uint32_t p = 0; p < mc; ++p) {
-            const uint8_t* c = a_mn ? chunk_of(g.A, z, k, m0 + p) : chunk_of(g.A, z, m0 + p, k);
-            bulk_load(a + p * kChunkBytes, c, kChunkBytes, &full[s]);
-            bulk_load(a + (2 + p) * kChunkBytes, c + kChunkBytes, kChunkBytes, &full[s]);
-          }
-          uint8_t* b = a + S::kA;
-          for (uint32_t p = 0; p < nc; ++p) {
-            const uint8_t* c = b_mn ? chunk_of(g.B, z, k, n0 + p) : chunk_of(g.B, z, n0 + p, k);
-            bulk_load(b + p * kChunkBytes, c, kChunkBytes, &full[s]);
-            bulk_load(b + (S::kBChunks + p) * kChunkBytes, c + kChunkBytes, kChunkBytes, &full[s]);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDownRegs));
+    if (warp == kEpi) {
+      if (elect_one()) {
+        uint32_t it = 0;
+        bool ok = true;
+        while (ok && run.next(sg)) {
+          uint32_t z, ti, tj;
+          tile_at(g, sg.tile, z, ti, tj);
+          const uint32_t m0 = ti * (S::kTileRows / 64) + rank * 2, n0 = tj * (BN / 64) + rank * S::kBChunks;
+          const uint32_t mc = m0 < mchunks ? min(2u, mchunks - m0) : 0;
+          const uint32_t nc = n0 < nchunks ? min(S::kBChunks, nchunks - n0) : 0;
+          for (uint32_t k = sg.k0; k < sg.k1; ++k, ++it) {
+            const uint32_t s = it % S::kStages;
+            ok = mbar_wait(&empty[s], ((it / S::kStages) & 1) ^ 1, err);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&full[s], (mc + nc) * kPairBytes);
+            const bool a_mn = transposed(g.A, ti, k), b_mn = transposed(g.B, tj, k);
+            uint8_t* a = sm + s * S::kStage;
+            for (uint32_t p = 0; p < mc; ++p) {
+              const uint8_t* c = a_mn ? chunk_of(g.A, z, k, m0 + p) : chunk_of(g.A, z, m0 + p, k);
+              bulk_load(a + p * kChunkBytes, c, kChunkBytes, &full[s]);
+              bulk_load(a + (2 + p) * kChunkBytes, c + kChunkBytes, kChunkBytes, &full[s]);
+            }
+            uint8_t* b = a + S::kA;
+            for (uint32_t p = 0; p < nc; ++p) {
+              const uint8_t* c = b_mn ? chunk_of(g.B, z, k, n0 + p) : chunk_of(g.B, z, n0 + p, k);
+              bulk_load(b + p * kChunkBytes, c, kChunkBytes, &full[s]);
+              bulk_load(b + (S::kBChunks + p) * kChunkBytes, c + kChunkBytes, kChunkBytes, &full[s]);
+            }
           }
         }
+        // every copy has landed before the block may end
+        for (uint32_t u = it > (uint32_t)S::kStages ? it - S::kStages : 0; u < it; ++u)
+          mbar_wait(&full[u % S::kStages], (u / S::kStages) & 1, err);
       }
-      // every copy has landed before the block may end
-      for (uint32_t u = it > (uint32_t)S::kStages ? it - S::kStages : 0; u < it; ++u)
-        mbar_wait(&full[u % S::kStages], (u / S::kStages) & 1, err);
-    }
-  } else if (warp == kEpi + 1 && rank != 0) {
-    if (elect_one()) {                              // tells the even block of each chunk that has come in
-      uint32_t it = 0;
-      bool ok = true;
-      while (ok && run.next(sg))
-        for (uint32_t k = sg.k0; k < sg.k1 && ok; ++k, ++it) {
-          const uint32_t s = it % S::kStages;
-          ok = mbar_wait(&full[s], (it / S::kStages) & 1, err);
-          if (ok) mbar_arrive_at(&there[s], 0);
-        }
-    }
-  } else if (warp == kEpi + 1) {
-    if (elect_one()) {
-      auto mma = [](uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-        if constexpr (PAIR) umma_pair(d, a, b, idesc, add);
-        else umma(d, a, b, idesc, add);
-      };
-      auto commit = [](uint64_t* bar) {
-        if constexpr (PAIR) umma_commit_pair(bar);
-        else umma_commit(bar);
-      };
-      uint32_t it = 0, part = 0;
-      bool ok = true;
-      while (ok && run.next(sg)) {
-        uint32_t z, ti, tj;
-        tile_at(g, sg.tile, z, ti, tj);
-        for (uint32_t k0 = sg.k0; k0 < sg.k1 && ok; k0 += kDrain, ++part) {
-          const uint32_t buf = part % S::kBufs, d = tmem + buf * BN, k1 = min(sg.k1, k0 + kDrain);
-          ok = mbar_wait_cluster(&freed[buf], ((part / S::kBufs) & 1) ^ 1, err);
-          tc_fence_after();
-          for (uint32_t k = k0; k < k1 && ok; ++k, ++it) {
+    } else if (warp == kEpi + 1 && rank != 0) {
+      if (elect_one()) {                              // tells the even block of each chunk that has come in
+        uint32_t it = 0;
+        bool ok = true;
+        while (ok && run.next(sg))
+          for (uint32_t k = sg.k0; k < sg.k1 && ok; ++k, ++it) {
             const uint32_t s = it % S::kStages;
             ok = mbar_wait(&full[s], (it / S::kStages) & 1, err);
-            if (PAIR && ok) ok = mbar_wait_cluster(&there[s], (it / S::kStages) & 1, err);
-            if (!ok) break;
-            tc_fence_after();
-            const bool a_mn = transposed(g.A, ti, k), b_mn = transposed(g.B, tj, k);
-            const uint32_t idesc = umma_idesc(S::kTileRows, BN, a_mn, b_mn);
-            const uint32_t step_a = (a_mn ? 2048 : 32) / 16, step_b = (b_mn ? 2048 : 32) / 16;   // 16 rows, or 16 columns
-            const uint32_t a = smem_addr(sm + s * S::kStage), b = a + S::kA;
-            const uint64_t ah = umma_desc(a, kChunkBytes, 1024), bh = umma_desc(b, kChunkBytes, 1024);
-            const uint64_t al = ah + 2 * kChunkBytes / 16, bl = bh + S::kBChunks * kChunkBytes / 16;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              mma(d, al + q * step_a, bh + q * step_b, idesc, k != k0 || q != 0);
-              mma(d, ah + q * step_a, bl + q * step_b, idesc, true);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) mma(d, ah + q * step_a, bh + q * step_b, idesc, true);
-            commit(&empty[s]);
+            if (ok) mbar_arrive_at(&there[s], 0);
           }
-          commit(&done[buf]);
+      }
+    } else if (warp == kEpi + 1) {
+      if (elect_one()) {
+        auto mma = [](uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+          if constexpr (PAIR) umma_pair(d, a, b, idesc, add);
+          else umma(d, a, b, idesc, add);
+        };
+        auto commit = [](uint64_t* bar) {
+          if constexpr (PAIR) umma_commit_pair(bar);
+          else umma_commit(bar);
+        };
+        uint32_t it = 0, part = 0;
+        bool ok = true;
+        while (ok && run.next(sg)) {
+          uint32_t z, ti, tj;
+          tile_at(g, sg.tile, z, ti, tj);
+          for (uint32_t k0 = sg.k0; k0 < sg.k1 && ok; k0 += kDrain, ++part) {
+            const uint32_t buf = part % S::kBufs, d = tmem + buf * BN, k1 = min(sg.k1, k0 + kDrain);
+            ok = mbar_wait_cluster(&freed[buf], ((part / S::kBufs) & 1) ^ 1, err);
+            tc_fence_after();
+            for (uint32_t k = k0; k < k1 && ok; ++k, ++it) {
+              const uint32_t s = it % S::kStages;
+              ok = mbar_wait(&full[s], (it / S::kStages) & 1, err);
+              if (PAIR && ok) ok = mbar_wait_cluster(&there[s], (it / S::kStages) & 1, err);
+              if (!ok) break;
+              tc_fence_after();
+              const bool a_mn = transposed(g.A, ti, k), b_mn = transposed(g.B, tj, k);
+              const uint32_t idesc = umma_idesc(S::kTileRows, BN, a_mn, b_mn);
+              // 16 rows, or 16 columns
+              const uint32_t step_a = (a_mn ? 2048 : 32) / 16, step_b = (b_mn ? 2048 : 32) / 16;
+              const uint32_t a = smem_addr(sm + s * S::kStage), b = a + S::kA;
+              const uint64_t ah = umma_desc(a, kChunkBytes, 1024), bh = umma_desc(b, kChunkBytes, 1024);
+              const uint64_t al = ah + 2 * kChunkBytes / 16, bl = bh + S::kBChunks * kChunkBytes / 16;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                mma(d, al + q * step_a, bh + q * step_b, idesc, k != k0 || q != 0);
+                mma(d, ah + q * step_a, bl + q * step_b, idesc, true);
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q) mma(d, ah + q * step_a, bh + q * step_b, idesc, true);
+              commit(&empty[s]);
+            }
+            commit(&done[buf]);
+          }
         }
       }
     }
-  }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kUpRegs));
     constexpr int W = BN / 2;                     // columns of a thread's row
     const uint32_t side = warp >> 2;
     uint8_t* stage = sm + S::kStages * S::kStage + warp * kStaging;
@@ -308,7 +310,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
           prefetch(d + kChunkBytes);
         }
       if (g.update && i0 + lane < g.M)
-        for (uint32_t c = 0; c < W && j0 + c < g.N; c += 32) prefetch(g.out + ((uint64_t)z * g.M + i0 + lane) * g.N + j0 + c);
+        for (uint32_t c = 0; c < W && j0 + c < g.N; c += 32)
+          prefetch(g.out + ((uint64_t)z * g.M + i0 + lane) * g.N + j0 + c);
       float acc[W];
 #pragma unroll
       for (int c = 0; c < W; ++c) acc[c] = 0.f;
@@ -824,8 +827,8 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const __grid_const
       constexpr uint32_t id = umma_idesc(128, 64, false, true);
       for (int k = 0; k < C; ++k) {
         for (int h = 0; h < (deep1 ? 2 : 1); ++h)
-          three(tmem + (apart ? 2 * k + h : k) * 64, p + h * kBlock, x + k * kBlock + h * (kChunkBytes / 16), 2, 128, kLow, id,
-                !apart && h, h ? deep1 : deep0);
+          three(tmem + (apart ? 2 * k + h : k) * 64, p + h * kBlock, x + k * kBlock + h * (kChunkBytes / 16), 2, 128,
+                kLow, id, !apart && h, h ? deep1 : deep0);
         umma_commit(&ready[k]);
       }
     }
@@ -928,6 +931,7 @@ struct Layout {
 template <typename K>
 cudaError_t workers_of(K kernel, bool pair, size_t smem, int* workers) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) e = launched_with(kernel, kThreads, kRegs);
   *workers = dev_info().sm_count;
   if (e != cudaSuccess || !pair) return e;
   cudaLaunchConfig_t cfg = {};
