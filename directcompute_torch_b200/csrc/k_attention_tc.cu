@@ -1146,8 +1146,15 @@ cudaError_t backward(const AttnArgs& a, const Layout& L, const Tiles& t, cudaStr
 
 }  // namespace
 
+// The tensor cores' way has more launches and a pass over the operands before it; the CUDA
+// cores' time goes with the work (here all pairs times features), and for few rows with the
+// bytes of the keys.  Microseconds, CUDA cores against tensor cores, forward: 8.4 million 20
+// and 28, 50 million 40 and 29, 67 million 33 to 37 and 32 to 35, 262 million 116 and 66; 8
+// rows a key head over 1000 keys 26 and 42, 16 rows over 2000 72 and 61.  Forward and
+// backward: 11.5 million 42 and 50, 34 million 62 to 114 and 47 to 62, 67 million 96 and 52.
 bool attn_tensor_fits(const AttnArgs& a, bool backward) {
-  return a.batch && a.kv_len && (int64_t)a.q_len * a.group >= 32;
+  const double work = (double)a.batch * a.q_heads * a.q_len * a.kv_len * a.dim;
+  return backward ? work >= 12e6 : work >= 30e6 && (int64_t)a.q_len * a.group >= 16;
 }
 
 size_t attn_tensor_ws_bytes(const AttnArgs& a, bool backward) { return Layout(a, backward).total; }

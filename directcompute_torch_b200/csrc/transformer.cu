@@ -113,7 +113,8 @@ void copy3(int64_t* to, const int64_t* from) {
   for (int i = 0; i < 3; ++i) to[i] = from[i];
 }
 
-constexpr uint64_t kMost = 1ull << 30;       // positions, and positions times heads, of one call
+constexpr uint64_t kMost = 1ull << 30;       // tokens or features of one call
+constexpr uint64_t kMostRows = 1ull << 28;   // positions times heads: sums of a few of them are 32-bit
 
 // ---------------------------------------------------------------------------
 // attention
@@ -126,8 +127,8 @@ int attention(const char* what, const DctAttention* p, void* q, void* k, void* v
     return refuse(DCT_ERR_ARG, "%s: head_dim is %u (1 to 128)", what, p->head_dim);
   if (!p->q_heads || !p->kv_heads || p->q_heads % p->kv_heads)
     return refuse(DCT_ERR_ARG, "%s: %u query heads over %u key heads", what, p->q_heads, p->kv_heads);
-  if ((unsigned __int128)p->q_len * p->q_heads * std::max(1u, p->batch) >= kMost ||
-      (unsigned __int128)p->kv_len * p->kv_heads * std::max(1u, p->batch) >= kMost)
+  if ((unsigned __int128)p->q_len * p->q_heads * std::max(1u, p->batch) >= kMostRows ||
+      (unsigned __int128)p->kv_len * p->kv_heads * std::max(1u, p->batch) >= kMostRows)
     return refuse(DCT_ERR_ARG, "%s: too many rows in one call", what);
   if (!isfinite(p->scale)) return refuse(DCT_ERR_ARG, "%s: scale is not finite", what);
   const uint64_t B = p->batch, D = p->head_dim;
@@ -168,7 +169,7 @@ int attention(const char* what, const DctAttention* p, void* q, void* k, void* v
   a.batch = p->batch; a.q_heads = p->q_heads; a.kv_heads = p->kv_heads; a.group = p->q_heads / p->kv_heads;
   a.q_len = p->q_len; a.kv_len = p->kv_len; a.dim = p->head_dim;
   a.causal = p->causal != 0;
-  a.window = (int)std::min<uint32_t>(p->window, (uint32_t)kMost);
+  a.window = p->window >= p->q_len + p->kv_len ? 0 : (int)p->window;      // as wide as that hides nothing
   a.scale = p->scale != 0.f ? p->scale : (float)(1.0 / sqrt((double)p->head_dim));
   OnDevice guard;
   cudaStream_t st = rt_stream();

@@ -212,17 +212,20 @@ def test_attention(dev, shape, mask):
     _hold(_attention(dev, q, k, v, go, **mask), T.attention(q, k, v, go, **mask), ALL)
 
 
+@pytest.mark.parametrize("size", [(90, 150, 64), (260, 270, 128), (200, 330, 64)])
 @pytest.mark.parametrize("mask", MASKS, ids=str)
-def test_attention_ragged(dev, mask):
+def test_attention_ragged(dev, mask, size):
     """Lengths of 0, 1, whole ones and ones past the end (clamped), queries fewer and more than keys."""
-    q, k, v, go = _inputs(7, 90, 150, 4, 2, 64)
-    lens = {"q_lens": [90, 0, 1, 37, 64, 99, 90], "kv_lens": [150, 150, 1, 20, 65, 1000, 0]}
+    t, n, d = size
+    q, k, v, go = _inputs(7, t, n, 4, 2, d)
+    lens = {"q_lens": [t, 0, 1, 37, 64, t + 9, t], "kv_lens": [n, n, 1, 20, 65, 1000, 0]}
     want = T.attention(q, k, v, go, **mask, **lens)
     _hold(_attention(dev, q, k, v, go, **mask, **lens), want, ALL)
 
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, 3e38])
-@pytest.mark.parametrize("shape", [(2, 70, 140, 4, 2, 64), (2, 1, 300, 4, 2, 128), (2, 5, 300, 2, 2, 32)], ids=str)
+@pytest.mark.parametrize("shape", [(2, 70, 140, 4, 2, 64), (2, 1, 300, 4, 2, 128), (2, 5, 300, 2, 2, 32),
+                                   (2, 210, 400, 4, 2, 64), (2, 300, 300, 4, 1, 100)], ids=str)
 def test_attention_masked_places_do_not_reach_results(dev, bad, shape):
     q, k, v, go = _inputs(*shape)
     t, n = shape[1], shape[2]
@@ -234,9 +237,10 @@ def test_attention_masked_places_do_not_reach_results(dev, bad, shape):
 
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
-def test_attention_later_keys_do_not_reach_earlier_queries(dev, bad):
+@pytest.mark.parametrize("t", [200, 520])
+def test_attention_later_keys_do_not_reach_earlier_queries(dev, bad, t):
     """A value that a causal mask hides from a query does not reach it, inside a tile too."""
-    q, k, v, go = _inputs(1, 200, 200, 2, 2, 64)
+    q, k, v, go = _inputs(1, t, t, 2, 2, 64)
     want = T.attention(q, k, v, go, causal=True)
     v[0, 150, 1], k[0, 170, 1] = bad, bad
     got = _attention(dev, q, k, v, causal=True)
@@ -245,10 +249,11 @@ def test_attention_later_keys_do_not_reach_earlier_queries(dev, bad):
     assert not np.isfinite(got["out"][0, 150:, 1]).any() if np.isnan(bad) else not np.isfinite(got["out"][0, 150, 1]).any()
 
 
-@pytest.mark.parametrize("spread", [0, 8, 30])
-def test_attention_far_apart_magnitudes(dev, spread):
+@pytest.mark.parametrize("spread", [0, 8, 13, 30])
+@pytest.mark.parametrize("t", [150, 520])
+def test_attention_far_apart_magnitudes(dev, spread, t):
     """Rows whose sizes lie 2^spread apart, and inputs far from 1."""
-    q, k, v, go = _inputs(1, 150, 150, 2, 1, 64)
+    q, k, v, go = _inputs(1, t, t, 2, 1, 64)
     r = np.random.default_rng(5)
     for x in (v, go):
         x *= np.exp2(-r.integers(0, spread + 1, x.shape[:3] + (1,))).astype(np.float32)
@@ -259,10 +264,11 @@ def test_attention_far_apart_magnitudes(dev, spread):
 
 
 @pytest.mark.parametrize("offset", [0, 1, 4])
-def test_attention_strides(dev, offset):
+@pytest.mark.parametrize("t,d", [(100, 64), (300, 64), (260, 128), (280, 50)])
+def test_attention_strides(dev, offset, t, d):
     """Packed projections and heads before positions, at aligned and unaligned starts; nothing is
     written between an output's rows."""
-    b, t, h, hk, d = 2, 100, 4, 2, 64
+    b, h, hk = 2, 4, 2
     q, k, v, go = _inputs(b, t, t, h, hk, d)
     w = (h + 2 * hk) * d + 4
     st = {"q": (t * w, w, d), "k": (t * w, w, d), "v": (hk * t * d, d, t * d), "o": (h * t * d, d, t * d),
@@ -280,16 +286,65 @@ def test_attention_one_new_token(dev, group, n, d):
     _hold(_attention(dev, q, k, v, **kw), T.attention(q, k, v, **kw), ("out", "lse"))
 
 
-def test_attention_is_the_same_from_run_to_run(dev):
-    q, k, v, go = _inputs(2, 190, 190, 4, 2, 64)
+@pytest.mark.parametrize("shape,mask", [
+    ((2, 192, 192, 8, 2, 64), {"causal": True, "window": 50}), ((3, 16, 1500, 16, 4, 128), {"causal": True}),
+    ((1, 700, 900, 6, 6, 72), {"window": 300}), ((2, 5, 3000, 16, 2, 128), {"causal": True}),
+    ((4, 260, 260, 8, 1, 33), {"causal": True}), ((1, 1, 5000, 8, 1, 128), {}), ((2, 300, 2000, 4, 4, 128), {"window": 1}),
+    ((1, 1000, 130, 4, 2, 64), {"causal": True}), ((2, 385, 385, 4, 4, 112), {})], ids=str)
+def test_attention_larger(dev, shape, mask):
+    """Sizes that take the tensor cores, forward with the keys split where rows are few."""
+    q, k, v, go = _inputs(*shape)
+    _hold(_attention(dev, q, k, v, go, **mask), T.attention(q, k, v, go, **mask), ALL)
+
+
+@pytest.mark.parametrize("bad", ["nan", "inf", "rows", "values", "scores"])
+@pytest.mark.parametrize("t", [40, 300])
+def test_attention_heads_apart(dev, bad, t):
+    """One key head that float16 pairs cannot hold leaves the other heads as they were, and is right itself."""
+    q, k, v, go = _inputs(2, t, 1500, 4, 2, 64)
+    fine = _attention(dev, q, k, v, go, causal=True)
+    if bad in ("nan", "inf"):
+        v[1, 700, 1, 3] = np.nan if bad == "nan" else np.inf
+    elif bad == "rows":
+        k[1, 130, 1] *= np.float32(2.0 ** -30)
+    elif bad == "values":
+        v[1, 128:, 1] *= np.float32(2.0 ** -80)
+    else:
+        q[1, :, 2:] *= 3e4
+    got = _attention(dev, q, k, v, go, causal=True)
+    for x in ALL[2:] + ("out",):
+        heads = 2 if x in ("out", "dq") else 1
+        assert np.array_equal(got[x][0], fine[x][0]) and np.array_equal(got[x][1][:, :heads], fine[x][1][:, :heads])
+    if bad in ("rows", "values"):
+        _hold(got, T.attention(q, k, v, go, causal=True), ALL)
+    elif bad == "scores":
+        _hold(got, T.attention(q, k, v, go, causal=True), ("out", "lse"))
+    else:
+        first = max(0, 700 - (1500 - t))                     # queries that see key 700
+        assert not np.isfinite(got["out"][1, first:, 2:, 3]).any()
+
+
+def test_attention_over_a_cache_with_room(dev):
+    """Keys in a cache longer than its valid part, heads before positions."""
+    b, t, n, h, hk, d, room = 3, 20, 900, 8, 2, 64, 1024
+    q, k, v, go = _inputs(b, t, n, h, hk, d)
+    st = {x: (hk * room * d, d, room * d) for x in ("k", "v", "dk", "dv")}
+    kw = {"causal": True, "kv_lens": [900, 1, 555]}
+    _hold(_attention(dev, q, k, v, go, strides=st, **kw), T.attention(q, k, v, go, **kw), ALL)
+
+
+@pytest.mark.parametrize("t", [190, 350])
+def test_attention_is_the_same_from_run_to_run(dev, t):
+    q, k, v, go = _inputs(2, t, t, 4, 2, 64)
     one, two = (_attention(dev, q, k, v, go, causal=True) for _ in range(2))
     assert all(np.array_equal(one[x], two[x]) for x in ALL)
     none = _attention(dev, q, k, v, causal=True, lse=False)
     assert np.array_equal(none["out"], one["out"]) and np.isnan(none["lse"]).all()
 
 
-def test_attention_scale_of_either_sign(dev):
-    q, k, v, go = _inputs(1, 70, 70, 2, 2, 64)
+@pytest.mark.parametrize("t", [70, 520])
+def test_attention_scale_of_either_sign(dev, t):
+    q, k, v, go = _inputs(1, t, t, 2, 2, 64)
     for scale in (0.5, -0.1, 1e-20):
         _hold(_attention(dev, q, k, v, go, scale=scale), T.attention(q, k, v, go, scale=scale), ALL)
 
@@ -363,7 +418,9 @@ def _muon(shape, **kw):
 
 
 MATRICES = [(1, 1, 1), (1, 1, 9), (2, 9, 1), (1, 17, 33), (3, 64, 64), (1, 127, 333), (1, 333, 127), (2, 128, 256),
-            (1, 260, 130), (5, 96, 200), (1, 513, 700), (1, 700, 513), (2, 256, 1025)]
+            (1, 260, 130), (5, 96, 200), (1, 513, 700), (1, 700, 513), (2, 256, 1025), (1, 128, 2560), (2, 2561, 128),
+            (1, 129, 640), (3, 64, 321), (1, 5, 3000), (1, 2100, 1), (40, 100, 70), (1, 1030, 1300), (3, 600, 600),
+            (1, 2048, 2050)]
 
 
 @pytest.mark.parametrize("shape", MATRICES, ids=str)
