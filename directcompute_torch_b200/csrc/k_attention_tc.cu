@@ -431,16 +431,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
   tc_fence_after();
   // S twice, P V, the operand Q
   const uint32_t tm_s = ctl.tmem, tm_o = tm_s + 256, tm_q = tm_s + 384;
-  pdl_entry();
-  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads;
-  const int split = blockIdx.x / heads % splits, tile = row_tiles - 1 - blockIdx.x / heads / splits;  // long rows first
+  const int heads = a.batch * a.kv_heads, bh = blockIdx.x % heads, rest = blockIdx.x / heads;
+  const int split = rest % splits, tile = row_tiles - 1 - rest / splits;                     // long rows first
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const bool splits_head = head_splits(w.stats[bh], a.scale, a.dim);
-  if (!splits_head && threadIdx.x == 0) *w.any = 1;          // work for the float32 kernels
-  const AttnSpan span(a, b);
   const int rows = a.q_len * a.group, r0 = tile * kTile;
-  // keys of the tile's rows
-  const int i0 = r0 / a.group, i1 = min(min(r0 + kTile, rows) - 1, span.m * a.group - 1) / a.group;
+  const int i0 = r0 / a.group, i_end = (min(r0 + kTile, rows) - 1) / a.group;    // positions of the tile's rows
+  pdl_entry();
+  const AttnStats stats = w.stats[bh];
+  const AttnSpan span(a, b);
+  const bool splits_head = head_splits(stats, a.scale, a.dim);
+  if (!splits_head && threadIdx.x == 0) *w.any = 1;          // work for the float32 kernels
+  const int i1 = min(i_end, span.m - 1);
   int t0 = 0, n = 0;
   if (splits_head && i0 < span.m) {
     const int k0 = span.lo(a, i0), k1 = span.hi(a, i1);
@@ -678,14 +679,16 @@ DCT_DEV void attn_dq(const AttnArgs& a, const Tiles& w, int block, int row_tiles
   tc_fence_after();
   // S and dP twice, the operand dout, the accumulator
   const uint32_t tm_s = ctl.tmem, tm_dp = tm_s + 128, tm_go = tm_s + 256, tm_acc = tm_s + 384;
-  pdl_entry();
   const int heads = a.batch * a.kv_heads, bh = block % heads, tile = row_tiles - 1 - block / heads;
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const bool splits_head = head_splits(w.stats[bh], a.scale, a.dim);
-  if (!splits_head && threadIdx.x == 0) *w.any = 1;          // work for the float32 kernels
-  const AttnSpan span(a, b);
   const int rows = a.q_len * a.group, r0 = tile * kTile;
-  const int i0 = r0 / a.group, i1 = min(min(r0 + kTile, rows) - 1, span.m * a.group - 1) / a.group;
+  const int i0 = r0 / a.group, i_end = (min(r0 + kTile, rows) - 1) / a.group;
+  pdl_entry();
+  const AttnStats stats = w.stats[bh];
+  const AttnSpan span(a, b);
+  const bool splits_head = head_splits(stats, a.scale, a.dim);
+  if (!splits_head && threadIdx.x == 0) *w.any = 1;          // work for the float32 kernels
+  const int i1 = min(i_end, span.m - 1);
   int t0 = 0, n = 0;
   if (splits_head && i0 < span.m) {
     const int k0 = span.lo(a, i0), k1 = span.hi(a, i1);
@@ -861,12 +864,13 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
   tc_fence_after();
   // the accumulators, the operand V, S and dP (each also P's and dS's place)
   const uint32_t tm_dk = ctl.tmem, tm_dv = tm_dk + 128, tm_v = tm_dk + 256, tm_s = tm_dk + 384, tm_dp = tm_dk + 448;
-  pdl_entry();
   const int heads = a.batch * a.kv_heads, bh = block % heads, tile = block / heads;    // long ones first
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const bool splits_head = head_splits(w.stats[bh], a.scale, a.dim);
-  if (!splits_head && threadIdx.x == 0) *w.any = 1;          // work for the float32 kernels
+  pdl_entry();
+  const AttnStats stats = w.stats[bh];
   const AttnSpan span(a, b);
+  const bool splits_head = head_splits(stats, a.scale, a.dim);
+  if (!splits_head && threadIdx.x == 0) *w.any = 1;          // work for the float32 kernels
   const int j0 = tile * kTile, j1 = min(j0 + kTile, span.n) - 1;
   int t0 = 0, n = 0;
   if (splits_head && j0 < span.n) {

@@ -185,10 +185,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
-  pdl_entry();
   const uint32_t mchunks = (g.M + 63) / 64, nchunks = (g.N + 63) / 64;
+  // the first segment before the wait for the kernel before: its divisions take 2 us
   Run run(total, g.kb, unit, used, worker, PAIR ? gridDim.x / 2 : gridDim.x);
   Segment sg;
+  uint32_t z, ti, tj;
+  auto next = [&]() {
+    if (!run.next(sg)) return false;
+    tile_at(g, sg.tile, z, ti, tj);
+    return true;
+  };
+  bool more = next();
+  pdl_entry();
   // whether chunk k of an operand's tile is read with its rows as the contraction: its own
   // layout, or the mirror image of a chunk above the diagonal
   auto transposed = [](const Operand& o, uint32_t tile, uint32_t k) {
@@ -201,9 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
       if (elect_one()) {
         uint32_t it = 0;
         bool ok = true;
-        while (ok && run.next(sg)) {
-          uint32_t z, ti, tj;
-          tile_at(g, sg.tile, z, ti, tj);
+          for (; ok && more; more = next()) {
           const uint32_t m0 = ti * (S::kTileRows / 64) + rank * 2, n0 = tj * (BN / 64) + rank * S::kBChunks;
           const uint32_t mc = m0 < mchunks ? min(2u, mchunks - m0) : 0;
           const uint32_t nc = n0 < nchunks ? min(S::kBChunks, nchunks - n0) : 0;
@@ -235,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
       if (elect_one()) {                              // tells the even block of each chunk that has come in
         uint32_t it = 0;
         bool ok = true;
-        while (ok && run.next(sg))
+        for (; ok && more; more = next())
           for (uint32_t k = sg.k0; k < sg.k1 && ok; ++k, ++it) {
             const uint32_t s = it % S::kStages;
             ok = mbar_wait(&full[s], (it / S::kStages) & 1, err);
@@ -254,9 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
         };
         uint32_t it = 0, part = 0;
         bool ok = true;
-        while (ok && run.next(sg)) {
-          uint32_t z, ti, tj;
-          tile_at(g, sg.tile, z, ti, tj);
+        for (; ok && more; more = next()) {
           for (uint32_t k0 = sg.k0; k0 < sg.k1 && ok; k0 += kDrain, ++part) {
             const uint32_t buf = part % S::kBufs, d = tmem + buf * BN, k1 = min(sg.k1, k0 + kDrain);
             ok = mbar_wait_cluster(&freed[buf], ((part / S::kBufs) & 1) ^ 1, err);
@@ -297,9 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
     // once a wait has run out the loop goes on without waiting: the other warps still count
     // on meeting this one
     bool ok = true;
-    while (run.next(sg)) {
-      uint32_t z, ti, tj;
-      tile_at(g, sg.tile, z, ti, tj);
+    for (; more; more = next()) {
       // the warp's 32 rows from i0, the thread's columns from j0
       const uint32_t i0 = ti * S::kTileRows + rank * kRows + (warp & 3) * 32, j0 = tj * BN + side * W;
       // what the end of the tile reads, into L2 by then
@@ -961,10 +963,10 @@ cudaError_t product_as(Product g, uint32_t batch, cudaStream_t st) {
   if (g.half) g.tiles = g.mt * (g.mt + 1) / 2;
   const uint64_t total = (uint64_t)g.tiles * batch, work = total * g.kb;
   if (total >= (1ull << 31)) return cudaErrorInvalidConfiguration;
-  // The tiles that do not go around: whole, or cut in runs of 4 chunks or more, whichever ends
-  // first.  A cut tile's meeting in memory costs about as much as 6 chunks (one matrix of
+  // The tiles that do not go around: whole, or cut in runs of 4 chunks or more (2 of the
+  // smallest tiles), whichever ends first.  A cut tile's meeting in memory costs about as much as 6 chunks (one matrix of
   // 1024 x 8192: 700 us cut, 1079 us whole; twelve of 768 x 768: 552 and 550 us).
-  constexpr uint64_t kShortest = 4, kMeeting = 6;
+  constexpr uint64_t kShortest = BN == 64 ? 2 : 4, kMeeting = 6;
   const uint64_t workers = std::min<uint64_t>(work / kShortest + 1, most), left = total % workers;
   const uint64_t cut = std::max<uint64_t>(kShortest, (left * g.kb + workers - 1) / workers) + kMeeting;
   const uint32_t unit = g.kb <= cut ? g.kb : 1;
@@ -995,10 +997,11 @@ cudaError_t product(int tile, const Product& g, uint32_t batch, cudaStream_t st)
 
 // Pairs with tiles of 256 where these fill a fifth of the SMs or more with one symmetric
 // product (twelve of 768 x 768: 479 us, 509 with tiles of 128; 4096 x 4096: 3.3 ms, 4.9);
-// below, smaller tiles divide better (1500 x 1500: 519 us, 419 with 128).
+// below, smaller tiles divide better (1500 x 1500: 519 us, 419 with 128; 256 x 1000: 259, 173
+// and 159 with 64; 512 x 2048: 327, 222 and 214).
 int tile_of(const MuonArgs& a) {
   const uint64_t s = std::min(a.rows, a.cols), n = (s + 255) / 256;
-  return s <= 64 ? 64 : n * (n + 1) / 2 * a.batch * 5 >= (uint64_t)dev_info().sm_count ? 256 : 128;
+  return n * (n + 1) / 2 * a.batch * 5 >= (uint64_t)dev_info().sm_count ? 256 : s <= 512 ? 64 : 128;
 }
 
 // the power of two that brings `most` to at most 2^15
