@@ -80,6 +80,8 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
                                                     int tq, int tk, bool vec) {
   constexpr int kGroups = 8 * BLOCKS, kStep = 512 / kGroups, kPasses = kTile / kStep;
   __shared__ uint32_t sh[3];
+  touch(a);
+  touch(w);
   pdl_entry();
   const int heads = a.batch * a.kv_heads;
   int x = blockIdx.x, t = 0;
@@ -436,6 +438,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
   const int rows = a.q_len * a.group, r0 = tile * kTile;
   const int i0 = r0 / a.group, i_end = (min(r0 + kTile, rows) - 1) / a.group;    // positions of the tile's rows
+  touch(a);
+  touch(w);
   pdl_entry();
   const AttnStats stats = w.stats[bh];
   const AttnSpan span(a, b);
@@ -683,6 +687,8 @@ DCT_DEV void attn_dq(const AttnArgs& a, const Tiles& w, int block, int row_tiles
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
   const int rows = a.q_len * a.group, r0 = tile * kTile;
   const int i0 = r0 / a.group, i_end = (min(r0 + kTile, rows) - 1) / a.group;
+  touch(a);
+  touch(w);
   pdl_entry();
   const AttnStats stats = w.stats[bh];
   const AttnSpan span(a, b);
@@ -866,6 +872,8 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
   const uint32_t tm_dk = ctl.tmem, tm_dv = tm_dk + 128, tm_v = tm_dk + 256, tm_s = tm_dk + 384, tm_dp = tm_dk + 448;
   const int heads = a.batch * a.kv_heads, bh = block % heads, tile = block / heads;    // long ones first
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+  touch(a);
+  touch(w);
   pdl_entry();
   const AttnStats stats = w.stats[bh];
   const AttnSpan span(a, b);

@@ -88,19 +88,21 @@ struct Segment {
   uint32_t tile, k0, k1;     // chunks [k0, k1) of the tile
   uint32_t first, count;     // the worker with the tile's first segment, the tile's segments
 };
-struct Run {
-  uint64_t at, end, units;   // of the tiles that are left
+struct Run {                 // fewer than `workers` tiles are left, of at most 2^17 chunks: 32 bits hold the products
+  uint32_t at, end, units;   // of the tiles that are left
   uint32_t kb, unit, worker, workers, round, rounds, used;
   DCT_DEV Run(uint32_t tiles, uint32_t kb_, uint32_t unit_, uint32_t used_, uint32_t worker_, uint32_t workers_)
-      : units((uint64_t)(tiles % workers_) * (kb_ / unit_)), kb(kb_), unit(unit_), worker(worker_), workers(workers_),
-        round(0), rounds(tiles / workers_), used(used_) {
+      : kb(kb_), unit(unit_), worker(worker_), workers(workers_), round(0), rounds(tiles / workers_), used(used_) {
+    units = (tiles - rounds * workers) * (unit == 1 ? kb : 1);
     at = end = 0;
     if (worker < used) {
       at = worker * units / used * unit;
       end = (worker + 1) * units / used * unit;
     }
   }
-  DCT_DEV uint32_t worker_of(uint64_t chunk) const { return (uint32_t)(((chunk / unit + 1) * used - 1) / units); }
+  DCT_DEV uint32_t worker_of(uint32_t chunk) const {
+    return (((unit == 1 ? chunk : chunk / unit) + 1) * used - 1) / units;
+  }
   DCT_DEV bool next(Segment& s) {
     if (round < rounds) {
       s.tile = round++ * workers + worker;
@@ -110,11 +112,10 @@ struct Run {
       return true;
     }
     if (at >= end) return false;
-    const uint32_t t = (uint32_t)(at / kb);
-    const uint64_t base = (uint64_t)t * kb;
+    const uint32_t t = at / kb, base = t * kb;
     s.tile = rounds * workers + t;
-    s.k0 = (uint32_t)(at - base);
-    s.k1 = (uint32_t)min((uint64_t)kb, end - base);
+    s.k0 = at - base;
+    s.k1 = min(kb, end - base);
     s.first = worker_of(base);
     s.count = worker_of(base + kb - 1) - s.first + 1;
     at = base + s.k1;
@@ -962,7 +963,7 @@ cudaError_t product_as(Product g, uint32_t batch, cudaStream_t st) {
   g.tiles = g.mt * g.nt;
   if (g.half) g.tiles = g.mt * (g.mt + 1) / 2;
   const uint64_t total = (uint64_t)g.tiles * batch, work = total * g.kb;
-  if (total >= (1ull << 31)) return cudaErrorInvalidConfiguration;
+  if (total >= (1ull << 31) || g.kb > (1u << 17)) return cudaErrorInvalidConfiguration;
   // The tiles that do not go around: whole, or cut in runs of 4 chunks or more (2 of the
   // smallest tiles), whichever ends first.  A cut tile's meeting in memory costs about as much as 6 chunks (one matrix of
   // 1024 x 8192: 700 us cut, 1079 us whole; twelve of 768 x 768: 552 and 550 us).

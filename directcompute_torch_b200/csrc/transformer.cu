@@ -199,7 +199,7 @@ int attention(const char* what, const DctAttention* p, void* q, void* k, void* v
 // Fills the shape, the polynomial and the largest singular value that its steps can give.
 int muon_args(const char* what, const DctMuon* p, MuonArgs& a) {
   if (!p) return refuse(DCT_ERR_ARG, "%s: no parameters", what);
-  if (p->batch > 65535 || (uint64_t)p->rows * p->cols >= kMost || p->rows >= (1u << 24) || p->cols >= (1u << 24))
+  if (p->batch > 65535 || (uint64_t)p->rows * p->cols >= kMost || p->rows > (1u << 23) || p->cols > (1u << 23))
     return refuse(DCT_ERR_ARG, "%s: %u matrices of %u x %u are too many or too large", what, p->batch, p->rows,
                   p->cols);
   if (p->steps > 16) return refuse(DCT_ERR_ARG, "%s: %u steps (0 to 16)", what, p->steps);
