@@ -303,17 +303,23 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ AttnA
   store_row(a, bh / a.kv_heads, RowAt(a, bh % a.kv_heads, (int)(row % rows)), f, o, best, sum);
 }
 
-// delta = sum_d dout out, a warp per (batch, head, position)
+// delta = sum_d dout out, an octet per (batch, head, position).  The products are summed as the
+// gradients sum dout v: a row that sees one key, whose out is that key's v, gets
+// dP - delta = 0 and gradients of exactly 0.
+template <int NV, bool VEC>
 __global__ void __launch_bounds__(128) k_attn_delta(const __grid_constant__ AttnArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (int64_t)a.batch * a.q_heads * a.q_len) return;
-  const int i = (int)(row % a.q_len), b = (int)(row / a.q_len / a.q_heads), h = (int)(row / a.q_len % a.q_heads);
-  const int64_t o = at(a.os, b, i, h);
-  float s = 0.f;
-  if (i < AttnSpan(a, b).m)
-    for (int f = threadIdx.x & 31; f < a.dim; f += 32) s = fmaf(a.dout[o + f], a.out[o + f], s);
-  s = warp_sum_f(s);
-  if ((threadIdx.x & 31) == 0)
+  const int64_t rows = (int64_t)a.batch * a.q_heads * a.q_len, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 3);
+  const int64_t r = min(row, rows - 1);
+  const int lane = threadIdx.x & 7;
+  const int i = (int)(r % a.q_len), b = (int)(r / a.q_len / a.q_heads), h = (int)(r / a.q_len % a.q_heads);
+  const bool in = row < rows && i < AttnSpan(a, b).m;
+  float go[4 * NV] = {}, o[4 * NV] = {};
+  if (in) {
+    load_row<NV, VEC>(go, a.dout + at(a.os, b, i, h), lane, a.dim);
+    load_row<NV, VEC>(o, a.out + at(a.os, b, i, h), lane, a.dim);
+  }
+  const float s = octet_sum(dot(go, o));
+  if (row < rows && lane == 0)
     a.delta[((int64_t)b * a.kv_heads + h / a.group) * padded_rows(a) + (int64_t)i * a.group + h % a.group] = s;
 }
 
@@ -551,8 +557,10 @@ cudaError_t launch_attn_join(const AttnArgs& a, int splits, float* part, bool te
 cudaError_t launch_attn_delta(const AttnArgs& a, cudaStream_t st) {
   const int64_t rows = (int64_t)a.batch * a.q_heads * a.q_len;
   if (!rows) return cudaSuccess;
-  k_attn_delta<<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(a);
-  return cudaGetLastError();
+  return by_width(a.dim, a.dim % 4 == 0 && aligned(a.dout, a.os) && aligned(a.out, a.os), [&](auto nv, auto v) {
+    k_attn_delta<decltype(nv)::value, decltype(v)::value><<<(unsigned)((rows + 15) / 16), 128, 0, st>>>(a);
+    return cudaGetLastError();
+  });
 }
 
 cudaError_t launch_attn_rows_backward(const AttnArgs& a, cudaStream_t st) {

@@ -324,6 +324,19 @@ def test_attention_heads_apart(dev, bad, t):
         assert not np.isfinite(got["out"][1, first:, 2:, 3]).any()
 
 
+@pytest.mark.parametrize("d", [64, 128, 37])
+def test_attention_of_a_single_key_has_no_gradient_of_its_score(dev, d):
+    """softmax of one score is 1 whatever it is: dq and dk are exactly 0, dv is the sum of dout."""
+    q, k, v, go = _inputs(3, 5, 1, 4, 2, d)
+    got = _attention(dev, q, k, v, go)
+    assert not got["dq"].any() and not got["dk"].any()
+    assert np.array_equal(got["out"], np.repeat(v, 2, 2) + 0 * q)
+    _hold(got, T.attention(q, k, v, go), ALL)
+    q, k, v, go = _inputs(2, 30, 30, 4, 2, d)
+    got = _attention(dev, q, k, v, go, window=1)
+    assert not got["dq"].any() and not got["dk"].any()
+
+
 def test_attention_over_a_cache_with_room(dev):
     """Keys in a cache longer than its valid part, heads before positions."""
     b, t, n, h, hk, d, room = 3, 20, 900, 8, 2, 64, 1024
