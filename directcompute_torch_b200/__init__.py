@@ -10,7 +10,7 @@ holds the loader and the Python host side:
 * `ops`     -- the NumPy-semantics ops the reference has no GPU kernel for
   (broadcast binary ops with broadcast gradients, exp/log/tanh, axis and full
   reductions, fused softmax-CE, bias + ReLU with the fused backward,
-  BatchNorm2d); `ops.bind(nn_engine)` builds them on the reference's own
+  BatchNorm2d, rotary positions, attention, the orthogonalised update); `ops.bind(nn_engine)` builds them on the reference's own
   Tensor instead;
 * `dist`    -- leading-dimension sharding across the GPUs of one node (one
   process per GPU, NCCL for the reduced-axis exchanges).

@@ -1,8 +1,9 @@
 // Shared device helpers for libdct_cuda (sm_100a).
 //
-// Every kernel of the library is memory-bound fp32 work: 128-bit vector
+// Most kernels of the library are memory-bound fp32 work: 128-bit vector
 // loads/stores, streaming cache hints, float64 accumulation for every sum, and
-// grids sized as a multiple of the SM count.  Nothing here uses tensor cores.
+// grids sized as a multiple of the SM count.  The contractions (attention, the
+// orthogonalised update) are on the tensor cores: dct_umma.cuh.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>

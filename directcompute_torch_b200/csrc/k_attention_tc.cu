@@ -1152,8 +1152,8 @@ cudaError_t backward(const AttnArgs& a, const Layout& L, const Tiles& t, cudaStr
   if (nq + nk > INT_MAX) return cudaErrorInvalidConfiguration;
   const bool vec = a.dim % 4 == 0;
   return launch_pdl(k_attn_backward<BLOCKS, FULL>, dim3((unsigned)(nq + nk)), dim3(kThreads), kSmem, st, a, t,
-                    (int)L.row_tiles, (int)nk, vec && aligned(a.dq, a.dqs), vec && aligned(a.dk, a.dks) && aligned(a.dv, a.dvs),
-                    device_error_word());
+                    (int)L.row_tiles, (int)nk, vec && aligned(a.dq, a.dqs),
+                    vec && aligned(a.dk, a.dks) && aligned(a.dv, a.dvs), device_error_word());
 }
 
 }  // namespace

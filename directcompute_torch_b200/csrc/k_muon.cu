@@ -965,8 +965,9 @@ cudaError_t product_as(Product g, uint32_t batch, cudaStream_t st) {
   const uint64_t total = (uint64_t)g.tiles * batch, work = total * g.kb;
   if (total >= (1ull << 31) || g.kb > (1u << 17)) return cudaErrorInvalidConfiguration;
   // The tiles that do not go around: whole, or cut in runs of 4 chunks or more (2 of the
-  // smallest tiles), whichever ends first.  A cut tile's meeting in memory costs about as much as 6 chunks (one matrix of
-  // 1024 x 8192: 700 us cut, 1079 us whole; twelve of 768 x 768: 552 and 550 us).
+  // smallest tiles), whichever ends first.  A cut tile's meeting in memory costs about as
+  // much as 6 chunks (when this rule was chosen, one matrix of 1024 x 8192: 700 us cut,
+  // 1079 us whole; twelve of 768 x 768: 552 and 550 us).
   constexpr uint64_t kShortest = BN == 64 ? 2 : 4, kMeeting = 6;
   const uint64_t workers = std::min<uint64_t>(work / kShortest + 1, most), left = total % workers;
   const uint64_t cut = std::max<uint64_t>(kShortest, (left * g.kb + workers - 1) / workers) + kMeeting;

@@ -359,7 +359,7 @@ DCT_API int dct_attention_backward(const DctAttention* p, void* q, void* k, void
  * (on the shorter side; X^T X for tall matrices), which moves the singular values
  * toward 1.  a = b = c = 0 means 3.4445, -4.7750, 2.0315; steps 0..16; the polynomial
  * a s + b s^3 + c s^5 must keep [0, 1] below 64 over the steps (DCT_ERR_ARG).
- * y may be x. */
+ * y may be x.  batch <= 65535, rows and cols <= 2^23, rows cols < 2^30. */
 typedef struct DctMuon {
   uint32_t batch, rows, cols, steps;
   double a, b, c;
