@@ -96,6 +96,30 @@ int check(const char* what, Arg& a) {
 
 bool overlap(const Arg& a, const Arg& b) { return a.extent && b.extent && a.lo() < b.hi() && b.lo() < a.hi(); }
 
+// Whether no element of one output is one of the other.  Ranges that meet are told apart
+// where the two lie side by side in every step of a common buffer, as the parts of a packed
+// projection do: equal strides of batch and position, the heads of one behind the other's.
+bool apart(const Arg& a, const Arg& b) {
+  if (!overlap(a, b)) return true;
+  const Arg &first = a.lo() <= b.lo() ? a : b, &second = a.lo() <= b.lo() ? b : a;
+  auto width = [](const Arg& x) { return x.dim + (x.size[2] - 1) * (uint64_t)x.stride[2]; };
+  const uint64_t ahead = (uint64_t)(second.lo() - first.lo()) / 4;
+  if (ahead < width(first)) return false;
+  uint64_t stride[2], size[2], span = ahead + width(second);
+  for (int i = 0; i < 2; ++i) {
+    if (a.size[i] > 1 && b.size[i] > 1 && a.stride[i] != b.stride[i]) return false;
+    stride[i] = (uint64_t)(a.size[i] > 1 ? a : b).stride[i];
+    size[i] = std::max(a.size[i], b.size[i]);
+  }
+  const int inner = size[0] > 1 && (size[1] <= 1 || stride[0] < stride[1]) ? 0 : 1;
+  for (const int i : {inner, 1 - inner}) {
+    if (size[i] <= 1) continue;
+    if (stride[i] < span) return false;
+    span += (size[i] - 1) * stride[i];
+  }
+  return true;
+}
+
 // an int32 tensor of n words, or null
 int words(const char* what, const char* name, void* handle, uint64_t n, const int32_t** out) {
   *out = nullptr;
@@ -151,6 +175,9 @@ int attention(const char* what, const DctAttention* p, void* q, void* k, void* v
     for (int j = 0; j < n; ++j)
       if (args[i].output && !args[j].output && overlap(args[i], args[j]))
         return refuse(DCT_ERR_ARG, "%s: %s overlaps %s", what, args[i].name, args[j].name);
+    for (int j = i + 1; j < n; ++j)
+      if (args[i].output && args[j].output && !apart(args[i], args[j]))
+        return refuse(DCT_ERR_ARG, "%s: %s and %s share elements", what, args[i].name, args[j].name);
     if ((args[i].output || l.output) && overlap(args[i], l))
       return refuse(DCT_ERR_ARG, "%s: %s overlaps lse", what, args[i].name);
   }

@@ -301,9 +301,10 @@ DCT_API int dct_batchnorm_forward_train_noalloc(const float* x, const float* gam
  * projection or of a cache with spare room needs no copy (for a tensor that starts
  * inside a buffer, wrap its first element).  Strides are not negative, the elements of
  * an output are distinct, and no output shares its address range with an input, except
- * where a call says that it works in place (DCT_ERR_ARG otherwise).  Index tensors are
- * int32 words.  A size of 0 is allowed for batch and lengths.  The calls use the
- * library's stream and scratch workspace; a stream that is being captured into a
+ * where a call says that it works in place (DCT_ERR_ARG otherwise).  Two outputs may lie
+ * interleaved in one buffer, with equal strides of batch and position and the heads of
+ * one behind those of the other.  Index tensors are int32 words.  A size of 0 is allowed
+ * for batch and lengths.  The calls use the library's stream and scratch workspace; a stream that is being captured into a
  * graph is refused (DCT_ERR_UNSUPPORTED), since a later call may move the workspace.
  * Results are the same, bit for bit, from run to run. */
 

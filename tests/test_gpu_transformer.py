@@ -613,3 +613,47 @@ def test_refused_while_the_stream_is_captured(dev, call):
         dev.sync()
         dev.free(*h)
         dev.clear_error()
+
+
+# ---------------------------------------------------------------------------
+# gradients in one buffer
+# ---------------------------------------------------------------------------
+def test_attention_gradients_packed(dev):
+    """dq, dk and dv interleaved in one buffer are those of three buffers; shared elements are refused."""
+    lib = dev.lib
+    b, t, h, d = 2, 5, 2, 8
+    q, k, v, go = _inputs(b, t, t, h, h, d)
+    apart = _attention(dev, q, k, v, go)
+    st, packed = _packed(q.shape), (3 * t * h * d, 3 * h * d, d)
+    hold = [dev.buf(x.ravel()) for x in (q, k, v, go)]
+    out, lse, base = dev.empty(q.size), dev.empty(b * h * t), dev.empty(3 * q.size, fill=np.nan)
+    hold += [out, lse, base]
+    part = []
+    for x in range(3):
+        at = x * h * d
+        part.append(lib.dct_wrap_device_ptr(lib.dct_buffer_device_ptr(base) + 4 * at, 3 * q.size - at))
+    hold += part
+
+    def back(dq, dk, dv, **kw):
+        p = _abi.Attention(batch=b, q_heads=h, kv_heads=h, q_len=t, kv_len=t, head_dim=d,
+                           **{x + "_stride": st for x in "qkvo"},
+                           **{**{x + "_stride": packed for x in ("dq", "dk", "dv")}, **kw})
+        return lib.dct_attention_backward(ctypes.byref(p), *hold[:3], None, None, out, lse, hold[3], dq, dk, dv)
+    try:
+        p = _abi.Attention(batch=b, q_heads=h, kv_heads=h, q_len=t, kv_len=t, head_dim=d,
+                           **{x + "_stride": st for x in "qkvo"})
+        _abi.check(lib, lib.dct_attention_forward(ctypes.byref(p), *hold[:3], None, None, out, lse))
+        for order in ((0, 1, 2), (2, 0, 1)):
+            _abi.check(lib, back(*(part[i] for i in order)))
+            got = dev.read(base).reshape(b, t, 3, h, d)
+            for name, i in zip(("dq", "dk", "dv"), order):
+                assert np.array_equal(got[:, :, i], apart[name]), (name, order)
+        assert back(part[0], part[1], part[1]) == ERR["ARG"]
+        assert back(part[0], part[0], part[2]) == ERR["ARG"]
+        assert back(part[0], part[1], part[2], dv_stride=(packed[0], h * d, d)) == ERR["ARG"]
+        near = lib.dct_wrap_device_ptr(lib.dct_buffer_device_ptr(base) + 4 * (h * d - 1), 3 * q.size - h * d + 1)
+        hold.append(near)
+        assert back(part[0], near, part[2]) == ERR["ARG"]
+    finally:
+        dev.free(*reversed(hold))
+        dev.clear_error()
