@@ -41,7 +41,6 @@ struct Tiles {
   uint32_t* any;               // set where a head does not take the tensor cores
   float *lse2, *delta;         // [heads][padded rows], backward: log-sums in log2 units, sum dout out
   int64_t tiles[4];            // of a head
-  int blocks;                  // of 64 features
 };
 
 // the rows of operand t of a head that are valid, and one of them
@@ -1113,7 +1112,6 @@ cudaError_t prepare(const AttnArgs& a, const Layout& L, uint8_t* w, bool backwar
   }
   t.lse2 = reinterpret_cast<float*>(w + L.lse2);
   t.delta = reinterpret_cast<float*>(w + L.delta);
-  t.blocks = (int)L.blocks;
   cudaError_t e = cudaMemsetAsync(t.stats, 0, sizeof(AttnStats) * L.heads + sizeof(uint32_t), st);
   if (e != cudaSuccess) return e;
   const int64_t split = L.heads * ((backward ? 2 : 1) * L.row_tiles + 2 * L.key_tiles);
