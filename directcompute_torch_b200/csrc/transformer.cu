@@ -184,11 +184,15 @@ int attention(const char* what, const DctAttention* p, void* q, void* k, void* v
   AttnArgs a{};
   if (const int rc = words(what, "q_lens", q_lens, B, &a.q_lens)) return rc;
   if (const int rc = words(what, "kv_lens", kv_lens, B, &a.kv_lens)) return rc;
-  for (int i = 0; i < n; ++i)
-    for (const int32_t* w : {a.q_lens, a.kv_lens})
-      if (w && args[i].output && args[i].extent && reinterpret_cast<const char*>(w) < args[i].hi() &&
-          args[i].lo() < reinterpret_cast<const char*>(w + B))
-        return refuse(DCT_ERR_ARG, "%s: %s overlaps the lengths", what, args[i].name);
+  for (const int32_t* w : {a.q_lens, a.kv_lens}) {
+    auto meets = [&](const Arg& x) {
+      return w && x.output && x.extent && reinterpret_cast<const char*>(w) < x.hi() &&
+             x.lo() < reinterpret_cast<const char*>(w + B);
+    };
+    for (int i = 0; i < n; ++i)
+      if (meets(args[i])) return refuse(DCT_ERR_ARG, "%s: %s overlaps the lengths", what, args[i].name);
+    if (meets(l)) return refuse(DCT_ERR_ARG, "%s: lse overlaps the lengths", what);
+  }
   a.q = args[0].buf->d; a.k = args[1].buf->d; a.v = args[2].buf->d;
   a.out = args[3].buf->d;
   a.lse = l.buf ? l.buf->d : nullptr;

@@ -657,3 +657,20 @@ def test_attention_gradients_packed(dev):
     finally:
         dev.free(*reversed(hold))
         dev.clear_error()
+
+
+def test_attention_refuses_log_sums_over_the_lengths(dev):
+    lib = dev.lib
+    h = [dev.empty(96) for _ in range(4)]
+    lse = dev.empty(12)
+    tail = lib.dct_wrap_device_ptr(lib.dct_buffer_device_ptr(lse) + 4 * 10, 2)
+    st = (48, 16, 8)
+    p = _abi.Attention(batch=2, q_heads=2, kv_heads=2, q_len=3, kv_len=3, head_dim=8,
+                       **{x + "_stride": st for x in "qkvo"})
+    try:
+        for lens in ((lse, None), (None, lse), (tail, None), (None, tail)):
+            assert lib.dct_attention_forward(ctypes.byref(p), *h[:3], *lens, h[3], lse) == ERR["ARG"], lens
+        assert lib.dct_attention_forward(ctypes.byref(p), *h[:3], tail, None, h[3], None) == 0
+    finally:
+        dev.free(tail, lse, *h)
+        dev.clear_error()
