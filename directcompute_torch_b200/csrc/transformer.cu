@@ -151,8 +151,9 @@ int attention(const char* what, const DctAttention* p, void* q, void* k, void* v
     return refuse(DCT_ERR_ARG, "%s: head_dim is %u (1 to 128)", what, p->head_dim);
   if (!p->q_heads || !p->kv_heads || p->q_heads % p->kv_heads)
     return refuse(DCT_ERR_ARG, "%s: %u query heads over %u key heads", what, p->q_heads, p->kv_heads);
-  if ((unsigned __int128)p->q_len * p->q_heads * std::max(1u, p->batch) >= kMostRows ||
-      (unsigned __int128)p->kv_len * p->kv_heads * std::max(1u, p->batch) >= kMostRows)
+  // heads and batch entries count where there are no positions too: the kernels' are 32-bit
+  if ((unsigned __int128)std::max(1u, p->q_len) * p->q_heads * std::max(1u, p->batch) >= kMostRows ||
+      (unsigned __int128)std::max(1u, p->kv_len) * p->kv_heads * std::max(1u, p->batch) >= kMostRows)
     return refuse(DCT_ERR_ARG, "%s: too many rows in one call", what);
   if (!isfinite(p->scale)) return refuse(DCT_ERR_ARG, "%s: scale is not finite", what);
   const uint64_t B = p->batch, D = p->head_dim;

@@ -674,3 +674,20 @@ def test_attention_refuses_log_sums_over_the_lengths(dev):
     finally:
         dev.free(tail, lse, *h)
         dev.clear_error()
+
+
+def test_attention_refuses_too_many_heads_without_positions(dev):
+    """Heads and batch entries are bounded where the lengths are 0 as well."""
+    lib = dev.lib
+    h = [dev.empty(8) for _ in range(9)]
+    try:
+        for size in ({"q_heads": 1 << 31}, {"batch": 1 << 31}, {"batch": 1 << 20, "q_heads": 1 << 20},
+                     {"q_heads": 1 << 28, "kv_heads": 1 << 28}, {"batch": (1 << 32) - 1}):
+            p = _abi.Attention(**{"batch": 1, "q_heads": 1, "kv_heads": 1, "q_len": 0, "kv_len": 0, "head_dim": 8,
+                                  **size})
+            assert lib.dct_attention_forward(ctypes.byref(p), *h[:3], None, None, h[3], h[4]) == ERR["ARG"], size
+            assert lib.dct_attention_backward(ctypes.byref(p), *h[:3], None, None, h[3], h[4], *h[5:9]) == \
+                ERR["ARG"], size
+    finally:
+        dev.free(*h)
+        dev.clear_error()
