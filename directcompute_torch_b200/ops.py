@@ -548,6 +548,8 @@ def _words(a, shape, what):
     a = np.asarray(a)
     if not np.issubdtype(a.dtype, np.integer):
         raise ValueError(f"{what}: integers expected, got {a.dtype}")
+    if a.size and not (-2 ** 31 <= int(a.min()) and int(a.max()) < 2 ** 31):
+        raise ValueError(f"{what}: integers of 32 bits expected, got {a.min()} to {a.max()}")
     a = np.ascontiguousarray(np.broadcast_to(a, shape), dtype=np.int32)
     if not a.size:
         return _buf(1)
@@ -555,6 +557,13 @@ def _words(a, shape, what):
     if not h:
         raise MemoryError("libdct_cuda: " + (lib.dct_last_error() or b"").decode())
     return h
+
+
+def _within(value, low, high, what):
+    """An integer of [low, high]: a field of the call's struct would keep its low bits only."""
+    if value != int(value) or not low <= value <= high:
+        raise ValueError(f"{what} is {value} (an integer of {low} to {high})")
+    return int(value)
 
 
 def _strides(shape):
@@ -607,7 +616,9 @@ def rotary(x, positions=None, start=0, rotated=None, interleaved=False, base=100
     first so many features turn (default all).  interleaved: pairs (2j, 2j+1) instead of
     (j, j + rotated/2).  factor, original, low, high, magnitude: scaling for contexts longer
     than `original` (see DctRotary in include/dct_cuda.h)."""
-    return RotaryFunc().forward(x, positions, start=start, rotated=x.shape[-1] if rotated is None else rotated,
+    rotated = x.shape[-1] if rotated is None else _within(rotated, 0, 256, "rotary: rotated")
+    start = _within(start, -2 ** 31, 2 ** 31 - 1, "rotary: start")
+    return RotaryFunc().forward(x, positions, start=start, rotated=rotated,
                                 interleaved=bool(interleaved), base=base, factor=factor, original=original, low=low,
                                 high=high, magnitude=magnitude)
 
@@ -620,13 +631,18 @@ class AttentionFunc(Node):
         if len(q.shape) != 4 or len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or \
                 q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
             raise ValueError(f"attention: q {q.shape}, k {k.shape} and v {v.shape} do not match")
+        window = _within(window, 0, 2 ** 32 - 1, "attention: window")
+        if scale is not None and not np.float32(scale):
+            raise ValueError(f"attention: scale {scale} is 0 in float32")
         self.inputs = (q, k, v)
         b, t, h, d = q.shape
-        self.words = [_words(q_lens, (b,), "attention q_lens"), _words(kv_lens, (b,), "attention kv_lens")]
+        self.words = []                       # released by __del__, also where the second is refused
+        for lens, what in ((q_lens, "attention q_lens"), (kv_lens, "attention kv_lens")):
+            self.words.append(_words(lens, (b,), what))
         qs, ks = _strides(q.shape), _strides(k.shape)
         self.p = Attention(batch=b, q_heads=h, kv_heads=k.shape[2], q_len=t, kv_len=k.shape[1], head_dim=d,
                            causal=bool(causal), window=window, q_stride=qs, k_stride=ks, v_stride=ks, o_stride=qs,
-                           dq_stride=qs, dk_stride=ks, dv_stride=ks, scale=scale or 0.0)
+                           dq_stride=qs, dk_stride=ks, dv_stride=ks, scale=0.0 if scale is None else scale)
         oh, lh = _buf(q.size), _buf(b * t * h)
         rc = lib.dct_attention_forward(ctypes.byref(self.p), q.gpu_buf, k.gpu_buf, v.gpu_buf, *self.words, oh, lh)
         if rc:
@@ -681,6 +697,7 @@ def _muon(x, steps, coefficients, eps, **kw):
     if len(x.shape) < 2:
         raise ValueError("orthogonalize: matrices [..., rows, cols] expected")
     a, b, c = coefficients
+    steps = _within(steps, 0, 16, "orthogonalize: steps")
     return Muon(batch=_size(x.shape[:-2]), rows=x.shape[-2], cols=x.shape[-1], steps=steps, a=a, b=b, c=c, eps=eps,
                 **kw)
 
@@ -688,8 +705,9 @@ def _muon(x, steps, coefficients, eps, **kw):
 def orthogonalize(x, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
     """Matrices x [..., rows, cols] with their singular values moved toward 1 by
     Newton-Schulz steps (no gradient)."""
+    p = _muon(x, steps, coefficients, eps)
     h = _buf(x.size)
-    rc = lib.dct_orthogonalize(ctypes.byref(_muon(x, steps, coefficients, eps)), x.gpu_buf, h)
+    rc = lib.dct_orthogonalize(ctypes.byref(p), x.gpu_buf, h)
     if rc:
         _release(h)
     check(lib, rc, "dct_orthogonalize")
