@@ -30,7 +30,9 @@ DCT_DEV float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^e for -126 <= e <= 127; the tiles' exponents and their sums are clamped to that
+// 2^e for -126 <= e <= 127, clamped to that.  A tile's exponent is -30 to 74 and the sum of two
+// up to 148: harmless for scores (2^-126 of a number below 2^37 is as good as nothing in an
+// exponent), but not for what is added to something as small.
 DCT_DEV float pow2(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
 DCT_DEV uint32_t lane_bits(int warp) { return (uint32_t)(warp & 3) * 32u << 16; }
 
@@ -620,6 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
 // against its keys) and for dk and dv (a tile of keys against the rows that see them): seven
 // products instead of five, but every gradient has one owner, no atomics and one order.
 constexpr float kUpP = 14.f;                       // P <= 1 is held as 2^14 P
+constexpr float kDownP = 1.f / 16384.f;            // and back
 
 // The accumulators are drained after every tile of the inner side, whose scales they carry.
 template <int N>
@@ -964,7 +967,7 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
       // The gradients of a tile of rows are drained at the end of it (dv) and after the next
       // tile's first P (dk), when their last products are done and no matrix instruction yet
       // waits for the accumulator.
-      float f = 0.f, fd = 0.f, fp = 0.f, back_v = 0.f, back_k = 0.f;
+      float f = 0.f, fd = 0.f, up = 0.f, back_v = 0.f, back_k = 0.f;
       int group = 0;
       auto take_dv = [&]() {
         wait(&ctl.dv_full, group);
@@ -985,8 +988,8 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
         if (first) {
           const int eds = scale_of_ds(gt.norm, vt.norm);
           f = a.scale * kLog2e * pow2(-qt.e - ek);
-          fd = pow2(-gt.e - vt.e);
-          fp = pow2(eds - (int)kUpP);                      // P from 2^14 P, and dS's scale
+          fd = pow2(eds - gt.e - vt.e);
+          up = pow2(eds);
           back_v = pow2(-(int)kUpP - gt.e);
           back_k_next = ldexpf(a.scale, -eds - qt.e);
           const int next = ((t0 + j) >> 1) + 1;
@@ -1027,10 +1030,10 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const float4 d = del[e / 4];
-          p[e] = p[e] * fp * fmaf(__uint_as_float(x[e]), fd, -d.x);
-          p[e + 1] = p[e + 1] * fp * fmaf(__uint_as_float(x[e + 1]), fd, -d.y);
-          p[e + 2] = p[e + 2] * fp * fmaf(__uint_as_float(x[e + 2]), fd, -d.z);
-          p[e + 3] = p[e + 3] * fp * fmaf(__uint_as_float(x[e + 3]), fd, -d.w);
+          p[e] = p[e] * kDownP * fmaf(__uint_as_float(x[e]), fd, -d.x * up);
+          p[e + 1] = p[e + 1] * kDownP * fmaf(__uint_as_float(x[e + 1]), fd, -d.y * up);
+          p[e + 2] = p[e + 2] * kDownP * fmaf(__uint_as_float(x[e + 2]), fd, -d.z * up);
+          p[e + 3] = p[e + 3] * kDownP * fmaf(__uint_as_float(x[e + 3]), fd, -d.w * up);
         }
         store_operand<16>(tm_dp + off, p);
         tmem_wait_st();
