@@ -50,7 +50,6 @@ DCT_DEV int64_t at(const int64_t* s, int b, int t, int h) { return b * s[0] + t 
 // [2^14, 2^15); an element is then off by 2^-23 of itself or 2^-40 of that largest one.
 struct AttnTile {
   int32_t e;
-  float norm;                  // of v and dout: a bound on its rows' norms
 };
 // Of a key head: magnitudes as float bits, which order like integers, so that they meet by
 // atomic maximum from 0 (the same in any order).

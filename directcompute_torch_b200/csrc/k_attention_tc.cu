@@ -32,7 +32,7 @@ DCT_DEV float ex2(float x) {
 }
 // 2^e for -126 <= e <= 127, clamped to that.  A tile's exponent is -30 to 74 and the sum of two
 // up to 148: harmless for scores (2^-126 of a number below 2^37 is as good as nothing in an
-// exponent), but not for what is added to something as small.
+// exponent), but dP and delta stay in units of dout's tile, and sums are scaled back in two steps.
 DCT_DEV float pow2(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
 DCT_DEV uint32_t lane_bits(int warp) { return (uint32_t)(warp & 3) * 32u << 16; }
 
@@ -41,7 +41,8 @@ struct Tiles {
   AttnTile* info[4];           // [heads][tiles]
   AttnStats* stats;            // [heads]
   uint32_t* any;               // set where a head does not take the tensor cores
-  float *lse2, *delta;         // [heads][padded rows], backward: log-sums in log2 units, sum dout out
+  float *lse2, *delta;         // [heads][padded rows], backward: log-sums in log2 units, sum dout out in
+                               // units of dout's tile
   int64_t tiles[4];            // of a head
 };
 
@@ -80,7 +81,7 @@ template <int BLOCKS>
 __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ AttnArgs a, const __grid_constant__ Tiles w,
                                                     int tq, int tk, bool vec) {
   constexpr int kGroups = 8 * BLOCKS, kStep = 512 / kGroups, kPasses = kTile / kStep;
-  __shared__ uint32_t sh[3];
+  __shared__ uint32_t sh[2];
   touch(a);
   touch(w);
   pdl_entry();
@@ -96,10 +97,10 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
   const AttnSpan span(a, b);
   const int rows = rows_of(a, span, t);
   if (tile * kTile >= rows && t != 3) return;      // nothing reads it (dout's log-sums are read by whole tiles)
-  if (threadIdx.x < 3) sh[threadIdx.x] = 0;
+  if (threadIdx.x < 2) sh[threadIdx.x] = 0;
   __syncthreads();
-  float v[kPasses][8];
-  uint32_t top = 0, low = 0, norm = 0;
+  float v[kPasses][8], delta[kPasses];
+  uint32_t top = 0, low = 0;
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
     const int r = tile * kTile + row0 + p * kStep;
@@ -127,14 +128,10 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
     for (int o = 1; o < kGroups; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     top = max(top, m);
     if (m) low = max(low, ~m);
-    if (t >= 2) {
-      // the row's norm through its own scale, so that squares neither vanish nor overflow
-      const float f = __uint_as_float(m), i = m ? 1.f / f : 0.f;
-      float s = 0.f, d = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf(v[p][e] * i, v[p][e] * i, s);
+    if (t == 3) {
+      float d = 0.f;
       const int r = tile * kTile + row0 + p * kStep;
-      if (t == 3 && r < rows) {
+      if (r < rows) {
         const RowAt q(a, hk, r);
         const float* o = a.out + at(a.os, b, q.i, q.h) + g * 8;
 #pragma unroll
@@ -142,12 +139,8 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
           if (g * 8 + e < a.dim) d = fmaf(v[p][e], o[e], d);
       }
 #pragma unroll
-      for (int o = 1; o < kGroups; o <<= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        d += __shfl_xor_sync(0xffffffffu, d, o);
-      }
-      if (m < 0x7f800000u) norm = max(norm, __float_as_uint(1.001f * f * sqrtf(s)));
-      if (t == 3 && g == 0) {
+      for (int o = 1; o < kGroups; o <<= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+      if (g == 0) {
         const int64_t at_row = (int64_t)bh * padded_rows(a) + r;
         float l = INFINITY;                        // a row that sees nothing: P = 2^(s - inf) = 0
         if (r < rows) {
@@ -156,24 +149,22 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
           if (l == -INFINITY) l = INFINITY;
         }
         w.lse2[at_row] = l;
-        w.delta[at_row] = d;
+        a.delta[at_row] = delta[p] = d;
       }
     }
   }
   top = __reduce_max_sync(0xffffffffu, top);
   low = __reduce_max_sync(0xffffffffu, low);
-  norm = __reduce_max_sync(0xffffffffu, norm);
   if ((threadIdx.x & 31) == 0) {
     atomicMax(&sh[0], top);
     atomicMax(&sh[1], low);
-    atomicMax(&sh[2], norm);
   }
   __syncthreads();
   top = sh[0];
   const bool splits = tile_splits(top, ~sh[1]);
   const int e = top && splits ? 14 - ((int)(top >> 23) - 127) : 0;
   if (threadIdx.x == 0) {
-    w.info[t][bh * w.tiles[t] + tile] = AttnTile{e, __uint_as_float(sh[2])};
+    w.info[t][bh * w.tiles[t] + tile] = AttnTile{e};
     if (t == 0) atomicMax(&w.stats[bh].top_q, top);
     if (t == 1) atomicMax(&w.stats[bh].top_k, top);
     if (t == 2 && top) {
@@ -184,6 +175,11 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
   }
   if (!splits) return;
   const float f = pow2(e);
+  if (t == 3 && g == 0) {
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p)
+      w.delta[(int64_t)bh * padded_rows(a) + tile * kTile + row0 + p * kStep] = delta[p] * f;
+  }
   if (g >= (a.dim + 15) / 16 * 2) return;          // features that no product reads
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
@@ -622,9 +618,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
 // against its keys) and for dk and dv (a tile of keys against the rows that see them): seven
 // products instead of five, but every gradient has one owner, no atomics and one order.
 constexpr float kUpP = 14.f;                       // P <= 1 is held as 2^14 P
-constexpr float kDownP = 1.f / 16384.f;            // and back
 
-// The accumulators are drained after every tile of the inner side, whose scales they carry.
+// The accumulators are drained whenever the scales that they carry change: dv after every
+// tile of the inner side, dq and dk after every half tile.
 template <int N>
 DCT_DEV void drain(uint32_t addr, float f, float (&acc)[N]) {
 #pragma unroll
@@ -636,12 +632,39 @@ DCT_DEV void drain(uint32_t addr, float f, float (&acc)[N]) {
     for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(__uint_as_float(v[e]), f, acc[c + e]);
   }
 }
-
-// dS is held as 2^eds dS / scale, from |dS / (P scale)| <= 2 max|dout row| max|v row|
-DCT_DEV int scale_of_ds(float norm_do, float norm_v) {
-  const float n = norm_do * norm_v;
-  return n > 0.f ? min(13 - ((int)(__float_as_uint(n) >> 23) - 127), 120) : 0;
+template <int N>
+DCT_DEV void drain(uint32_t addr, float2 f, float (&acc)[N]) {
+#pragma unroll
+  for (int c = 0; c < N; c += 16) {
+    uint32_t v[16];
+    tmem_load16(addr + c, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(__uint_as_float(v[e]) * f.x, f.y, acc[c + e]);
+  }
 }
+
+// dS = P (dP - delta) can be anything up to the sizes of dout and the largest v of the whole
+// row, and is small where P is or where another row of the tile has the large dout.  So it is
+// scaled by what it is: for each row of the product that takes it (a query in dq, a key in dk)
+// the largest |dS| of the half tile comes to [2^14, 2^15), and the row's accumulator is drained
+// with the reverse of that after every half tile.  (Bounds from the tiles' norms instead lost
+// the accuracy of rows far below the bound, and passed float16 where delta came from
+// other tiles' v.)  The four threads of a row meet here: returns the exponent for theirs.
+template <int N>
+DCT_DEV int scale_of_ds(const float (&ds)[N], uint8_t (&top)[2][kTile][4], int j, int row, int quarter, int warp) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) m = max(m, __float_as_uint(ds[e]) & 0x7fffffffu);
+  top[j & 1][row][quarter] = (uint8_t)(m >> 23);      // the exponent: order enough
+  rows_sync(warp);               // (the other half of `top` is in use until all have passed this)
+  const uint32_t x = *reinterpret_cast<const uint32_t*>(top[j & 1][row]);
+  const uint32_t y = max(max(x & 255, x >> 8 & 255), max(x >> 16 & 255, x >> 24));
+  return min(14 + 127 - (int)y, 120);
+}
+// f 2^e as two factors, neither of which leaves float32 where their product with an
+// accumulator does not
+DCT_DEV float2 factors(float f, int e) { return make_float2(pow2(e >> 1), f * pow2(e - (e >> 1))); }
 
 template <int BLOCKS>
 struct Dq : Sizes<BLOCKS> {
@@ -651,10 +674,12 @@ struct Dq : Sizes<BLOCKS> {
     Ring<kValues> v;
     uint64_t q_full, go_full, s_full[2], ds_full[2], acc_full, acc_empty;
     uint32_t tmem;
+    __align__(4) uint8_t top[2][kTile][4];
   };
   static constexpr uint32_t kK = Sizes<BLOCKS>::kTileBytes, kV = kK + kKeys * Sizes<BLOCKS>::kSlotBytes;
   static constexpr uint32_t kEnd = kV + kValues * Sizes<BLOCKS>::kSlotBytes;
   static constexpr size_t kSmem = kEnd + sizeof(Control);
+  static_assert(kSmem <= 227 * 1024);
 };
 
 // dq of a tile of 128 rows: dS = P (dP - delta), dq = scale dS K.  Q rests in shared memory,
@@ -737,17 +762,15 @@ DCT_DEV void attn_dq(const AttnArgs& a, const Tiles& w, int block, int row_tiles
           ctl.v.release(j);
           umma_commit(&ctl.s_full[j & 1]);
         };
-        int group = 0;
         scores(0);
         for (int j = 0; j < n && wait.ok; ++j) {
           if (j + 1 < n) scores(j + 1);
           wait(&ctl.ds_full[j & 1], j >> 1);
-          const bool first = j == 0 || !((t0 + j) & 1), last = j == n - 1 || ((t0 + j) & 1);   // of its tile
-          if (first) wait(&ctl.acc_empty, group++ ^ 1);
+          wait(&ctl.acc_empty, j ^ 1);
           if (!wait.ok) break;
-          mma_rows<BLOCKS, 16>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(key(j), 2 * kChunkBytes, 1024), !first, steps);
+          mma_rows<BLOCKS, 16>(tm_acc, tm_s + (j & 1) * kHalf, umma_desc(key(j), 2 * kChunkBytes, 1024), false, steps);
           ctl.k.release(j);
-          if (last) umma_commit(&ctl.acc_full);
+          umma_commit(&ctl.acc_full);
         }
       }
     }
@@ -759,7 +782,7 @@ DCT_DEV void attn_dq(const AttnArgs& a, const Tiles& w, int block, int row_tiles
     const int lo = in ? span.lo(a, at_row.i) : 0, hi = in ? span.hi(a, at_row.i) : 0;
     const AttnTile *ki = w.info[1] + bh * w.tiles[1], *vi = w.info[2] + bh * w.tiles[2];
     const int eq = w.info[0][bh * w.tiles[0] + tile].e;
-    const AttnTile go = w.info[3][bh * w.tiles[3] + tile];
+    const int eg = w.info[3][bh * w.tiles[3] + tile].e;
     float acc[S::kF];
 #pragma unroll
     for (int e = 0; e < S::kF; ++e) acc[e] = 0.f;
@@ -769,23 +792,21 @@ DCT_DEV void attn_dq(const AttnArgs& a, const Tiles& w, int block, int row_tiles
       tile_to_tmem<BLOCKS>(w.p[3] + (bh * w.tiles[3] + tile) * (int64_t)S::kTileBytes, tm_go, warp, row);
       tmem_wait_st();
       arrive_warp(&ctl.go_full);
-      float f = 0.f, fd = 0.f, ds_delta = 0.f, back = 0.f;
-      int group = 0;
-      auto take = [&](int group) {
-        wait(&ctl.acc_full, group);
+      float f = 0.f, fd = 0.f;
+      float2 back = {};
+      auto take = [&](int j) {
+        wait(&ctl.acc_full, j);
         drain(tm_acc + lane_bits(warp) + quarter * S::kF, back, acc);
         arrive_warp(&ctl.acc_empty);
       };
       AttnTile kt = ki[t0 >> 1], vt = vi[t0 >> 1];
+      int ek = 0;
       for (int j = 0; j < n; ++j) {
         const int key = (t0 + j) * kHalf + quarter * 16;
-        float back_next = back;
         if (j == 0 || !((t0 + j) & 1)) {           // another tile of K and V
-          const int eds = scale_of_ds(go.norm, vt.norm);
-          f = a.scale * kLog2e * pow2(-eq - kt.e);
-          fd = pow2(eds - go.e - vt.e);
-          ds_delta = delta * pow2(eds);
-          back_next = ldexpf(a.scale, -eds - kt.e);
+          ek = kt.e;
+          f = a.scale * kLog2e * pow2(-eq - ek);
+          fd = pow2(-vt.e);
           const int next = ((t0 + j) >> 1) + 1;
           if (next <= (t0 + n - 1) >> 1) {
             kt = ki[next];
@@ -801,19 +822,23 @@ DCT_DEV void attn_dq(const AttnArgs& a, const Tiles& w, int block, int row_tiles
         float ds[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          ds[e] = ex2(fmaf(__uint_as_float(x[e]), f, -lse2)) * fmaf(__uint_as_float(y[e]), fd, -ds_delta);
+          ds[e] = ex2(fmaf(__uint_as_float(x[e]), f, -lse2)) * fmaf(__uint_as_float(y[e]), fd, -delta);
         if (__any_sync(0xffffffffu, key < lo || key + 16 > hi)) {
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (key + e < lo || key + e >= hi) ds[e] = 0.f;
         }
+        const int eds = scale_of_ds(ds, ctl.top, j, row, quarter, warp);
+        const float up = pow2(eds);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[e] *= up;
         store_operand<16>(tm_s + off, ds);
         tmem_wait_st();
         arrive_warp(&ctl.ds_full[j & 1]);
-        if (j && !((t0 + j) & 1)) take(group++);
-        back = back_next;
+        if (j) take(j - 1);
+        back = factors(a.scale, -eds - eg - ek);
       }
-      take(group);
+      take(n - 1);
     }
     if (r < rows) {
       store_features<S::kF>(a.dq + at(a.dqs, b, at_row.i, at_row.h), quarter * S::kF, a.dim, vec_out, acc);
@@ -830,6 +855,7 @@ struct Dkv : Sizes<BLOCKS> {
   static constexpr int kRowsQ = BLOCKS == 1 ? 5 : 3, kRowsGo = BLOCKS == 1 ? 4 : 2;  // halves of Q, of dout
   struct Control {
     float lse[kRowsQ][kHalf], delta[kRowsQ][kHalf];  // with Q; 16-byte aligned: the bulk copies' targets
+    __align__(4) uint8_t top[2][kTile][4];
     Ring<kRowsQ> q;
     Ring<kRowsGo> go;
     uint64_t k_full, v_full, s_full, dp_full, p_full, ds_full, dv_full, dv_empty, dk_full, dk_empty;
@@ -838,6 +864,7 @@ struct Dkv : Sizes<BLOCKS> {
   static constexpr uint32_t kQ = Sizes<BLOCKS>::kTileBytes, kGo = kQ + kRowsQ * Sizes<BLOCKS>::kSlotBytes;
   static constexpr uint32_t kEnd = kGo + kRowsGo * Sizes<BLOCKS>::kSlotBytes;
   static constexpr size_t kSmem = kEnd + sizeof(Control);
+  static_assert(kSmem <= 227 * 1024);
 };
 
 // dk and dv of a tile of 128 keys: dv = P^T dout, dk = scale dS^T Q.  K rests in shared
@@ -933,18 +960,18 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
         for (int j = 0; j < n && wait.ok; ++j) {
           const bool first = j == 0 || !((t0 + j) & 1), last = j == n - 1 || ((t0 + j) & 1);   // of its tile
           wait(&ctl.p_full, j);
-          if (first) wait(&ctl.dv_empty, group ^ 1);
+          if (first) wait(&ctl.dv_empty, group++ ^ 1);
           if (!wait.ok) break;
           mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(grad(j), 2 * kChunkBytes, 1024), !first, steps);
           ctl.go.release(j);
           if (last) umma_commit(&ctl.dv_full);
           if (j + 1 < n) scores(j + 1);
           wait(&ctl.ds_full, j);
-          if (first) wait(&ctl.dk_empty, group++ ^ 1);
+          wait(&ctl.dk_empty, j ^ 1);
           if (!wait.ok) break;
-          mma_rows<BLOCKS, 16>(tm_dk, tm_dp, umma_desc(query(j), 2 * kChunkBytes, 1024), !first, steps);
+          mma_rows<BLOCKS, 16>(tm_dk, tm_dp, umma_desc(query(j), 2 * kChunkBytes, 1024), false, steps);
           ctl.q.release(j);
-          if (last) umma_commit(&ctl.dk_full);
+          umma_commit(&ctl.dk_full);
           if (j + 1 < n) dps(j + 1);
         }
       }
@@ -956,7 +983,7 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
     const int lo = key < span.n ? span.first(a, key) * a.group : 0, hi = key < span.n ? span.last(a, key) * a.group : 0;
     const AttnTile *qi = w.info[0] + bh * w.tiles[0], *gi = w.info[3] + bh * w.tiles[3];
     const int ek = w.info[1][bh * w.tiles[1] + tile].e;
-    const AttnTile vt = w.info[2][bh * w.tiles[2] + tile];
+    const int ev = w.info[2][bh * w.tiles[2] + tile].e;
     float dk[S::kF], dv[S::kF];
 #pragma unroll
     for (int e = 0; e < S::kF; ++e) dk[e] = dv[e] = 0.f;
@@ -964,34 +991,33 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
       tile_to_tmem<BLOCKS>(w.p[2] + (bh * w.tiles[2] + tile) * (int64_t)S::kTileBytes, tm_v, warp, row);
       tmem_wait_st();
       arrive_warp(&ctl.v_full);
-      // The gradients of a tile of rows are drained at the end of it (dv) and after the next
-      // tile's first P (dk), when their last products are done and no matrix instruction yet
-      // waits for the accumulator.
-      float f = 0.f, fd = 0.f, up = 0.f, back_v = 0.f, back_k = 0.f;
+      // dv of a tile of rows is drained at the end of it, dk of a half tile after the next one's
+      // first P, when their last products are done and no matrix instruction yet waits for the
+      // accumulator.
+      const float fd = pow2(-ev);
+      float f = 0.f, back_v = 0.f;
+      float2 back_k = {};
       int group = 0;
       auto take_dv = [&]() {
-        wait(&ctl.dv_full, group);
+        wait(&ctl.dv_full, group++);
         drain(tm_dv + lane_bits(warp) + quarter * S::kF, back_v, dv);
         arrive_warp(&ctl.dv_empty);
       };
-      auto take_dk = [&]() {
-        wait(&ctl.dk_full, group++);
+      auto take_dk = [&](int j) {
+        wait(&ctl.dk_full, j);
         drain(tm_dk + lane_bits(warp) + quarter * S::kF, back_k, dk);
         arrive_warp(&ctl.dk_empty);
       };
       AttnTile qt = qi[t0 >> 1], gt = gi[t0 >> 1];
+      int eq = 0, eg = 0;
       const uint32_t off = lane_bits(warp) + quarter * 16;
       for (int j = 0; j < n; ++j) {
         const int r = (t0 + j) * kHalf + quarter * 16;
-        const bool first = j == 0 || !((t0 + j) & 1);      // of another tile of Q and dout
-        float back_k_next = back_k;
-        if (first) {
-          const int eds = scale_of_ds(gt.norm, vt.norm);
-          f = a.scale * kLog2e * pow2(-qt.e - ek);
-          fd = pow2(eds - gt.e - vt.e);
-          up = pow2(eds);
-          back_v = pow2(-(int)kUpP - gt.e);
-          back_k_next = ldexpf(a.scale, -eds - qt.e);
+        if (j == 0 || !((t0 + j) & 1)) {                   // another tile of Q and dout
+          eq = qt.e;
+          f = a.scale * kLog2e * pow2(-eq - ek);
+          eg = gt.e;
+          back_v = pow2(-(int)kUpP - eg);
           const int next = ((t0 + j) >> 1) + 1;
           if (next <= (t0 + n - 1) >> 1) {
             qt = qi[next];
@@ -1022,25 +1048,29 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
         store_operand<16>(tm_s + off, p);
         tmem_wait_st();
         arrive_warp(&ctl.p_full);
-        if (j && first) take_dk();
-        back_k = back_k_next;
+        if (j) take_dk(j - 1);
         wait(&ctl.dp_full, j);
         tmem_load16(tm_dp + off, x);
         tmem_wait_ld();
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const float4 d = del[e / 4];
-          p[e] = p[e] * kDownP * fmaf(__uint_as_float(x[e]), fd, -d.x * up);
-          p[e + 1] = p[e + 1] * kDownP * fmaf(__uint_as_float(x[e + 1]), fd, -d.y * up);
-          p[e + 2] = p[e + 2] * kDownP * fmaf(__uint_as_float(x[e + 2]), fd, -d.z * up);
-          p[e + 3] = p[e + 3] * kDownP * fmaf(__uint_as_float(x[e + 3]), fd, -d.w * up);
+          p[e] *= fmaf(__uint_as_float(x[e]), fd, -d.x);
+          p[e + 1] *= fmaf(__uint_as_float(x[e + 1]), fd, -d.y);
+          p[e + 2] *= fmaf(__uint_as_float(x[e + 2]), fd, -d.z);
+          p[e + 3] *= fmaf(__uint_as_float(x[e + 3]), fd, -d.w);
         }
+        const int eds = scale_of_ds(p, ctl.top, j, row, quarter, warp);
+        const float up = pow2(eds);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] *= up;
+        back_k = factors(a.scale, -eds - (int)kUpP - eg - eq);
         store_operand<16>(tm_dp + off, p);
         tmem_wait_st();
         arrive_warp(&ctl.ds_full);
         if (j == n - 1 || ((t0 + j) & 1)) take_dv();
       }
-      take_dk();
+      take_dk(n - 1);
     }
     if (key < a.kv_len) {
       store_features<S::kF>(a.dk + at(a.dks, b, key, hk), quarter * S::kF, a.dim, vec_out, dk);
@@ -1068,7 +1098,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_backward(const __grid_cons
 // ---------------------------------------------------------------------------
 struct Layout {
   int64_t heads, row_tiles, key_tiles, blocks;
-  size_t stats, tile[4], info[4], lse2, delta, part, total;
+  size_t stats, tile[4], info[4], lse2, delta, plain, part, total;
   int splits;
   Layout(const AttnArgs& a, bool backward) {
     heads = (int64_t)a.batch * a.kv_heads;
@@ -1088,10 +1118,11 @@ struct Layout {
       tile[t] = take(tiles * blocks * kBlockBytes);
       info[t] = take(tiles * sizeof(AttnTile));
     }
-    lse2 = delta = part = 0;
+    lse2 = delta = plain = part = 0;
     if (backward) {
       lse2 = take(sizeof(float) * heads * row_tiles * kTile);
       delta = take(sizeof(float) * heads * row_tiles * kTile);
+      plain = take(sizeof(float) * heads * row_tiles * kTile);
     } else {
       part = take(std::max(attn_rows_ws_bytes(a),
                            splits > 1 ? sizeof(float) * heads * a.group * a.q_len * splits * (size_t)(a.dim + 2) : 0));
@@ -1194,11 +1225,11 @@ cudaError_t launch_attn_tensor_backward(const AttnArgs& args, void* ws, cudaStre
   AttnArgs a = args;
   const Layout L(a, true);
   Tiles t;
+  a.delta = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + L.plain);
   cudaError_t e = prepare(a, L, static_cast<uint8_t*>(ws), true, t, st);
   if (e != cudaSuccess) return e;
   a.stats = t.stats;
   a.any = t.any;
-  a.delta = t.delta;
   const auto run = L.blocks == 1 ? (a.dim == 64 ? backward<1, true> : backward<1, false>)
                                  : (a.dim == 128 ? backward<2, true> : backward<2, false>);
   e = run(a, L, t, st);

@@ -25,3 +25,34 @@ def test_attention_gradients_of_small_and_large_operands(dev, t, d, sizes):
     v *= np.float32(2.0 ** sizes[1])
     go *= np.float32(2.0 ** sizes[2])
     _both(dev, q, k, v, go)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("size", [1.0, 1e-6, 1e6])
+@pytest.mark.parametrize("tile", [2.0 ** -10, 2.0 ** -20, 2.0 ** -40, 0.0])
+@pytest.mark.parametrize("t,d", [(512, 64), (400, 128)])
+def test_attention_gradients_where_a_run_of_values_is_small(dev, t, d, tile, size, causal):
+    """128 keys whose v is small or 0: their dS is delta's, which the other keys' v make."""
+    q, k, v, go = _inputs(1, t, t, 2, 1, d)
+    v[:, 128:256] *= np.float32(tile)
+    go *= np.float32(size)
+    _both(dev, q, k, v, go, causal=causal)
+
+
+@pytest.mark.parametrize("spread", [8, 13])
+def test_attention_gradients_where_douts_rows_are_apart(dev, spread):
+    """Rows of dout up to 2^spread apart, and last ones (which alone see the last keys) all small."""
+    q, k, v, go = _inputs(1, 2048, 2048, 1, 1, 64)
+    r = np.random.default_rng(6)
+    go *= np.exp2(-r.integers(0, spread + 1, go.shape[:3] + (1,))).astype(np.float32)
+    _both(dev, q, k, v, go)
+    go[:, -40:] *= np.float32(2.0 ** -spread) / np.abs(go[:, -40:]).max(-1, keepdims=True)
+    _both(dev, q, k, v, go, causal=True)
+
+
+@pytest.mark.parametrize("spread", [8, 13])
+def test_attention_gradients_where_values_rows_are_apart(dev, spread):
+    q, k, v, go = _inputs(1, 1500, 1500, 1, 1, 128)
+    r = np.random.default_rng(7)
+    v *= np.exp2(-r.integers(0, spread + 1, v.shape[:3] + (1,))).astype(np.float32)
+    _both(dev, q, k, v, go)
