@@ -617,10 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_forward(const __grid_const
 // Two kinds of blocks that each form the scores and dP = dout V^T again, for dq (a tile of rows
 // against its keys) and for dk and dv (a tile of keys against the rows that see them): seven
 // products instead of five, but every gradient has one owner, no atomics and one order.
-constexpr float kUpP = 14.f;                       // P <= 1 is held as 2^14 P
-
-// The accumulators are drained whenever the scales that they carry change: dv after every
-// tile of the inner side, dq and dk after every half tile.
+// The accumulators carry scales of their half tile, so they are drained after each.
 template <int N>
 DCT_DEV void drain(uint32_t addr, float f, float (&acc)[N]) {
 #pragma unroll
@@ -644,23 +641,36 @@ DCT_DEV void drain(uint32_t addr, float2 f, float (&acc)[N]) {
   }
 }
 
+// The largest of four numbers of [0, 255], one of each thread of a row.  (`top` may be written
+// again when all have passed another meeting.)
+DCT_DEV int meet(uint32_t mine, uint8_t (&top)[kTile][4], int row, int quarter, int warp) {
+  top[row][quarter] = (uint8_t)mine;
+  rows_sync(warp);
+  const uint32_t x = *reinterpret_cast<const uint32_t*>(top[row]);
+  return (int)max(max(x & 255, x >> 8 & 255), max(x >> 16 & 255, x >> 24));
+}
 // dS = P (dP - delta) can be anything up to the sizes of dout and the largest v of the whole
 // row, and is small where P is or where another row of the tile has the large dout.  So it is
 // scaled by what it is: for each row of the product that takes it (a query in dq, a key in dk)
 // the largest |dS| of the half tile comes to [2^14, 2^15), and the row's accumulator is drained
 // with the reverse of that after every half tile.  (Bounds from the tiles' norms instead lost
 // the accuracy of rows far below the bound, and passed float16 where delta came from
-// other tiles' v.)  The four threads of a row meet here: returns the exponent for theirs.
+// other tiles' v.)  Returns the exponent.
 template <int N>
-DCT_DEV int scale_of_ds(const float (&ds)[N], uint8_t (&top)[2][kTile][4], int j, int row, int quarter, int warp) {
+DCT_DEV int scale_of_ds(const float (&ds)[N], uint8_t (&top)[kTile][4], int row, int quarter, int warp) {
   uint32_t m = 0;
 #pragma unroll
   for (int e = 0; e < N; ++e) m = max(m, __float_as_uint(ds[e]) & 0x7fffffffu);
-  top[j & 1][row][quarter] = (uint8_t)(m >> 23);      // the exponent: order enough
-  rows_sync(warp);               // (the other half of `top` is in use until all have passed this)
-  const uint32_t x = *reinterpret_cast<const uint32_t*>(top[j & 1][row]);
-  const uint32_t y = max(max(x & 255, x >> 8 & 255), max(x >> 16 & 255, x >> 24));
-  return min(14 + 127 - (int)y, 120);
+  return min(14 + 127 - meet(m >> 23, top, row, quarter, warp), 120);     // exponents: order enough
+}
+// P = 2^y of a key's rows likewise: a key that no row gives much weight has a dv as small, with
+// as many bits.  (Down to weights of 2^-36; smaller ones keep steps of 2^-75.)
+template <int N>
+DCT_DEV int scale_of_p(const float (&y)[N], uint8_t (&top)[kTile][4], int row, int quarter, int warp) {
+  float m = y[0];
+#pragma unroll
+  for (int e = 1; e < N; ++e) m = fmaxf(m, y[e]);
+  return 14 + 50 - meet(__float2int_rd(fminf(fmaxf(m, -36.f), 100.f)) + 50, top, row, quarter, warp);
 }
 // f 2^e as two factors, neither of which leaves float32 where their product with an
 // accumulator does not
@@ -828,7 +838,7 @@ DCT_DEV void attn_dq(const AttnArgs& a, const Tiles& w, int block, int row_tiles
           for (int e = 0; e < 16; ++e)
             if (key + e < lo || key + e >= hi) ds[e] = 0.f;
         }
-        const int eds = scale_of_ds(ds, ctl.top, j, row, quarter, warp);
+        const int eds = scale_of_ds(ds, ctl.top[j & 1], row, quarter, warp);
         const float up = pow2(eds);
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[e] *= up;
@@ -956,15 +966,13 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
         };
         scores(0);
         dps(0);
-        int group = 0;
         for (int j = 0; j < n && wait.ok; ++j) {
-          const bool first = j == 0 || !((t0 + j) & 1), last = j == n - 1 || ((t0 + j) & 1);   // of its tile
           wait(&ctl.p_full, j);
-          if (first) wait(&ctl.dv_empty, group++ ^ 1);
+          wait(&ctl.dv_empty, j ^ 1);
           if (!wait.ok) break;
-          mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(grad(j), 2 * kChunkBytes, 1024), !first, steps);
+          mma_rows<BLOCKS, 16>(tm_dv, tm_s, umma_desc(grad(j), 2 * kChunkBytes, 1024), false, steps);
           ctl.go.release(j);
-          if (last) umma_commit(&ctl.dv_full);
+          umma_commit(&ctl.dv_full);
           if (j + 1 < n) scores(j + 1);
           wait(&ctl.ds_full, j);
           wait(&ctl.dk_empty, j ^ 1);
@@ -991,18 +999,11 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
       tile_to_tmem<BLOCKS>(w.p[2] + (bh * w.tiles[2] + tile) * (int64_t)S::kTileBytes, tm_v, warp, row);
       tmem_wait_st();
       arrive_warp(&ctl.v_full);
-      // dv of a tile of rows is drained at the end of it, dk of a half tile after the next one's
-      // first P, when their last products are done and no matrix instruction yet waits for the
-      // accumulator.
+      // dv of a half tile is drained at the end of it, dk after the next one's P, when their
+      // products are done and no matrix instruction yet waits for the accumulator.
       const float fd = pow2(-ev);
-      float f = 0.f, back_v = 0.f;
+      float f = 0.f;
       float2 back_k = {};
-      int group = 0;
-      auto take_dv = [&]() {
-        wait(&ctl.dv_full, group++);
-        drain(tm_dv + lane_bits(warp) + quarter * S::kF, back_v, dv);
-        arrive_warp(&ctl.dv_empty);
-      };
       auto take_dk = [&](int j) {
         wait(&ctl.dk_full, j);
         drain(tm_dk + lane_bits(warp) + quarter * S::kF, back_k, dk);
@@ -1017,7 +1018,6 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
           eq = qt.e;
           f = a.scale * kLog2e * pow2(-eq - ek);
           eg = gt.e;
-          back_v = pow2(-(int)kUpP - eg);
           const int next = ((t0 + j) >> 1) + 1;
           if (next <= (t0 + n - 1) >> 1) {
             qt = qi[next];
@@ -1035,16 +1035,19 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const float4 l = lse[e / 4];
-          p[e] = ex2(fmaf(__uint_as_float(x[e]), f, kUpP - l.x));
-          p[e + 1] = ex2(fmaf(__uint_as_float(x[e + 1]), f, kUpP - l.y));
-          p[e + 2] = ex2(fmaf(__uint_as_float(x[e + 2]), f, kUpP - l.z));
-          p[e + 3] = ex2(fmaf(__uint_as_float(x[e + 3]), f, kUpP - l.w));
+          p[e] = fmaf(__uint_as_float(x[e]), f, -l.x);
+          p[e + 1] = fmaf(__uint_as_float(x[e + 1]), f, -l.y);
+          p[e + 2] = fmaf(__uint_as_float(x[e + 2]), f, -l.z);
+          p[e + 3] = fmaf(__uint_as_float(x[e + 3]), f, -l.w);
         }
         if (__any_sync(0xffffffffu, r < lo || r + 16 > hi)) {
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (r + e < lo || r + e >= hi) p[e] = 0.f;
+            if (r + e < lo || r + e >= hi) p[e] = -INFINITY;
         }
+        const int ep = scale_of_p(p, ctl.top[0], row, quarter, warp);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] = ex2(p[e] + (float)ep);
         store_operand<16>(tm_s + off, p);
         tmem_wait_st();
         arrive_warp(&ctl.p_full);
@@ -1060,15 +1063,17 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
           p[e + 2] *= fmaf(__uint_as_float(x[e + 2]), fd, -d.z);
           p[e + 3] *= fmaf(__uint_as_float(x[e + 3]), fd, -d.w);
         }
-        const int eds = scale_of_ds(p, ctl.top, j, row, quarter, warp);
+        const int eds = scale_of_ds(p, ctl.top[1], row, quarter, warp);
         const float up = pow2(eds);
 #pragma unroll
         for (int e = 0; e < 16; ++e) p[e] *= up;
-        back_k = factors(a.scale, -eds - (int)kUpP - eg - eq);
+        back_k = factors(a.scale, -eds - ep - eg - eq);
         store_operand<16>(tm_dp + off, p);
         tmem_wait_st();
         arrive_warp(&ctl.ds_full);
-        if (j == n - 1 || ((t0 + j) & 1)) take_dv();
+        wait(&ctl.dv_full, j);
+        drain(tm_dv + lane_bits(warp) + quarter * S::kF, pow2(-ep - eg), dv);
+        arrive_warp(&ctl.dv_empty);
       }
       take_dk(n - 1);
     }

@@ -56,3 +56,21 @@ def test_attention_gradients_where_values_rows_are_apart(dev, spread):
     r = np.random.default_rng(7)
     v *= np.exp2(-r.integers(0, spread + 1, v.shape[:3] + (1,))).astype(np.float32)
     _both(dev, q, k, v, go)
+
+
+def _sink(t, n, h, d, above, small):
+    """The first key's score lies `above` over the others' mean, its value 2^-small of theirs."""
+    q, k, v, go = _inputs(1, t, n, h, 1, d)
+    k[..., 0] = 0
+    k[:, 0] = 0
+    k[:, 0, :, 0] = 40
+    q[..., 0] = above * np.sqrt(d) / 40
+    v[:, 0] *= np.float32(2.0 ** -small)
+    return q, k, v, go
+
+
+@pytest.mark.parametrize("above", [16, 20])
+@pytest.mark.parametrize("t,n,h,d", [(16, 300, 2, 64), (160, 2000, 2, 128), (700, 700, 4, 64)])
+def test_attention_gradients_of_keys_of_little_weight(dev, t, n, h, d, above):
+    """Weights of 2^-24 to 2^-34 for all keys but one: their dv is as small, with as many bits."""
+    _both(dev, *_sink(t, n, h, d, above, 0), names=("dk", "dv"))
