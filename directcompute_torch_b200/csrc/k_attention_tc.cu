@@ -376,8 +376,10 @@ DCT_DEV bool misaligned(const uint8_t* sm, uint32_t* err) {
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
-// P is held as 2^7 P: a weight is at most 1, and hi + lo reach 2^-32 of it
-constexpr float kUp = 7.f;
+// P is held as 2^15 P: a weight is at most 1 (and what a score's rounding adds: 2^0.02 at 2^18),
+// and hi + lo reach 2^-40 of its row's largest one so far.  That is a choice: a row whose result
+// is made of weights below 2^-17 of its largest has them in fewer bits than float32.
+constexpr float kUp = 15.f;
 
 template <int BLOCKS>
 struct Forward : Sizes<BLOCKS> {

@@ -74,3 +74,23 @@ def _sink(t, n, h, d, above, small):
 def test_attention_gradients_of_keys_of_little_weight(dev, t, n, h, d, above):
     """Weights of 2^-24 to 2^-34 for all keys but one: their dv is as small, with as many bits."""
     _both(dev, *_sink(t, n, h, d, above, 0), names=("dk", "dv"))
+
+
+@pytest.mark.parametrize("above,small", [(16, 6), (20, 10)])
+@pytest.mark.parametrize("t,n,h,d", [(16, 300, 2, 64), (160, 2000, 2, 128), (2048, 4096, 8, 64)])
+def test_attention_where_one_key_takes_most(dev, t, n, h, d, above, small):
+    """Results that are made of the small weights, which the first key's small value leaves over."""
+    _both(dev, *_sink(t, n, h, d, above, small), names=("out", "dq", "dk", "dv"))
+
+
+def test_attention_of_scores_near_the_limit(dev):
+    """Scores up to 2^18 of either sign: what their rounding adds to a weight stays in float16, and
+    results stay between the values."""
+    q, k, v, go = _inputs(1, 300, 700, 2, 1, 64)
+    q = np.float32(0.9 * 2.0 ** 8) * (1 + np.float32(0.01) * np.clip(q, -4, 4))
+    k = np.float32(2.0 ** 7) * (1 + np.float32(0.01) * np.clip(k, -4, 4))
+    k[:, ::2] *= -1
+    for scale in (None, -0.125):
+        got = _attention(dev, q, k, v, go, scale=scale)
+        assert all(np.isfinite(got[x]).all() for x in got)
+        assert np.abs(got["out"]).max() <= 1.00001 * np.abs(v).max()
