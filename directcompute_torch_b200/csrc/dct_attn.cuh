@@ -60,11 +60,13 @@ struct AttnStats {
   uint32_t pad[3];
 };
 // Tiles of infinities or NaN, of sizes whose scaling could leave float32, or with rows so far
-// apart that the small ones would lose their own accuracy to the common scale, cannot be
-// split.  `low` is the smallest row maximum that is not 0.
+// apart that the small ones would lose their own accuracy to the common scale (2^-14 of it
+// leaves 26 bits), cannot be split.  `low` is the smallest row maximum that is not 0.  Neither
+// can those whose features are as far apart, where they make a result's features.
+constexpr int kApart = 14;
 DCT_DEV bool tile_splits(uint32_t top, uint32_t low) {
   const int t = (int)(top >> 23) - 127, l = (int)(low >> 23) - 127;
-  return top == 0 || (t >= -60 && t <= 44 && l >= t - 14);
+  return top == 0 || (t >= -60 && t <= 44 && l >= t - kApart);
 }
 // Whether a head takes the tensor cores: scores beyond 2^18 would amplify a tile's 2^-40 past
 // float32's own error; tiles of v further than 2^60 apart could overflow the running outputs,

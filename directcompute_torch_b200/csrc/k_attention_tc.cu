@@ -78,10 +78,11 @@ DCT_DEV void store_features(float* row, int first, int dim, bool vec, const floa
 // once.  With dout come delta = sum dout out and the log-sums.  Bound by memory: 8 bytes a
 // feature (12 for dout).
 template <int BLOCKS>
-__global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ AttnArgs a, const __grid_constant__ Tiles w,
+__global__ void __launch_bounds__(512, BLOCKS == 1 ? 3 : 2) k_attn_split(const __grid_constant__ AttnArgs a, const __grid_constant__ Tiles w,
                                                     int tq, int tk, bool vec) {
   constexpr int kGroups = 8 * BLOCKS, kStep = 512 / kGroups, kPasses = kTile / kStep;
   __shared__ uint32_t sh[2];
+  __shared__ uint2 sizes[16][kGroups];             // exponents of 8 features' largest |x|, a warp's rows
   touch(a);
   touch(w);
   pdl_entry();
@@ -97,6 +98,8 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
   const AttnSpan span(a, b);
   const int rows = rows_of(a, span, t);
   if (tile * kTile >= rows && t != 3) return;      // nothing reads it (dout's log-sums are read by whole tiles)
+  // operands whose features are a result's: v in out, q in dk, k in dq, dout in dv
+  const bool by_feature = a.dout ? t != 2 : t == 2;
   if (threadIdx.x < 2) sh[threadIdx.x] = 0;
   __syncthreads();
   float v[kPasses][8], delta[kPasses];
@@ -153,9 +156,26 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
       }
     }
   }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (by_feature) {
+    uint32_t c[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) m = max(m, __float_as_uint(v[p][e]) & 0x7fffffffu);
+      c[e >> 2] |= max(m >> 23, min(m, 1u)) << 8 * (e & 3);                // 0: nothing but zeros
+    }
+#pragma unroll
+    for (int o = kGroups; o < 32; o <<= 1) {
+      c[0] = __vmaxu4(c[0], __shfl_xor_sync(0xffffffffu, c[0], o));
+      c[1] = __vmaxu4(c[1], __shfl_xor_sync(0xffffffffu, c[1], o));
+    }
+    if (lane < kGroups) sizes[warp][lane] = make_uint2(c[0], c[1]);
+  }
   top = __reduce_max_sync(0xffffffffu, top);
   low = __reduce_max_sync(0xffffffffu, low);
-  if ((threadIdx.x & 31) == 0) {
+  if (lane == 0) {
     atomicMax(&sh[0], top);
     atomicMax(&sh[1], low);
   }
@@ -172,6 +192,14 @@ __global__ void __launch_bounds__(512) k_attn_split(const __grid_constant__ Attn
       atomicMax(&w.stats[bh].low_v, ~top);
     }
     if (!splits) w.stats[bh].bad = 1;
+  }
+  if (by_feature && warp == 1 && lane < 2 * kGroups) {     // 4 features a lane
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c = __vmaxu4(c, lane & 1 ? sizes[i][lane >> 1].y : sizes[i][lane >> 1].x);
+#pragma unroll
+    for (int e = 0; e < 32; e += 8)
+      if ((c >> e & 255) && (c >> e & 255) + kApart < top >> 23) w.stats[bh].bad = 1;
   }
   if (!splits) return;
   const float f = pow2(e);

@@ -94,3 +94,18 @@ def test_attention_of_scores_near_the_limit(dev):
         got = _attention(dev, q, k, v, go, scale=scale)
         assert all(np.isfinite(got[x]).all() for x in got)
         assert np.abs(got["out"]).max() <= 1.00001 * np.abs(v).max()
+
+
+@pytest.mark.parametrize("apart", [10, 20, 26])
+@pytest.mark.parametrize("t,d", [(512, 64), (384, 80)])
+def test_attention_where_features_are_apart(dev, t, d, apart):
+    """Features of an operand 2^apart below its others: they keep the accuracy of their own size."""
+    small = np.array([1, 17, d - 1])
+    for which in range(4):
+        x = list(_inputs(1, t, t, 2, 1, d))
+        x[which][..., small] *= np.float32(2.0 ** -apart)
+        got = _attention(dev, *x)
+        hold(got, *x)
+        name = ("dk", "dq", "out", "dv")[which]             # the result whose features are the operand's
+        pick = {y: got[y][..., small] if y == name else got[y] for y in got}
+        hold(pick, *x, names=(name,), features={name: small})
