@@ -31,7 +31,7 @@ struct AttnSpan {
   }
   DCT_DEV int last(const AttnArgs& a, int j) const {
     if (j >= n) return 0;
-    return a.window ? min(m, j - (n - m) + a.window) : m;
+    return a.window ? max(0, min(m, j - (n - m) + a.window)) : m;     // not negative: rows are `group` times as many
   }
 };
 

@@ -691,3 +691,19 @@ def test_attention_refuses_too_many_heads_without_positions(dev):
     finally:
         dev.free(*h)
         dev.clear_error()
+
+
+@pytest.mark.parametrize("rows", [False, True])
+def test_attention_window_over_a_long_cache_of_many_query_heads(dev, rows):
+    """Keys times query heads of a key head past 2^31: the rows that see an early key are none, as
+    32-bit numbers too.  rows: a head that float16 pairs cannot hold."""
+    n, h, d, w, near = 600_000, 4096, 4, 100, 200
+    q, k, v, go = _inputs(1, 1, near, h, 1, d)
+    if rows:
+        k[0, -1] *= np.float32(2.0 ** -30)
+    far_k, far_v = (np.concatenate((np.ones((1, n - near, 1, d), np.float32), x), 1) for x in (k, v))
+    kw = {"causal": True, "window": w}
+    got = _attention(dev, q, far_k, far_v, go, **kw)
+    assert not got["dk"][:, :n - near].any() and not got["dv"][:, :n - near].any()
+    got["dk"], got["dv"] = got["dk"][:, n - near:], got["dv"][:, n - near:]
+    _hold(got, T.attention(q, k, v, go, **kw), ALL)
