@@ -891,6 +891,15 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const __grid_const
   if (warp == 0) tmem_free(tmem, 512);
 }
 
+// One block an SM, whatever it needs: each takes all 512 columns of tensor memory, and two
+// clusters that share SMs could each hold the columns that the other waits for.
+constexpr size_t kSmShared = 228 * 1024;          // of an SM
+constexpr size_t small_smem(int chunks) {
+  const size_t need = (size_t)(chunks + 2) * 4 * kChunkBytes, alone = kSmShared / 2 + 1024;
+  return need > alone ? need : alone;
+}
+static_assert(2 * small_smem(1) > kSmShared && small_smem(kMostChunks) <= 227 * 1024);
+
 // Blocks of a matrix's cluster, or 0 where the general way takes it.  A chunk costs a block
 // about 2300 cycles a step, the meeting of several blocks' sums 6800.
 int small_blocks(const MuonArgs& a) {
@@ -1049,9 +1058,9 @@ cudaError_t launch_small(const MuonArgs& a, int blocks, void* ws, cudaStream_t s
   g.next_x = (float)a.a;
   g.last_p = pow2(-w.x - w.p);
   g.last_x = (float)(a.a * pow2(-w.x));
-  const size_t smem = (size_t)(g.chunks + 2) * 4 * kChunkBytes;
+  const size_t smem = small_smem(g.chunks);
   static const cudaError_t set = cudaFuncSetAttribute(k_muon_small, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                      (kMostChunks + 2) * 4 * kChunkBytes);
+                                                      (int)small_smem(kMostChunks));
   if (set != cudaSuccess) return set;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];

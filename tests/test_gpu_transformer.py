@@ -707,3 +707,19 @@ def test_attention_window_over_a_long_cache_of_many_query_heads(dev, rows):
     assert not got["dk"][:, :n - near].any() and not got["dv"][:, :n - near].any()
     got["dk"], got["dv"] = got["dk"][:, n - near:], got["dv"][:, n - near:]
     _hold(got, T.attention(q, k, v, go, **kw), ALL)
+
+
+def test_orthogonalize_many_short_matrices(dev):
+    """More clusters of one and two chunks a block than there are SMs, which no two may share."""
+    r = np.random.default_rng(2)
+    for shape in ((400, 16, 60), (300, 90, 100), (160, 40, 500)):
+        x = r.normal(size=shape).astype(np.float32)
+        h, y = dev.buf(x), dev.empty(x.size)
+        try:
+            _abi.check(dev.lib, dev.lib.dct_orthogonalize(ctypes.byref(_muon(shape, steps=2)), h, y))
+            got = dev.read(y).reshape(shape)
+        finally:
+            dev.free(h, y)
+        for i in range(0, len(x), 37):
+            want, err = T.orthogonalize(x[i], steps=2)
+            assert np.linalg.norm(got[i] - want) <= err
