@@ -916,10 +916,14 @@ int small_blocks(const MuonArgs& a) {
   return best;
 }
 
+// Scratch of one launch's matrices.  A thin matrix is padded to 64 on its short side, up to 128
+// times its data with both copies of X, so a batch goes in groups that stay below this.
+constexpr uint64_t kMostScratch = 2ull << 30;
+
 struct Layout {
   uint32_t rb, cb, sb;              // chunks of rows, columns, the shorter side
   uint64_t x, s;                    // bytes of X's and of a Gram matrix's chunks
-  size_t x0, x1, gram, poly, part, cut, arrived, total;
+  size_t x0 = 0, x1 = 0, gram = 0, poly = 0, part, cut = 0, arrived, total;
   explicit Layout(const MuonArgs& a) {
     rb = (a.rows + 63) / 64;
     cb = (a.cols + 63) / 64;
@@ -928,14 +932,22 @@ struct Layout {
     s = (uint64_t)sb * sb * kPairBytes;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 1023) & ~size_t(1023); return o; };
-    x0 = take(x * a.batch);
-    x1 = take(x * a.batch);
-    gram = take(s * a.batch);
-    poly = take(s * a.batch);
     part = take(8 * kMostParts * (size_t)a.batch);
-    cut = take(2ull * dev_info().sm_count * kRows * 256 * sizeof(float));
     arrived = take(sizeof(uint32_t) * dev_info().sm_count);
+    if (a.steps) {                  // without, the direction is only scaled
+      x0 = take(x * a.batch);
+      x1 = take(x * a.batch);
+      gram = take(s * a.batch);
+      poly = take(s * a.batch);
+      cut = take(2ull * dev_info().sm_count * kRows * 256 * sizeof(float));
+    }
     total = at;
+  }
+  static uint64_t a_matrix(const MuonArgs& a) {
+    MuonArgs one = a;
+    one.batch = 1;
+    const Layout l(one);
+    return 8 * kMostParts + (a.steps ? 2 * (l.x + l.s) : 0);
   }
 };
 
@@ -1034,11 +1046,14 @@ struct Powers {
   }
 };
 
-}  // namespace
-
-size_t muon_ws_bytes(const MuonArgs& a) {
-  if (const int n = small_blocks(a)) return n > 1 ? (size_t)a.batch * n * 16384 * sizeof(float) : 0;
-  return Layout(a).total;
+// The matrices of a launch: all, or as many as the scratch allows, in groups of (almost) one size.
+uint32_t group_of(const MuonArgs& a) {
+  const int n = small_blocks(a);
+  const uint64_t one = n ? (n > 1 ? n * 16384 * sizeof(float) : 0) : Layout::a_matrix(a);
+  const uint64_t most = one ? std::max<uint64_t>(1, kMostScratch / one) : a.batch;
+  if (a.batch <= most) return a.batch;
+  const uint32_t groups = (uint32_t)((a.batch + most - 1) / most);
+  return (a.batch + groups - 1) / groups;
 }
 
 cudaError_t launch_small(const MuonArgs& a, int blocks, void* ws, cudaStream_t st) {
@@ -1076,8 +1091,7 @@ cudaError_t launch_small(const MuonArgs& a, int blocks, void* ws, cudaStream_t s
   return cudaLaunchKernelEx(&cfg, k_muon_small, g, device_error_word());
 }
 
-cudaError_t launch_muon(const MuonArgs& a, void* ws, cudaStream_t st) {
-  if (!a.rows || !a.cols || !a.batch) return cudaSuccess;
+cudaError_t launch_group(const MuonArgs& a, void* ws, cudaStream_t st) {
   if (const int n = small_blocks(a)) return launch_small(a, n, ws, st);
   const Layout L(a);
   uint8_t* w = static_cast<uint8_t*>(ws);
@@ -1143,6 +1157,32 @@ cudaError_t launch_muon(const MuonArgs& a, void* ws, cudaStream_t st) {
     }
     e = product(tile, q, a.batch, st);
     std::swap(x, y);
+  }
+  return e;
+}
+
+}  // namespace
+
+size_t muon_ws_bytes(const MuonArgs& a) {
+  if (!a.rows || !a.cols || !a.batch) return 0;
+  MuonArgs g = a;
+  g.batch = group_of(a);
+  if (const int n = small_blocks(g)) return n > 1 ? (size_t)g.batch * n * 16384 * sizeof(float) : 0;
+  return Layout(g).total;
+}
+
+cudaError_t launch_muon(const MuonArgs& a, void* ws, cudaStream_t st) {
+  if (!a.rows || !a.cols || !a.batch) return cudaSuccess;
+  const uint32_t most = group_of(a);
+  cudaError_t e = cudaSuccess;
+  for (uint32_t z = 0; z < a.batch && e == cudaSuccess; z += most) {
+    MuonArgs g = a;
+    const uint64_t at = (uint64_t)z * a.rows * a.cols;
+    g.batch = std::min(most, a.batch - z);
+    g.g += at;
+    if (a.update) { g.w += at; g.m += at; }
+    else g.y += at;
+    e = launch_group(g, ws, st);
   }
   return e;
 }

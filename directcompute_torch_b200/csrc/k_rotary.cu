@@ -162,7 +162,7 @@ cudaError_t launch_rotary(const RotaryArgs& a, const RotaryTurns& f, cudaStream_
   const uint32_t width = a.heads * a.head_dim;
   g.per_block = width >= 4096 ? 1 : 4096 / width;
   if (g.per_block > g.tokens) g.per_block = g.tokens;
-  // a table of at most 32 KB (one feature-wide heads aside, 4096 features hold at most 2048 pairs)
+  // a table of at most 16 KB: 4096 features hold at most 2048 pairs, a wider token's heads at most 128
   g.by_length = FastDiv(g.length); g.by_units = FastDiv(g.units); g.by_heads = FastDiv(g.heads);
   const uint32_t blocks = (g.tokens + g.per_block - 1) / g.per_block;
   const size_t smem = sizeof(float2) * g.per_block * g.half;

@@ -360,7 +360,10 @@ DCT_API int dct_attention_backward(const DctAttention* p, void* q, void* k, void
  * (on the shorter side; X^T X for tall matrices), which moves the singular values
  * toward 1.  a = b = c = 0 means 3.4445, -4.7750, 2.0315; steps 0..16; the polynomial
  * a s + b s^3 + c s^5 must keep [0, 1] below 64 over the steps (DCT_ERR_ARG).
- * y may be x.  batch <= 65535, rows and cols <= 2^23, rows cols < 2^30. */
+ * y may be x.  batch <= 65535, rows and cols <= 2^23, rows cols < 2^30.  Scratch: 8 bytes for
+ * each element of a matrix padded to multiples of 64 rows and columns, and for each of the
+ * shorter side's square, with a batch in groups of at most 2 GB (or one matrix); less than 1 MB
+ * a matrix where the shorter side is 128 or less and the longer 2560. */
 typedef struct DctMuon {
   uint32_t batch, rows, cols, steps;
   double a, b, c;

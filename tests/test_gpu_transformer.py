@@ -723,3 +723,47 @@ def test_orthogonalize_many_short_matrices(dev):
         for i in range(0, len(x), 37):
             want, err = T.orthogonalize(x[i], steps=2)
             assert np.linalg.norm(got[i] - want) <= err
+
+
+@pytest.mark.parametrize("shape,update", [((4000, 4, 2600), False), ((4000, 2600, 4), True), ((11000, 2, 2500), False),
+                                          ((11000, 2500, 2), True)], ids=str)
+def test_orthogonalize_of_a_batch_in_groups(dev, shape, update):
+    """Thin matrices whose scratch would be far more than their data: a bounded part of it, in turn."""
+    import torch
+    r = np.random.default_rng(8)
+    x = r.normal(size=shape).astype(np.float32)
+    w = r.normal(size=shape).astype(np.float32)
+    hs = [dev.buf(x), dev.buf(w), dev.buf(np.zeros(shape, np.float32))]
+    before = torch.cuda.mem_get_info()[0]
+    try:
+        p = _muon(shape, steps=2, lr=0.5, momentum=0.9, scale=1.0)
+        if update:
+            _abi.check(dev.lib, dev.lib.dct_muon(ctypes.byref(p), hs[1], hs[2], hs[0]))
+        else:
+            _abi.check(dev.lib, dev.lib.dct_orthogonalize(ctypes.byref(p), hs[0], hs[1]))
+        got, m = dev.read(hs[1]).reshape(shape), dev.read(hs[2]).reshape(shape)
+        assert before - torch.cuda.mem_get_info()[0] < 5 << 30
+    finally:
+        dev.free(*hs)
+    for i in (0, 1, len(x) // 2 - 1, len(x) // 2, len(x) // 2 + 1, len(x) - 1):
+        want, err = T.orthogonalize(x[i], steps=2)
+        if update:
+            assert np.array_equal(m[i], x[i])
+            want, err = w[i] - 0.5 * want, 0.5 * err + T.U * 2 * (np.linalg.norm(w[i]) + np.linalg.norm(want))
+        assert np.linalg.norm(got[i] - want) <= err
+
+
+def test_scaling_alone_takes_no_scratch_of_its_steps(dev):
+    """Without steps a thin matrix is only divided by its norm."""
+    import torch
+    shape = (2, 1, 1 << 23)
+    x = np.ones(shape, np.float32)
+    hs = [dev.buf(x), dev.empty(x.size)]
+    before = torch.cuda.mem_get_info()[0]
+    try:
+        _abi.check(dev.lib, dev.lib.dct_orthogonalize(ctypes.byref(_muon(shape, steps=0)), *hs))
+        got = dev.read(hs[1])
+        assert before - torch.cuda.mem_get_info()[0] < 1 << 30
+    finally:
+        dev.free(*hs)
+    assert np.abs(got * np.sqrt(1 << 23) - 1).max() <= 4 * T.U
