@@ -623,6 +623,13 @@ def rotary(x, positions=None, start=0, rotated=None, interleaved=False, base=100
                                 high=high, magnitude=magnitude)
 
 
+class _LogSums(Node):
+    """Behind attention's log-sums: a gradient that reaches them would be lost without a word."""
+
+    def backward(self, g):
+        raise NotImplementedError("attention: the log-sums have no gradient; use their values (ops.to_numpy) instead")
+
+
 class AttentionFunc(Node):
     """softmax(scale q k^T + mask) v; the backward recomputes the probabilities from the
     saved log-sums."""
@@ -648,10 +655,11 @@ class AttentionFunc(Node):
         if rc:
             _release(oh, lh)
         check(lib, rc, "dct_attention_forward")
-        self.lse = _wrap(lh, (b, h, t))
+        grad = q.requires_grad or k.requires_grad or v.requires_grad
+        self.lse = _wrap(lh, (b, h, t), _LogSums(q, k, v) if grad else None, grad)
         lib.AddRefBuffer(oh)                  # the buffer, not the tensor: that would be a cycle
         self.out = oh
-        return _wrap(oh, q.shape, self, q.requires_grad or k.requires_grad or v.requires_grad)
+        return _wrap(oh, q.shape, self, grad)
 
     def backward(self, g):
         q, k, v = self.inputs
@@ -684,7 +692,8 @@ def attention(q, k, v, causal=False, window=0, scale=None, q_lens=None, kv_lens=
     causal: a query sees the keys up to its own position, the last query standing at the
     last key.  window > 0: only the nearest `window` positions.  scale: default
     1/sqrt(features).  q_lens, kv_lens: valid positions of each batch entry.  A query that
-    sees nothing gets 0 (and log-sum -inf)."""
+    sees nothing gets 0 (and log-sum -inf).  return_lse: (result, log-sums [batch, head, position]);
+    a backward pass through the log-sums raises NotImplementedError."""
     f = AttentionFunc()
     out = f.forward(q, k, v, causal, window, scale, q_lens, kv_lens)
     return (out, f.lse) if return_lse else out

@@ -767,3 +767,22 @@ def test_scaling_alone_takes_no_scratch_of_its_steps(dev):
     finally:
         dev.free(*hs)
     assert np.abs(got * np.sqrt(1 << 23) - 1).max() <= 4 * T.U
+
+
+def test_a_gradient_of_the_log_sums_is_refused(dev):
+    """It has no formula here: refused where one reaches them, not left out of the sum."""
+    from directcompute_torch_b200 import ops
+    q, k, v, go = _inputs(1, 5, 7, 2, 1, 8)
+    t = [ops.tensor(x, requires_grad=True) for x in (q, k, v)]
+    out, lse = ops.attention(*t, return_lse=True)
+    want = T.attention(q, k, v, go)
+    assert _max_over(np.abs(ops.to_numpy(lse) - want["lse"]), want["lse_tol"]) <= 1
+    with pytest.raises(NotImplementedError):
+        ops.add(ops.mul(out, out), ops.sum(ops.exp(lse))).backward()
+    for x in t:
+        x.grad = None
+    out, lse = ops.attention(*t, return_lse=True)            # beside a backward pass that leaves them out
+    out.backward(ops.tensor(go))
+    got = {x: ops.to_numpy(y.grad) for x, y in zip(("dq", "dk", "dv"), t)}
+    _hold(got, want, ("dq", "dk", "dv"))
+    assert not ops.attention(*(ops.tensor(x) for x in (q, k, v)), return_lse=True)[1].requires_grad
