@@ -8,7 +8,8 @@ pass cannot do without, and `exact(case, seed)` gives its result in 64 bits.
 
 All tensors are float32 with the features of a head adjacent in memory, [batch, position,
 head, feature]; index tensors are int32.  The library's calls take buffer handles; a program
-that holds torch tensors wraps their device pointers for the call.
+that holds torch tensors wraps their device pointers for the call.  The calls are ordered on the
+library's own stream and on no other, so such a program puts torch's work on that stream.
 """
 import ctypes
 import math
@@ -110,7 +111,19 @@ def _lengths(case):
     return [min(q, x) if case["op"] == "train" or q > 1 else q for x in kv], kv
 
 
+def _on_library_stream():
+    """Torch's work on the library's stream: what it writes before a call is there for it, and what a
+    call writes is there for torch."""
+    from directcompute_torch_b200 import load_library
+    lib = load_library()
+    if not lib.InitEngine():
+        raise RuntimeError("libdct_cuda: " + lib.dct_last_error().decode())
+    torch.cuda.set_stream(torch.cuda.ExternalStream(lib.dct_stream(), device=lib.dct_device()))
+
+
 def prepare(case, seed):
+    if own:
+        _on_library_stream()
     g = torch.Generator(device="cuda")
     g.manual_seed(int(seed))
 
