@@ -203,7 +203,11 @@ DCT_API void* dct_create_buffer(uint64_t count);
 DCT_API void* dct_buffer_device_ptr(void* handle);
 DCT_API uint64_t dct_buffer_count(void* handle);
 DCT_API int dct_buffer_refcount(void* handle);
-/* non-owning handle over caller device memory (released with ReleaseBuffer, never freed) */
+/* non-owning handle over caller device memory (released with ReleaseBuffer, never freed).
+ * The library's stream (dct_stream) is a non-blocking one, ordered with no other stream, the
+ * default one included: work of another stream on this memory has to be waited for on both
+ * sides of a call, by events or dct_synchronize, or be put on dct_stream() itself (in torch:
+ * torch.cuda.set_stream(torch.cuda.ExternalStream(lib.dct_stream()))). */
 DCT_API void* dct_wrap_device_ptr(void* dptr, uint64_t count);
 DCT_API int dct_copy_h2d(void* handle, const void* src, uint64_t offset, uint64_t count);   /* async */
 DCT_API int dct_copy_d2h(void* handle, void* dst, uint64_t offset, uint64_t count);         /* waits */
