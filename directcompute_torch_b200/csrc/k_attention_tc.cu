@@ -1076,8 +1076,9 @@ DCT_DEV void attn_dkv(const AttnArgs& a, const Tiles& w, int block, int row_tile
             if (r + e < lo || r + e >= hi) p[e] = -INFINITY;
         }
         const int ep = scale_of_p(p, ctl.top[0], row, quarter, warp);
+        const float up_p = pow2(ep);               // (not in the exponent, which would be rounded again)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) p[e] = ex2(p[e] + (float)ep);
+        for (int e = 0; e < 16; ++e) p[e] = ex2(p[e]) * up_p;
         store_operand<16>(tm_s + off, p);
         tmem_wait_st();
         arrive_warp(&ctl.p_full);

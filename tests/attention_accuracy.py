@@ -8,6 +8,12 @@ off by 2^-24 at most) is off by a few times as much, so FACTOR is 8.  A row whos
 is small by chance, or whose terms cancel (one visible key), gets a floor beside it: FLOOR
 roundings of each of its terms, u (half a step) of the term's size before cancellation, as
 independent errors: in length the root of the sum of squares, not the sum.
+
+For dv, whose last key may have a single row's weight to be made of, the floor counts what the
+weight exp(s - lse) is off by when lse is a float32 number, as the interface has it.  Its exponent
+is off by at most u |s| (the factor that takes the score to the exponent's base), u |lse| (lse
+itself), u |lse| (in that base) and u |s - lse| (the difference), each half a step of a number of
+that size, and the weight relatively by as much: |s| 4, |lse| 6, |s - lse| 10 make 26 u.
 """
 from __future__ import annotations
 
@@ -45,9 +51,13 @@ def _floors(q, k, v, go, see, scale, r):
     q, k, v, go = (x.astype(np.float64) for x in (q, k, v, go))
     p, lq, lk, lv, lg = r["p"], _len(q), _len(k), _len(v), _len(go)
     term = abs(scale) * p * (lg[:, None] * lv[None] + np.abs(r["delta"]))      # of dS
+    s = np.where(see, scale * (q @ k.T), 0.0)
+    with np.errstate(divide="ignore"):
+        away = np.where(p > 0, -np.log(p), 0.0)                                # lse - s
+    weight = p * (1 + (np.abs(s) + 2 * np.abs(np.where(see, s + away, 0)) + away) / FLOOR)
     # an error of delta is one for the whole row: it meets the sum of the weighted keys
     shared = abs(scale) * lg * _len(r["out"]) * _len(p @ k)
-    return {"out": U * np.sqrt((p * p) @ (lv * lv)), "dv": U * np.sqrt((p * p).T @ (lg * lg)),
+    return {"out": U * np.sqrt((p * p) @ (lv * lv)), "dv": U * np.sqrt((weight * weight).T @ (lg * lg)),
             "dq": U * (np.sqrt((term * term) @ (lk * lk)) + shared), "dk": U * np.sqrt((term * term).T @ (lq * lq))}
 
 

@@ -1,16 +1,29 @@
 """The transformer operators' results as near their definition as float32 arithmetic comes
 (tests.attention_accuracy), where operands, weights or gradients are far apart in size."""
+import ctypes
+
 import numpy as np
 import pytest
 
+from directcompute_torch_b200 import _abi
+from oracle import transformer as T
 from tests.attention_accuracy import hold
-from tests.test_gpu_transformer import _attention, _inputs
+from tests.test_gpu_transformer import _attention, _inputs, _muon
 
 pytestmark = pytest.mark.gpu
 
 
 def _both(dev, q, k, v, go, names=("out", "dq", "dk", "dv"), **kw):
     hold(_attention(dev, q, k, v, go, **kw), q, k, v, go, names=names, **kw)
+
+
+@pytest.mark.parametrize("mask", [{}, {"causal": True}, {"causal": True, "window": 200}], ids=str)
+@pytest.mark.parametrize("shape", [(2, 70, 70, 4, 2, 64), (1, 300, 300, 2, 2, 96), (3, 16, 1500, 16, 4, 128),
+                                   (1, 400, 400, 4, 1, 128), (2, 385, 385, 4, 4, 112), (1, 1500, 1500, 2, 1, 64),
+                                   (4, 260, 260, 8, 1, 33), (1, 700, 900, 6, 6, 72)], ids=str)
+def test_attention_as_near_as_float32(dev, shape, mask):
+    """Ordinary inputs, on the CUDA cores and the tensor cores."""
+    _both(dev, *_inputs(*shape), **mask)
 
 
 @pytest.mark.parametrize("t,d", [(60, 64), (512, 64), (384, 128), (400, 40)])
@@ -109,3 +122,77 @@ def test_attention_where_features_are_apart(dev, t, d, apart):
         name = ("dk", "dq", "out", "dv")[which]             # the result whose features are the operand's
         pick = {y: got[y][..., small] if y == name else got[y] for y in got}
         hold(pick, *x, names=(name,), features={name: small})
+
+
+def _newton_schulz(x, dtype, steps=5, coefficients=T.COEFFICIENTS, eps=1e-7):
+    """The definition in one type (the norm in float64, as everywhere here)."""
+    a, b, c = (dtype(v) for v in coefficients)
+    tall = x.shape[0] > x.shape[1]
+    x = x.astype(np.float64)
+    x = ((x.T if tall else x) / (np.linalg.norm(x) + eps)).astype(dtype)
+    for _ in range(steps):
+        g = x @ x.T
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return (x.T if tall else x).astype(np.float64)
+
+
+def _near(got, x, **kw):
+    """got is off by at most 8 times what float32 is (see tests.attention_accuracy), or what roundings of
+    x alone become in these steps."""
+    want, own = _newton_schulz(x, np.float64, **kw), _newton_schulz(x, np.float32, **kw)
+    r = np.random.default_rng(1)
+    moved = _newton_schulz(x * (1 + T.U * r.choice([-1.0, 1.0], x.shape)), np.float64, **kw)
+    off, own, moved = (np.linalg.norm(y - want) for y in (got, own, moved))
+    assert off <= 8 * own + 8 * moved + 4 * T.U * np.linalg.norm(want), (off, own, moved)
+
+
+@pytest.mark.parametrize("kind", ["even", "few", "falling"])
+@pytest.mark.parametrize("steps", [1, 2, 3, 5])
+@pytest.mark.parametrize("shape", [(40, 24), (128, 128), (333, 127), (60, 2500), (130, 257), (300, 300), (700, 520),
+                                   (1100, 1300), (150, 4000)], ids=str)
+def test_orthogonalize_as_near_as_float32(dev, shape, steps, kind):
+    """Matrices of even, of few and of steadily falling singular values, through each way and the steps between."""
+    r = np.random.default_rng(4)
+    x = r.normal(size=shape)
+    if kind != "even":
+        n = min(shape)
+        u, s, v = np.linalg.svd(x, full_matrices=False)
+        s = np.where(np.arange(n) < max(1, n // 8), 1.0, 1e-3) if kind == "few" else 10.0 ** -np.linspace(0, 4, n)
+        x = (u * s) @ v
+    x = x.astype(np.float32)
+    h, y = dev.buf(x), dev.empty(x.size)
+    try:
+        _abi.check(dev.lib, dev.lib.dct_orthogonalize(ctypes.byref(_muon((1, *shape), steps=steps)), h, y))
+        _near(dev.read(y).reshape(shape), x, steps=steps)
+    finally:
+        dev.free(h, y)
+
+
+@pytest.mark.parametrize("shape", [(90, 200), (400, 260)], ids=str)
+@pytest.mark.parametrize("coefficients", [(1.5, -0.5, 0.0), (2.0, -1.5, 0.5)], ids=str)
+def test_orthogonalize_other_polynomials_as_near_as_float32(dev, shape, coefficients):
+    x = np.random.default_rng(5).normal(size=shape).astype(np.float32)
+    a, b, c = coefficients
+    h, y = dev.buf(x), dev.empty(x.size)
+    try:
+        p = _muon((1, *shape), steps=12, a=a, b=b, c=c)
+        _abi.check(dev.lib, dev.lib.dct_orthogonalize(ctypes.byref(p), h, y))
+        _near(dev.read(y).reshape(shape), x, steps=12, coefficients=coefficients)
+    finally:
+        dev.free(h, y)
+
+
+@pytest.mark.parametrize("shape", [(2, 130, 257), (3, 128, 128)], ids=str)
+def test_muon_step_as_near_as_float32(dev, shape):
+    r = np.random.default_rng(6)
+    w, m, g = (f * r.normal(size=shape).astype(np.float32) for f in (np.float32(0.01), 1, 1))
+    hs = [dev.buf(x) for x in (w, m, g)]
+    try:
+        p = _muon(shape, lr=0.5, momentum=0.9, weight_decay=0.5, nesterov=1, scale=2.0)
+        _abi.check(dev.lib, dev.lib.dct_muon(ctypes.byref(p), *hs))
+        got = dev.read(hs[0]).reshape(shape)
+    finally:
+        dev.free(*hs)
+    for i in range(shape[0]):
+        u = g[i] + np.float32(0.9) * (np.float32(0.9) * m[i] + g[i])
+        _near(0.75 * w[i].astype(np.float64) - got[i], u)        # w is small, its roundings too: lr scale is 1
