@@ -688,10 +688,10 @@ DCT_DEV int meet(uint32_t mine, uint8_t (&top)[kTile][4], int row, int quarter, 
 // other tiles' v.)  Returns the exponent.
 template <int N>
 DCT_DEV int scale_of_ds(const float (&ds)[N], uint8_t (&top)[kTile][4], int row, int quarter, int warp) {
-  uint32_t m = 0;
+  float m = 0.f;
 #pragma unroll
-  for (int e = 0; e < N; ++e) m = max(m, __float_as_uint(ds[e]) & 0x7fffffffu);
-  return min(14 + 127 - meet(m >> 23, top, row, quarter, warp), 120);     // exponents: order enough
+  for (int e = 0; e < N; ++e) m = fmaxf(m, fabsf(ds[e]));
+  return min(14 + 127 - meet(__float_as_uint(m) >> 23, top, row, quarter, warp), 120);
 }
 // P = 2^y of a key's rows likewise: a key that no row gives much weight has a dv as small, with
 // as many bits.  (Down to weights of 2^-36; smaller ones keep steps of 2^-75.)
