@@ -8,8 +8,7 @@ pass cannot do without, and `exact(case, seed)` gives its result in 64 bits.
 
 All tensors are float32 with the features of a head adjacent in memory, [batch, position,
 head, feature]; index tensors are int32.  The library's calls take buffer handles; a program
-that holds torch tensors wraps their device pointers for the call.  The calls are ordered on the
-library's own stream and on no other, so such a program puts torch's work on that stream.
+that holds torch tensors wraps their device pointers for the call.
 """
 import ctypes
 import math
@@ -111,19 +110,7 @@ def _lengths(case):
     return [min(q, x) if case["op"] == "train" or q > 1 else q for x in kv], kv
 
 
-def _on_library_stream():
-    """Torch's work on the library's stream: what it writes before a call is there for it, and what a
-    call writes is there for torch."""
-    from directcompute_torch_b200 import load_library
-    lib = load_library()
-    if not lib.InitEngine():
-        raise RuntimeError("libdct_cuda: " + lib.dct_last_error().decode())
-    torch.cuda.set_stream(torch.cuda.ExternalStream(lib.dct_stream(), device=lib.dct_device()))
-
-
 def prepare(case, seed):
-    if own:
-        _on_library_stream()
     g = torch.Generator(device="cuda")
     g.manual_seed(int(seed))
 
@@ -265,10 +252,24 @@ def _plain_muon(s):
 # ---------------------------------------------------------------------------
 # the library's calls
 # ---------------------------------------------------------------------------
+def _library():
+    """The library.  Its calls are ordered on its own stream and on no other, so torch's work goes there from
+    the first call on: what torch has written is there for a call, and what a call writes for torch."""
+    from directcompute_torch_b200 import load_library
+    lib = load_library()
+    if not hasattr(_library, "stream"):
+        if not lib.InitEngine():
+            raise RuntimeError("libdct_cuda: " + lib.dct_last_error().decode())
+        _library.stream = torch.cuda.ExternalStream(lib.dct_stream(), device=lib.dct_device())
+        _library.stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(_library.stream)
+    return lib
+
+
 def _call(function, struct, *tensors):
     """One library call over torch tensors: their device pointers wrapped as handles for its time."""
-    from directcompute_torch_b200 import _abi, load_library
-    lib = load_library()
+    from directcompute_torch_b200 import _abi
+    lib = _library()
     handles = [None if t is None else lib.dct_wrap_device_ptr(t.data_ptr(), 1 + sum(
         (n - 1) * st for n, st in zip(t.shape, t.stride()))) for t in tensors]
     status = getattr(lib, function)(ctypes.byref(struct), *handles)
