@@ -9,8 +9,8 @@
 // one bulk copy brings it and it serves as either operand: with its features as the
 // contraction (scores) or with its rows (the products with P, dS).
 //
-// Heads that the split cannot hold (infinities, NaN, rows of very different size) take the
-// kernels of k_attention.cu, which pick them by the same test on the device.
+// Heads that the split cannot hold (infinities, NaN, rows or features of very different size)
+// take the kernels of k_attention.cu, which pick them by the same test on the device.
 #include <limits.h>
 
 #include <algorithm>
@@ -76,10 +76,12 @@ DCT_DEV void store_features(float* row, int first, int dim, bool vec, const floa
 // blocks [tensor][head][tile] of 512 threads; a thread takes 8 features of every 32nd (64th)
 // row and holds them while the block finds the tile's magnitude, so each operand is read
 // once.  With dout come delta = sum dout out and the log-sums.  Bound by memory: 8 bytes a
-// feature (12 for dout).
+// feature (12 for dout).  Three blocks an SM for 64 features: training with a window 196 us with
+// two, 191.5 with three.
 template <int BLOCKS>
-__global__ void __launch_bounds__(512, BLOCKS == 1 ? 3 : 2) k_attn_split(const __grid_constant__ AttnArgs a, const __grid_constant__ Tiles w,
-                                                    int tq, int tk, bool vec) {
+__global__ void __launch_bounds__(512, BLOCKS == 1 ? 3 : 2) k_attn_split(const __grid_constant__ AttnArgs a,
+                                                                         const __grid_constant__ Tiles w, int tq,
+                                                                         int tk, bool vec) {
   constexpr int kGroups = 8 * BLOCKS, kStep = 512 / kGroups, kPasses = kTile / kStep;
   __shared__ uint32_t sh[2];
   __shared__ uint2 sizes[16][kGroups];             // exponents of 8 features' largest |x|, a warp's rows

@@ -344,7 +344,8 @@ DCT_API int dct_rotary(const DctRotary* p, void* x, void* positions, void* y);
  * What a masked place holds, NaN and infinity too, does not reach a result.  lse is
  * [batch, q_heads, q_len], adjacent; it may be null in the forward call.  The backward
  * call takes the forward call's out and lse and recomputes the probabilities; dout has
- * o_stride. */
+ * o_stride.  Results have the accuracy of float32 arithmetic; the forward call holds a row's
+ * weights to 2^-40 of the largest, so those below 2^-17 of it in fewer bits. */
 typedef struct DctAttention {
   uint32_t batch, q_heads, kv_heads, q_len, kv_len, head_dim;
   int32_t causal;
