@@ -365,6 +365,8 @@ DCT_API int dct_attention_backward(const DctAttention* p, void* q, void* k, void
  * (on the shorter side; X^T X for tall matrices), which moves the singular values
  * toward 1.  a = b = c = 0 means 3.4445, -4.7750, 2.0315; steps 0..16; the polynomial
  * a s + b s^3 + c s^5 must keep [0, 1] below 64 over the steps (DCT_ERR_ARG).
+ * X is held in steps of 2^-38 of the largest singular value that these can reach (1.2 for the
+ * default): where |x|_F is 1e-5 of eps or less, and X as small, that leaves few bits or none.
  * y may be x.  batch <= 65535, rows and cols <= 2^23, rows cols < 2^30.  Scratch: 8 bytes for
  * each element of a matrix padded to multiples of 64 rows and columns, and for each of the
  * shorter side's square, with a batch in groups of at most 2 GB (or one matrix); less than 1 MB
